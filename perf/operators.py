@@ -164,9 +164,11 @@ def _inputs(case, seed):
         if op == "grad":
             # the forward's statistics, which a training step keeps, and the two gradients
             x = s["logits"].double()
-            lse = torch.logsumexp(x, -1)
-            s["lse"] = lse.float()
-            s["entropy"] = (lse - ((x - lse[:, None]).exp() * x).sum(-1)).float()
+            m = x.amax(-1)
+            e = (x - m[:, None]).exp()
+            z = e.sum(-1)
+            s["m"], s["l"] = m.float(), z.float()
+            s["entropy"] = (z.log() - (e * (x - m[:, None])).sum(-1) / z).float()
             s["dlogp"], s["dentropy"] = _normal(g, (n,), torch.float32), _normal(g, (n,), torch.float32, 0.1)
         return s
     b, dk, seq = case["batch"], case["dk"], case["seq"]
@@ -208,7 +210,7 @@ def prepare(case, seed):
                                device="cuda", dtype=dt)
     elif op == "score":
         n, k = case["rows"], case["top_k"]
-        s["out"] = {name: torch.zeros((n,), device="cuda") for name in ("logp", "entropy", "lse")}
+        s["out"] = {name: torch.zeros((n,), device="cuda") for name in ("logp", "entropy", "m", "l")}
         if k:
             s["out"]["top_ids"] = torch.zeros((n, k), device="cuda", dtype=torch.int64)
             s["out"]["top_logp"] = torch.zeros((n, k), device="cuda")
@@ -315,21 +317,20 @@ def _score_plain(s, c):
     t = x - top
     e = torch.exp(t)
     z = e.sum(-1)
-    lse = top[:, 0] + torch.log(z)
     entropy = torch.log(z) - (e * torch.where(e == 0, zero, t)).sum(-1) / z
-    logp = x.gather(1, target.clamp_min(0)[:, None])[:, 0] - lse
+    logp = t.gather(1, target.clamp_min(0)[:, None])[:, 0] - torch.log(z)
     out = {"logp": torch.where(kept, logp, zero), "entropy": torch.where(kept, entropy, zero),
-           "lse": torch.where(kept, lse, zero)}
+           "m": torch.where(kept, top[:, 0], zero), "l": torch.where(kept, z, zero)}
     if c["top_k"]:
         best, ids = torch.sort(x, dim=-1, descending=True, stable=True)
-        ids, best = ids[:, :c["top_k"]], best[:, :c["top_k"]] - lse[:, None]
+        ids, best = ids[:, :c["top_k"]], best[:, :c["top_k"]] - top - torch.log(z)[:, None]
         out["top_ids"] = torch.where(kept[:, None], ids, torch.full_like(ids, -1))
         out["top_logp"] = torch.where(kept[:, None], best, zero)
     return out
 
 
 def _grad_plain(s, c):
-    logp = s["logits"].float() - s["lse"][:, None]
+    logp = s["logits"].float() - s["m"][:, None] - torch.log(s["l"])[:, None]
     p = torch.exp(logp)
     d = -s["dlogp"][:, None] * p
     d -= s["dentropy"][:, None] * p * torch.where(p == 0, torch.zeros_like(p),
@@ -381,7 +382,7 @@ def _score_own(N, s, c):
     o, k = s["out"], c["top_k"]
     N.check(N.lib.nml_token_logprobs_device(
         s["logits"].data_ptr(), c["vocab"], s["targets"].data_ptr(), c["rows"], c["vocab"], IGNORE,
-        1, k, o["logp"].data_ptr(), o["entropy"].data_ptr(), o["lse"].data_ptr(),
+        1, k, o["logp"].data_ptr(), o["entropy"].data_ptr(), o["m"].data_ptr(), o["l"].data_ptr(),
         o["top_ids"].data_ptr() if k else None, o["top_logp"].data_ptr() if k else None,
         s["err"].data_ptr(), CODES[c["dtype"]]))
     return o
@@ -389,8 +390,8 @@ def _score_own(N, s, c):
 
 def _grad_own(N, s, c):
     N.check(N.lib.nml_token_logprobs_backward_device(
-        s["logits"].data_ptr(), c["vocab"], s["targets"].data_ptr(), s["lse"].data_ptr(),
-        s["entropy"].data_ptr(), s["dlogp"].data_ptr(), s["dentropy"].data_ptr(), c["rows"],
+        s["logits"].data_ptr(), c["vocab"], s["targets"].data_ptr(), s["m"].data_ptr(),
+        s["l"].data_ptr(), s["entropy"].data_ptr(), s["dlogp"].data_ptr(), s["dentropy"].data_ptr(), c["rows"],
         c["vocab"], IGNORE, 1, s["out"].data_ptr(), c["vocab"], s["err"].data_ptr(),
         CODES[c["dtype"]]))
     return s["out"]
@@ -417,8 +418,8 @@ def work(case):
     if op in ("score", "grad"):
         n = case["rows"] * case["vocab"]
         if op == "grad":
-            return {"bytes": 2 * es * n + 24 * case["rows"], "flops": 8 * n}
-        return {"bytes": es * n + (20 + 12 * case["top_k"]) * case["rows"], "flops": 6 * n}
+            return {"bytes": 2 * es * n + 28 * case["rows"], "flops": 8 * n}
+        return {"bytes": es * n + (24 + 12 * case["top_k"]) * case["rows"], "flops": 6 * n}
     tokens = case["batch"] * case["seq"] * (0.5 if case["ragged"] and case["batch"] > 1 else 1)
     if op != "attend":
         vectors = 2 * tokens * case["heads"]  # K's and V's
@@ -462,7 +463,7 @@ def exact(case, seed):
         keep = (t != IGNORE).double()
         at = t.clamp_min(0)[:, None]
         if op == "grad":
-            lp = x - s["lse"].double()[:, None]
+            lp = x - s["m"].double()[:, None] - s["l"].double().log()[:, None]
             p = lp.exp()
             hot = torch.zeros_like(x).scatter_(1, at, 1.0)
             d = s["dlogp"].double()[:, None] * (hot - p)
@@ -471,7 +472,7 @@ def exact(case, seed):
         lse = torch.logsumexp(x, -1)
         lp = x - lse[:, None]
         out = {"logp": lp.gather(1, at)[:, 0] * keep, "entropy": -(lp.exp() * lp).sum(-1) * keep,
-               "lse": lse * keep}
+               "m": x.amax(-1) * keep, "l": (x - x.amax(-1, keepdim=True)).exp().sum(-1) * keep}
         if case["top_k"]:
             out["top_ids"] = None
             out["top_logp"] = torch.topk(lp, case["top_k"], -1).values * keep[:, None]
