@@ -162,6 +162,55 @@ int nml_decode_attention_device(const void* q, const void* kcache, const void* v
                                 const int32_t* lens, void* out, size_t batch, size_t heads,
                                 size_t max_seq, size_t dk, float scale_div, int* err, int dtype);
 
+/* ---- a KV cache in 4 bits ----
+ * No reference counterpart (its generate() keeps no cache, models/generate.py:101-103): the
+ * cache of nml_decode_attention_device at 4.25 bits a value. A head's vector of dk values is cut
+ * into nb = ⌈dk/32⌉ blocks of 32 (the last padded with zeros); a block is 32 E2M1 codes (0, ½,
+ * 1, 1½, 2, 3, 4, 6 and sign; code i in half i % 2 of byte i / 2, the low half first) and a
+ * scale byte e for 2^(e − 127), 255 for NaN. With 2^k ≤ max|x| < 2^(k+1) a block's scale is
+ * 2^(k−2), or 2^(k−1) where max|x| ≥ 1.75·2^k, within [2^-120, 2^125] (2^13 for float16
+ * values); a value goes to the nearest multiple, ties to the even code, at most ±6. A block with
+ * an infinite or NaN value reads back as NaN throughout.
+ *   k_codes, v_codes:   uint8 (batch, kv_heads, max_seq, nb, 16), 16-byte aligned
+ *   k_scales, v_scales: uint8 (batch, kv_heads, max_seq, nb)
+ * pos, counts, lens: device int32 (batch). *err: device int, may be NULL, cleared by the caller;
+ * bit 0 is set for a position outside the cache, a count outside [0, seq] or a length outside
+ * [0, max_seq] (counts and lengths are clamped). Any head dim 1 ≤ dk ≤ 256; all asynchronous. */
+
+/* Quantises seq new tokens of each row into the cache: token s of row b, s < counts[b] (NULL:
+ * seq), goes to position pos[b] + s (NULL: s). Element d of head h of that token is at
+ * k[b·stride_b + h·stride_h + s·stride_s + d], v alike (strides in elements: a projection's
+ * (batch, seq, heads, dk) or head-major (batch, heads, seq, dk)). Other positions, and tokens
+ * outside the cache, are left as they were. Rows of one call must not share positions. */
+int nml_kv4_write_device(const void* k, const void* v, size_t stride_b, size_t stride_h,
+                         size_t stride_s, uint8_t* k_codes, uint8_t* k_scales, uint8_t* v_codes,
+                         uint8_t* v_scales, const int32_t* pos, const int32_t* counts,
+                         size_t batch, size_t heads, size_t seq, size_t max_seq, size_t dk,
+                         int* err, int dtype);
+/* The values of those positions, k_out and v_out: (batch, heads, seq, dk) in dtype (rounded to
+ * it where it is float16 and the cache was written from float32). Tokens from counts[b] on are
+ * left as they were; a position outside the cache reads as zeros. */
+int nml_kv4_read_device(const uint8_t* k_codes, const uint8_t* k_scales, const uint8_t* v_codes,
+                        const uint8_t* v_scales, const int32_t* pos, const int32_t* counts,
+                        void* k_out, void* v_out, size_t batch, size_t heads, size_t seq,
+                        size_t max_seq, size_t dk, int* err, int dtype);
+/* Causal attention of each row's counts[b] (NULL: seq) last cached tokens over the cache: token
+ * s stands at position lens[b] − counts[b] + s and sees the keys up to itself,
+ *   s_j = (q·k_j) / scale_div, softmax, Σ_j p_j·v_j     (scores and sums in float32)
+ * with the cache's values exactly; a token that sees no key (a length below the count) gives
+ * zeros. A NaN block reaches only the tokens that see its key. seq = 1 is a decode step.
+ *   q: (batch, heads, seq, dk); out: (batch, seq, heads·dk), rows from counts[b] on left as
+ *   they were; query head h reads KV head h / (heads / kv_heads)
+ *   ws: nml_kv4_attention_workspace bytes, 16-byte aligned; nothing is kept in it from one call
+ *   to the next, but calls that run at the same time need one each. */
+int nml_kv4_attention_workspace(size_t batch, size_t heads, size_t kv_heads, size_t seq,
+                                size_t max_seq, size_t dk, size_t* bytes);
+int nml_kv4_attention_device(const void* q, const uint8_t* k_codes, const uint8_t* k_scales,
+                             const uint8_t* v_codes, const uint8_t* v_scales, const int32_t* lens,
+                             const int32_t* counts, void* out, size_t batch, size_t heads,
+                             size_t kv_heads, size_t seq, size_t max_seq, size_t dk,
+                             float scale_div, void* ws, size_t ws_bytes, int* err, int dtype);
+
 /* Mean tied-head cross-entropy (kernels/fused_tied_crossentropy.py:8-24 →
  * fused_crossentropy.py:14-30) without materialising all (rows, vocab) logits at once.
  * has_ignore: drop rows with label == ignore_index (losses/_ce_prepare.py:46-69).
@@ -191,6 +240,34 @@ int nml_sample_device(const void* logits, size_t batch, size_t vocab, float temp
                       int top_k, float top_p, float repetition_penalty, const double* u,
                       const int64_t* history, size_t history_stride, const int32_t* hist_len,
                       int64_t* out_ids, int dtype);
+
+/* Log probabilities of given tokens, with no reference kernel: the float32 counterpart, row by
+ * row, of what losses/cross_entropy.py:109-192 averages and models/generate.py:23-59 draws from.
+ * logits: (rows, vocab) at a row stride of ld elements (dtype), targets: int64 (rows).
+ *   m = max_v x_v, l = Σ_v exp(x_v − m) (the log-sum-exp is m + log l)
+ *   logp = x[target] − m − log l
+ *   entropy = −Σ_v p_v·log p_v          (p_v = exp(x_v − m) / l; a logit of −inf adds nothing)
+ *   top_ids, top_logp: (rows, top_k), the largest logits' ids and log probabilities, largest
+ *             first, of equal ones the lower id first (NaN ranks above all); top_k ≤ 64
+ * Outputs are float32 (ids int64); logp, entropy, m, l may each be NULL, targets too without
+ * logp. has_ignore: a row whose target is ignore_index is not read and gives zeros and ids −1.
+ * A target outside [0, vocab) gives a logp of NaN and sets bit 0 of *err (device int, may be
+ * NULL; the caller clears it). A row holding NaN, or nothing above −inf, has no distribution:
+ * its statistics are NaN. Asynchronous, no workspace. */
+int nml_token_logprobs_device(const void* logits, size_t ld, const int64_t* targets, size_t rows,
+                              size_t vocab, int64_t ignore_index, int has_ignore, size_t top_k,
+                              float* logp, float* entropy, float* m, float* l,
+                              int64_t* top_ids, float* top_logp, int* err, int dtype);
+/* Its gradient: dlogits (rows, vocab) at stride ld_d, of the logits' dtype, is overwritten with
+ *   dlogp·([v = target] − p_v) − dentropy·p_v·(log p_v + entropy)
+ * from the forward's m, l and entropy; dlogp, dentropy: float32 (rows), NULL for none (without
+ * dentropy, entropy may be NULL). Ignored rows: zeros. dlogits may be logits itself. A target
+ * outside [0, vocab) makes its row NaN and sets bit 0 of *err. Asynchronous, no workspace. */
+int nml_token_logprobs_backward_device(const void* logits, size_t ld, const int64_t* targets,
+                                       const float* m, const float* l, const float* entropy,
+                                       const float* dlogp, const float* dentropy, size_t rows,
+                                       size_t vocab, int64_t ignore_index, int has_ignore, void* dlogits,
+                                       size_t ld_d, int* err, int dtype);
 
 /* Optimizer step, float32 state, in place on device buffers.
  * adamw_step (native/src/module.cpp:175-188 → adamw_step_cpu, native/src/adamw.cpp:6-20):

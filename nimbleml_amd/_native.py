@@ -63,6 +63,15 @@ _SIGS = {
     "nml_embedding_backward_device": [vp, vp, vp, sz, sz, sz, i32],
     "nml_causal_attention_device": [vp, vp, vp, vp, sz, sz, sz, f32, i32],
     "nml_decode_attention_device": [vp, vp, vp, vp, vp, sz, sz, sz, sz, f32, vp, i32],
+    "nml_kv4_write_device": [vp, vp, sz, sz, sz, vp, vp, vp, vp, vp, vp, sz, sz, sz, sz, sz, vp,
+                             i32],
+    "nml_kv4_read_device": [vp, vp, vp, vp, vp, vp, vp, vp, sz, sz, sz, sz, sz, vp, i32],
+    "nml_kv4_attention_workspace": [sz, sz, sz, sz, sz, sz, C.POINTER(sz)],
+    "nml_kv4_attention_device": [vp, vp, vp, vp, vp, vp, vp, vp, sz, sz, sz, sz, sz, sz, f32, vp,
+                                 sz, vp, i32],
+    "nml_token_logprobs_device": [vp, sz, vp, sz, sz, i64, i32, sz, vp, vp, vp, vp, vp, vp, vp, i32],
+    "nml_token_logprobs_backward_device": [vp, sz, vp, vp, vp, vp, vp, vp, sz, sz, i64, i32, vp,
+                                           sz, vp, i32],
     "nml_sdpa_forward_device": [vp, vp, vp, vp, vp, sz, sz, sz, f32, i32, i32],
     "nml_tied_ce_forward_device": [vp, vp, vp, sz, sz, sz, i64, i32, C.POINTER(C.c_double), i32],
     "nml_tied_ce_forward_device_noalloc": [vp, vp, vp, sz, sz, sz, i64, i32,

@@ -196,6 +196,92 @@ struct SampleArgs {
 };
 int launch_sample(int dt, const SampleArgs& a, hipStream_t st);
 
+// The KV cache in 4 bits (ops_kv4.hip). Codes (B, Hkv, P, ⌈dk/32⌉, 16) and scales
+// (B, Hkv, P, ⌈dk/32⌉) bytes, for K and for V; P positions a row.
+//
+// Write: token s < counts[b] (null: S) of row b goes to position pos[b] + s (null: s); element d
+// of head h is at k + b·stride_b + h·stride_h + s·stride_s + d, v alike. A position outside the
+// cache is not written and sets bit 0 of *err (may be null), a count outside [0, S] is clamped
+// and does so too.
+struct Kv4WriteArgs {
+  const void* k;
+  const void* v;
+  long long stride_b, stride_h, stride_s;
+  uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
+  const int32_t* pos;
+  const int32_t* counts;
+  int B, H, S, P, dk;
+  int* err;
+};
+int launch_kv4_write(int dt, const Kv4WriteArgs& a, hipStream_t st);
+
+// Read: the same positions into k_out and v_out, (B, H, S, dk) of type dt; tokens from counts[b]
+// on are left as they were, a position outside the cache reads as zeros (and sets the bit).
+struct Kv4ReadArgs {
+  const uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
+  const int32_t* pos;
+  const int32_t* counts;
+  void* k_out;
+  void* v_out;
+  int B, H, S, P, dk;
+  int* err;
+};
+int launch_kv4_read(int dt, const Kv4ReadArgs& a, hipStream_t st);
+
+// Attention of counts[b] (null: S) new tokens of each row, the last of the row's lens[b] cached
+// ones: token s sees keys 0 … lens[b] − counts[b] + s, none of them: zeros. q (B, H, S, dk),
+// out (B, S, H·dk); query head h reads KV head h / (H / Hkv). Rows of out from counts[b] on are
+// left as they were. ws: kv4_attention_workspace bytes, contents free before and after.
+struct Kv4AttnArgs {
+  const void* q;
+  const uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
+  const int32_t* lens;
+  const int32_t* counts;
+  void* out;
+  int B, H, Hkv, S, P, dk;
+  float scale;  // divisor of the scores
+  void* ws;
+  int* err;
+};
+size_t kv4_attention_workspace(int B, int H, int Hkv, int S, int P, int dk);
+int launch_kv4_attention(int dt, const Kv4AttnArgs& a, hipStream_t st);
+
+// Log probabilities of given tokens (ops_logprob.hip): per row of logits (rows, V) at stride ld,
+// m = max x, l = Σ exp(x − m), logp = x[target] − m − log l, entropy = −Σ p log p and the top_k largest logits'
+// ids and log probabilities in order (of equal ones the lower id first). Any of logp, entropy,
+// m, l may be null. A row whose target is ignore_index (with has_ignore) gives zeros, ids −1; a
+// target outside [0, V) gives NaN and sets bit 0 of *err (may be null).
+struct LogprobArgs {
+  const void* logits;
+  long long ld;
+  const int64_t* targets;  // null: no logp, no row ignored
+  int rows, V;
+  long long ignore_index;
+  int has_ignore, top_k;
+  float *logp, *entropy, *m, *l;
+  int64_t* top_ids;
+  float* top_logp;
+  int* err;
+};
+constexpr int kMaxTopLogprobs = 64;
+int launch_logprobs(int dt, const LogprobArgs& a, hipStream_t st);
+
+// Its gradient: dlogits = dlogp·([v = target] − p_v) − dentropy·p_v·(log p_v + entropy), from the
+// forward's m, l and entropy; dlogp, dentropy: null for zero. May overwrite logits in place.
+struct LogprobBwdArgs {
+  const void* logits;
+  long long ld;
+  const int64_t* targets;
+  const float *m, *l, *entropy, *dlogp, *dentropy;
+  int rows, V;
+  long long ignore_index;
+  int has_ignore;
+  void* dlogits;
+  long long ld_d;
+  int* err;
+};
+int launch_logprobs_backward(int dt, const LogprobBwdArgs& a, hipStream_t st);
+
 // ------------------------------------------------------------ training
 // Every launch takes the model's storage type dt (F32 or F16) for the activation-side
 // tensors; parameter gradients, partial sums and the softmax statistics are float32.

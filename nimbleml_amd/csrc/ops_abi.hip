@@ -177,6 +177,23 @@ int noalloc_scratch(void** out) {
   return 0;
 }
 
+int kv4_codes_ok(const char* what, const void* k_codes, const void* v_codes) {
+  NML_REQUIRE(((reinterpret_cast<uintptr_t>(k_codes) | reinterpret_cast<uintptr_t>(v_codes)) & 15) == 0,
+              "%s: codes must be 16-byte aligned", what);
+  return 0;
+}
+
+// Sizes of a 4-bit cache call: a launch of four lanes a block, 32-bit element numbers within a
+// row of the batch.
+int kv4_shape_ok(const char* what, size_t batch, size_t heads, size_t seq, size_t max_seq, size_t dk) {
+  NML_REQUIRE(dk >= 1 && dk <= (size_t)kMaxHeadDim, "%s: head_dim %zu outside [1, %d]", what, dk, kMaxHeadDim);
+  NML_REQUIRE(batch <= 65535 && heads <= 65535, "%s: %zu rows × %zu heads too many", what, batch, heads);
+  NML_REQUIRE(max_seq >= 1 && max_seq <= (size_t)1 << 30, "%s: max_seq %zu outside [1, 2^30]", what, max_seq);
+  NML_REQUIRE(seq <= ((size_t)1 << 26) / (heads ? heads : 1), "%s: %zu tokens × %zu heads too many", what, seq,
+              heads);
+  return 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -518,6 +535,182 @@ int nml_sample_device(const void* logits, size_t batch, size_t vocab, float temp
   a.hist_len = history ? hist_len : nullptr;
   a.out_ids = out_ids;
   return launch_sample(dtype, a, nml::stream());
+}
+
+int nml_kv4_write_device(const void* k, const void* v, size_t stride_b, size_t stride_h, size_t stride_s,
+                         uint8_t* k_codes, uint8_t* k_scales, uint8_t* v_codes, uint8_t* v_scales,
+                         const int32_t* pos, const int32_t* counts, size_t batch, size_t heads, size_t seq,
+                         size_t max_seq, size_t dk, int* err, int dtype) {
+  NML_TRY(check_dtype(dtype));
+  NML_TRY(kv4_shape_ok("kv4 write", batch, heads, seq, max_seq, dk));
+  if (batch == 0 || heads == 0 || seq == 0) return 0;
+  NML_REQUIRE(k && v && k_codes && k_scales && v_codes && v_scales, "kv4 write: a buffer is null");
+  NML_TRY(kv4_codes_ok("kv4 write", k_codes, v_codes));
+  const size_t limit = (size_t)1 << 40;
+  NML_REQUIRE(stride_b < limit && stride_h < limit && stride_s < limit, "kv4 write: a stride is out of range");
+  Kv4WriteArgs a{};
+  a.k = k;
+  a.v = v;
+  a.stride_b = (long long)stride_b;
+  a.stride_h = (long long)stride_h;
+  a.stride_s = (long long)stride_s;
+  a.k_codes = k_codes;
+  a.k_scales = k_scales;
+  a.v_codes = v_codes;
+  a.v_scales = v_scales;
+  a.pos = pos;
+  a.counts = counts;
+  a.B = (int)batch;
+  a.H = (int)heads;
+  a.S = (int)seq;
+  a.P = (int)max_seq;
+  a.dk = (int)dk;
+  a.err = err;
+  return launch_kv4_write(dtype, a, nml::stream());
+}
+
+int nml_kv4_read_device(const uint8_t* k_codes, const uint8_t* k_scales, const uint8_t* v_codes,
+                        const uint8_t* v_scales, const int32_t* pos, const int32_t* counts, void* k_out,
+                        void* v_out, size_t batch, size_t heads, size_t seq, size_t max_seq, size_t dk, int* err,
+                        int dtype) {
+  NML_TRY(check_dtype(dtype));
+  NML_TRY(kv4_shape_ok("kv4 read", batch, heads, seq, max_seq, dk));
+  if (batch == 0 || heads == 0 || seq == 0) return 0;
+  NML_REQUIRE(k_out && v_out && k_codes && k_scales && v_codes && v_scales, "kv4 read: a buffer is null");
+  NML_TRY(kv4_codes_ok("kv4 read", k_codes, v_codes));
+  Kv4ReadArgs a{};
+  a.k_codes = k_codes;
+  a.k_scales = k_scales;
+  a.v_codes = v_codes;
+  a.v_scales = v_scales;
+  a.pos = pos;
+  a.counts = counts;
+  a.k_out = k_out;
+  a.v_out = v_out;
+  a.B = (int)batch;
+  a.H = (int)heads;
+  a.S = (int)seq;
+  a.P = (int)max_seq;
+  a.dk = (int)dk;
+  a.err = err;
+  return launch_kv4_read(dtype, a, nml::stream());
+}
+
+static int kv4_attention_ok(size_t batch, size_t heads, size_t kv_heads, size_t seq, size_t max_seq, size_t dk) {
+  NML_TRY(kv4_shape_ok("kv4 attention", batch, heads, seq, max_seq, dk));
+  NML_REQUIRE(kv_heads >= 1 ? heads % kv_heads == 0 : heads == 0,
+              "kv4 attention: heads (%zu) must be divisible by kv_heads (%zu)", heads, kv_heads);
+  return 0;
+}
+
+int nml_kv4_attention_workspace(size_t batch, size_t heads, size_t kv_heads, size_t seq, size_t max_seq,
+                                size_t dk, size_t* bytes) {
+  NML_REQUIRE(bytes != nullptr, "kv4 attention: bytes is null");
+  *bytes = 0;
+  NML_TRY(kv4_attention_ok(batch, heads, kv_heads, seq, max_seq, dk));
+  if (batch && heads && seq)
+    *bytes = kv4_attention_workspace((int)batch, (int)heads, (int)kv_heads, (int)seq, (int)max_seq, (int)dk);
+  return 0;
+}
+
+int nml_kv4_attention_device(const void* q, const uint8_t* k_codes, const uint8_t* k_scales,
+                             const uint8_t* v_codes, const uint8_t* v_scales, const int32_t* lens,
+                             const int32_t* counts, void* out, size_t batch, size_t heads, size_t kv_heads,
+                             size_t seq, size_t max_seq, size_t dk, float scale_div, void* ws, size_t ws_bytes,
+                             int* err, int dtype) {
+  NML_TRY(check_dtype(dtype));
+  NML_TRY(kv4_attention_ok(batch, heads, kv_heads, seq, max_seq, dk));
+  NML_REQUIRE(scale_div > 0.f && std::isfinite(scale_div), "kv4 attention: scale_div must be positive");
+  if (batch == 0 || heads == 0 || seq == 0) return 0;
+  NML_REQUIRE(q && k_codes && k_scales && v_codes && v_scales && lens && out, "kv4 attention: a buffer is null");
+  NML_TRY(kv4_codes_ok("kv4 attention", k_codes, v_codes));
+  const size_t need =
+      kv4_attention_workspace((int)batch, (int)heads, (int)kv_heads, (int)seq, (int)max_seq, (int)dk);
+  NML_REQUIRE(ws_bytes >= need && (need == 0 || ws != nullptr),
+              "kv4 attention: a workspace of %zu bytes is needed, %zu given", need, ws ? ws_bytes : (size_t)0);
+  NML_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 15) == 0, "kv4 attention: the workspace must be 16-byte aligned");
+  Kv4AttnArgs a{};
+  a.q = q;
+  a.k_codes = k_codes;
+  a.k_scales = k_scales;
+  a.v_codes = v_codes;
+  a.v_scales = v_scales;
+  a.lens = lens;
+  a.counts = counts;
+  a.out = out;
+  a.B = (int)batch;
+  a.H = (int)heads;
+  a.Hkv = (int)kv_heads;
+  a.S = (int)seq;
+  a.P = (int)max_seq;
+  a.dk = (int)dk;
+  a.scale = scale_div;
+  a.ws = ws;
+  a.err = err;
+  return launch_kv4_attention(dtype, a, nml::stream());
+}
+
+int nml_token_logprobs_device(const void* logits, size_t ld, const int64_t* targets, size_t rows, size_t vocab,
+                              int64_t ignore_index, int has_ignore, size_t top_k, float* logp, float* entropy,
+                              float* m, float* l, int64_t* top_ids, float* top_logp, int* err, int dtype) {
+  NML_TRY(check_dtype(dtype));
+  NML_REQUIRE(rows <= 0x7fffffff && vocab >= 1 && vocab <= (size_t)1 << 30 && ld >= vocab && ld < (size_t)1 << 40,
+              "token logprobs: %zu rows of %zu logits at stride %zu out of range", rows, vocab, ld);
+  NML_REQUIRE(top_k <= (size_t)kMaxTopLogprobs && top_k <= vocab,
+              "token logprobs: top_k %zu above %d or the vocabulary", top_k, kMaxTopLogprobs);
+  if (rows == 0) return 0;
+  NML_REQUIRE(logits != nullptr, "token logprobs: logits is null");
+  NML_REQUIRE(targets != nullptr || logp == nullptr, "token logprobs: logp needs targets");
+  NML_REQUIRE(top_k == 0 || (top_ids && top_logp), "token logprobs: top_k needs top_ids and top_logp");
+  LogprobArgs a{};
+  a.logits = logits;
+  a.ld = (long long)ld;
+  a.targets = targets;
+  a.rows = (int)rows;
+  a.V = (int)vocab;
+  a.ignore_index = ignore_index;
+  a.has_ignore = has_ignore;
+  a.top_k = (int)top_k;
+  a.logp = logp;
+  a.entropy = entropy;
+  a.m = m;
+  a.l = l;
+  a.top_ids = top_ids;
+  a.top_logp = top_logp;
+  a.err = err;
+  return launch_logprobs(dtype, a, nml::stream());
+}
+
+int nml_token_logprobs_backward_device(const void* logits, size_t ld, const int64_t* targets, const float* m,
+                                       const float* l, const float* entropy, const float* dlogp,
+                                       const float* dentropy,
+                                       size_t rows, size_t vocab, int64_t ignore_index, int has_ignore,
+                                       void* dlogits, size_t ld_d, int* err, int dtype) {
+  NML_TRY(check_dtype(dtype));
+  NML_REQUIRE(rows <= 0x7fffffff && vocab >= 1 && vocab <= (size_t)1 << 30 && ld >= vocab && ld < (size_t)1 << 40 &&
+                  ld_d >= vocab && ld_d < (size_t)1 << 40,
+              "token logprobs backward: %zu rows of %zu logits at strides %zu, %zu out of range", rows, vocab, ld,
+              ld_d);
+  if (rows == 0) return 0;
+  NML_REQUIRE(logits && targets && m && l && dlogits, "token logprobs backward: a buffer is null");
+  NML_REQUIRE(dentropy == nullptr || entropy != nullptr, "token logprobs backward: dentropy needs entropy");
+  LogprobBwdArgs a{};
+  a.logits = logits;
+  a.ld = (long long)ld;
+  a.targets = targets;
+  a.m = m;
+  a.l = l;
+  a.entropy = entropy;
+  a.dlogp = dlogp;
+  a.dentropy = dentropy;
+  a.rows = (int)rows;
+  a.V = (int)vocab;
+  a.ignore_index = ignore_index;
+  a.has_ignore = has_ignore;
+  a.dlogits = dlogits;
+  a.ld_d = (long long)ld_d;
+  a.err = err;
+  return launch_logprobs_backward(dtype, a, nml::stream());
 }
 
 }  // extern "C"

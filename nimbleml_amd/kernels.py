@@ -7,6 +7,12 @@ Each takes host arrays or ``DeviceArray``s in the compute dtype and returns
   fused_sdpa_forward          kernels/fused_sdpa.py:256-289 (any additive mask, or none)
   decode_attention            one cached decode step of that attention (the KV-cache seam of
                               models/generate.py:93-100; no reference kernel)
+  KV4Cache, kv4_write, kv4_read, kv4_attention
+                              a KV cache in 4 bits: quantised as it is written, read back,
+                              attended to by one or several new tokens (no reference kernel)
+  token_logprobs, token_logprobs_backward
+                              log probabilities of given tokens, entropies and the best
+                              alternatives, and their gradient (no reference kernel)
   embedding_lookup            kernels/embedding_scatter.py:25-36
   fused_tied_crossentropy_forward  kernels/fused_tied_crossentropy.py:8-24 (loss only)
   linear                      the `x @ W + b` of neural_network/_fused_arrays.py:25-30
@@ -280,3 +286,169 @@ def clip_grad_norm(grads, max_norm):
     N.check(N.lib.nml_clip_grad_norm_device(ptrs, sizes, len(grads), float(max_norm),
                                             C.byref(norm)))
     return float(norm.value)
+
+
+class KV4Cache:
+    """K and V of ``max_seq`` positions a row in 4 bits (blocks of 32 E2M1 codes and a
+    power-of-two scale): ``k_codes``/``v_codes`` uint8 (batch, kv_heads, max_seq, blocks, 16),
+    ``k_scales``/``v_scales`` uint8 (batch, kv_heads, max_seq, blocks). Starts zeroed."""
+
+    def __init__(self, batch, kv_heads, max_seq, dk):
+        self.batch, self.kv_heads = int(batch), int(kv_heads)
+        self.max_seq, self.dk = int(max_seq), int(dk)
+        shape = (self.batch, self.kv_heads, self.max_seq, -(-self.dk // 32))
+        self.k_codes, self.k_scales, self.v_codes, self.v_scales = arrs = [
+            N.DeviceArray(shape + (16,) * (i % 2 == 0), np.uint8) for i in range(4)]
+        for a in arrs:
+            N.check(N.lib.nml_memset(a.ptr, 0, a.nbytes))
+
+    @property
+    def pointers(self):
+        return (self.k_codes.ptr, self.k_scales.ptr, self.v_codes.ptr, self.v_scales.ptr)
+
+
+def _rows_i32(x, batch, what):
+    """A device int32 (batch,) array, or None."""
+    if x is None:
+        return None
+    d = _dev(x if isinstance(x, N.DeviceArray) else np.ascontiguousarray(x, dtype=np.int32),
+             np.int32)
+    if d.shape != (batch,):
+        raise ValueError(f"{what} must be ({batch},), got {d.shape}")
+    return d
+
+
+def _check_flag(err, message):
+    if int(err.numpy()[0]):
+        raise ValueError(message)
+
+
+def kv4_write(cache, k, v, pos=None, counts=None):
+    """Quantise K and V (batch, kv_heads, seq, dk) of new tokens into ``cache``: token s of row
+    b, s < ``counts[b]`` (None: all), goes to position ``pos[b] + s`` (None: s). Raises
+    ValueError for a position outside the cache (the others are written) or a count outside
+    [0, seq]."""
+    dt = _float_dtype(k)
+    kd, vd = _dev(k, dt), _dev(v, dt)
+    want = (cache.batch, cache.kv_heads, kd.shape[2] if kd.ndim == 4 else -1, cache.dk)
+    if kd.shape != want or vd.shape != want:
+        raise ValueError(f"kv4_write: k {kd.shape}, v {vd.shape} for a cache of ({cache.batch}, "
+                         f"{cache.kv_heads}, seq, {cache.dk})")
+    seq = want[2]
+    pd = _rows_i32(pos, cache.batch, "kv4_write: pos")
+    cd = _rows_i32(counts, cache.batch, "kv4_write: counts")
+    err = N.DeviceArray.from_host(np.zeros(1, np.int32))
+    N.check(N.lib.nml_kv4_write_device(
+        kd.ptr, vd.ptr, cache.kv_heads * seq * cache.dk, seq * cache.dk, cache.dk,
+        *cache.pointers, N.ptr(pd), N.ptr(cd), cache.batch, cache.kv_heads, seq, cache.max_seq,
+        cache.dk, err.ptr, N.np_dtype_code(dt)))
+    _check_flag(err, f"kv4_write: a position is outside [0, {cache.max_seq}) or a count outside "
+                     f"[0, {seq}]")
+
+
+def kv4_read(cache, seq, pos=None, counts=None, dtype=None):
+    """The values (K, V), each (batch, kv_heads, seq, dk) in ``dtype`` (None: the compute
+    dtype), that ``cache`` holds at positions ``pos[b] …`` (None: 0); zeros from ``counts[b]``
+    on. Raises ValueError for a position outside the cache."""
+    dt = np.dtype(np_backend.dtype if dtype is None else dtype)
+    pd = _rows_i32(pos, cache.batch, "kv4_read: pos")
+    cd = _rows_i32(counts, cache.batch, "kv4_read: counts")
+    out = [N.DeviceArray((cache.batch, cache.kv_heads, int(seq), cache.dk), dt) for _ in range(2)]
+    if cd is not None:
+        for o in out:
+            N.check(N.lib.nml_memset(o.ptr, 0, o.nbytes))
+    err = N.DeviceArray.from_host(np.zeros(1, np.int32))
+    N.check(N.lib.nml_kv4_read_device(
+        *cache.pointers, N.ptr(pd), N.ptr(cd), out[0].ptr, out[1].ptr, cache.batch,
+        cache.kv_heads, int(seq), cache.max_seq, cache.dk, err.ptr, N.np_dtype_code(dt)))
+    _check_flag(err, f"kv4_read: a position is outside [0, {cache.max_seq}) or a count outside "
+                     f"[0, {seq}]")
+    return out[0], out[1]
+
+
+def kv4_attention(q, cache, lens, scale, counts=None):
+    """Causal attention of each row's ``counts[b]`` (None: all ``seq``) last cached tokens over
+    ``cache``: ``q`` (batch, heads, seq, dk), ``lens`` (batch,) tokens cached per row, these
+    included, ``scale`` the sqrt(dk) divisor; query head h reads KV head
+    h // (heads // kv_heads). Returns the merged-head output (batch, seq, heads·dk), zeros for
+    tokens from ``counts[b]`` on and for tokens that see no key. Raises ValueError for a length
+    outside [0, max_seq] or a count outside [0, seq]."""
+    dt = _float_dtype(q)
+    qd = _dev(q, dt)
+    if qd.ndim != 4 or qd.shape[0] != cache.batch or qd.shape[3] != cache.dk:
+        raise ValueError(f"kv4_attention: q {qd.shape} for a cache of {cache.batch} rows, head "
+                         f"dim {cache.dk}")
+    batch, heads, seq, dk = qd.shape
+    ld = _rows_i32(lens, batch, "kv4_attention: lens")
+    if ld is None:
+        raise ValueError("kv4_attention: lens is required")
+    cd = _rows_i32(counts, batch, "kv4_attention: counts")
+    sizes = (batch, heads, cache.kv_heads, seq, cache.max_seq, dk)
+    need = C.c_size_t()
+    N.check(N.lib.nml_kv4_attention_workspace(*sizes, C.byref(need)))
+    ws = N.DeviceArray((need.value,), np.uint8) if need.value else None
+    out = N.DeviceArray((batch, seq, heads * dk), dt)
+    if cd is not None:
+        N.check(N.lib.nml_memset(out.ptr, 0, out.nbytes))
+    err = N.DeviceArray.from_host(np.zeros(1, np.int32))
+    N.check(N.lib.nml_kv4_attention_device(
+        qd.ptr, *cache.pointers, ld.ptr, N.ptr(cd), out.ptr, *sizes, float(scale), N.ptr(ws),
+        need.value, err.ptr, N.np_dtype_code(dt)))
+    _check_flag(err, f"kv4_attention: a length is outside [0, {cache.max_seq}] or a count outside "
+                     f"[0, {seq}]")
+    return out
+
+
+def _logit_rows(logits, targets):
+    dt = _float_dtype(logits)
+    ld = _dev(logits, dt)
+    rows = ld.size // ld.shape[-1]
+    td = targets
+    if not isinstance(td, N.DeviceArray):
+        td = N.DeviceArray.from_host(np.ascontiguousarray(targets, dtype=np.int64).reshape(-1))
+    if td.dtype != np.int64 or td.size != rows:
+        raise ValueError(f"label count ({td.size}) must match batch size ({rows})")
+    return ld, td, rows, ld.shape[-1], N.np_dtype_code(dt)
+
+
+def token_logprobs(logits, targets, top_k=0, ignore_index=None):
+    """Log probabilities of ``targets`` (rows,) under ``logits`` (..., vocab), row by row:
+    ``(logp, entropy, m, l, top_ids, top_logp)`` as ``DeviceArray``s — float32 (rows,) each (m, l:
+    the largest logit and Σ exp(x − m)), the ``top_k`` most probable ids (int64) and their log probabilities (rows, top_k), most probable
+    first, or None without ``top_k``. Rows whose target is ``ignore_index`` give zeros and ids
+    −1. Raises ValueError for a target outside [0, vocab)."""
+    ld, td, rows, vocab, code = _logit_rows(logits, targets)
+    logp, entropy, m, lsum = (N.DeviceArray((rows,), np.float32) for _ in range(4))
+    ids = top = None
+    if top_k:
+        ids, top = N.DeviceArray((rows, top_k), np.int64), N.DeviceArray((rows, top_k), np.float32)
+    err = N.DeviceArray.from_host(np.zeros(1, np.int32))
+    has = ignore_index is not None
+    N.check(N.lib.nml_token_logprobs_device(
+        ld.ptr, vocab, td.ptr, rows, vocab, int(ignore_index) if has else 0, int(has), int(top_k),
+        logp.ptr, entropy.ptr, m.ptr, lsum.ptr, N.ptr(ids), N.ptr(top), err.ptr, code))
+    _check_flag(err, f"label out of range [0, {vocab})")
+    return logp, entropy, m, lsum, ids, top
+
+
+def token_logprobs_backward(logits, targets, m, lsum, entropy, dlogp=None, dentropy=None,
+                            ignore_index=None):
+    """The gradient with respect to ``logits`` (its shape and dtype) of Σ dlogp·logp +
+    dentropy·entropy, from ``token_logprobs``' ``m``, ``l`` and ``entropy``; ``dlogp``, ``dentropy``
+    (rows,) float32 or None."""
+    ld, td, rows, vocab, code = _logit_rows(logits, targets)
+    stats = []
+    for name, x in (("m", m), ("l", lsum), ("entropy", entropy), ("dlogp", dlogp),
+                    ("dentropy", dentropy)):
+        d = None if x is None else _dev(x, np.float32)
+        if d is not None and d.size != rows:
+            raise ValueError(f"token_logprobs_backward: {name} must have {rows} values, got {d.size}")
+        stats.append(d)
+    out = N.DeviceArray(ld.shape, ld.dtype)
+    err = N.DeviceArray.from_host(np.zeros(1, np.int32))
+    has = ignore_index is not None
+    N.check(N.lib.nml_token_logprobs_backward_device(
+        ld.ptr, vocab, td.ptr, *(N.ptr(s) for s in stats), rows, vocab,
+        int(ignore_index) if has else 0, int(has), out.ptr, vocab, err.ptr, code))
+    _check_flag(err, f"label out of range [0, {vocab})")
+    return out
