@@ -346,3 +346,35 @@ def test_offsets_past_32_bits(gpu):
         want = w @ hv[j] / (w.sum() + p - n)
         tol = np.abs(hv[j]).max() * w.sum() / p * 1e-3 + 2.0**-11 * np.abs(want).max() + 2.0**-25
         assert np.abs(out[j] - want).max() <= tol
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dk, group, seq", [(64, 1, 1), (128, 2, 1), (32, 1, 5), (80, 3, 2), (256, 1, 1)])
+def test_long_rows_in_pieces(gpu, dtype, dk, group, seq):
+    """Few rows and long ones: a row's keys in many pieces, beside rows of one piece and of a
+    piece and a key."""
+    check_attention(np.random.RandomState(dk), dtype, dk, 1, group, seq, [3001, 128, 129, 1, 1280])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_pieces_of_very_different_scores(gpu, dtype):
+    """One piece holds scores hundreds above the others', one holds a NaN block that the last
+    token alone sees."""
+    r = np.random.RandomState(14)
+    dk, n = 64, 2050
+    k, v = normal(r, (1, 1, n, dk), dtype), normal(r, (1, 1, n, dk), dtype)
+    q = normal(r, (1, 1, 2, dk), dtype)
+    k[0, 0, 700:720] *= 40
+    scale = 8.0
+    got = K.kv4_attention(q, cache_of(k, v), [n], scale).numpy().astype(np.float64)
+    hk, hv = R.held(k), R.held(v)
+    err = np.abs(got - R.attention(q, hk, hv, [n], None, scale)).max()
+    assert err <= bound(q, hk, hv, scale, dtype)
+    clean = got
+    v[0, 0, n - 1, 10] = np.inf
+    got = K.kv4_attention(q, cache_of(k, v), [n], scale).numpy().astype(np.float64)[0]
+    assert np.array_equal(got[0], clean[0, 0])
+    assert np.isnan(got[1, :32]).all() and np.array_equal(got[1, 32:], clean[0, 1, 32:])
+    k[0, 0, n - 1, 40] = np.nan
+    got = K.kv4_attention(q, cache_of(k, v), [n], scale).numpy().astype(np.float64)[0]
+    assert np.array_equal(got[0], clean[0, 0]) and np.isnan(got[1]).all()
