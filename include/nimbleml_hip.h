@@ -201,8 +201,9 @@ int nml_kv4_read_device(const uint8_t* k_codes, const uint8_t* k_scales, const u
  * zeros. A NaN block reaches only the tokens that see its key. seq = 1 is a decode step.
  *   q: (batch, heads, seq, dk); out: (batch, seq, heads·dk), rows from counts[b] on left as
  *   they were; query head h reads KV head h / (heads / kv_heads)
- *   ws: nml_kv4_attention_workspace bytes, 16-byte aligned; nothing is kept in it from one call
- *   to the next, but calls that run at the same time need one each. */
+ *   ws: nml_kv4_attention_workspace bytes, 16-byte aligned, zeroed once before its first use;
+ *   every call leaves its counters zero, so one serves any number of calls one after another,
+ *   whatever their sizes, and calls that can run at the same time need one each. */
 int nml_kv4_attention_workspace(size_t batch, size_t heads, size_t kv_heads, size_t seq,
                                 size_t max_seq, size_t dk, size_t* bytes);
 int nml_kv4_attention_device(const void* q, const uint8_t* k_codes, const uint8_t* k_scales,

@@ -231,7 +231,7 @@ int launch_kv4_read(int dt, const Kv4ReadArgs& a, hipStream_t st);
 // Attention of counts[b] (null: S) new tokens of each row, the last of the row's lens[b] cached
 // ones: token s sees keys 0 … lens[b] − counts[b] + s, none of them: zeros. q (B, H, S, dk),
 // out (B, S, H·dk); query head h reads KV head h / (H / Hkv). Rows of out from counts[b] on are
-// left as they were. ws: kv4_attention_workspace bytes, contents free before and after.
+// left as they were. ws: kv4_attention_workspace bytes, zeroed before the first launch with it.
 struct Kv4AttnArgs {
   const void* q;
   const uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
@@ -239,6 +239,8 @@ struct Kv4AttnArgs {
   const int32_t* counts;
   void* out;
   int B, H, Hkv, S, P, dk;
+  int group;    // H / Hkv
+  int slots;    // set by the launch
   float scale;  // divisor of the scores
   void* ws;
   int* err;

@@ -600,6 +600,13 @@ static int kv4_attention_ok(size_t batch, size_t heads, size_t kv_heads, size_t 
   NML_TRY(kv4_shape_ok("kv4 attention", batch, heads, seq, max_seq, dk));
   NML_REQUIRE(kv_heads >= 1 ? heads % kv_heads == 0 : heads == 0,
               "kv4 attention: heads (%zu) must be divisible by kv_heads (%zu)", heads, kv_heads);
+  if (batch && heads && seq) {
+    // the kernel numbers pieces of 128 keys in 32 bits
+    const size_t tiles = (heads / kv_heads * seq + 15) / 16 * kv_heads;
+    NML_REQUIRE(tiles * batch <= 0x7fffffff / ((max_seq + 127) / 128),
+                "kv4 attention: %zu rows × %zu heads × %zu tokens over %zu positions too many", batch, heads, seq,
+                max_seq);
+  }
   return 0;
 }
 
@@ -641,6 +648,7 @@ int nml_kv4_attention_device(const void* q, const uint8_t* k_codes, const uint8_
   a.B = (int)batch;
   a.H = (int)heads;
   a.Hkv = (int)kv_heads;
+  a.group = (int)(heads / kv_heads);
   a.S = (int)seq;
   a.P = (int)max_seq;
   a.dk = (int)dk;

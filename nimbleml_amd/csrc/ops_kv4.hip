@@ -10,6 +10,8 @@
 // saturating the largest value at 6 would cost more than the coarser step (signal to error on
 // normal values 19.02 dB with the change at 1.75, 18.75 at 1.5, 18.79 without it; 16.33, 15.41
 // and 16.30 with one channel of 32 six times as large).
+#include <algorithm>
+
 #include "kernels.hpp"
 
 namespace nml {
@@ -180,54 +182,128 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4ReadArgs a) {
 // The queries that share a KV head — its group's heads times the new tokens — are the columns of
 // 16-wide MFMA tiles: S = K·Qᵀ takes 16 keys' blocks as its rows (a lane converts the codes it
 // loaded and has its operand, no LDS), O = Vᵀ·Pᵀ takes the probabilities from the lanes where S
-// left them, with the keys of the contraction in that order. Only V passes through LDS, for the
-// transpose of its read. The codes' values are exact in bf16, a query is split in two (float16)
-// or three (float32) bf16 parts without loss and a probability into as many, so every product
-// is exact and scores, statistics and outputs are float32 sums.
+// left them, with the keys of the contraction in that order. V passes through LDS for the
+// transpose of its read; Q is split and laid out in LDS once a workgroup. The codes' values are
+// exact in bf16, a query is split in two (float16) or three (float32) bf16 parts without loss and
+// a probability into as many, so every product is exact and scores, statistics and outputs are
+// float32 sums.
 //
 // A wave goes through tiles of 32 keys on its own: its loads of the next tile are in flight
 // during this one; the running maximum that the exponentials refer to moves only when a score
 // passes it by 2^8 (probabilities are then at most 2^8, all the same to float32), which skips
-// the rescaling of O on nearly every tile. Waves merge in LDS, the splits of a long row in a
-// second launch.
+// the rescaling of O on nearly every tile. A workgroup's eight waves merge in LDS.
+//
+// A (row, KV head, 16 queries) is one workgroup's unless its keys are many: pieces of a long one
+// go to several, as many in all as the card holds at once, and the last to finish merges them in
+// their order. A piece costs its startup and the merge about as much as four spans of keys, so it
+// has at least so many.
 
+typedef float f2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
 typedef unsigned u2 __attribute__((ext_vector_type(2)));
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 8;
+constexpr int kThreads = 64 * kWaves;
 constexpr int kKeys = 32;                  // keys of a wave's tile
-constexpr int kSpan = kWaves * kKeys;      // a split takes a multiple of these
+constexpr int kSpan = kWaves * kKeys;      // keys of a workgroup's round
 constexpr float kSlack = 8.f;              // in powers of two
 
-// Keys of a split when a row's are dealt to `splits`.
-__host__ __device__ __forceinline__ int split_keys(int len, int splits) {
-  const int per = (len + splits - 1) / splits;
-  return per < kSpan ? kSpan : (per + kSpan - 1) / kSpan * kSpan;
-}
+// Workgroups that the card's 256 CUs hold at once, by registers and LDS.
+__host__ __device__ constexpr int capacity(int nb) { return nb == 1 ? 768 : nb <= 4 ? 512 : 256; }
+// Spans that a piece has at least: what it costs to begin one and to merge it.
+__host__ __device__ constexpr int least_spans(int nb) { return nb <= 2 ? 8 : nb <= 4 ? 4 : 2; }
 
-// One row of the batch: cached length and new tokens, in range.
-struct RowInfo {
+// ws: a counter for each tile in pieces (zero before and after every launch, in the same place
+// for calls of any size), then for each piece its rows' maxima and Σ p, then their Σ p·v. Tiles in
+// pieces are fewer than the card's workgroups (a piece is at least their even share), and so their
+// pieces fewer than twice as many.
+constexpr int kCounters = 2048, kCounterStep = 16;  // a line for each
+
+// Rows of the batch, 64 at a time with one in each lane: cached length and new tokens, in range.
+struct Rows {
   int len, n;
+  __device__ __forceinline__ void load(const Kv4AttnArgs& a, int b, int* err) {
+    len = n = 0;
+    if (b < a.B) {
+      const int x = a.lens[b], y = a.counts ? a.counts[b] : a.S;
+      len = min(max(x, 0), a.P);
+      n = min(max(y, 0), a.S);
+      if (err && (x != len || y != n)) __hip_atomic_fetch_or(err, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  // Spans of the lane's row (at least one: its outputs are to be written).
+  __device__ __forceinline__ int spans() const { return n > 0 ? max(1, (len + kSpan - 1) / kSpan) : 1; }
 };
-__device__ __forceinline__ RowInfo row_info(const Kv4AttnArgs& a, int b, int* err) {
-  RowInfo r;
-  r.n = row_count(a.counts, b, a.S, err);
-  const int len = a.lens[b];
-  r.len = len < 0 ? 0 : (len > a.P ? a.P : len);
-  if (r.len != len && err) __hip_atomic_fetch_or(err, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return r;
+
+// Inclusive sum over the wave's lanes (data-parallel-primitive moves: within rows of 16, then the
+// rows' last lanes to the rows behind).
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);  // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);  // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);  // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return v;
 }
 
-// x = Σ of NP bf16 parts (the rest lost is below 2^-8·NP of x).
+// What this workgroup does: piece `piece` of `pieces` of tile (b, e), whose row has len keys and n
+// new tokens; `slot`: where the tile's first piece is in ws. b < 0: nothing.
+struct Work {
+  int b, e, piece, pieces, slot, len, n, spans;
+};
+__device__ __forceinline__ Work find_work(const Kv4AttnArgs& a, int each, int nb, int lane) {
+  Work w{};
+  Rows rows;
+  int total = 0;
+  for (int i = 0; i < a.B; i += 64) {
+    rows.load(a, i + lane, blockIdx.x == 0 ? a.err : nullptr);
+    total += __builtin_amdgcn_readlane(wave_scan(i + lane < a.B ? rows.spans() : 0), 63);
+  }
+  // pieces go to the places that the tiles' own workgroups leave (a quarter where they leave none:
+  // for a row much longer than the others)
+  const int cap = capacity(nb), room = max(cap - static_cast<int>(min(static_cast<long long>(each) * a.B, 1LL * cap)), cap / 4);
+  const int least = max(least_spans(nb), static_cast<int>((static_cast<long long>(total) * each + room - 1) / room));
+  const int at = static_cast<int>(blockIdx.x / each);
+  int before = 0, slots = 0;
+  for (int i = 0; i < a.B; i += 64) {
+    if (a.B > 64) rows.load(a, i + lane, nullptr);
+    const int spans = i + lane < a.B ? rows.spans() : 0;
+    const int pieces = spans <= least ? min(spans, 1) : (spans + least - 1) / least;
+    const int sum = wave_scan(pieces), sum_slots = wave_scan(pieces > 1 ? pieces : 0);
+    const unsigned long long past = __ballot(before + sum > at);
+    if (past) {
+      const int l = __ffsll(past) - 1;
+      w.pieces = __builtin_amdgcn_readlane(pieces, l);
+      w.spans = __builtin_amdgcn_readlane(spans, l);
+      w.len = __builtin_amdgcn_readlane(rows.len, l);
+      w.n = __builtin_amdgcn_readlane(rows.n, l);
+      const int first = before + __builtin_amdgcn_readlane(sum, l) - w.pieces;
+      const int local = static_cast<int>(blockIdx.x) - first * each;
+      w.b = i + l;
+      w.e = w.pieces == 1 ? local : local / w.pieces;
+      w.piece = local - w.e * w.pieces;
+      w.slot = (slots + __builtin_amdgcn_readlane(sum_slots, l) - w.pieces) * each + w.e * w.pieces;
+      return w;
+    }
+    before += __builtin_amdgcn_readlane(sum, 63);
+    slots += __builtin_amdgcn_readlane(sum_slots, 63);
+  }
+  w.b = -1;
+  return w;
+}
+
+// x = Σ of NP bf16 parts, two values at once (what is lost is below 2^(1 − 8·NP − NP) of x).
 template <int NP>
-__device__ __forceinline__ void split_bf16(float x, __bf16* part) {
+__device__ __forceinline__ void split_bf16(f2 x, bf2* part) {
 #pragma unroll
   for (int p = 0; p < NP; ++p) {
-    part[p] = static_cast<__bf16>(x);
-    x -= static_cast<float>(part[p]);
+    part[p] = __builtin_convertvector(x, bf2);
+    if (p + 1 < NP) x -= __builtin_convertvector(part[p], f2);
   }
 }
 
@@ -239,18 +315,19 @@ struct Kv4Tile {
   unsigned e[2][W];
 };
 
+// Tile at `codes` and `scales` (those of its first key). Keys past `last` (of the tile): that key
+// again; blocks that pad nb: the last one again.
 template <int NB>
 __device__ __forceinline__ void load_tile(Kv4Tile<NB>& t, const uint8_t* __restrict__ codes,
-                                          const uint8_t* __restrict__ scales, int k0, int last, int nb, int lane) {
+                                          const uint8_t* __restrict__ scales, int last, int nb, int lane) {
   constexpr int W = Kv4Tile<NB>::W;
   const int g = lane >> 4;
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
-    const int key = min(k0 + 16 * s + (lane & 15), last);  // (past the end: the last key again)
+    const unsigned key = min(16 * s + (lane & 15), last);
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const int blk = min(g * NB / 4 + w, nb - 1);  // (blocks that pad nb: the last one again)
-      const size_t at = static_cast<size_t>(key) * nb + blk;
+      const unsigned at = key * nb + min(g * NB / 4 + w, nb - 1);
       const uint8_t* p = codes + at * kBlockBytes;
       if constexpr (NB >= 4) {
         const u4 v = *reinterpret_cast<const u4*>(p);
@@ -277,6 +354,9 @@ __device__ __forceinline__ bf8 convert8(unsigned c, float s) {
   return bf8{a.x, a.y, b.x, b.y, d.x, d.y, e.x, e.y};
 }
 
+// As scale_value, of a byte that the write made (never 0; zeroed memory holds codes of 0 only).
+__device__ __forceinline__ float tile_scale(unsigned e) { return __builtin_bit_cast(float, e << 23); }
+
 // Keys of a 16-key subtile (bit i: key i) that hold a NaN block, from the lanes' scales; the
 // NaN blocks themselves become zeros. `of`: per block, the keys; null: any block.
 template <int NB>
@@ -302,84 +382,121 @@ __device__ __forceinline__ unsigned take_nan(Kv4Tile<NB>& t, int s, unsigned* of
   return any;
 }
 
+// V in LDS: a key's 32·NB values in a row, its 32-byte pairs exchanged by the key so that the
+// 16 rows that a transposing read takes 32 bytes each of lie in different banks.
+template <int NB>
+__device__ __forceinline__ int v_pair(int key, int pair) {
+  return pair ^ (NB >= 4 ? key & 7 : NB == 2 ? key >> 1 & 3 : key >> 2 & 1);
+}
+
+// Partial results pass between workgroups of any XCD: stores and loads at agent scope (past the
+// L2s) and a count that each workgroup adds to once its stores have arrived. (An acquire in the
+// last one and plain loads instead cost 20 µs a launch: it empties that XCD's L2.)
+__device__ __forceinline__ void put2(float* p, f2 v) {
+  __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), __builtin_bit_cast(unsigned long long, v), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f2 get2(const float* p) {
+  return __builtin_bit_cast(f2, __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED,
+                                                  __HIP_MEMORY_SCOPE_AGENT));
+}
+
 template <typename T, int NB>
-__global__ __launch_bounds__(256) void kv4_attention_kernel(Kv4AttnArgs a, int splits) {
+__global__ __launch_bounds__(kThreads, NB <= 4 ? 4 : 2) void kv4_attention_kernel(Kv4AttnArgs a) {
   constexpr int NP = sizeof(T) == 2 ? 2 : 3;
   constexpr int W = Kv4Tile<NB>::W, DT = 2 * NB;  // DT: 16-wide tiles of the head dim
-  constexpr int kRow = 64 * NB + 32;              // bytes of a key's values in LDS (+32: banks)
-  constexpr int kWaveLds = kKeys * kRow;          // and 16 rows of 32·NB floats fit as well
+  constexpr int kRow = 64 * NB;                   // bytes of a key's values in LDS
+  constexpr int kWaveLds = kKeys * kRow;          // and as many of 16 rows of 32·NB floats
+  constexpr int D = 32 * NB;
   __shared__ __align__(16) char lds[kWaves * kWaveLds];
+  __shared__ __align__(16) bf8 qs[NP][NB][64];
   __shared__ float sm[kWaves][16], sl[kWaves][16];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x % splits, tile = blockIdx.x / splits, hk = blockIdx.y, b = blockIdx.z;
-  const int nb = (a.dk + kBlock - 1) / kBlock, group = a.H / a.Hkv, R = group * a.S;
-  const RowInfo row = row_info(a, b, split == 0 ? a.err : nullptr);
-  const int per = split_keys(row.len, splits), active = max(1, (row.len + per - 1) / per);
-  if (split >= active) return;
-  const int k0 = split * per, k1 = min(row.len, k0 + per);
+  __shared__ unsigned arrived;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, g = lane >> 4;
+  const int nb = (a.dk + kBlock - 1) / kBlock, R = a.group * a.S, tiles = (R + 15) / 16;
+  const Work work = find_work(a, a.Hkv * tiles, NB, lane);
+  if (work.b < 0 || work.n == 0) return;
+  const int hk = tiles == 1 ? work.e : work.e / tiles, tile = work.e - hk * tiles;
+  const int per = work.pieces == 1 ? work.spans : (work.spans + work.pieces - 1) / work.pieces;
+  const int k0 = work.piece * per * kSpan, k1 = min(work.len, k0 + per * kSpan);
 
-  // This lane's query: row r of the KV head's R, token s of head hk·group + r / S. It sees keys
-  // up to lim; a column without a query (or of the padding) runs along with zeros.
-  const int r = tile * 16 + col, s = r % a.S;
-  const bool live = r < R && s < row.n;
-  const int h = hk * group + r / a.S;
-  const int lim = live ? row.len - row.n + s : 0x7fffffff;
+  // The query of column c of this tile: row r of the KV head's R, token s of head hk·group + r / S.
+  // It sees keys up to lim; a column without a query (or of the padding) runs along with zeros.
+  auto token = [&](int r) { return a.S == 1 ? 0 : r % a.S; };
+  auto head = [&](int r) { return hk * a.group + (a.S == 1 ? r : r / a.S); };
+  const int r = tile * 16 + col, s = token(r);
+  const bool live = r < R && s < work.n;
+  const int lim = live ? work.len - work.n + s : 0x7fffffff;
+
+  // Q as it lies in memory, eight values a lane (wave t: step t of the product), in flight while
+  // the keys' loads are issued
+  typedef T v8 __attribute__((ext_vector_type(8), aligned(16)));
+  v8 raw = {};
+  const int d0 = 8 * (g * NB + w);
+  if (w < NB && live) {
+    const T* qp = static_cast<const T*>(a.q) + ((static_cast<size_t>(work.b) * a.H + head(r)) * a.S + s) * a.dk;
+    if ((a.dk & 7) == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0) {
+      if (d0 < a.dk) raw = *reinterpret_cast<const v8*>(qp + d0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (d0 + i < a.dk) raw[i] = qp[d0 + i];
+    }
+  }
+
+  const size_t base = (static_cast<size_t>(work.b) * a.Hkv + hk) * a.P * nb;
+  const uint8_t* kc = a.k_codes + base * kBlockBytes;
+  const uint8_t* ks = a.k_scales + base;
+  const uint8_t* vc = a.v_codes + base * kBlockBytes;
+  const uint8_t* vs = a.v_scales + base;
+  // A tile of keys from `at` on. Past the piece's end: its first key again and again, so that
+  // every round issues as many loads (the waits before their use count them).
+  Kv4Tile<NB> k, v;
+  auto fetch = [&](int at) {
+    const int from = at < k1 ? at : k0, last = at < k1 ? work.len - 1 - at : 0;
+    const size_t o = static_cast<size_t>(from) * nb;
+    load_tile<NB>(k, kc + o * kBlockBytes, ks + o, last, nb, lane);
+    load_tile<NB>(v, vc + o * kBlockBytes, vs + o, last, nb, lane);
+  };
+  int j = k0 + w * kKeys;
+  if (k0 < k1) fetch(j);
+
+  if (w < NB) {
+    bf8 q[NP];
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      bf2 part[NP];
+      split_bf16<NP>(f2{static_cast<float>(raw[i]), static_cast<float>(raw[i + 1])}, part);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) q[p][i] = part[p].x, q[p][i + 1] = part[p].y;
+    }
+#pragma unroll
+    for (int p = 0; p < NP; ++p) qs[p][w][lane] = q[p];
+  }
   int least = lim;
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) least = min(least, __shfl_xor(least, o, 64));
-
-  bf8 q[NP][NB];
-  {
-    const T* qp = static_cast<const T*>(a.q) + ((static_cast<size_t>(b) * a.H + (live ? h : 0)) * a.S + (live ? s : 0)) * a.dk;
-    const bool vec = (a.dk & 7) == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0;
-#pragma unroll
-    for (int t = 0; t < NB; ++t) {
-      float x[8];
-      const int d0 = 8 * (g * NB + t);
-      if (vec) load8<T, true>(qp, d0, a.dk, x);
-      else load8<T, false>(qp, d0, a.dk, x);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        __bf16 part[NP];
-        split_bf16<NP>(live ? x[i] : 0.f, part);
-#pragma unroll
-        for (int p = 0; p < NP; ++p) q[p][t][i] = part[p];
-      }
-    }
-  }
   const float scale = 1.44269504088896341f / a.scale;  // scores in powers of two
+  const float slack = kSlack * 0.69314718055994531f * a.scale;
   floatx4 o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = floatx4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, ref = 0.f, l = 0.f;  // l: of this lane's keys
+  float m = -INFINITY, ref = 0.f, l = 0.f;  // m: of q·k; ref: m·scale, finite; l: of this lane's keys
   unsigned nan_blocks = 0;                  // blocks of the output that a NaN block of V reached
-
-  const size_t head = (static_cast<size_t>(b) * a.Hkv + hk) * a.P * nb;
-  const uint8_t* kc = a.k_codes + head * kBlockBytes;
-  const uint8_t* ks = a.k_scales + head;
-  const uint8_t* vc = a.v_codes + head * kBlockBytes;
-  const uint8_t* vs = a.v_scales + head;
   char* mine = lds + w * kWaveLds;
-  Kv4Tile<NB> kt, vt;
-  int j = k0 + w * kKeys;
-  if (j < k1) {
-    load_tile<NB>(kt, kc, ks, j, row.len - 1, nb, lane);
-    load_tile<NB>(vt, vc, vs, j, row.len - 1, nb, lane);
-  }
+  __syncthreads();
+
   for (; j < k1; j += kSpan) {
-    Kv4Tile<NB> k = kt, v = vt;
-    if (j + kSpan < k1) {
-      load_tile<NB>(kt, kc, ks, j + kSpan, row.len - 1, nb, lane);
-      load_tile<NB>(vt, vc, vs, j + kSpan, row.len - 1, nb, lane);
-    }
-    unsigned bad_e = 0;
+    unsigned worst = 0;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < W; ++i) bad_e = max(bad_e, max(k.e[t][i], v.e[t][i]));
-    const bool nan = __ballot(bad_e == kScaleNaN) != 0;
+      for (int i = 0; i < W; ++i) worst = max(worst, max(k.e[t][i], v.e[t][i]));
+    const bool nan = __ballot(worst == kScaleNaN) != 0;
     unsigned k_nan[2] = {0, 0};
     if (nan) {
+#pragma unroll
       for (int t = 0; t < 2; ++t) {
         k_nan[t] = take_nan<NB>(k, t, nullptr);
         unsigned of[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -393,25 +510,32 @@ __global__ __launch_bounds__(256) void kv4_attention_kernel(Kv4AttnArgs a, int s
     }
     // S = K·Qᵀ: this lane's are keys 4g … 4g+3 of both subtiles with its query
     float x[8];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+    {
+      floatx4 acc[2] = {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        const bf8 kk = convert8(k.c[t][i], scale_value(k.e[t][W == 2 ? i / 4 : 0]));
+        const bf8 k0v = convert8(k.c[0][i], tile_scale(k.e[0][W == 2 ? i / 4 : 0]));
+        const bf8 k1v = convert8(k.c[1][i], tile_scale(k.e[1][W == 2 ? i / 4 : 0]));
 #pragma unroll
-        for (int p = 0; p < NP; ++p) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[p][i], acc, 0, 0, 0);
+        for (int p = 0; p < NP; ++p) {
+          const bf8 q = qs[p][i][lane];
+          acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0v, q, acc[0], 0, 0, 0);
+          acc[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1v, q, acc[1], 0, 0, 0);
+        }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[4 * t + i] = acc[i] * scale;
+      for (int i = 0; i < 8; ++i) x[i] = acc[i / 4][i % 4];
     }
     // V to LDS, a key a row
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < NB; ++i)
-        *reinterpret_cast<bf8*>(mine + (16 * t + col) * kRow + 16 * (g * NB + i)) =
-            convert8(v.c[t][i], scale_value(v.e[t][W == 2 ? i / 4 : 0]));
+      for (int i = 0; i < NB; ++i) {
+        const int key = 16 * t + col, chunk = g * NB + i;
+        *reinterpret_cast<bf8*>(mine + key * kRow + v_pair<NB>(key, chunk >> 1) * 32 + (chunk & 1) * 16) =
+            convert8(v.c[t][i], tile_scale(v.e[t][W == 2 ? i / 4 : 0]));
+      }
+    fetch(j + kSpan);
     if (nan) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -425,10 +549,10 @@ __global__ __launch_bounds__(256) void kv4_attention_kernel(Kv4AttnArgs a, int s
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
-    if (__ballot(top > m + kSlack)) {
+    if (__ballot(top > m + slack)) {
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float mn = fmaxf(m, top), rn = mn == -INFINITY ? 0.f : mn;
+      const float mn = fmaxf(m, top), rn = mn == -INFINITY ? 0.f : mn * scale;
       const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - rn);
       m = mn;
       ref = rn;
@@ -438,23 +562,25 @@ __global__ __launch_bounds__(256) void kv4_attention_kernel(Kv4AttnArgs a, int s
     }
     bf8 p[NP];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float e = __builtin_amdgcn_exp2f(x[i] - ref);
-      l += e;
-      __bf16 part[NP];
+    for (int i = 0; i < 8; i += 2) {
+      const f2 e = {__builtin_amdgcn_exp2f(__builtin_fmaf(x[i], scale, -ref)),
+                    __builtin_amdgcn_exp2f(__builtin_fmaf(x[i + 1], scale, -ref))};
+      l += e.x;
+      l += e.y;
+      bf2 part[NP];
       split_bf16<NP>(e, part);
 #pragma unroll
-      for (int c = 0; c < NP; ++c) p[c][i] = part[c];
+      for (int c = 0; c < NP; ++c) p[c][i] = part[c].x, p[c][i + 1] = part[c].y;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (LDS of this wave alone, in order)
     // O += Vᵀ·Pᵀ: four keys of either subtile and 16 dims a transposing read
-    const char* at = mine + (4 * g + col / 4) * kRow + (col % 4) * 8;
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       typedef __attribute__((address_space(3))) s4 lds_s4;
-      const s4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + 32 * d));
-      const s4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + 16 * kRow + 32 * d));
-      typedef short s8 __attribute__((ext_vector_type(8)));
+      const int key = 4 * g + col / 4;  // (and 16 on: the same pair)
+      const char* at = mine + key * kRow + v_pair<NB>(key, d) * 32 + (col % 4) * 8;
+      const s4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)at);
+      const s4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + 16 * kRow));
       const bf8 vv = __builtin_bit_cast(bf8, s8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
 #pragma unroll
       for (int c = 0; c < NP; ++c) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, p[c], o[d], 0, 0, 0);
@@ -465,10 +591,10 @@ __global__ __launch_bounds__(256) void kv4_attention_kernel(Kv4AttnArgs a, int s
   // The waves' parts: o[d] holds dims 16d + 4g … + 3 of this lane's query.
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
-  if (g == 0) sm[w][col] = m, sl[w][col] = l;
-  float* part = reinterpret_cast<float*>(mine);
-  constexpr int D = 32 * NB;
-  if (live) {
+  if (g == 0) sm[w][col] = m == -INFINITY ? m : ref, sl[w][col] = l;
+  const int rows = min(16, R - tile * 16);
+  if (col < rows) {
+    float* part = reinterpret_cast<float*>(mine);
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       if (nan_blocks >> (d / 2) & 1u) o[d] = floatx4{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
@@ -476,55 +602,107 @@ __global__ __launch_bounds__(256) void kv4_attention_kernel(Kv4AttnArgs a, int s
     }
   }
   __syncthreads();
-  const int rows = min(16, R - tile * 16);
-  for (int i = threadIdx.x; i < rows * D; i += 256) {
-    const int c = i / D, d = i % D, rr = tile * 16 + c, ss = rr % a.S;
-    if (ss >= row.n || d >= a.dk) continue;
+  // Output value d of row c of the tile.
+  auto finish = [&](int c, int d, float lt, float ot) {
+    const int rr = tile * 16 + c, ss = token(rr);
+    T* out = static_cast<T*>(a.out) + ((static_cast<size_t>(work.b) * a.S + ss) * a.H + head(rr)) * a.dk;
+    if (ss < work.n && d < a.dk) out[d] = static_cast<T>(work.len - work.n + ss < 0 ? 0.f : ot / lt);
+  };
+  const int slot_rows = min(16, R);
+  const size_t parts = a.slots;  // pieces that ws has room for
+  float* ml = reinterpret_cast<float*>(static_cast<char*>(a.ws) + sizeof(unsigned) * kCounters * kCounterStep);
+  float* po = ml + parts * slot_rows * 2;
+  for (int i = 2 * threadIdx.x; i < rows * D; i += 2 * kThreads) {
+    const int c = i / D, d = i % D;
     float mm = sm[0][c];
 #pragma unroll
     for (int y = 1; y < kWaves; ++y) mm = fmaxf(mm, sm[y][c]);
     const float rf = mm == -INFINITY ? 0.f : mm;
-    float lt = 0.f, ot = 0.f;
+    float lt = 0.f;
+    f2 ot = {0.f, 0.f};
 #pragma unroll
     for (int y = 0; y < kWaves; ++y) {
       const float f = __builtin_amdgcn_exp2f(sm[y][c] - rf);  // (−inf: 0)
+      const f2 p = *reinterpret_cast<const f2*>(lds + y * kWaveLds + 4 * i);
       lt += sl[y][c] * f;
-      ot += reinterpret_cast<const float*>(lds + y * kWaveLds)[c * D + d] * f;
+      ot += p * f;
     }
-    const int hh = hk * group + rr / a.S;
-    if (active == 1) {
-      T* out = static_cast<T*>(a.out) + (static_cast<size_t>(b) * a.S + ss) * a.H * a.dk + static_cast<size_t>(hh) * a.dk;
-      out[d] = static_cast<T>(row.len - row.n + ss < 0 ? 0.f : ot / lt);
+    if (work.pieces == 1) {
+      finish(c, d, lt, ot.x);
+      finish(c, d + 1, lt, ot.y);
     } else {
-      const size_t p = ((static_cast<size_t>(b) * a.H + hh) * a.S + ss) * splits + split;
-      float* ws = static_cast<float*>(a.ws);
-      const size_t parts = static_cast<size_t>(a.B) * a.H * a.S * splits;
-      if (d == 0) ws[2 * p] = mm, ws[2 * p + 1] = lt;
-      ws[2 * parts + p * a.dk + d] = ot;
+      const size_t slot = static_cast<size_t>(work.slot + work.piece) * slot_rows;
+      if (d == 0) put2(ml + (slot + c) * 2, f2{mm, lt});
+      put2(po + slot * D + i, ot);
     }
   }
-}
+  if (work.pieces == 1) return;
 
-// The splits of one query's row, in order.
-template <typename T>
-__global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4AttnArgs a, int splits) {
-  const int s = blockIdx.x, h = blockIdx.y, b = blockIdx.z, d = threadIdx.x;
-  const RowInfo row = row_info(a, b, nullptr);
-  const int per = split_keys(row.len, splits), active = max(1, (row.len + per - 1) / per);
-  if (active == 1 || s >= row.n || d >= a.dk) return;
-  const size_t p = ((static_cast<size_t>(b) * a.H + h) * a.S + s) * splits;
-  const float* ml = static_cast<const float*>(a.ws) + 2 * p;
-  const float* o = static_cast<const float*>(a.ws) + 2 * static_cast<size_t>(a.B) * a.H * a.S * splits + p * a.dk + d;
-  float m = -INFINITY, l = 0.f, v = 0.f;
-  for (int i = 0; i < active; ++i) m = fmaxf(m, ml[2 * i]);
-  const float ref = m == -INFINITY ? 0.f : m;
-  for (int i = 0; i < active; ++i) {
-    const float f = __builtin_amdgcn_exp2f(ml[2 * i] - ref);
-    l += ml[2 * i + 1] * f;
-    v += o[static_cast<size_t>(i) * a.dk] * f;
+  // The last of a tile's workgroups to arrive merges its pieces, in their order.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  unsigned* counter = static_cast<unsigned*>(a.ws) + static_cast<size_t>(work.slot) * kCounterStep;
+  if (threadIdx.x == 0)
+    arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (arrived + 1 != static_cast<unsigned>(work.pieces)) return;
+  if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  // four dims of a row a thread, the pieces over as many threads as there are
+  constexpr int Q = D / 4, kBatch = 4;
+  struct Sum {
+    floatx4 o;
+    float m, l;
+  };
+  Sum* sums = reinterpret_cast<Sum*>(lds);
+  static_assert(kThreads * sizeof(Sum) <= sizeof(lds), "a sum a thread");
+  const int cols = rows * Q, ways = cols >= kThreads ? 1 : kThreads / cols, way = ways == 1 ? 0 : threadIdx.x / cols;
+  for (int i = threadIdx.x - way * cols; i < cols; i += kThreads) {
+    const int c = i / Q, dq = i % Q;
+    Sum t{floatx4{0.f, 0.f, 0.f, 0.f}, -INFINITY, 0.f};
+    for (int y = way; y < work.pieces && way < ways; y += kBatch * ways) {
+      f2 st[kBatch], p[kBatch][2];
+#pragma unroll
+      for (int z = 0; z < kBatch; ++z) {  // (every load of a batch before the first use)
+        st[z] = f2{-INFINITY, 0.f};
+        p[z][0] = p[z][1] = f2{0.f, 0.f};
+        if (y + z * ways < work.pieces) {
+          const size_t at = static_cast<size_t>(work.slot + y + z * ways) * slot_rows + c;
+          st[z] = get2(ml + 2 * at);
+          p[z][0] = get2(po + at * D + 4 * dq);
+          p[z][1] = get2(po + at * D + 4 * dq + 2);
+        }
+      }
+      float mn = t.m;
+#pragma unroll
+      for (int z = 0; z < kBatch; ++z) mn = fmaxf(mn, st[z].x);
+      const float rf = mn == -INFINITY ? 0.f : mn, f0 = __builtin_amdgcn_exp2f(t.m - rf);
+      t.m = mn;
+      t.l *= f0;
+      t.o *= f0;
+#pragma unroll
+      for (int z = 0; z < kBatch; ++z) {
+        const float f = __builtin_amdgcn_exp2f(st[z].x - rf);
+        t.l += st[z].y * f;
+        t.o += floatx4{p[z][0].x, p[z][0].y, p[z][1].x, p[z][1].y} * f;
+      }
+    }
+    if (ways > 1) {
+      sums[threadIdx.x] = t;
+      __syncthreads();
+      if (way == 0)
+        for (int y = 1; y < ways; ++y) {
+          const Sum v = sums[y * cols + i];
+          const float mn = fmaxf(t.m, v.m), rf = mn == -INFINITY ? 0.f : mn;
+          const float f0 = __builtin_amdgcn_exp2f(t.m - rf), f1 = __builtin_amdgcn_exp2f(v.m - rf);
+          t.m = mn;
+          t.l = t.l * f0 + v.l * f1;
+          t.o = t.o * f0 + v.o * f1;
+        }
+    }
+    if (way == 0)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) finish(c, 4 * dq + x, t.l, t.o[x]);
   }
-  T* out = static_cast<T*>(a.out) + (static_cast<size_t>(b) * a.S + s) * a.H * a.dk + static_cast<size_t>(h) * a.dk;
-  out[d] = static_cast<T>(row.len - row.n + s < 0 ? 0.f : v / l);
 }
 
 unsigned quads(int S, int H, int dk) {
@@ -557,33 +735,36 @@ int read_launch(const Kv4ReadArgs& a, hipStream_t st) {
   return 0;
 }
 
-// Workgroups that fill the card (four on each of 256 CUs); a row's keys are split until there
-// are as many, in pieces of at least kSpan keys.
-int attention_splits(int B, int H, int Hkv, int S, int P) {
-  const long long tiles = (static_cast<long long>(H / Hkv) * S + 15) / 16;
-  const long long groups = tiles * Hkv * B, want = (1024 + groups - 1) / groups, most = (P + kSpan - 1) / kSpan;
-  return static_cast<int>(want < most ? want : most);
+// Most pieces of one tile, and in all those of tiles in pieces that there can be.
+struct Pieces {
+  long long tiles, most, slots;
+};
+Pieces attention_pieces(int B, int H, int Hkv, int S, int P, int dk) {
+  Pieces p;
+  const int nb = (dk + kBlock - 1) / kBlock, spans = (P - 1) / kSpan + 1;
+  p.tiles = (static_cast<long long>(H / Hkv) * S + 15) / 16 * Hkv * B;
+  p.most = (spans - 1) / least_spans(nb) + 1;
+  p.slots = p.most == 1 ? 0 : std::min(p.tiles * p.most, 2LL * capacity(nb));
+  return p;
 }
 
 template <typename T, int NB>
-int attention_launch_nb(const Kv4AttnArgs& a, int splits, hipStream_t st) {
-  const unsigned tiles = (static_cast<unsigned>(a.H / a.Hkv) * a.S + 15) / 16;
-  kv4_attention_kernel<T, NB><<<dim3(tiles * splits, a.Hkv, a.B), 256, 0, st>>>(a, splits);
+int attention_launch_nb(Kv4AttnArgs a, hipStream_t st) {
+  const Pieces p = attention_pieces(a.B, a.H, a.Hkv, a.S, a.P, a.dk);
+  a.slots = static_cast<int>(p.slots);
+  // every tile's workgroup, and those that pieces add
+  kv4_attention_kernel<T, NB><<<static_cast<unsigned>(std::min(p.tiles + p.slots, p.tiles * p.most)), kThreads, 0, st>>>(a);
   NML_LAUNCHED();
-  if (splits > 1) {
-    kv4_combine_kernel<T><<<dim3(a.S, a.H, a.B), a.dk <= 64 ? 64 : a.dk <= 128 ? 128 : 256, 0, st>>>(a, splits);
-    NML_LAUNCHED();
-  }
   return 0;
 }
 
 template <typename T>
 int attention_launch(const Kv4AttnArgs& a, hipStream_t st) {
-  const int splits = attention_splits(a.B, a.H, a.Hkv, a.S, a.P), nb = (a.dk + kBlock - 1) / kBlock;
-  if (nb == 1) return attention_launch_nb<T, 1>(a, splits, st);
-  if (nb == 2) return attention_launch_nb<T, 2>(a, splits, st);
-  if (nb <= 4) return attention_launch_nb<T, 4>(a, splits, st);
-  return attention_launch_nb<T, 8>(a, splits, st);
+  const int nb = (a.dk + kBlock - 1) / kBlock;
+  if (nb == 1) return attention_launch_nb<T, 1>(a, st);
+  if (nb == 2) return attention_launch_nb<T, 2>(a, st);
+  if (nb <= 4) return attention_launch_nb<T, 4>(a, st);
+  return attention_launch_nb<T, 8>(a, st);
 }
 
 }  // namespace
@@ -597,8 +778,11 @@ int launch_kv4_read(int dt, const Kv4ReadArgs& a, hipStream_t st) {
 }
 
 size_t kv4_attention_workspace(int B, int H, int Hkv, int S, int P, int dk) {
-  const int splits = attention_splits(B, H, Hkv, S, P);
-  return splits == 1 ? 0 : sizeof(float) * static_cast<size_t>(B) * H * S * splits * (dk + 2);
+  const Pieces p = attention_pieces(B, H, Hkv, S, P, dk);
+  if (p.slots == 0) return 0;
+  const long long R = static_cast<long long>(H / Hkv) * S, nb = (dk + kBlock - 1) / kBlock;
+  const long long d = kBlock * (nb <= 2 ? nb : nb <= 4 ? 4 : 8);
+  return sizeof(unsigned) * kCounters * kCounterStep + sizeof(float) * p.slots * std::min<long long>(16, R) * (2 + d);
 }
 
 int launch_kv4_attention(int dt, const Kv4AttnArgs& a, hipStream_t st) {

@@ -387,6 +387,8 @@ def kv4_attention(q, cache, lens, scale, counts=None):
     need = C.c_size_t()
     N.check(N.lib.nml_kv4_attention_workspace(*sizes, C.byref(need)))
     ws = N.DeviceArray((need.value,), np.uint8) if need.value else None
+    if ws is not None:
+        N.check(N.lib.nml_memset(ws.ptr, 0, ws.nbytes))
     out = N.DeviceArray((batch, seq, heads * dk), dt)
     if cd is not None:
         N.check(N.lib.nml_memset(out.ptr, 0, out.nbytes))

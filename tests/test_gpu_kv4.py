@@ -231,7 +231,7 @@ def test_ragged_counts_leave_the_padding(gpu, dtype):
                                                 np.full((b, seq, h * dk), 7, dtype))]
     need = N.C.c_size_t()
     N.check(N.lib.nml_kv4_attention_workspace(b, h, h, seq, p, dk, N.C.byref(need)))
-    ws = N.DeviceArray((need.value,), np.uint8)
+    ws = N.DeviceArray.from_host(np.zeros(need.value, np.uint8))
     N.check(N.lib.nml_kv4_attention_device(dev[0].ptr, *c.pointers, dev[1].ptr, dev[2].ptr,
                                            dev[3].ptr, b, h, h, seq, p, dk, 8.0, ws.ptr, need.value,
                                            None, N.np_dtype_code(dtype)))
@@ -378,3 +378,49 @@ def test_pieces_of_very_different_scores(gpu, dtype):
     k[0, 0, n - 1, 40] = np.nan
     got = K.kv4_attention(q, cache_of(k, v), [n], scale).numpy().astype(np.float64)[0]
     assert np.array_equal(got[0], clean[0, 0]) and np.isnan(got[1]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dk, group, seq", [(32, 1, 1), (64, 3, 2)])
+def test_one_long_row_among_short_ones(gpu, dtype, dk, group, seq):
+    """One row's keys in more pieces than are merged at a time, beside forty rows of a few."""
+    r = np.random.RandomState(dk)
+    lens = r.randint(0, 4, 40)
+    lens[17] = 9001
+    check_attention(r, dtype, dk, 1, group, seq, lens)
+
+
+def test_many_rows(gpu):
+    """More rows than a wave's lanes, with and without keys, tokens or both."""
+    r = np.random.RandomState(15)
+    lens, counts = r.randint(0, 150, 200), r.randint(0, 4, 200)
+    lens[::7] = 0
+    check_attention(r, np.float16, 32, 2, 1, 3, lens, counts, 150)
+
+
+def test_one_workspace_serves_calls_of_any_size(gpu):
+    """Calls of different shapes follow each other on one workspace, zeroed once."""
+    r = np.random.RandomState(16)
+    shapes = [(3, 2, 1, 1, 64, 900), (1, 1, 4, 5, 32, 3000), (40, 4, 1, 1, 128, 260),
+              (2, 2, 2, 3, 256, 700), (1, 1, 1, 1, 16, 5000)]
+    need = N.C.c_size_t()
+    most = 0
+    for b, kv, g, s, dk, n in shapes:
+        N.check(N.lib.nml_kv4_attention_workspace(b, kv * g, kv, s, n, dk, N.C.byref(need)))
+        most = max(most, need.value)
+    ws = N.DeviceArray.from_host(np.zeros(most, np.uint8))
+    made = []
+    for b, kv, g, s, dk, n in shapes:
+        k, v, q = normal(r, (b, kv, n, dk), np.float32), normal(r, (b, kv, n, dk), np.float32), \
+            normal(r, (b, kv * g, s, dk), np.float32)
+        lens = r.randint(s, n + 1, b)
+        c = cache_of(k, v)
+        made.append((c, N.DeviceArray.from_host(q), N.DeviceArray.from_host(lens.astype(np.int32)),
+                     K.kv4_attention(q, c, lens, 8.0).numpy()))
+    for _ in range(3):
+        for (b, kv, g, s, dk, n), (c, q, lens, want) in zip(shapes, made):
+            out = N.DeviceArray((b, s, kv * g * dk), np.float32)
+            N.check(N.lib.nml_kv4_attention_device(
+                q.ptr, *c.pointers, lens.ptr, None, out.ptr, b, kv * g, kv, s, n, dk, 8.0, ws.ptr,
+                most, None, N.F32))
+            assert np.array_equal(out.numpy(), want)
