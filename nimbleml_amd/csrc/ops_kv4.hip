@@ -312,7 +312,7 @@ template <int NB>
 struct Kv4Tile {
   static constexpr int W = NB > 4 ? 2 : 1;  // blocks a lane's values touch
   unsigned c[2][NB];
-  unsigned e[2][W];
+  uint8_t e[2][W];  // (as loaded: widened at their use, or the wait for them moves up to the load)
 };
 
 // Tile at `codes` and `scales` (those of its first key). Keys past `last` (of the tile): that key
@@ -490,23 +490,12 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 4 : 2) void kv4_attention_kerne
   for (; j < k1; j += kSpan) {
     unsigned worst = 0;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < W; ++i) worst = max(worst, max(k.e[t][i], v.e[t][i]));
+    for (int i = 0; i < W; ++i) worst = max(worst, max<unsigned>(k.e[0][i], k.e[1][i]));
     const bool nan = __ballot(worst == kScaleNaN) != 0;
     unsigned k_nan[2] = {0, 0};
     if (nan) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        k_nan[t] = take_nan<NB>(k, t, nullptr);
-        unsigned of[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        take_nan<NB>(v, t, of);
-        const int seen = min(max(min(lim, k1 - 1) - (j + 16 * t) + 1, 0), 16);
-        const unsigned vis = (1u << seen) - 1u;
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
-          if (of[i] & vis) nan_blocks |= 1u << i;
-      }
+      for (int t = 0; t < 2; ++t) k_nan[t] = take_nan<NB>(k, t, nullptr);
     }
     // S = K·Qᵀ: this lane's are keys 4g … 4g+3 of both subtiles with its query
     float x[8];
@@ -525,6 +514,21 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 4 : 2) void kv4_attention_kerne
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = acc[i / 4][i % 4];
+    }
+    worst = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) worst = max(worst, max<unsigned>(v.e[0][i], v.e[1][i]));
+    if (__ballot(worst == kScaleNaN)) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        unsigned of[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        take_nan<NB>(v, t, of);
+        const int seen = min(max(min(lim, k1 - 1) - (j + 16 * t) + 1, 0), 16);
+        const unsigned vis = (1u << seen) - 1u;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+          if (of[i] & vis) nan_blocks |= 1u << i;
+      }
     }
     // V to LDS, a key a row
 #pragma unroll
