@@ -239,18 +239,6 @@ struct Rows {
   __device__ __forceinline__ int spans() const { return n > 0 ? max(1, (len + kSpan - 1) / kSpan) : 1; }
 };
 
-// Inclusive sum over the wave's lanes (data-parallel-primitive moves: within rows of 16, then the
-// rows' last lanes to the rows behind).
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);  // row_shr:2
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);  // row_shr:4
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);  // row_shr:8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
-  return v;
-}
-
 // What this workgroup does: piece `piece` of `pieces` of tile (b, e), whose row has len keys and n
 // new tokens; `slot`: where the tile's first piece is in ws. b < 0: nothing.
 struct Work {

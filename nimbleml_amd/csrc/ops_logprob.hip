@@ -8,15 +8,20 @@
 // either dtype. A logit of −inf has probability 0 and adds
 // nothing; a row of nothing else has no distribution: logp and entropy are NaN, as log_softmax's.
 //
-// A workgroup takes a row. Rows are read as the aligned 16-byte pieces that hold them (a row of
-// an odd vocabulary starts anywhere); what such a piece holds of the neighbouring rows is not
-// read but taken as −inf.
+// A workgroup takes a row and goes over it once: each thread keeps Σ exp(t) and Σ exp(t)·t of its
+// logits relative to a reference of its own, which moves only when a logit passes it by 8 (so the
+// sums are scaled a few times a row, not once a logit); the threads' sums meet at the end. Rows
+// are read as the aligned 16-byte pieces that hold them (a row of an odd vocabulary starts
+// anywhere); what such a piece holds of the neighbouring rows is not read but taken as −inf.
 #include "kernels.hpp"
 
 namespace nml {
 
 namespace {
 
+#ifndef LP_ROWS
+#define LP_ROWS 512
+#endif
 // Gathered candidates of the alternatives; more than this takes the rounds below.
 constexpr int kCandidates = 1024;
 
@@ -29,13 +34,9 @@ __device__ __forceinline__ unsigned order_of(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-__device__ __forceinline__ unsigned wave_umax(unsigned v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const unsigned w = __shfl_xor(v, o, 64);
-    v = v > w ? v : w;
-  }
-  return v;
+// The logit of such a word.
+__device__ __forceinline__ float value_of(unsigned o) {
+  return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 
 __device__ __forceinline__ unsigned long long wave_umax64(unsigned long long v) {
@@ -62,26 +63,88 @@ struct RowPieces {
   __device__ vec load(int c) const {
     const int i = first(c);
     if (i >= 0 && i + E <= V) return *reinterpret_cast<const vec*>(row + i);
-    vec r;
+    return edge(i);
+  }
+  // (word by word: as a vector its values would take a register each beside the whole pieces)
+  __device__ vec edge(int i) const {
+    typedef unsigned u4 __attribute__((ext_vector_type(4)));
+    u4 r;
 #pragma unroll
-    for (int e = 0; e < E; ++e) r[e] = i + e >= 0 && i + e < V ? row[i + e] : static_cast<T>(-INFINITY);
-    return r;
+    for (int w = 0; w < 4; ++w) {
+      if constexpr (E == 4) {
+        r[w] = i + w >= 0 && i + w < V ? __builtin_bit_cast(unsigned, row[i + w]) : 0xff800000u;
+      } else {
+        unsigned half[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int at = i + 2 * w + e;
+          half[e] = at >= 0 && at < V ? __builtin_bit_cast(unsigned short, row[at]) : 0xfc00u;
+        }
+        r[w] = half[0] | half[1] << 16;
+      }
+    }
+    return __builtin_bit_cast(vec, r);
   }
 };
 
-// NCH pieces a thread in registers; NCH = 0: any number, read again for every pass.
+constexpr float kLowest = -1e4f;          // exp of it is 0, its product with that too
+constexpr float kNone = -3.402823466e38f;  // a reference below every finite logit
+
+// A thread's part of Σ exp(x − ref) and Σ exp(x − ref)·(x − ref), and the largest x it has seen.
+struct Part {
+  float top, ref, z, zt;
+  // of another reference r (at least the largest x, or this part's own)
+  __device__ __forceinline__ void move(float r) {
+    const float d = fmaxf(ref - r, kLowest), f = exp_of(d);
+    zt = f * (zt + z * d);
+    z *= f;
+    ref = r;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ float piece_max(const typename RowPieces<T>::vec& v);
+template <>
+__device__ __forceinline__ float piece_max<float>(const typename RowPieces<float>::vec& v) {
+  return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+}
+template <>
+__device__ __forceinline__ float piece_max<half_t>(const typename RowPieces<half_t>::vec& v) {
+  typedef half_t h2 __attribute__((ext_vector_type(2)));
+  const h2 a = __builtin_elementwise_max(h2{v[0], v[1]}, h2{v[2], v[3]});
+  const h2 b = __builtin_elementwise_max(h2{v[4], v[5]}, h2{v[6], v[7]});
+  const h2 c = __builtin_elementwise_max(a, b);
+  return fmaxf(static_cast<float>(c.x), static_cast<float>(c.y));
+}
+
+template <typename T>
+__device__ __forceinline__ void add_piece(Part& s, const typename RowPieces<T>::vec& v) {
+  const float top = piece_max<T>(v);  // (NaN is not seen here; it reaches the sums)
+  s.top = fmaxf(s.top, top);
+  if (__ballot(top > s.ref + 8.f)) s.move(fmaxf(s.ref, top));
+#pragma unroll
+  for (int e = 0; e < RowPieces<T>::E; ++e) {
+    const float t = static_cast<float>(v[e]) - s.ref, p = exp_of(t);
+    s.z += p;
+    s.zt += p * fmaxf(t, kLowest);
+  }
+}
+
+// NCH pieces a thread, all loaded at once and kept for the alternatives; NCH = 0: any number, four
+// in flight, read again for the alternatives.
 template <typename T, int NT, int NCH>
 __global__ __launch_bounds__(NT) void logprob_kernel(LogprobArgs a) {
   constexpr int NW = NT / 64;
   typedef RowPieces<T> Row;
   constexpr int E = Row::E;
   typedef typename Row::vec vec;
-  __shared__ float red[2][16];
-  __shared__ unsigned thr_w[16];
-  __shared__ unsigned long long best_w[16];
+  typedef unsigned u4 __attribute__((ext_vector_type(4)));
+  __shared__ Part parts[NW];
+  __shared__ float thr_w[NW];
+  __shared__ unsigned long long best_w[NW];
   __shared__ unsigned long long cand[kCandidates];
-  __shared__ int ncand;
-  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  __shared__ int ncand, counts[NW];
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t y = a.targets ? a.targets[r] : 0;
   if (a.targets && a.has_ignore && y == a.ignore_index) {
     if (tid == 0) {
@@ -98,125 +161,168 @@ __global__ __launch_bounds__(NT) void logprob_kernel(LogprobArgs a) {
   }
   const T* l = static_cast<const T*>(a.logits) + static_cast<size_t>(r) * a.ld;
   const Row row(l, a.V);
-  vec reg[NCH > 0 ? NCH : 1];
-  const int per = NCH > 0 ? NCH : (row.n + NT - 1) / NT;
+  const bool bad = a.targets && (y < 0 || y >= a.V);
+  const float target = a.targets && !bad ? static_cast<float>(l[y]) : __builtin_nanf("");
+  u4 reg[NCH > 0 ? NCH : 1];
+  auto none = [] {
+    vec v;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = static_cast<T>(-INFINITY);
+    return v;
+  };
   if (NCH > 0) {
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       const int c = tid + NT * k;
-      if (c < row.n) {
-        reg[k] = row.load(c);
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) reg[k][e] = static_cast<T>(-INFINITY);
-      }
+      reg[k] = __builtin_bit_cast(u4, c < row.n ? row.load(c) : none());
     }
   }
-  // f(piece's first element, its values) for each of this thread's pieces
+  // f(piece's first element, its values) for each of this thread's pieces (a wave together: for
+  // lanes past the row −inf)
   auto each = [&](auto f) {
     if (NCH > 0) {
 #pragma unroll
-      for (int k = 0; k < NCH; ++k) f(row.first(tid + NT * k), reg[k]);
+      for (int k = 0; k < NCH; ++k)
+        if (NT * k + 64 * w < row.n) {
+          int c = tid + NT * k;
+          asm volatile("" : "+v"(reg[k]), "+v"(c));  // (as loaded, nothing made of it kept from pass to pass)
+          f(row.first(c), __builtin_bit_cast(vec, reg[k]));
+          __builtin_amdgcn_sched_barrier(0);
+        }
     } else {
-      for (int k = 0; k < per; ++k)
-        if (tid + NT * k < row.n) f(row.first(tid + NT * k), row.load(tid + NT * k));
+      constexpr int F = 4;
+      for (int c = tid; c - lane < row.n; c += F * NT) {
+        vec v[F];
+#pragma unroll
+        for (int k = 0; k < F; ++k) v[k] = c + NT * k < row.n ? row.load(c + NT * k) : none();
+#pragma unroll
+        for (int k = 0; k < F; ++k)
+          if (c - lane + NT * k < row.n) f(row.first(c + NT * k), v[k]);
+      }
     }
   };
-  float mine = -INFINITY;
-  each([&](int, const vec& v) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) mine = fmaxf(mine, static_cast<float>(v[e]));
-  });
-  float mx = wave_max(mine);
-  if (lane == 0) red[0][w] = mx;
+  Part s{-INFINITY, kNone, 0.f, 0.f};
+  each([&](int, const vec& v) { add_piece<T>(s, v); });
+  const float mine = s.top;
+  // the wave's sums, then the row's, relative to the largest logit (−inf where nothing is above:
+  // then to a finite reference, and the row has no distribution)
+  {
+    const float top = wave_max_dpp(s.top), ref = wave_max_dpp(s.ref);
+    s.move(fmaxf(ref, top));
+    s.z = wave_sum_dpp(s.z);
+    s.zt = wave_sum_dpp(s.zt);
+    s.top = top;
+    if (lane == 0) parts[w] = s;
+  }
   __syncthreads();
-  mx = red[0][0];
-#pragma unroll
-  for (int i = 1; i < NW; ++i) mx = fmaxf(mx, red[0][i]);
-  __syncthreads();
-  float z = 0.f, zt = 0.f;
-  each([&](int, const vec& v) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float t = static_cast<float>(v[e]) - mx, p = exp_of(t);
-      z += p;
-      zt += p * fmaxf(t, -1e4f);  // (p is 0 there)
-    }
-  });
-  z = wave_sum(z);
-  zt = wave_sum(zt);
-  if (lane == 0) red[0][w] = z, red[1][w] = zt;
-  __syncthreads();
-  z = 0.f, zt = 0.f;
-#pragma unroll
-  for (int i = 0; i < NW; ++i) z += red[0][i], zt += red[1][i];
+  // (one wave's part a lane: every thread going over all sixteen took 1.5 µs of a row's 9)
+  Part p = lane < NW ? parts[lane] : Part{-INFINITY, kNone, 0.f, 0.f};
+  const float mx = wave_max_dpp(p.top);
+  p.move(fmaxf(mx, kNone));
+  float z = wave_sum_dpp(p.z);
+  const float zt = wave_sum_dpp(p.zt);
+  if (mx == -INFINITY) z = __builtin_nanf("");
   const float lz = logf(z);
   if (tid == 0) {
-    const bool bad = a.targets && (y < 0 || y >= a.V);
     if (bad && a.err) __hip_atomic_fetch_or(a.err, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (a.logp) a.logp[r] = bad ? __builtin_nanf("") : (static_cast<float>(l[y]) - mx) - lz;
+    if (a.logp) a.logp[r] = (target - mx) - lz;
     if (a.entropy) a.entropy[r] = lz - zt / z;
     if (a.m) a.m[r] = mx;
     if (a.l) a.l[r] = z;
   }
   if (a.top_k == 0) return;
 
-  // A word that at least top_k logits reach: in each wave whose lanes all hold some of the row,
+  // A value that at least top_k logits reach: in each wave whose lanes all hold some of the row,
   // the q-th largest of the lanes' maxima, the least of them over those waves.
   const int full = min(NW, row.n / 64);
+  float thr = -INFINITY;
   if (tid == 0) ncand = 0;
-  unsigned thr = 0;
   if (full > 0) {
-    unsigned top = 0;
-    each([&](int i, const vec& v) {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (i + e >= 0 && i + e < a.V) {
-          const unsigned o = order_of(static_cast<float>(v[e]));
-          top = top > o ? top : o;
-        }
-    });
     const int q = (a.top_k + full - 1) / full;
-    unsigned m = 0;
+    float top = mine, m = 0.f;
+    bool out = false;
     for (int i = 0; i < q; ++i) {
-      m = wave_umax(top);
-      const unsigned long long at = __ballot(top == m);
-      if (lane == __ffsll(at) - 1) top = 0;
+      m = wave_max_dpp(out ? -INFINITY : top);
+      const unsigned long long at = __ballot(!out && top == m);
+      if (lane == __ffsll(at) - 1) out = true;
     }
     if (lane == 0) thr_w[w] = m;
     __syncthreads();
     thr = thr_w[0];
-    for (int i = 1; i < full; ++i) thr = min(thr, thr_w[i]);
+    for (int i = 1; i < full; ++i) thr = fminf(thr, thr_w[i]);
   }
   __syncthreads();
   auto key = [](float x, int i) { return static_cast<unsigned long long>(order_of(x)) << 32 | ~static_cast<unsigned>(i); };
-  each([&](int i, const vec& v) {
+  const bool ordered = z == z;  // no NaN among the logits
+  if (ordered && NCH > 0) {
+    // kept pieces: a first pass counts, a second one writes to places known by then (what a piece
+    // holds past the row counts where the bound is −inf, with a word below every logit's)
+    int n = 0;
+    each([&](int, const vec& v) {
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (i + e >= 0 && i + e < a.V && order_of(static_cast<float>(v[e])) >= thr) {
-        const int at = atomicAdd(&ncand, 1);
-        if (at < kCandidates) cand[at] = key(static_cast<float>(v[e]), i + e);
+      for (int e = 0; e < E; ++e) n += static_cast<float>(v[e]) >= thr;
+    });
+    int at = wave_scan(n);
+    if (lane == 63) counts[w] = at;
+    at -= n;
+    __syncthreads();
+    const int before = wave_scan(lane < NW ? counts[lane] : 0);
+    if (w > 0) at += __builtin_amdgcn_readlane(before, w - 1);
+    if (tid == 0) ncand = __builtin_amdgcn_readlane(before, 63);
+    each([&](int i, const vec& v) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (static_cast<float>(v[e]) >= thr) {
+          if (at < kCandidates) cand[at] = i + e >= 0 && i + e < a.V ? key(static_cast<float>(v[e]), i + e) : 0;
+          ++at;
+        }
+    });
+  } else if (ordered) {
+    each([&](int i, const vec& v) {
+      if (!__ballot(piece_max<T>(v) >= thr)) return;
+      // places for the wave's candidates of this piece at once
+      unsigned long long take[E];
+      int n = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        take[e] = __ballot(static_cast<float>(v[e]) >= thr && i + e >= 0 && i + e < a.V);
+        n += __popcll(take[e]);
       }
-  });
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&ncand, n);
+      at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int mine = at + __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(take[e] >> 32),
+                                                        __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(take[e]), 0));
+        if (take[e] >> lane & 1 && mine < kCandidates) cand[mine] = key(static_cast<float>(v[e]), i + e);
+        at += __popcll(take[e]);
+      }
+    });
+  }
   __syncthreads();
   int64_t* ids = a.top_ids + static_cast<size_t>(r) * a.top_k;
   float* lps = a.top_logp + static_cast<size_t>(r) * a.top_k;
   auto put = [&](int at, unsigned long long k) {
-    const unsigned id = ~static_cast<unsigned>(k);
-    ids[at] = id;
-    lps[at] = (static_cast<float>(l[id]) - mx) - lz;
+    ids[at] = ~static_cast<unsigned>(k);
+    lps[at] = (value_of(static_cast<unsigned>(k >> 32)) - mx) - lz;
   };
   const int n = ncand;
-  if (n <= kCandidates) {  // each candidate's place: how many come before it
-    for (int i = tid; i < n; i += NT) {
-      const unsigned long long k = cand[i];
+  if (ordered && n <= kCandidates) {  // each candidate's place: how many come before it
+    constexpr int kShare = 8;         // lanes to a candidate
+    for (int i0 = 0; i0 < n; i0 += NT / kShare) {
+      const int i = i0 + tid / kShare;
+      const unsigned long long k = i < n ? cand[i] : ~0ull;
       int before = 0;
-      for (int j = 0; j < n; ++j) before += cand[j] > k;
-      if (before < a.top_k) put(before, k);
+      for (int j = tid % kShare; j < n; j += kShare) before += cand[j] > k;
+      before += __shfl_xor(before, 1, 64);
+      before += __shfl_xor(before, 2, 64);
+      before += __shfl_xor(before, 4, 64);
+      if (i < n && tid % kShare == 0 && before < a.top_k) put(before, k);
     }
     return;
   }
-  // Many equal logits (masked vocabularies): the next one in order, top_k times.
+  // Many equal logits (masked vocabularies) or NaN: the next one in order, top_k times.
   unsigned long long last = ~0ull;
   for (int t = 0; t < a.top_k; ++t) {
     unsigned long long best = 0;
@@ -271,7 +377,7 @@ __global__ __launch_bounds__(256) void logprob_bwd_kernel(LogprobBwdArgs a) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const float lp = (static_cast<float>(x[e]) - m) - lz, p = exp_of(lp);
-      float g = -p * (dl + dh * (fmaxf(lp, -1e4f) + h));  // (p is 0 below)
+      float g = -p * (dl + dh * (fmaxf(lp, kLowest) + h));
       if (i0 + e == y) g += dl;
       d[e] = static_cast<T>(g);
     }
@@ -290,10 +396,12 @@ int logprobs_launch(const LogprobArgs& a, hipStream_t st) {
   constexpr int E = RowPieces<T>::E;
   const int pieces = (a.V + 2 * (E - 1)) / E;  // at most, wherever a row starts
 #define NML_LOGPROB(NT, NCH) logprob_kernel<T, NT, NCH><<<a.rows, NT, 0, st>>>(a)
+  // Few rows: all of a row's loads at once, over as many lanes as a workgroup has. Many rows
+  // overlap each other's latency: four waves a row.
   if (pieces <= 256 * 4) NML_LOGPROB(256, 4);
-  else if (pieces <= 512 * 8) NML_LOGPROB(512, 8);
-  else if (pieces <= 512 * 16) NML_LOGPROB(512, 16);
-  else if (pieces <= 1024 * 16) NML_LOGPROB(1024, 16);
+  else if (a.rows > LP_ROWS) NML_LOGPROB(256, 0);
+  else if (pieces <= 1024 * 4) NML_LOGPROB(1024, 4);
+  else if (pieces <= 1024 * 8) NML_LOGPROB(1024, 8);
   else NML_LOGPROB(1024, 0);
 #undef NML_LOGPROB
   NML_LAUNCHED();
