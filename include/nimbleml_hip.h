@@ -372,6 +372,15 @@ int nml_model_mha_backward(nml_model* m, const void* dout, void* dx);
 int nml_model_loss(nml_model* m, const int64_t* ids, const int64_t* labels, size_t batch,
                    size_t seq, int64_t ignore_index, int has_ignore, double* loss);
 
+/* Log probabilities of labels (device int64, batch × seq) at every position of ids, with the
+ * entropies and the top_k most probable tokens: nml_token_logprobs_device over the logits that
+ * nml_model_forward would give, in row chunks, never all at once. Outputs are device arrays over
+ * batch·seq rows (top_ids, top_logp: × top_k); logp, entropy may be NULL. Returns after the device
+ * finishes; reports an id or a label (other than ignore_index, with has_ignore) out of range. */
+int nml_model_logprobs(nml_model* m, const int64_t* ids, const int64_t* labels, size_t batch,
+                       size_t seq, int64_t ignore_index, int has_ignore, size_t top_k, float* logp,
+                       float* entropy, int64_t* top_ids, float* top_logp);
+
 /* ---- training (float32 and float16 models) -------------------------------------------
  * compute_loss with the autograd graph kept, then loss.backward() (models/gpt.py:123-137;
  * Tensor.backward, utils/tensor.py:286-332; the array-level backward of
@@ -448,6 +457,11 @@ int nml_model_adamw_update(nml_model* m, int kind, int layer, size_t offset, siz
 /* KV cache for batch rows: K and V per layer, (batch, heads, max_seq, head_dim) each.
  * The seam generate() probes for (models/generate.py:93-100). */
 int nml_cache_create(nml_model* m, size_t batch, nml_cache** out);
+/* The same cache in 4 bits (blocks of 32 E2M1 codes and a scale, as nml_kv4_write_device makes
+ * them): 3.76 times fewer bytes than float16's. Every call that takes a cache takes it; attention
+ * sees the values that the cache holds, the new tokens' own among them, whether they come one by
+ * one or as a prompt. Beside the codes it holds one layer's K and V in the compute dtype. */
+int nml_cache_create_kv4(nml_model* m, size_t batch, nml_cache** out);
 int nml_cache_destroy(nml_cache* c);
 /* The length of row 0 (rows prefilled with nml_model_prefill_ragged may differ). */
 int nml_cache_length(nml_cache* c, size_t* len);
@@ -477,6 +491,12 @@ int nml_model_generate(nml_model* m, const int64_t* prompts, size_t prompt_strid
                        const int32_t* prompt_len, size_t batch, size_t max_new,
                        float temperature, int top_k, float top_p, float repetition_penalty,
                        const double* u, int64_t* tokens_out, size_t out_stride, int use_graph);
+
+/* nml_model_generate over a cache in 4 bits (nml_cache_create_kv4). */
+int nml_model_generate_kv4(nml_model* m, const int64_t* prompts, size_t prompt_stride,
+                           const int32_t* prompt_len, size_t batch, size_t max_new,
+                           float temperature, int top_k, float top_p, float repetition_penalty,
+                           const double* u, int64_t* tokens_out, size_t out_stride, int use_graph);
 
 /* Timing helper for the benchmark: average device time of one decode step
  * (embedding … sampling) over `steps` steps of the last generate() call shape. */

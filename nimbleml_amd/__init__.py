@@ -14,6 +14,7 @@ from nimbleml_amd.gpt import GPT, KVCache
 from nimbleml_amd.layers import (Dense, Embedding, FeedForward, FusedGPTTrunk,
                                  FusedTransformerBlock, Module, MultiHeadAttention, RMSNorm,
                                  Sequential, TransformerBlock)
+from nimbleml_amd.logprobs import token_log_probs
 from nimbleml_amd.mask import causal_mask_tensor, make_causal_mask
 from nimbleml_amd.np_backend import device, set_device, set_dtype, using_gpu
 from nimbleml_amd.optim import Adam, AdamW
@@ -28,5 +29,5 @@ __all__ = [
     "Sequential", "save", "load", "load_arrays", "named_parameters", "save_checkpoint",
     "load_checkpoint", "Adam", "AdamW", "device", "using_gpu",
     "set_device", "set_dtype", "np_backend", "no_grad", "enable_grad", "is_grad_enabled",
-    "causal_mask_tensor", "make_causal_mask",
+    "causal_mask_tensor", "make_causal_mask", "token_log_probs",
 ]

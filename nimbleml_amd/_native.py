@@ -91,6 +91,7 @@ _SIGS = {
     "nml_model_mha_forward_train": [vp, i32, vp, vp, sz, sz, i32, vp],
     "nml_model_mha_backward": [vp, vp, vp],
     "nml_model_loss": [vp, vp, vp, sz, sz, i64, i32, C.POINTER(C.c_double)],
+    "nml_model_logprobs": [vp, vp, vp, sz, sz, i64, i32, sz, vp, vp, vp, vp],
     "nml_model_zero_grad": [vp],
     "nml_model_grad_ptr": [vp, i32, i32, C.POINTER(C.c_void_p)],
     "nml_model_loss_train": [vp, vp, vp, sz, sz, i64, i32, C.POINTER(C.c_double)],
@@ -103,11 +104,13 @@ _SIGS = {
     "nml_model_adam_master": [vp, i32, i32, C.POINTER(C.c_void_p)],
     "nml_model_adamw_update": [vp, i32, i32, sz, sz, f32, f32, f32, f32, f32, f32, f32],
     "nml_cache_create": [vp, sz, C.POINTER(vp)],
+    "nml_cache_create_kv4": [vp, sz, C.POINTER(vp)],
     "nml_cache_destroy": [vp],
     "nml_cache_length": [vp, C.POINTER(sz)],
     "nml_model_forward_cached": [vp, vp, vp, sz, sz, vp, i32],
     "nml_model_prefill_ragged": [vp, vp, vp, sz, PI32, sz, vp],
     "nml_model_generate": [vp, vp, sz, PI32, sz, sz, f32, i32, f32, f32, vp, vp, sz, i32],
+    "nml_model_generate_kv4": [vp, vp, sz, PI32, sz, sz, f32, i32, f32, f32, vp, vp, sz, i32],
     "nml_model_last_decode_ms": [vp, C.POINTER(f32)],
     "nml_model_last_decode_path": [vp, C.POINTER(C.c_int)],
 }

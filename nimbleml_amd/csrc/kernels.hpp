@@ -212,6 +212,7 @@ struct Kv4WriteArgs {
   const int32_t* counts;
   int B, H, S, P, dk;
   int* err;
+  int src_at_pos;  // token s is read where it goes to: element d of head h at … + (pos[b] + s)·stride_s + d
 };
 int launch_kv4_write(int dt, const Kv4WriteArgs& a, hipStream_t st);
 
@@ -225,6 +226,7 @@ struct Kv4ReadArgs {
   void* v_out;
   int B, H, S, P, dk;
   int* err;
+  int out_tokens;  // tokens that k_out and v_out have room for, ≥ S (0: S)
 };
 int launch_kv4_read(int dt, const Kv4ReadArgs& a, hipStream_t st);
 
@@ -241,6 +243,7 @@ struct Kv4AttnArgs {
   int B, H, Hkv, S, P, dk;
   int group;    // H / Hkv
   int slots;    // set by the launch
+  int more;     // keys of a row beyond lens[b]: lens may hold the position of the first new token
   float scale;  // divisor of the scores
   void* ws;
   int* err;

@@ -21,8 +21,15 @@ using namespace nml;
 struct nml_cache {
   nml_model* m;
   int B;
-  void* k = nullptr;  // L × B × H × P × dk
+  // L × B × H × P × dk; of a cache in 4 bits one layer's, through which each layer's new tokens
+  // pass (and, for many of them, the values read back)
+  void* k = nullptr;
   void* v = nullptr;
+  // A cache in 4 bits: codes (L × B × H × P × ⌈dk/32⌉ × 16) and scales, else null; attention
+  // workspaces of a batch and of the halves of a split one.
+  uint8_t *k_codes = nullptr, *k_scales = nullptr, *v_codes = nullptr, *v_scales = nullptr;
+  char* ws4[2] = {nullptr, nullptr};
+  size_t ws4_bytes = 0;
   int32_t* len_dev = nullptr;  // B
   std::vector<int32_t> len;    // host mirror
   // Single-token steps (forward_with_cache with one token per row): the fed ids at their
@@ -151,7 +158,80 @@ struct KVView {
   void* k;
   void* v;
   long long sb, sh;
+  // A cache in 4 bits: this layer's part of it (k and v then hold P positions of one layer in the
+  // compute dtype), and an attention workspace. Null: none.
+  uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
+  void* ws4;
 };
+
+// Layer l of cache c from row b0 on; half: which of the cache's workspaces.
+KVView cache_view(nml_model* m, const nml_cache* c, int l, int b0, int half) {
+  const long long sb = (long long)m->H * m->P * m->dk, sh = (long long)m->P * m->dk;
+  const size_t layer = c->k_codes ? 0 : (size_t)l * c->B * m->H * m->P * m->dk * m->es;
+  const size_t at = layer + (size_t)b0 * m->H * m->P * m->dk * m->es;
+  KVView v{static_cast<char*>(c->k) + at, static_cast<char*>(c->v) + at, sb, sh, nullptr, nullptr, nullptr, nullptr,
+           nullptr};
+  if (c->k_codes) {
+    const size_t blocks = ((size_t)l * c->B + b0) * m->H * m->P * ((m->dk + 31) / 32);
+    v.k_codes = c->k_codes + blocks * 16;
+    v.k_scales = c->k_scales + blocks;
+    v.v_codes = c->v_codes + blocks * 16;
+    v.v_scales = c->v_scales + blocks;
+    v.ws4 = c->ws4[half];
+  }
+  return v;
+}
+
+// Most new tokens a row that attend to a cache in 4 bits as it lies: 16 queries are one tile of
+// the kernel. More of them (a prompt or a piece of one) read the values back and take the
+// prefill kernels.
+constexpr int kKv4Tokens = 16;
+
+// The S new tokens of B rows, in c.k and c.v from position pos on, into the cache in 4 bits.
+// counts: tokens of each row (null: S).
+int kv4_append(nml_model* m, const KVView& c, int B, int S, const int32_t* pos, const int32_t* counts, hipStream_t st) {
+  Kv4WriteArgs w{};
+  w.k = c.k;
+  w.v = c.v;
+  w.stride_b = c.sb;
+  w.stride_h = c.sh;
+  w.stride_s = m->dk;
+  w.k_codes = c.k_codes;
+  w.k_scales = c.k_scales;
+  w.v_codes = c.v_codes;
+  w.v_scales = c.v_scales;
+  w.pos = pos;
+  w.counts = counts;
+  w.B = B;
+  w.H = m->H;
+  w.S = S;
+  w.P = m->P;
+  w.dk = m->dk;
+  w.src_at_pos = 1;
+  return launch_kv4_write(m->dt, w, st);
+}
+
+// Attention of the S newest tokens of B rows over a cache in 4 bits; the first of them is at pos.
+int kv4_attend(nml_model* m, const KVView& c, const void* q, void* out, int B, int S, const int32_t* pos, hipStream_t st) {
+  Kv4AttnArgs a{};
+  a.q = q;
+  a.k_codes = c.k_codes;
+  a.k_scales = c.k_scales;
+  a.v_codes = c.v_codes;
+  a.v_scales = c.v_scales;
+  a.lens = pos;
+  a.more = S;
+  a.out = out;
+  a.B = B;
+  a.H = a.Hkv = m->H;
+  a.group = 1;
+  a.S = S;
+  a.P = m->P;
+  a.dk = m->dk;
+  a.scale = sqrtf((float)m->dk);
+  a.ws = c.ws4;
+  return launch_kv4_attention(m->dt, a, st);
+}
 
 // Sequences of different lengths packed row after row (device arrays): row r is
 // position s of sequence b with row_seg[r] = (b << 16) | s; sequence b has seq_len[b]
@@ -172,10 +252,11 @@ struct AttnMode {
 
 // One attention sublayer over R rows of xin: [q | k | v] = xin·W_qkvᵀ + b (q head-major
 // into acts.q, k and v through c), RoPE when `rope`, attention into acts.att, then
-// out = acts.att·W_oᵀ + b_o (+ resid when non-null; out may equal resid).
+// out = acts.att·W_oᵀ + b_o (+ resid when non-null; out may equal resid). keys: with a cache in 4
+// bits, the most keys of a row once the new tokens are in it.
 int attention_sublayer(nml_model* m, const Layer& w, const void* xin, const Acts& a, int B, int S,
                        const int32_t* pos_base, const KVView& c, bool rope, const AttnMode& am,
-                       const void* resid, void* out, hipStream_t st, const Ragged* rg) {
+                       const void* resid, void* out, hipStream_t st, const Ragged* rg, int keys = 0) {
   const int R = rg ? rg->R : B * S, d = m->d;
   LinearArgs qkv{};
   qkv.x = xin;
@@ -192,6 +273,25 @@ int attention_sublayer(nml_model* m, const Layer& w, const void* xin, const Acts
   if (rope)  // models/gpt.py:62-64 → _fused_arrays.py:95-98
     NML_TRY(launch_rope(m->dt, a.q, c.k, c.sb, c.sh, B, m->H, S, m->dk, pos_base,
                         rg ? rg->seq_len : nullptr, m->rope_cos, m->rope_sin, m->P, st));
+  if (c.k_codes) {
+    NML_TRY(kv4_append(m, c, B, S, pos_base, rg ? rg->seq_len : nullptr, st));
+    if (rg || S > kKv4Tokens) {  // the values that the cache now holds, in place of the computed ones
+      Kv4ReadArgs r{};
+      r.k_codes = c.k_codes;
+      r.k_scales = c.k_scales;
+      r.v_codes = c.v_codes;
+      r.v_scales = c.v_scales;
+      r.counts = rg ? rg->seq_len : nullptr;
+      r.k_out = c.k;
+      r.v_out = c.v;
+      r.B = B;
+      r.H = m->H;
+      r.S = keys;
+      r.P = r.out_tokens = m->P;
+      r.dk = m->dk;
+      NML_TRY(launch_kv4_read(m->dt, r, st));
+    }
+  }
   AttnArgs at{};
   at.q = a.q;
   at.k = c.k;
@@ -211,7 +311,10 @@ int attention_sublayer(nml_model* m, const Layer& w, const void* xin, const Acts
     at.seq_len = rg->seq_len;
     at.row_start = rg->row_start;
   }
-  NML_TRY(launch_attention_prefill(m->dt, at, st));
+  if (c.k_codes && !rg && S <= kKv4Tokens)
+    NML_TRY(kv4_attend(m, c, a.q, a.att, B, S, pos_base, st));
+  else
+    NML_TRY(launch_attention_prefill(m->dt, at, st));
   LinearArgs wo{};
   wo.x = a.att;
   wo.lda = d;
@@ -234,14 +337,14 @@ int attention_sublayer(nml_model* m, const Layer& w, const void* xin, const Acts
 template <typename KVF>
 int trunk(nml_model* m, const Acts& a, int B, int S, const int32_t* pos_base, KVF kv,
           hipStream_t st, const Ragged* rg = nullptr, bool final_norm = true,
-          const AttnMode& am = AttnMode{}) {
+          const AttnMode& am = AttnMode{}, int keys = 0) {
   const int R = rg ? rg->R : B * S, d = m->d;
   for (int l = 0; l < m->L; ++l) {
     const Layer& w = m->layers[l];
     const KVView c = kv(l);
     NML_TRY(launch_rmsnorm(m->dt, a.x, w.ln1, a.xn, nullptr, nullptr, R, d, kEps, st));
     NML_TRY(attention_sublayer(m, w, a.xn, a, B, S, pos_base, c, rope_on(m), am, a.x, a.x, st,
-                               rg));
+                               rg, keys));
     NML_TRY(launch_rmsnorm(m->dt, a.x, w.ln2, a.xn, nullptr, nullptr, R, d, kEps, st));
     LinearArgs f1{};
     f1.x = a.xn;
@@ -304,9 +407,6 @@ int decode_step(nml_model* m, nml_cache* c, const Acts& a, int b0, int Bn, const
   logits = static_cast<char*>(logits) + (size_t)b0 * m->V * m->es;
   NML_TRY(launch_embed_decode(m->dt, tokens, tok_stride, pos, m->emb, posw(m), a.x, B, d, m->V,
                               m->P, err, st));
-  // the cache holds all c->B rows per layer; this step's rows start at row b0
-  const size_t layer_kv = (size_t)c->B * m->H * m->P * m->dk * m->es;
-  const size_t row0 = (size_t)b0 * m->H * m->P * m->dk * m->es;
   // RMSNorm fused into the GEMMs that consume it (fp16, 8 < B ≤ 64): the residual GEMMs
   // (W_o, W2) leave per-piece sums of squares of x in a.ssq, and QKV, W1 and the head
   // normalise x on load; layer 0's input (the embedding) still takes the RMSNorm kernel.
@@ -317,9 +417,10 @@ int decode_step(nml_model* m, nml_cache* c, const Acts& a, int b0, int Bn, const
                     linear_norm_fusable(m->dt, B, d, m->V);
   for (int l = 0; l < m->L; ++l) {
     const Layer& w = m->layers[l];
-    void* kl = static_cast<char*>(c->k) + l * layer_kv + row0;
-    void* vl = static_cast<char*>(c->v) + l * layer_kv + row0;
-    const long long sb = (long long)m->H * m->P * m->dk, sh = (long long)m->P * m->dk;
+    // the cache holds all c->B rows per layer; this step's rows start at row b0
+    const KVView view = cache_view(m, c, l, b0, b0 > 0);
+    void *kl = view.k, *vl = view.v;
+    const long long sb = view.sb, sh = view.sh;
     const bool fuse_in = fuse && l > 0;
     if (!fuse_in) NML_TRY(launch_rmsnorm(m->dt, a.x, w.ln1, a.xn, nullptr, nullptr, B, d, kEps, st));
     LinearArgs qkv{};
@@ -354,7 +455,12 @@ int decode_step(nml_model* m, nml_cache* c, const Acts& a, int b0, int Bn, const
     at.S = 1;
     at.dk = m->dk;
     at.scale = sqrtf((float)m->dk);
-    NML_TRY(launch_attention_decode(m->dt, at, pos, max_len, a.part, st));
+    if (view.k_codes) {
+      NML_TRY(kv4_append(m, view, B, 1, pos, nullptr, st));
+      NML_TRY(kv4_attend(m, view, a.q, a.att, B, 1, pos, st));
+    } else {
+      NML_TRY(launch_attention_decode(m->dt, at, pos, max_len, a.part, st));
+    }
     LinearArgs wo{};
     wo.x = a.att;
     wo.lda = d;
@@ -583,8 +689,7 @@ int prefill_rows(nml_model* m, nml_cache* c, const int64_t* prompts, size_t prom
     maxp = plen[b] > maxp ? plen[b] : maxp;
     same = same && plen[b] == plen[0];
   }
-  const size_t layer_kv = (size_t)B * m->H * m->P * m->dk * m->es;
-  const long long sb = (long long)m->H * m->P * m->dk, sh = (long long)m->P * m->dk;
+  auto kv = [&](int l) { return cache_view(m, c, l, 0, 0); };
   NML_HIP(hipMemsetAsync(sm.zeros, 0, B * 4, st));
   if (same) {
     const int S = plen[0];
@@ -599,12 +704,7 @@ int prefill_rows(nml_model* m, nml_cache* c, const int64_t* prompts, size_t prom
       NML_TRY(launch_embed(m->dt, prompts, m->emb, posw(m), nullptr, a.x, B, S, m->d, m->V, m->P,
                            sm.err, st));
     }
-    NML_TRY(trunk(m, a, B, S, sm.zeros,
-                  [&](int l) {
-                    return KVView{static_cast<char*>(c->k) + l * layer_kv,
-                                  static_cast<char*>(c->v) + l * layer_kv, sb, sh};
-                  },
-                  st));
+    NML_TRY(trunk(m, a, B, S, sm.zeros, kv, st, nullptr, true, AttnMode{}, S));
     NML_TRY(head(m, a, B, S, logits, 1, st));
   } else {
     // Packed rows: (b << 16) | s per row, then the lengths and row starts.
@@ -631,12 +731,7 @@ int prefill_rows(nml_model* m, nml_cache* c, const int64_t* prompts, size_t prom
       NML_TRY(launch_embed(m->dt, prompts + (size_t)b * prompt_stride, m->emb, posw(m), nullptr,
                            static_cast<char*>(a.x) + (size_t)starts[b] * m->d * m->es, 1, plen[b],
                            m->d, m->V, m->P, sm.err, st));
-    NML_TRY(trunk(m, a, B, maxp, sm.zeros,
-                  [&](int l) {
-                    return KVView{static_cast<char*>(c->k) + l * layer_kv,
-                                  static_cast<char*>(c->v) + l * layer_kv, sb, sh};
-                  },
-                  st, &rg));
+    NML_TRY(trunk(m, a, B, maxp, sm.zeros, kv, st, &rg, true, AttnMode{}, maxp));
     gather_last_rows_kernel<<<B, 128, 0, st>>>(static_cast<const char*>(a.xn), rg.row_start,
                                                rg.seq_len, static_cast<char*>(a.att),
                                                m->d * (int)m->es);
@@ -948,14 +1043,81 @@ int nml_model_loss(nml_model* m, const int64_t* ids, const int64_t* labels, size
   return finish_loss(m, sm, st, loss);
 }
 
-int nml_cache_create(nml_model* m, size_t batch, nml_cache** out) {
+int nml_model_logprobs(nml_model* m, const int64_t* ids, const int64_t* labels, size_t batch, size_t seq,
+                       int64_t ignore_index, int has_ignore, size_t top_k, float* logp, float* entropy,
+                       int64_t* top_ids, float* top_logp) {
+  NML_TRY(check_ready(m));
+  NML_REQUIRE(seq <= (size_t)m->P, "Sequence length %zu exceeds maximum sequence length %d", seq,
+              m->P);
+  NML_REQUIRE(top_k <= (size_t)kMaxTopLogprobs && top_k <= (size_t)m->V,
+              "model logprobs: top_k %zu above %d or the vocabulary", top_k, kMaxTopLogprobs);
+  if (batch == 0 || seq == 0) return 0;
+  NML_REQUIRE(ids && labels, "model logprobs: ids and labels are required");
+  NML_REQUIRE(top_k == 0 || (top_ids && top_logp), "model logprobs: top_k needs top_ids and top_logp");
+  const int B = (int)batch, S = (int)seq, R = B * S;
+  hipStream_t st = nml::stream();
+  Acts a;
+  NML_TRY(acts_for(m, R, 0, &a));
+  const size_t kvb = align256((size_t)R * m->d * m->es);
+  NML_TRY(ensure(m, m->kvs, 2 * kvb));
+  void* kbuf = m->kvs.p;
+  void* vbuf = static_cast<char*>(m->kvs.p) + kvb;
+  Small sm;
+  NML_TRY(small_for(m, 1, &sm));
+  NML_HIP(hipMemsetAsync(sm.err, 0, 2 * sizeof(int), st));  // of the ids, of the labels
+  NML_TRY(launch_embed(m->dt, ids, m->emb, posw(m), nullptr, a.x, B, S, m->d, m->V, m->P, sm.err,
+                       st));
+  const long long sb = (long long)m->H * S * m->dk, sh = (long long)S * m->dk;
+  NML_TRY(trunk(m, a, B, S, nullptr, [&](int) { return KVView{kbuf, vbuf, sb, sh}; }, st));
+  // logits in row chunks, as nml_model_loss forms them
+  size_t chunk = R;
+  while (chunk > 1 && chunk * m->V * m->es > ((size_t)512 << 20)) chunk = (chunk + 1) / 2;
+  NML_TRY(ensure(m, m->logits_ws, align256(chunk * m->V * m->es)));
+  for (size_t r0 = 0; r0 < (size_t)R; r0 += chunk) {
+    const int n = (int)std::min(chunk, (size_t)R - r0);
+    LinearArgs lm{};
+    lm.x = static_cast<const char*>(a.xn) + r0 * m->d * m->es;
+    lm.lda = m->d;
+    lm.w = m->emb;
+    lm.out = m->logits_ws.p;
+    lm.M = n;
+    lm.N = m->V;
+    lm.K = m->d;
+    lm.epi = EPI_NONE;
+    NML_TRY(launch_linear(m->dt, lm, st));
+    LogprobArgs p{};
+    p.logits = m->logits_ws.p;
+    p.ld = m->V;
+    p.targets = labels + r0;
+    p.rows = n;
+    p.V = m->V;
+    p.ignore_index = ignore_index;
+    p.has_ignore = has_ignore;
+    p.top_k = (int)top_k;
+    p.logp = logp ? logp + r0 : nullptr;
+    p.entropy = entropy ? entropy + r0 : nullptr;
+    p.top_ids = top_k ? top_ids + r0 * top_k : nullptr;
+    p.top_logp = top_k ? top_logp + r0 * top_k : nullptr;
+    p.err = sm.err + 1;
+    NML_TRY(launch_logprobs(m->dt, p, st));
+  }
+  int herr[2] = {0, 0};
+  NML_HIP(hipMemcpyAsync(herr, sm.err, sizeof(herr), hipMemcpyDeviceToHost, st));
+  NML_HIP(hipStreamSynchronize(st));
+  NML_REQUIRE(herr[0] == 0, "Token ID out of range [0, %d)", m->V);
+  NML_REQUIRE(herr[1] == 0, "label out of range [0, %d)", m->V);
+  return 0;
+}
+
+static int cache_create(nml_model* m, size_t batch, bool four_bits, nml_cache** out) {
   *out = nullptr;
   NML_TRY(check_ready(m));
   NML_REQUIRE(batch > 0 && batch <= 4096, "cache batch %zu out of range", batch);
   nml_cache* c = new nml_cache();
   c->m = m;
   c->B = (int)batch;
-  const size_t bytes = (size_t)m->L * batch * m->H * m->P * m->dk * m->es;
+  const size_t rows = batch * m->H * m->P, blocks = four_bits ? (size_t)m->L * rows * ((m->dk + 31) / 32) : 0;
+  const size_t bytes = (four_bits ? 1 : (size_t)m->L) * rows * m->dk * m->es;
   auto room = [m](auto** p, size_t n) {
     const hipError_t e = hipMalloc(p, n);
     return e != hipSuccess && train_drop_logits(m) ? hipMalloc(p, n) : e;
@@ -963,18 +1125,31 @@ int nml_cache_create(nml_model* m, size_t batch, nml_cache** out) {
   hipError_t e1 = room(&c->k, bytes);
   hipError_t e2 = e1 == hipSuccess ? room(&c->v, bytes) : e1;
   hipError_t e3 = e2 == hipSuccess ? room(&c->len_dev, align256(batch * 4)) : e2;
+  if (four_bits) {
+    // a step of one token or of kKv4Tokens of the whole batch, and a step of half of it
+    for (int s : {1, kKv4Tokens})
+      for (int b : {c->B, (c->B + 1) / 2})
+        c->ws4_bytes = std::max(c->ws4_bytes, align256(kv4_attention_workspace(b, m->H, m->H, s, m->P, m->dk)));
+    for (auto p : {&c->k_codes, &c->v_codes}) e3 = e3 == hipSuccess ? room(p, blocks * 16) : e3;
+    for (auto p : {&c->k_scales, &c->v_scales}) e3 = e3 == hipSuccess ? room(p, blocks) : e3;
+    for (int i = 0; i < 2 && c->ws4_bytes; ++i) e3 = e3 == hipSuccess ? room(&c->ws4[i], c->ws4_bytes) : e3;
+  }
   if (e3 != hipSuccess) {
-    set_error("cache: allocation of 2 × %zu bytes failed: %s", bytes, hipGetErrorString(e3));
-    if (c->k) (void)hipFree(c->k);
-    if (c->v) (void)hipFree(c->v);
-    delete c;
+    set_error("cache: allocation of 2 × %zu bytes failed: %s", bytes + blocks * 17, hipGetErrorString(e3));
+    (void)nml_cache_destroy(c);
     return -1;
   }
   c->len.assign(batch, 0);
   NML_HIP(hipMemsetAsync(c->len_dev, 0, batch * 4, nml::stream()));
+  for (int i = 0; i < 2; ++i)
+    if (c->ws4[i]) NML_HIP(hipMemsetAsync(c->ws4[i], 0, c->ws4_bytes, nml::stream()));
   *out = c;
   return 0;
 }
+
+int nml_cache_create(nml_model* m, size_t batch, nml_cache** out) { return cache_create(m, batch, false, out); }
+
+int nml_cache_create_kv4(nml_model* m, size_t batch, nml_cache** out) { return cache_create(m, batch, true, out); }
 
 int nml_cache_destroy(nml_cache* c) {
   if (!c) return 0;
@@ -983,6 +1158,9 @@ int nml_cache_destroy(nml_cache* c) {
   if (c->v) (void)hipFree(c->v);
   if (c->len_dev) (void)hipFree(c->len_dev);
   if (c->tok) (void)hipFree(c->tok);
+  for (void* p : {(void*)c->k_codes, (void*)c->k_scales, (void*)c->v_codes, (void*)c->v_scales, (void*)c->ws4[0],
+                  (void*)c->ws4[1]})
+    if (p) (void)hipFree(p);
   delete c;
   return 0;
 }
@@ -1005,7 +1183,7 @@ int nml_model_forward_cached(nml_model* m, nml_cache* c, const int64_t* ids, siz
   NML_REQUIRE((size_t)start + seq <= (size_t)m->P,
               "Sequence length %zu exceeds maximum sequence length %d", start + seq, m->P);
   hipStream_t st = nml::stream();
-  if (B == 1 && S == 1 && persist_wanted() && !rope_on(m) &&
+  if (B == 1 && S == 1 && !c->k_codes && persist_wanted() && !rope_on(m) &&
       persist_supported(m->dt, m->d, m->H, m->F, B, m->P)) {
     // One token of one sequence: the persistent decode kernel (logits out, no choice).
     NML_TRY(cache_step_buffers(m, c));
@@ -1034,14 +1212,8 @@ int nml_model_forward_cached(nml_model* m, nml_cache* c, const int64_t* ids, siz
   NML_TRY(acts_for(m, B * S, 0, &a));
   NML_TRY(launch_embed(m->dt, ids, m->emb, posw(m), c->len_dev, a.x, B, S, m->d, m->V, m->P,
                        nullptr, st));
-  const size_t layer_kv = (size_t)B * m->H * m->P * m->dk * m->es;
-  const long long sb = (long long)m->H * m->P * m->dk, sh = (long long)m->P * m->dk;
-  NML_TRY(trunk(m, a, B, S, c->len_dev,
-                [&](int l) {
-                  return KVView{static_cast<char*>(c->k) + l * layer_kv,
-                                static_cast<char*>(c->v) + l * layer_kv, sb, sh};
-                },
-                st));
+  NML_TRY(trunk(m, a, B, S, c->len_dev, [&](int l) { return cache_view(m, c, l, 0, 0); }, st, nullptr, true,
+                AttnMode{}, start + S));
   NML_TRY(head(m, a, B, S, logits, last_only, st));
   add_scalar_kernel<<<(B + 255) / 256, 256, 0, st>>>(c->len_dev, B, S);
   NML_LAUNCHED();
@@ -1078,10 +1250,10 @@ int nml_model_prefill_ragged(nml_model* m, nml_cache* c, const int64_t* prompts,
   return 0;
 }
 
-int nml_model_generate(nml_model* m, const int64_t* prompts, size_t prompt_stride,
-                       const int32_t* prompt_len, size_t batch, size_t max_new,
-                       float temperature, int top_k, float top_p, float repetition_penalty,
-                       const double* u, int64_t* tokens_out, size_t out_stride, int use_graph) {
+static int generate(nml_model* m, const int64_t* prompts, size_t prompt_stride, const int32_t* prompt_len,
+                    size_t batch, size_t max_new, float temperature, int top_k, float top_p,
+                    float repetition_penalty, const double* u, int64_t* tokens_out, size_t out_stride,
+                    int use_graph, bool four_bits) {
   NML_TRY(check_ready(m));
   const int B = (int)batch;
   if (B == 0 || max_new == 0) return 0;
@@ -1103,7 +1275,7 @@ int nml_model_generate(nml_model* m, const int64_t* prompts, size_t prompt_strid
   hipStream_t st = nml::stream();
 
   nml_cache* c = nullptr;
-  NML_TRY(nml_cache_create(m, batch, &c));
+  NML_TRY(cache_create(m, batch, four_bits, &c));
   struct Guard {
     nml_cache* c;
     ~Guard() { nml_cache_destroy(c); }
@@ -1174,7 +1346,7 @@ int nml_model_generate(nml_model* m, const int64_t* prompts, size_t prompt_strid
   // Attention length bound of the decode steps: the last step feeds position
   // maxp + max_new - 2 and attends to every key up to it.
   const int decode_len = maxp + (int)max_new - 1;
-  const bool persistent = persist_wanted() && !rope_on(m) &&
+  const bool persistent = !four_bits && persist_wanted() && !rope_on(m) &&
                           persist_supported(m->dt, m->d, m->H, m->F, B, m->P);
   PersistArgs pa{};
   if (persistent)
@@ -1296,6 +1468,22 @@ int nml_model_generate(nml_model* m, const int64_t* prompts, size_t prompt_strid
   NML_REQUIRE((herr & 4) == 0, "persistent decode: a data exchange timed out");
   NML_REQUIRE(herr == 0, "Token ID out of range [0, %d)", m->V);
   return 0;
+}
+
+int nml_model_generate(nml_model* m, const int64_t* prompts, size_t prompt_stride,
+                       const int32_t* prompt_len, size_t batch, size_t max_new,
+                       float temperature, int top_k, float top_p, float repetition_penalty,
+                       const double* u, int64_t* tokens_out, size_t out_stride, int use_graph) {
+  return generate(m, prompts, prompt_stride, prompt_len, batch, max_new, temperature, top_k, top_p,
+                  repetition_penalty, u, tokens_out, out_stride, use_graph, false);
+}
+
+int nml_model_generate_kv4(nml_model* m, const int64_t* prompts, size_t prompt_stride,
+                           const int32_t* prompt_len, size_t batch, size_t max_new,
+                           float temperature, int top_k, float top_p, float repetition_penalty,
+                           const double* u, int64_t* tokens_out, size_t out_stride, int use_graph) {
+  return generate(m, prompts, prompt_stride, prompt_len, batch, max_new, temperature, top_k, top_p,
+                  repetition_penalty, u, tokens_out, out_stride, use_graph, true);
 }
 
 int nml_model_last_decode_ms(nml_model* m, float* ms_per_step) {

@@ -138,7 +138,7 @@ __global__ __launch_bounds__(kWriters) void kv4_write_kernel(Kv4WriteArgs a, Ite
       if (a.err) __hip_atomic_fetch_or(a.err, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     at[u] = ((static_cast<size_t>(b) * a.H + it.h) * a.P + p) * n.nb + it.blk;
-    if (here[u]) load8<T, VEC>(src + it.h * a.stride_h + it.s * a.stride_s, it.blk * kBlock + part * 8, a.dk, x[u]);
+    if (here[u]) load8<T, VEC>(src + it.h * a.stride_h + (a.src_at_pos ? p : it.s) * a.stride_s, it.blk * kBlock + part * 8, a.dk, x[u]);
   }
 #pragma unroll
   for (int u = 0; u < kEach; ++u) {
@@ -213,7 +213,7 @@ __global__ __launch_bounds__(kWriters) void kv4_read_kernel(Kv4ReadArgs a, Items
       for (int i = 0; i < 8; ++i) x[i] = __builtin_nanf("");
     }
     const int d0 = it[u].blk * kBlock + part * 8;
-    T* out = to + ((static_cast<size_t>(b) * a.H + it[u].h) * a.S + it[u].s) * a.dk + d0;
+    T* out = to + ((static_cast<size_t>(b) * a.H + it[u].h) * (a.out_tokens ? a.out_tokens : a.S) + it[u].s) * a.dk + d0;
     if (VEC) {
       v8 r;
 #pragma unroll
@@ -279,7 +279,7 @@ struct Rows {
   __device__ __forceinline__ void load(const Kv4AttnArgs& a, int b, int* err) {
     len = n = 0;
     if (b < a.B) {
-      const int x = a.lens[b], y = a.counts ? a.counts[b] : a.S;
+      const int x = a.lens[b] + a.more, y = a.counts ? a.counts[b] : a.S;
       len = min(max(x, 0), a.P);
       n = min(max(y, 0), a.S);
       if (err && (x != len || y != n)) __hip_atomic_fetch_or(err, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);

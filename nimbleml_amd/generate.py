@@ -14,6 +14,9 @@ order on the device, so a seeded run gives the reference's tokens. With ``eos_id
 the reference stops drawing at the eos step; the global generator is then rewound
 to the state those fewer draws leave, so later draws of the caller agree too.
 
+``kv_bits=4`` holds the KV cache in 4 bits (blocks of 32 values, a power-of-two scale): a long
+context's attention reads 3.76 times fewer bytes than float16's, and sees the rounded values.
+
 Ragged batches: ``input_ids`` may be a list of rows of different lengths; each
 row then generates as if run alone (the result is a list of arrays).
 """
@@ -44,11 +47,13 @@ def _rows(input_ids):
 
 def generate(model, input_ids, *, max_new_tokens: int = 64, temperature: float = 0.8,
              top_k: int = 0, top_p: float = 0.9, eos_id=None, repetition_penalty: float = 1.0,
-             use_kv_cache: bool = True, use_graph: bool = True):
-    from nimbleml_amd.gpt import GPT
+             use_kv_cache: bool = True, use_graph: bool = True, kv_bits=None):
+    from nimbleml_amd.gpt import GPT, check_kv_bits
 
     if not isinstance(model, GPT):
         raise TypeError("nimbleml_amd.generate drives nimbleml_amd.GPT models")
+    if check_kv_bits(kv_bits) and not use_kv_cache:
+        raise ValueError("kv_bits=4 needs use_kv_cache=True")
     rows, ragged = _rows(input_ids)
     batch = len(rows)
     n = int(max_new_tokens)
@@ -71,7 +76,7 @@ def generate(model, input_ids, *, max_new_tokens: int = 64, temperature: float =
 
     if use_kv_cache:
         tokens = _generate_device(model, rows, plen, n, temperature, top_k, top_p,
-                                  repetition_penalty, u, use_graph)
+                                  repetition_penalty, u, use_graph, kv_bits)
     else:
         tokens = _generate_reforward(model, rows, plen, n, temperature, top_k, top_p,
                                      repetition_penalty, u)
@@ -92,7 +97,9 @@ def generate(model, input_ids, *, max_new_tokens: int = 64, temperature: float =
     return out if ragged else np.asarray(out, dtype=np.int64)
 
 
-def _generate_device(model, rows, plen, n, temperature, top_k, top_p, penalty, u, use_graph):
+def _generate_device(model, rows, plen, n, temperature, top_k, top_p, penalty, u, use_graph,
+                     kv_bits=None):
+    run = N.lib.nml_model_generate_kv4 if kv_bits == 4 else N.lib.nml_model_generate
     h = model._device_model()
     batch = len(rows)
     stride = int(plen.max())
@@ -104,7 +111,7 @@ def _generate_device(model, rows, plen, n, temperature, top_k, top_p, penalty, u
     dtok = N.DeviceArray((batch, out_stride), np.int64)
     du = N.DeviceArray.from_host(np.ascontiguousarray(u, dtype=np.float64)) if u is not None else None
     plen_c = np.ascontiguousarray(plen, dtype=np.int32)
-    N.check(N.lib.nml_model_generate(
+    N.check(run(
         h, dprompt.ptr, stride, plen_c.ctypes.data_as(N.PI32), batch, n, float(temperature),
         int(top_k or 0), float(top_p if top_p is not None else 1.0), float(penalty),
         du.ptr if du is not None else None, dtok.ptr, out_stride, int(bool(use_graph))))

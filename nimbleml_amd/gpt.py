@@ -32,15 +32,26 @@ def _ids_array(input_ids) -> np.ndarray:
     return np.asarray(input_ids, dtype=np.int64)
 
 
-class KVCache:
-    """Per-layer K/V cache on the device (the ``cache`` of ``forward_with_cache``)."""
+def check_kv_bits(kv_bits):
+    """Whether a cache is to be held in 4 bits (``kv_bits=4``) or in the compute dtype (None)."""
+    if kv_bits not in (None, 4):
+        raise ValueError(f"kv_bits must be None (the compute dtype) or 4, got {kv_bits!r}")
+    return kv_bits == 4
 
-    def __init__(self, model: "GPT", batch: int):
+
+class KVCache:
+    """Per-layer K/V cache on the device (the ``cache`` of ``forward_with_cache``), in the
+    compute dtype or, with ``kv_bits=4``, in 4 bits."""
+
+    def __init__(self, model: "GPT", batch: int, kv_bits=None):
+        create = N.lib.nml_cache_create_kv4 if check_kv_bits(kv_bits) else N.lib.nml_cache_create
         self.model = model
         self.batch = int(batch)
+        self.kv_bits = kv_bits
         h = C.c_void_p()
+        self._h = None
         self._model_handle = model._device_model()
-        N.check(N.lib.nml_cache_create(self._model_handle, self.batch, C.byref(h)))
+        N.check(create(self._model_handle, self.batch, C.byref(h)))
         self._h = h
         self._owner = model._dev  # keeps the device model alive while the cache exists
         self.lengths = None  # per-row lengths of a ragged prefill (None: all rows alike)
@@ -389,9 +400,13 @@ class GPT(Module):
         N.check(N.lib.nml_model_forward(h, dids.ptr, b, s, out.ptr, 1))
         return Tensor(out, (b, self.vocab_size))
 
-    def forward_with_cache(self, input_ids, cache=None):
+    def forward_with_cache(self, input_ids, cache=None, *, kv_bits=None):
         """Append ``input_ids`` (batch, s) to the KV cache and return their logits
-        (batch, s, vocab) — the hook models/generate.py:93-100 looks for."""
+        (batch, s, vocab) — the hook models/generate.py:93-100 looks for. ``kv_bits=4``: a new
+        cache (``cache=None``) is held in 4 bits."""
+        check_kv_bits(kv_bits)
+        if cache is not None and kv_bits is not None and kv_bits != cache.kv_bits:
+            raise ValueError(f"the cache given has kv_bits={cache.kv_bits}, not {kv_bits}")
         ids = _ids_array(input_ids)
         if ids.ndim != 2:
             raise ValueError(f"input_ids must be 2D (batch, seq), got shape {ids.shape}.")
@@ -400,7 +415,7 @@ class GPT(Module):
         h = self._device_model()
         b, s = ids.shape
         if cache is None:
-            cache = KVCache(self, b)
+            cache = KVCache(self, b, kv_bits)
         if cache.model is not self or cache.batch != b:
             raise ValueError("cache was created for another model or batch size")
         if cache._model_handle is not h:
@@ -417,13 +432,14 @@ class GPT(Module):
             cache.lengths = cache.lengths + s
         return Tensor(out, (b, s, self.vocab_size)), cache
 
-    def prefill_ragged(self, rows):
+    def prefill_ragged(self, rows, *, kv_bits=None):
         """Prefill a new KV cache with rows of different lengths (a list of 1-D id arrays)
         in one packed pass, as ``generate`` does for a ragged batch; returns each row's
         last-position logits (batch, vocab) and the cache. Each row continues at its own
         position: ``forward_with_cache(ids (batch, 1), cache)`` then runs one step of the
         batched decode loop. (The reference runs such rows one at a time,
-        models/generate.py:80-89.)"""
+        models/generate.py:80-89.) ``kv_bits=4``: the cache is held in 4 bits."""
+        check_kv_bits(kv_bits)
         rows = [np.asarray(r, dtype=np.int64).reshape(-1) for r in rows]
         if not rows or any(r.size == 0 for r in rows):
             raise ValueError("prompts must not be empty")
@@ -440,13 +456,37 @@ class GPT(Module):
         for i, r in enumerate(rows):
             prompts[i, :r.size] = r
         h = self._device_model()
-        cache = KVCache(self, b)
+        cache = KVCache(self, b, kv_bits)
         out = self._logits_array((b, self.vocab_size))
         dp = N.DeviceArray.from_host(prompts)
         N.check(N.lib.nml_model_prefill_ragged(h, cache._h, dp.ptr, stride,
                                                plen.ctypes.data_as(N.PI32), b, out.ptr))
         cache.lengths = plen.astype(np.int64)
         return Tensor(out, (b, self.vocab_size)), cache
+
+    def log_probs(self, input_ids, labels, *, top_k=0, ignore_index=None):
+        """Log probabilities of ``labels`` (batch, seq) at every position of ``input_ids``, as
+        ``compute_loss`` averages them: a dict of ``DeviceArray``s — ``logp`` and ``entropy``
+        (batch, seq) float32 and, with ``top_k``, ``top_ids`` (int64) and ``top_logp``
+        (batch, seq, top_k), most probable first. Positions whose label is ``ignore_index`` give
+        zeros and ids −1. No gradient: ``token_log_probs`` takes the logits of ``forward``."""
+        ids = _ids_array(input_ids)
+        self._check_ids(ids)
+        b, s = ids.shape
+        lab = np_backend.as_label_indices(labels, batch_size=b * s)
+        h = self._device_model()
+        out = {"logp": N.DeviceArray((b, s), np.float32),
+               "entropy": N.DeviceArray((b, s), np.float32)}
+        if top_k:
+            out["top_ids"] = N.DeviceArray((b, s, top_k), np.int64)
+            out["top_logp"] = N.DeviceArray((b, s, top_k), np.float32)
+        dids, dlab = N.DeviceArray.from_host(ids), N.DeviceArray.from_host(lab)
+        has = ignore_index is not None
+        N.check(N.lib.nml_model_logprobs(
+            h, dids.ptr, dlab.ptr, b, s, int(ignore_index) if has else 0, int(has), int(top_k),
+            out["logp"].ptr, out["entropy"].ptr, N.ptr(out.get("top_ids")),
+            N.ptr(out.get("top_logp"))))
+        return out
 
     def compute_loss(self, input_ids, labels, ignore_index=None):
         """Mean tied-head cross-entropy (models/gpt.py:123-137); logits are formed in
