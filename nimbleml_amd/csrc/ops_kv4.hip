@@ -539,15 +539,25 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 4 : 2) void kv4_attention_kerne
     float x[8];
     {
       floatx4 acc[2] = {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}};
+      constexpr int F = NB < 2 ? NB : 2;
 #pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const bf8 k0v = convert8(k.c[0][i], tile_scale(k.e[0][W == 2 ? i / 4 : 0]));
-        const bf8 k1v = convert8(k.c[1][i], tile_scale(k.e[1][W == 2 ? i / 4 : 0]));
+      for (int i0 = 0; i0 < NB; i0 += F) {
+        bf8 q[NP][F];
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
-          const bf8 q = qs[p][i][lane];
-          acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0v, q, acc[0], 0, 0, 0);
-          acc[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1v, q, acc[1], 0, 0, 0);
+        for (int p = 0; p < NP; ++p)
+#pragma unroll
+          for (int f = 0; f < F; ++f) q[p][f] = qs[p][i0 + f][lane];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+          const int i = i0 + f;
+          const bf8 k0v = convert8(k.c[0][i], tile_scale(k.e[0][W == 2 ? i / 4 : 0]));
+          const bf8 k1v = convert8(k.c[1][i], tile_scale(k.e[1][W == 2 ? i / 4 : 0]));
+#pragma unroll
+          for (int p = 0; p < NP; ++p) {
+            acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0v, q[p][f], acc[0], 0, 0, 0);
+            acc[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1v, q[p][f], acc[1], 0, 0, 0);
+          }
         }
       }
 #pragma unroll
@@ -615,17 +625,27 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 4 : 2) void kv4_attention_kerne
       for (int c = 0; c < NP; ++c) p[c][i] = part[c].x, p[c][i + 1] = part[c].y;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (LDS of this wave alone, in order)
-    // O += Vᵀ·Pᵀ: four keys of either subtile and 16 dims a transposing read
+    // O += Vᵀ·Pᵀ: four keys of either subtile and 16 dims a transposing read; reads of four steps
+    // (two, where registers are short) at once, so that the wave waits for LDS once for them
+    constexpr int F = DT < 4 ? DT : NP == 3 && NB == 4 ? 2 : 4;
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      typedef __attribute__((address_space(3))) s4 lds_s4;
-      const int key = 4 * g + col / 4;  // (and 16 on: the same pair)
-      const char* at = mine + key * kRow + v_pair<NB>(key, d) * 32 + (col % 4) * 8;
-      const s4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)at);
-      const s4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + 16 * kRow));
-      const bf8 vv = __builtin_bit_cast(bf8, s8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
+    for (int d0 = 0; d0 < DT; d0 += F) {
+      bf8 vv[F];
 #pragma unroll
-      for (int c = 0; c < NP; ++c) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, p[c], o[d], 0, 0, 0);
+      for (int f = 0; f < F; ++f) {
+        typedef __attribute__((address_space(3))) s4 lds_s4;
+        const int key = 4 * g + col / 4;  // (and 16 on: the same pair)
+        const char* at = mine + key * kRow + v_pair<NB>(key, d0 + f) * 32 + (col % 4) * 8;
+        const s4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)at);
+        const s4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + 16 * kRow));
+        vv[f] = __builtin_bit_cast(bf8, s8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int c = 0; c < NP; ++c)
+#pragma unroll
+        for (int f = 0; f < F; ++f)
+          o[d0 + f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv[f], p[c], o[d0 + f], 0, 0, 0);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
