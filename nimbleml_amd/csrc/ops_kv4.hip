@@ -23,8 +23,9 @@ constexpr int kBlockBytes = 16;       // and their codes
 constexpr int kMinExp = -120;         // ½·2^-120 is a normal float32 and bf16
 constexpr unsigned kScaleNaN = 255u;
 // A writing or reading workgroup, and the blocks that a lane of it takes: four loads in flight
-// (with one, K and V of 4 × 4096 tokens of 16 heads × 128 fp16 values were written and read back
-// in 84 µs, now 72; reading 32 heads × 16384 tokens 45 µs, now 34, 5.0 TB/s).
+// (K and V of 4 × 4096 tokens of 16 heads × 128 float16 values: written and read back in 72 µs, 82
+// with one load; read in 34 µs, 45 with one. 5.0 TB/s: bound by memory. A step's few tokens take
+// the time of two launches).
 constexpr int kWriters = 256, kEach = 4;
 
 // New tokens of row b, and whether the count had to be clamped.
@@ -245,8 +246,12 @@ __global__ __launch_bounds__(kWriters) void kv4_read_kernel(Kv4ReadArgs a, Items
 //
 // A (row, KV head, 16 queries) is one workgroup's unless its keys are many: pieces of a long one
 // go to several, as many in all as the card holds at once, and the last to finish merges them in
-// their order. A piece costs its startup and the merge about as much as four spans of keys, so it
-// has at least so many.
+// their order.
+//
+// What bounds it: 8 rows of 8 Ki … 32 Ki keys, 8 KV heads of 128 with four query heads each, 39 µs,
+// 4.6 TB/s of memory. 32 rows of 128 … 1280 keys, 16 heads of 64, 12 µs: 2 TB/s, the latency of a
+// workgroup's few rounds. One row of 1023 keys 8 µs: 2.7 until the first tile is there and Q laid
+// out, 0.8 a round, 1.8 for the merge and the store.
 
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
@@ -264,7 +269,10 @@ constexpr float kSlack = 8.f;              // in powers of two
 
 // Workgroups that the card's 256 CUs hold at once, by registers and LDS.
 __host__ __device__ constexpr int capacity(int nb) { return nb == 1 ? 768 : nb <= 4 ? 512 : 256; }
-// Spans that a piece has at least: what it costs to begin one and to merge it.
+// Spans that a piece has at least: what it costs to begin one and to merge it. (Head dim 64, 32 rows
+// of 128 … 1280 keys: 12 µs at eight, where no row is split, 19 at two. 128, one row of 30 Ki keys
+// with 8 KV heads: 15.6 µs at four, 18.5 at two, 18.9 at eight. 256, 4 rows of up to 8 Ki keys with
+// 4 KV heads: 16.5 at two, 20.8 at four, 27.2 at eight.)
 __host__ __device__ constexpr int least_spans(int nb) { return nb <= 2 ? 8 : nb <= 4 ? 4 : 2; }
 
 // ws: a counter for each tile in pieces (zero before and after every launch, in the same place
@@ -275,18 +283,15 @@ constexpr int kCounters = 2048, kCounterStep = 16;  // a line for each
 
 // Rows of the batch, 64 at a time with one in each lane: cached length and new tokens, in range.
 struct Rows {
-  int len, n;
-  __device__ __forceinline__ void load(const Kv4AttnArgs& a, int b, int* err) {
-    len = n = 0;
-    if (b < a.B) {
-      const int x = a.lens[b] + a.more, y = a.counts ? a.counts[b] : a.S;
-      len = min(max(x, 0), a.P);
-      n = min(max(y, 0), a.S);
-      if (err && (x != len || y != n)) __hip_atomic_fetch_or(err, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
+  int len, n, spans;
+  // Spans of the lane's row: at least one (its outputs are to be written), none past the batch.
+  __device__ __forceinline__ bool load(const Kv4AttnArgs& a, int b) {
+    const int at = min(b, a.B - 1), x = a.lens[at] + a.more, y = a.counts ? a.counts[at] : a.S;
+    len = min(max(x, 0), a.P);
+    n = min(max(y, 0), a.S);
+    spans = b >= a.B ? 0 : n > 0 ? max(1, (len + kSpan - 1) / kSpan) : 1;
+    return x == len && y == n;  // (were in range)
   }
-  // Spans of the lane's row (at least one: its outputs are to be written).
-  __device__ __forceinline__ int spans() const { return n > 0 ? max(1, (len + kSpan - 1) / kSpan) : 1; }
 };
 
 // What this workgroup does: piece `piece` of `pieces` of tile (b, e), whose row has len keys and n
@@ -294,34 +299,70 @@ struct Rows {
 struct Work {
   int b, e, piece, pieces, slot, len, n, spans;
 };
-__device__ __forceinline__ Work find_work(const Kv4AttnArgs& a, int each, int nb, int lane) {
+// More than 64 rows are shared out to the waves, a run of rows each (2048 rows × 8 heads of up to
+// 512 keys of 64: 310 µs, 670 with every wave looking through them all); sums: of the waves.
+__device__ __forceinline__ Work find_work(const Kv4AttnArgs& a, int each, int nb, int lane, int wave, int (*sums)[3]) {
   Work w{};
   Rows rows;
+  const int run = a.B <= 64 ? 64 : (a.B + 64 * kWaves - 1) / (64 * kWaves) * 64;
+  const int first = a.B <= 64 ? 0 : wave * run, end = min(first + run, a.B);
   int total = 0;
-  for (int i = 0; i < a.B; i += 64) {
-    rows.load(a, i + lane, blockIdx.x == 0 ? a.err : nullptr);
-    total += __builtin_amdgcn_readlane(wave_scan(i + lane < a.B ? rows.spans() : 0), 63);
+  bool good = true;
+#pragma unroll 2
+  for (int i = first; i < end; i += 64) {
+    good &= rows.load(a, i + lane);
+    total += rows.spans;
+  }
+  if (!good && blockIdx.x == 0 && a.err) __hip_atomic_fetch_or(a.err, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  total = __builtin_amdgcn_readlane(wave_scan(total), 63);
+  if (a.B > 64) {
+    if (lane == 0) sums[wave][0] = total;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) total += sums[i][0];
   }
   // pieces go to the places that the tiles' own workgroups leave (a quarter where they leave none:
   // for a row much longer than the others)
   const int cap = capacity(nb), room = max(cap - static_cast<int>(min(static_cast<long long>(each) * a.B, 1LL * cap)), cap / 4);
   const int least = max(least_spans(nb), static_cast<int>((static_cast<long long>(total) * each + room - 1) / room));
+  auto pieces_of = [&](int spans) { return spans <= least ? min(spans, 1) : (spans + least - 1) / least; };
   const int at = static_cast<int>(blockIdx.x / each);
-  int before = 0, slots = 0;
-  for (int i = 0; i < a.B; i += 64) {
-    if (a.B > 64) rows.load(a, i + lane, nullptr);
-    const int spans = i + lane < a.B ? rows.spans() : 0;
-    const int pieces = spans <= least ? min(spans, 1) : (spans + least - 1) / least;
+  int before = 0, slots = 0, from = 0;
+  if (a.B > 64) {
+    int pieces = 0, split = 0;
+#pragma unroll 2
+    for (int i = first; i < end; i += 64) {
+      rows.load(a, i + lane);
+      const int p = pieces_of(rows.spans);
+      pieces += p;
+      split += p > 1 ? p : 0;
+    }
+    pieces = wave_scan(pieces);
+    split = wave_scan(split);
+    if (lane == 63) sums[wave][1] = pieces, sums[wave][2] = split;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i)  // the run that has this workgroup's row
+      if (from == i * run && before + sums[i][1] <= at) {
+        before += sums[i][1];
+        slots += sums[i][2];
+        from += run;
+      }
+  }
+  for (int i = from; i < min(from + run, a.B); i += 64) {
+    if (a.B > 64) rows.load(a, i + lane);
+    const int pieces = pieces_of(rows.spans);
     const int sum = wave_scan(pieces), sum_slots = wave_scan(pieces > 1 ? pieces : 0);
     const unsigned long long past = __ballot(before + sum > at);
     if (past) {
       const int l = __ffsll(past) - 1;
       w.pieces = __builtin_amdgcn_readlane(pieces, l);
-      w.spans = __builtin_amdgcn_readlane(spans, l);
+      w.spans = __builtin_amdgcn_readlane(rows.spans, l);
       w.len = __builtin_amdgcn_readlane(rows.len, l);
       w.n = __builtin_amdgcn_readlane(rows.n, l);
-      const int first = before + __builtin_amdgcn_readlane(sum, l) - w.pieces;
-      const int local = static_cast<int>(blockIdx.x) - first * each;
+      const int start = before + __builtin_amdgcn_readlane(sum, l) - w.pieces;
+      const int local = static_cast<int>(blockIdx.x) - start * each;
       w.b = i + l;
       w.e = w.pieces == 1 ? local : local / w.pieces;
       w.piece = local - w.e * w.pieces;
@@ -428,8 +469,9 @@ __device__ __forceinline__ int v_pair(int key, int pair) {
 }
 
 // Partial results pass between workgroups of any XCD: stores and loads at agent scope (past the
-// L2s) and a count that each workgroup adds to once its stores have arrived. (An acquire in the
-// last one and plain loads instead cost 20 µs a launch: it empties that XCD's L2.)
+// L2s) and a count that each workgroup adds to once its stores have arrived. (With an acquire in
+// the last one and plain loads, which empties that XCD's L2, 32 rows of 128 … 1280 keys took 32 µs
+// instead of 17.)
 __device__ __forceinline__ void put2(float* p, f2 v) {
   __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), __builtin_bit_cast(unsigned long long, v), __ATOMIC_RELAXED,
                      __HIP_MEMORY_SCOPE_AGENT);
@@ -440,7 +482,7 @@ __device__ __forceinline__ f2 get2(const float* p) {
 }
 
 template <typename T, int NB>
-__global__ __launch_bounds__(kThreads, NB <= 4 ? 4 : 2) void kv4_attention_kernel(Kv4AttnArgs a) {
+__global__ __launch_bounds__(kThreads, NB == 1 ? 6 : NB <= 4 ? 4 : 2) void kv4_attention_kernel(Kv4AttnArgs a) {
   constexpr int NP = sizeof(T) == 2 ? 2 : 3;
   constexpr int W = Kv4Tile<NB>::W, DT = 2 * NB;  // DT: 16-wide tiles of the head dim
   constexpr int kRow = 64 * NB;                   // bytes of a key's values in LDS
@@ -453,7 +495,7 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 4 : 2) void kv4_attention_kerne
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
   const int nb = (a.dk + kBlock - 1) / kBlock, R = a.group * a.S, tiles = (R + 15) / 16;
-  const Work work = find_work(a, a.Hkv * tiles, NB, lane);
+  const Work work = find_work(a, a.Hkv * tiles, NB, lane, w, reinterpret_cast<int(*)[3]>(lds));
   if (work.b < 0 || work.n == 0) return;
   const int hk = tiles == 1 ? work.e : work.e / tiles, tile = work.e - hk * tiles;
   const int per = work.pieces == 1 ? work.spans : (work.spans + work.pieces - 1) / work.pieces;
@@ -539,7 +581,7 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 4 : 2) void kv4_attention_kerne
     float x[8];
     {
       floatx4 acc[2] = {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}};
-      constexpr int F = NB < 2 ? NB : 2;
+      constexpr int F = NB < 2 || (NP == 3 && NB == 4) ? 1 : 2;  // (2 would spill there)
 #pragma unroll
       for (int i0 = 0; i0 < NB; i0 += F) {
         bf8 q[NP][F];
@@ -626,8 +668,8 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 4 : 2) void kv4_attention_kerne
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (LDS of this wave alone, in order)
     // O += Vᵀ·Pᵀ: four keys of either subtile and 16 dims a transposing read; reads of four steps
-    // (two, where registers are short) at once, so that the wave waits for LDS once for them
-    constexpr int F = DT < 4 ? DT : NP == 3 && NB == 4 ? 2 : 4;
+    // at once, so that the wave waits for LDS once for them (1–3 % of a call)
+    constexpr int F = DT < 4 ? DT : 4;
 #pragma unroll
     for (int d0 = 0; d0 < DT; d0 += F) {
       bf8 vv[F];

@@ -398,6 +398,41 @@ def test_many_rows(gpu):
     check_attention(r, np.float16, 32, 2, 1, 3, lens, counts, 150)
 
 
+@pytest.mark.parametrize("rows", [65, 128, 513, 1030])
+@pytest.mark.parametrize("dk, long", [(32, 7000), (64, 5000), (128, 3)])
+def test_many_rows_and_two_long_ones(gpu, rows, dk, long):
+    """More rows than one wave, or one load of all eight, looks through: two long ones in pieces,
+    the rest of a few keys or none; first and last rows among them."""
+    r = np.random.RandomState(rows)
+    kv, seq, p = 1, 2, max(long, 4)
+    lens = r.randint(0, 4, rows).astype(np.int32)
+    lens[0], lens[-1] = long, long - 1
+    picked = np.unique(np.r_[0, 1, 62:65, rows // 2, rows - 2:rows])
+    c = K.KV4Cache(rows, kv, p, dk)
+    k, v = (np.zeros((rows, kv, 4, dk), np.float16) for _ in range(2))
+    k[:], v[:] = normal(r, k.shape, np.float16), normal(r, v.shape, np.float16)
+    K.kv4_write(c, k, v)  # the first four keys of every row
+    tail = [normal(r, (1, kv, p, dk), np.float16) for _ in range(2)]
+    blocks = -(-dk // 32)
+    for row in (0, rows - 1):  # all of the two long ones
+        ptrs = [a.ptr + row * kv * p * blocks * size for a, size in
+                ((c.k_codes, 16), (c.k_scales, 1), (c.v_codes, 16), (c.v_scales, 1))]
+        dev = [N.DeviceArray.from_host(x) for x in tail]
+        N.check(N.lib.nml_kv4_write_device(dev[0].ptr, dev[1].ptr, 0, p * dk, dk, *ptrs, None, None, 1, kv,
+                                           p, p, dk, None, N.np_dtype_code(np.float16)))
+    q = normal(r, (rows, kv, seq, dk), np.float16)
+    got = K.kv4_attention(q, c, lens, 8.0).numpy().astype(np.float64)
+    for i in picked:
+        hk, hv = (R.held(t if i in (0, rows - 1) else x[i:i + 1]) for t, x in zip(tail, (k, v)))
+        want = R.attention(q[i:i + 1], hk, hv, lens[i:i + 1], None, 8.0)
+        assert np.abs(got[i] - want[0]).max() <= bound(q[i:i + 1], hk, hv, 8.0, np.float16), i
+    none = lens == 0
+    assert (got[none] == 0).all()
+    with pytest.raises(ValueError, match="outside"):
+        lens[rows - 5] = p + 1
+        K.kv4_attention(q, c, lens, 8.0)
+
+
 def test_one_workspace_serves_calls_of_any_size(gpu):
     """Calls of different shapes follow each other on one workspace, zeroed once."""
     r = np.random.RandomState(16)
