@@ -253,8 +253,8 @@ int nml_sample_device(const void* logits, size_t batch, size_t vocab, float temp
  * Outputs are float32 (ids int64); logp, entropy, m, l may each be NULL, targets too without
  * logp. has_ignore: a row whose target is ignore_index is not read and gives zeros and ids −1.
  * A target outside [0, vocab) gives a logp of NaN and sets bit 0 of *err (device int, may be
- * NULL; the caller clears it). A row holding NaN, or nothing above −inf, has no distribution:
- * its statistics are NaN. Asynchronous, no workspace. */
+ * NULL; the caller clears it). A row holding NaN or +inf, or nothing above −inf, has no
+ * distribution: logp, entropy and top_logp are NaN. Asynchronous, no workspace. */
 int nml_token_logprobs_device(const void* logits, size_t ld, const int64_t* targets, size_t rows,
                               size_t vocab, int64_t ignore_index, int has_ignore, size_t top_k,
                               float* logp, float* entropy, float* m, float* l,

@@ -184,7 +184,9 @@ KVView cache_view(nml_model* m, const nml_cache* c, int l, int b0, int half) {
 
 // Most new tokens a row that attend to a cache in 4 bits as it lies: 16 queries are one tile of
 // the kernel. More of them (a prompt or a piece of one) read the values back and take the
-// prefill kernels.
+// prefill kernels, whose tiles share a key's conversion among more queries. (8 layers of d 1024, 16
+// tokens on the cache as it lies and 17 on the values read back: 8 rows of 3000 keys 0.68 and
+// 1.04 ms, of 512 0.57 and 0.66; 1 row of 3000 0.42 and 0.72.)
 constexpr int kKv4Tokens = 16;
 
 // The S new tokens of B rows, in c.k and c.v from position pos on, into the cache in 4 bits.
@@ -1054,6 +1056,7 @@ int nml_model_logprobs(nml_model* m, const int64_t* ids, const int64_t* labels, 
   if (batch == 0 || seq == 0) return 0;
   NML_REQUIRE(ids && labels, "model logprobs: ids and labels are required");
   NML_REQUIRE(top_k == 0 || (top_ids && top_logp), "model logprobs: top_k needs top_ids and top_logp");
+  NML_REQUIRE(batch <= 0x7fffffff / seq, "model logprobs: batch %zu too large", batch);
   const int B = (int)batch, S = (int)seq, R = B * S;
   hipStream_t st = nml::stream();
   Acts a;

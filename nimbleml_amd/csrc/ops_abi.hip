@@ -601,9 +601,9 @@ static int kv4_attention_ok(size_t batch, size_t heads, size_t kv_heads, size_t 
   NML_REQUIRE(kv_heads >= 1 ? heads % kv_heads == 0 : heads == 0,
               "kv4 attention: heads (%zu) must be divisible by kv_heads (%zu)", heads, kv_heads);
   if (batch && heads && seq) {
-    // the kernel numbers pieces of 128 keys in 32 bits
+    // the kernel numbers pieces of 128 keys in 32 bits, and a launch its threads
     const size_t tiles = (heads / kv_heads * seq + 15) / 16 * kv_heads;
-    NML_REQUIRE(tiles * batch <= 0x7fffffff / ((max_seq + 127) / 128),
+    NML_REQUIRE(tiles * batch <= 0x7fffffff / ((max_seq + 127) / 128) && tiles * batch <= (size_t)1 << 22,
                 "kv4 attention: %zu rows × %zu heads × %zu tokens over %zu positions too many", batch, heads, seq,
                 max_seq);
   }
@@ -627,7 +627,7 @@ int nml_kv4_attention_device(const void* q, const uint8_t* k_codes, const uint8_
                              int* err, int dtype) {
   NML_TRY(check_dtype(dtype));
   NML_TRY(kv4_attention_ok(batch, heads, kv_heads, seq, max_seq, dk));
-  NML_REQUIRE(scale_div > 0.f && std::isfinite(scale_div), "kv4 attention: scale_div must be positive");
+  NML_REQUIRE(scale_div > 0.f && std::isnormal(scale_div), "kv4 attention: scale_div must be positive and normal");
   if (batch == 0 || heads == 0 || seq == 0) return 0;
   NML_REQUIRE(q && k_codes && k_scales && v_codes && v_scales && lens && out, "kv4 attention: a buffer is null");
   NML_TRY(kv4_codes_ok("kv4 attention", k_codes, v_codes));

@@ -470,6 +470,8 @@ class GPT(Module):
         (batch, seq) float32 and, with ``top_k``, ``top_ids`` (int64) and ``top_logp``
         (batch, seq, top_k), most probable first. Positions whose label is ``ignore_index`` give
         zeros and ids −1. No gradient: ``token_log_probs`` takes the logits of ``forward``."""
+        if not 0 <= top_k <= 64:
+            raise ValueError(f"log_probs: top_k must be in [0, 64], got {top_k}")
         ids = _ids_array(input_ids)
         self._check_ids(ids)
         b, s = ids.shape

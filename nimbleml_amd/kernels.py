@@ -416,9 +416,11 @@ def _logit_rows(logits, targets):
 def token_logprobs(logits, targets, top_k=0, ignore_index=None):
     """Log probabilities of ``targets`` (rows,) under ``logits`` (..., vocab), row by row:
     ``(logp, entropy, m, l, top_ids, top_logp)`` as ``DeviceArray``s — float32 (rows,) each (m, l:
-    the largest logit and Σ exp(x − m)), the ``top_k`` most probable ids (int64) and their log probabilities (rows, top_k), most probable
-    first, or None without ``top_k``. Rows whose target is ``ignore_index`` give zeros and ids
-    −1. Raises ValueError for a target outside [0, vocab)."""
+    the largest logit and Σ exp(x − m)), the ``top_k`` most probable ids (int64) and their log
+    probabilities (rows, top_k), most probable first, or None without ``top_k``. Rows whose target
+    is ``ignore_index`` give zeros and ids −1. Raises ValueError for a target outside [0, vocab)."""
+    if not 0 <= top_k <= 64:
+        raise ValueError(f"token_logprobs: top_k must be in [0, 64], got {top_k}")
     ld, td, rows, vocab, code = _logit_rows(logits, targets)
     logp, entropy, m, lsum = (N.DeviceArray((rows,), np.float32) for _ in range(4))
     ids = top = None

@@ -208,3 +208,20 @@ def test_statistics_alone(gpu):
     want = R.logprobs(x, np.zeros(4, np.int64), 3)
     assert np.array_equal(ids.numpy(), want[4])
     assert np.abs(en.numpy() - want[1]).max() <= tol_of(x) and np.abs(top.numpy() - want[5]).max() <= tol_of(x)
+
+
+def test_more_rows_than_one_launch_takes(gpu):
+    """2^21 + 5 rows: the first, the last and those at the seam are their own."""
+    r = np.random.RandomState(31)
+    rows, vocab = (1 << 21) + 5, 5
+    x = logits_of(r, rows, vocab, np.float16)
+    t = r.randint(0, vocab, rows)
+    t[-2] = 1 << 40  # ignored
+    got = [a.numpy() for a in K.token_logprobs(x, t, 2, 1 << 40)]
+    for s in (slice(0, 9), slice((1 << 21) - 7, rows)):
+        # (not bit for bit those of a call of their own: a row's sums are grouped by where its
+        # 16-byte pieces begin)
+        want = R.logprobs(x[s], t[s], 2, 1 << 40)
+        for g, w in zip(got, want):
+            assert g[s].shape == w.shape and np.abs(g[s] - w).max() <= tol_of(x[s]) * np.maximum(1, np.abs(w).max())
+        assert np.array_equal(got[4][s], want[4])

@@ -6,6 +6,8 @@ import numpy as np
 import pytest
 
 from nimbleml_amd import _native as N
+from nimbleml_amd import kernels as K
+from nimbleml_amd.gpt import check_kv_bits
 from oracle import kv4_ref as R
 
 P = 1 << 20  # a pointer that no call here may reach
@@ -40,6 +42,8 @@ def attend(batch=2, heads=4, kv=2, seq=1, max_seq=8, dk=64, scale=8.0, lens=P, w
     (read(dk=300), "head_dim"), (read(out=None), "null"), (read(dtype=-1), "dtype"),
     (attend(heads=5), "divisible"), (attend(kv=0), "divisible"), (attend(scale=0.0), "scale_div"),
     (attend(scale=float("nan")), "scale_div"), (attend(lens=None), "null"),
+    (attend(scale=1e-39), "normal"), (attend(scale=float("inf")), "normal"),
+    (attend(batch=4096, heads=2048, kv=2048), "too many"),
     (attend(ws=24), "aligned"), (attend(max_seq=0), "max_seq"), (attend(dk=512), "head_dim"),
 ])
 def test_kv4_refusals(call, match):
@@ -88,6 +92,23 @@ def test_logprobs_refusals(call, match):
 def test_logprobs_nothing_to_do():
     N.check(score(rows=0)[0](*score(rows=0)[1:]))
     N.check(grad(rows=0)[0](*grad(rows=0)[1:]))
+
+
+def test_python_refusals():
+    x, y = np.zeros((2, 7), np.float32), np.zeros(2, np.int64)
+    for k in (-1, 65):
+        with pytest.raises(ValueError, match="top_k"):
+            K.token_logprobs(x, y, k)
+    for bits in (8, 16, 0, "4"):
+        with pytest.raises(ValueError, match="kv_bits"):
+            check_kv_bits(bits)
+
+
+def test_models_that_are_not_there():
+    out = C.c_void_p(5)
+    refused(N.lib.nml_cache_create_kv4, None, 1, C.byref(out), match="null")
+    assert not out.value
+    refused(N.lib.nml_model_logprobs, None, P, P, 1, 1, 0, 0, 0, P, P, None, None, match="null")
 
 
 def test_oracle_rounds_to_the_nearest_code():
