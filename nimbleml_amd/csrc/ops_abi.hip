@@ -601,9 +601,9 @@ static int kv4_attention_ok(size_t batch, size_t heads, size_t kv_heads, size_t 
   NML_REQUIRE(kv_heads >= 1 ? heads % kv_heads == 0 : heads == 0,
               "kv4 attention: heads (%zu) must be divisible by kv_heads (%zu)", heads, kv_heads);
   if (batch && heads && seq) {
-    // the kernel numbers pieces of 128 keys in 32 bits, and a launch its threads
+    // the kernel numbers spans of 64 keys in 32 bits, and a launch its threads
     const size_t tiles = (heads / kv_heads * seq + 15) / 16 * kv_heads;
-    NML_REQUIRE(tiles * batch <= 0x7fffffff / ((max_seq + 127) / 128) && tiles * batch <= (size_t)1 << 22,
+    NML_REQUIRE(tiles * batch <= 0x7fffffff / ((max_seq + 63) / 64) && tiles * batch <= (size_t)1 << 22,
                 "kv4 attention: %zu rows × %zu heads × %zu tokens over %zu positions too many", batch, heads, seq,
                 max_seq);
   }

@@ -242,7 +242,7 @@ __global__ __launch_bounds__(kWriters) void kv4_read_kernel(Kv4ReadArgs a, Items
 // A wave goes through tiles of 32 keys on its own: its loads of the next tile are in flight
 // during this one; the running maximum that the exponentials refer to moves only when a score
 // passes it by 2^8 (probabilities are then at most 2^8, all the same to float32), which skips
-// the rescaling of O on nearly every tile. A workgroup's eight waves merge in LDS.
+// the rescaling of O on nearly every tile. A workgroup's waves merge in LDS.
 //
 // A (row, KV head, 16 queries) is one workgroup's unless its keys are many: pieces of a long one
 // go to several, as many in all as the card holds at once, and the last to finish merges them in
@@ -261,19 +261,23 @@ typedef short s8 __attribute__((ext_vector_type(8)));
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
 typedef unsigned u2 __attribute__((ext_vector_type(2)));
 
-constexpr int kWaves = 8;
-constexpr int kThreads = 64 * kWaves;
 constexpr int kKeys = 32;                  // keys of a wave's tile
-constexpr int kSpan = kWaves * kKeys;      // keys of a workgroup's round
 constexpr float kSlack = 8.f;              // in powers of two
 
+// Waves of a workgroup: eight, which share a tile's keys where tiles are few; four where there are
+// at least four times the workgroups of eight that the card holds, so that a short tile pays for
+// fewer waves' startup and merge (16 heads of 64, µs with eight and four: 512 rows of up to 2048 keys
+// 194, 157; 128 rows 54, 46; 128 rows of up to 8192 keys 154, 150; 512 rows of up to 512 keys and 8
+// heads 60, 40; two waves 154, 49, 164, 34). At head dims above 128 LDS has room for eight either way.
+constexpr int few_waves(int nb) { return nb <= 4 ? 4 : 8; }
+constexpr int kManyTiles = 4;
 // Workgroups that the card's 256 CUs hold at once, by registers and LDS.
-__host__ __device__ constexpr int capacity(int nb) { return nb == 1 ? 768 : nb <= 4 ? 512 : 256; }
+__host__ __device__ constexpr int capacity(int nb, int waves) { return (nb == 1 ? 768 : nb <= 4 ? 512 : 256) * 8 / waves; }
 // Spans that a piece has at least: what it costs to begin one and to merge it. (Head dim 64, 32 rows
 // of 128 … 1280 keys: 12 µs at eight, where no row is split, 19 at two. 128, one row of 30 Ki keys
 // with 8 KV heads: 15.6 µs at four, 18.5 at two, 18.9 at eight. 256, 4 rows of up to 8 Ki keys with
 // 4 KV heads: 16.5 at two, 20.8 at four, 27.2 at eight.)
-__host__ __device__ constexpr int least_spans(int nb) { return nb <= 2 ? 8 : nb <= 4 ? 4 : 2; }
+__host__ __device__ constexpr int least_spans(int nb, int waves) { return (nb <= 2 ? 8 : nb <= 4 ? 4 : 2) * 8 / waves; }
 
 // ws: a counter for each tile in pieces (zero before and after every launch, in the same place
 // for calls of any size), then for each piece its rows' maxima and Σ p, then their Σ p·v. Tiles in
@@ -281,7 +285,16 @@ __host__ __device__ constexpr int least_spans(int nb) { return nb <= 2 ? 8 : nb 
 // pieces fewer than twice as many.
 constexpr int kCounters = 2048, kCounterStep = 16;  // a line for each
 
-// Rows of the batch, 64 at a time with one in each lane: cached length and new tokens, in range.
+// Places for pieces: those that the tiles' own workgroups leave on the card (a quarter of it where
+// they leave none: for a row much longer than the others).
+__host__ __device__ inline int room_for(long long tiles, int cap) {
+  const int left = cap - static_cast<int>(tiles < cap ? tiles : cap);
+  return left > cap / 4 ? left : cap / 4;
+}
+
+// Rows of the batch, 64 at a time with one in each lane: cached length and new tokens, in range;
+// SPAN: keys of a workgroup's round.
+template <int SPAN>
 struct Rows {
   int len, n, spans;
   // Spans of the lane's row: at least one (its outputs are to be written), none past the batch.
@@ -289,7 +302,7 @@ struct Rows {
     const int at = min(b, a.B - 1), x = a.lens[at] + a.more, y = a.counts ? a.counts[at] : a.S;
     len = min(max(x, 0), a.P);
     n = min(max(y, 0), a.S);
-    spans = b >= a.B ? 0 : n > 0 ? max(1, (len + kSpan - 1) / kSpan) : 1;
+    spans = b >= a.B ? 0 : n > 0 ? max(1, (len + SPAN - 1) / SPAN) : 1;
     return x == len && y == n;  // (were in range)
   }
 };
@@ -300,11 +313,13 @@ struct Work {
   int b, e, piece, pieces, slot, len, n, spans;
 };
 // More than 64 rows are shared out to the waves, a run of rows each (2048 rows × 8 heads of up to
-// 512 keys of 64: 310 µs, 670 with every wave looking through them all); sums: of the waves.
-__device__ __forceinline__ Work find_work(const Kv4AttnArgs& a, int each, int nb, int lane, int wave, int (*sums)[3]) {
+// 512 keys of 64: 240 µs, of eight waves 310, 670 with every wave looking through them all); sums: of
+// the waves.
+template <int NB, int NW>
+__device__ __forceinline__ Work find_work(const Kv4AttnArgs& a, int each, int lane, int wave, int (*sums)[3]) {
   Work w{};
-  Rows rows;
-  const int run = a.B <= 64 ? 64 : (a.B + 64 * kWaves - 1) / (64 * kWaves) * 64;
+  Rows<NW * kKeys> rows;
+  const int run = a.B <= 64 ? 64 : (a.B + 64 * NW - 1) / (64 * NW) * 64;
   const int first = a.B <= 64 ? 0 : wave * run, end = min(first + run, a.B);
   int total = 0;
   bool good = true;
@@ -320,12 +335,10 @@ __device__ __forceinline__ Work find_work(const Kv4AttnArgs& a, int each, int nb
     __syncthreads();
     total = 0;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) total += sums[i][0];
+    for (int i = 0; i < NW; ++i) total += sums[i][0];
   }
-  // pieces go to the places that the tiles' own workgroups leave (a quarter where they leave none:
-  // for a row much longer than the others)
-  const int cap = capacity(nb), room = max(cap - static_cast<int>(min(static_cast<long long>(each) * a.B, 1LL * cap)), cap / 4);
-  const int least = max(least_spans(nb), static_cast<int>((static_cast<long long>(total) * each + room - 1) / room));
+  const int room = room_for(static_cast<long long>(each) * a.B, capacity(NB, NW));
+  const int least = max(least_spans(NB, NW), static_cast<int>((static_cast<long long>(total) * each + room - 1) / room));
   auto pieces_of = [&](int spans) { return spans <= least ? min(spans, 1) : (spans + least - 1) / least; };
   const int at = static_cast<int>(blockIdx.x / each);
   int before = 0, slots = 0, from = 0;
@@ -343,7 +356,7 @@ __device__ __forceinline__ Work find_work(const Kv4AttnArgs& a, int each, int nb
     if (lane == 63) sums[wave][1] = pieces, sums[wave][2] = split;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i)  // the run that has this workgroup's row
+    for (int i = 0; i < NW; ++i)  // the run that has this workgroup's row
       if (from == i * run && before + sums[i][1] <= at) {
         before += sums[i][1];
         slots += sums[i][2];
@@ -481,21 +494,22 @@ __device__ __forceinline__ f2 get2(const float* p) {
                                                   __HIP_MEMORY_SCOPE_AGENT));
 }
 
-template <typename T, int NB>
-__global__ __launch_bounds__(kThreads, NB == 1 ? 6 : NB <= 4 ? 4 : 2) void kv4_attention_kernel(Kv4AttnArgs a) {
+template <typename T, int NB, int NW>
+__global__ __launch_bounds__(64 * NW, NB == 1 ? 6 : NB <= 4 ? 4 : 2) void kv4_attention_kernel(Kv4AttnArgs a) {
   constexpr int NP = sizeof(T) == 2 ? 2 : 3;
   constexpr int W = Kv4Tile<NB>::W, DT = 2 * NB;  // DT: 16-wide tiles of the head dim
   constexpr int kRow = 64 * NB;                   // bytes of a key's values in LDS
   constexpr int kWaveLds = kKeys * kRow;          // and as many of 16 rows of 32·NB floats
-  constexpr int D = 32 * NB;
-  __shared__ __align__(16) char lds[kWaves * kWaveLds];
+  constexpr int D = 32 * NB, kThreads = 64 * NW, kSpan = NW * kKeys;
+  static_assert(NW >= NB, "a wave lays out a step of Q");
+  __shared__ __align__(16) char lds[NW * kWaveLds];
   __shared__ __align__(16) bf8 qs[NP][NB][64];
-  __shared__ float sm[kWaves][16], sl[kWaves][16];
+  __shared__ float sm[NW][16], sl[NW][16];
   __shared__ unsigned arrived;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
   const int nb = (a.dk + kBlock - 1) / kBlock, R = a.group * a.S, tiles = (R + 15) / 16;
-  const Work work = find_work(a, a.Hkv * tiles, NB, lane, w, reinterpret_cast<int(*)[3]>(lds));
+  const Work work = find_work<NB, NW>(a, a.Hkv * tiles, lane, w, reinterpret_cast<int(*)[3]>(lds));
   if (work.b < 0 || work.n == 0) return;
   const int hk = tiles == 1 ? work.e : work.e / tiles, tile = work.e - hk * tiles;
   const int per = work.pieces == 1 ? work.spans : (work.spans + work.pieces - 1) / work.pieces;
@@ -720,12 +734,12 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 6 : NB <= 4 ? 4 : 2) void kv4_a
     const int c = i / D, d = i % D;
     float mm = sm[0][c];
 #pragma unroll
-    for (int y = 1; y < kWaves; ++y) mm = fmaxf(mm, sm[y][c]);
+    for (int y = 1; y < NW; ++y) mm = fmaxf(mm, sm[y][c]);
     const float rf = mm == -INFINITY ? 0.f : mm;
     float lt = 0.f;
     f2 ot = {0.f, 0.f};
 #pragma unroll
-    for (int y = 0; y < kWaves; ++y) {
+    for (int y = 0; y < NW; ++y) {
       const float f = __builtin_amdgcn_exp2f(sm[y][c] - rf);  // (−inf: 0)
       const f2 p = *reinterpret_cast<const f2*>(lds + y * kWaveLds + 4 * i);
       lt += sl[y][c] * f;
@@ -834,27 +848,37 @@ int read_launch(const Kv4ReadArgs& a, hipStream_t st) {
   return 0;
 }
 
-// Most pieces of one tile, and in all those of tiles in pieces that there can be.
+// Waves of a workgroup; most pieces of one tile, and in all those of tiles in pieces that there
+// can be.
 struct Pieces {
+  int waves;
   long long tiles, most, slots;
 };
 Pieces attention_pieces(int B, int H, int Hkv, int S, int P, int dk) {
   Pieces p;
-  const int nb = (dk + kBlock - 1) / kBlock, spans = (P - 1) / kSpan + 1;
+  const int nb = (dk + kBlock - 1) / kBlock;
   p.tiles = (static_cast<long long>(H / Hkv) * S + 15) / 16 * Hkv * B;
-  p.most = (spans - 1) / least_spans(nb) + 1;
-  p.slots = p.most == 1 ? 0 : std::min(p.tiles * p.most, 2LL * capacity(nb));
+  p.waves = p.tiles >= kManyTiles * capacity(nb, 8) ? few_waves(nb) : 8;
+  const int span = p.waves * kKeys, spans = (P - 1) / span + 1;
+  p.most = (spans - 1) / least_spans(nb, p.waves) + 1;
+  p.slots = p.most == 1 ? 0 : std::min(p.tiles * p.most, 2LL * room_for(p.tiles, capacity(nb, p.waves)));
   return p;
+}
+
+template <typename T, int NB, int NW>
+int attention_launch_nw(const Kv4AttnArgs& a, const Pieces& p, hipStream_t st) {
+  // every tile's workgroup, and those that pieces add
+  kv4_attention_kernel<T, NB, NW><<<static_cast<unsigned>(std::min(p.tiles + p.slots, p.tiles * p.most)), 64 * NW, 0, st>>>(a);
+  NML_LAUNCHED();
+  return 0;
 }
 
 template <typename T, int NB>
 int attention_launch_nb(Kv4AttnArgs a, hipStream_t st) {
   const Pieces p = attention_pieces(a.B, a.H, a.Hkv, a.S, a.P, a.dk);
   a.slots = static_cast<int>(p.slots);
-  // every tile's workgroup, and those that pieces add
-  kv4_attention_kernel<T, NB><<<static_cast<unsigned>(std::min(p.tiles + p.slots, p.tiles * p.most)), kThreads, 0, st>>>(a);
-  NML_LAUNCHED();
-  return 0;
+  if (p.waves == 8) return attention_launch_nw<T, NB, 8>(a, p, st);
+  return attention_launch_nw<T, NB, few_waves(NB)>(a, p, st);
 }
 
 template <typename T>

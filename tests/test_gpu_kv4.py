@@ -433,6 +433,28 @@ def test_many_rows_and_two_long_ones(gpu, rows, dk, long):
         K.kv4_attention(q, c, lens, 8.0)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dk, group, seq", [(32, 1, 1), (64, 2, 3), (128, 1, 1), (256, 1, 1)])
+def test_many_tiles_of_every_length(gpu, dtype, dk, group, seq):
+    """Tiles far more than the card holds at once, one row in pieces; rows picked by length."""
+    r = np.random.RandomState(dk + seq)
+    rows, kv, p = 100, 33, 700
+    lens = r.randint(0, 40, rows)
+    lens[[3, 50, 99]] = 0, p, 300
+    k, v = normal(r, (1, kv, p, dk), dtype), normal(r, (1, kv, p, dk), dtype)
+    q = normal(r, (rows, kv * group, seq, dk), dtype)
+    one, c = cache_of(k, v), K.KV4Cache(rows, kv, p, dk)
+    for i in range(rows):  # every row holds the same keys
+        for a, b in ((one.k_codes, c.k_codes), (one.k_scales, c.k_scales), (one.v_codes, c.v_codes),
+                     (one.v_scales, c.v_scales)):
+            N.check(N.lib.nml_memcpy_d2d(b.ptr + i * a.nbytes, a.ptr, a.nbytes))
+    got = K.kv4_attention(q, c, lens, 8.0).numpy().astype(np.float64)
+    hk, hv = R.held(k), R.held(v)
+    for i in (0, 3, 49, 50, 51, 98, 99):
+        want = R.attention(q[i:i + 1], hk, hv, lens[i:i + 1], None, 8.0)
+        assert np.abs(got[i] - want[0]).max() <= bound(q[i:i + 1], hk, hv, 8.0, dtype), i
+
+
 def test_one_workspace_serves_calls_of_any_size(gpu):
     """Calls of different shapes follow each other on one workspace, zeroed once."""
     r = np.random.RandomState(16)
