@@ -357,6 +357,15 @@ def test_long_rows_in_pieces(gpu, dtype, dk, group, seq):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dk, group, seq", [(64, 1, 40), (128, 3, 7), (32, 2, 17)])
+def test_prompt_pieces_over_long_rows(gpu, dtype, dk, group, seq):
+    """More queries than a tile holds over rows in pieces; rows with fewer tokens than the call, and
+    a row whose first tokens see no key."""
+    check_attention(np.random.RandomState(seq), dtype, dk, 1, group, seq, [2600, 3, 2049, 40],
+                    [seq, min(seq, 9), 1, 0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_pieces_of_very_different_scores(gpu, dtype):
     """One piece holds scores hundreds above the others', one holds a NaN block that the last
     token alone sees."""

@@ -91,6 +91,24 @@ def test_ragged_prompts_and_steps(gpu):
             assert np.abs(a.numpy()[0, -1] - nxt[i][b, -1]).max() <= 1e-3
 
 
+@pytest.mark.parametrize("piece", [2, 16, 17, 25])
+def test_pieces_after_ragged_prompts(gpu, piece):
+    """Several tokens a row from different positions on, attended to in place and read back."""
+    w = make_weights(CFG, seed=15, dtype=np.float32, rich=True)
+    m = model(w, CFG, np.float32)
+    rows = [random_ids((n,), CFG.vocab_size, seed=n) for n in (7, 13, 1, 10)]
+    more = random_ids((4, piece), CFG.vocab_size, seed=98)
+    _, cache = m.prefill_ragged(rows, kv_bits=4)
+    got = m.forward_with_cache(more, cache)[0].numpy()
+    after = m.forward_with_cache(more[:, :1], cache)[0].numpy()
+    for b, row in enumerate(rows):
+        _, c = m.forward_with_cache(row[None], kv_bits=4)
+        want = m.forward_with_cache(more[b:b + 1], c)[0].numpy()
+        assert np.abs(want[0] - got[b]).max() <= 1e-3
+        want = m.forward_with_cache(more[b:b + 1, :1], c)[0].numpy()
+        assert np.abs(want[0] - after[b]).max() <= 1e-3
+
+
 @pytest.mark.parametrize("dtype", [np.float32, np.float16])
 @pytest.mark.parametrize("batch, graph", [(1, True), (3, False), (16, True)])
 def test_generate_is_the_argmax_of_cached_forwards(gpu, dtype, batch, graph):
