@@ -243,6 +243,10 @@ struct Kv4AttnArgs {
   int B, H, Hkv, S, P, dk;
   int group;    // H / Hkv
   int slots;    // set by the launch
+  // One new token a row (S = 1), at the row's last position of these (strides in elements, dk a
+  // position), not in the cache yet: the call writes it there. Null: it is.
+  const void *new_k, *new_v;
+  long long new_b, new_h;
   int more;     // keys of a row beyond lens[b]: lens may hold the position of the first new token
   float scale;  // divisor of the scores
   void* ws;

@@ -214,7 +214,10 @@ int kv4_append(nml_model* m, const KVView& c, int B, int S, const int32_t* pos, 
 }
 
 // Attention of the S newest tokens of B rows over a cache in 4 bits; the first of them is at pos.
-int kv4_attend(nml_model* m, const KVView& c, const void* q, void* out, int B, int S, const int32_t* pos, hipStream_t st) {
+// append: a single token, which goes from c.k and c.v into the cache on the way (saves the launch
+// of kv4_append).
+int kv4_attend(nml_model* m, const KVView& c, const void* q, void* out, int B, int S, const int32_t* pos, bool append,
+               hipStream_t st) {
   Kv4AttnArgs a{};
   a.q = q;
   a.k_codes = c.k_codes;
@@ -232,6 +235,12 @@ int kv4_attend(nml_model* m, const KVView& c, const void* q, void* out, int B, i
   a.dk = m->dk;
   a.scale = sqrtf((float)m->dk);
   a.ws = c.ws4;
+  if (append) {
+    a.new_k = c.k;
+    a.new_v = c.v;
+    a.new_b = c.sb;
+    a.new_h = c.sh;
+  }
   return launch_kv4_attention(m->dt, a, st);
 }
 
@@ -314,7 +323,7 @@ int attention_sublayer(nml_model* m, const Layer& w, const void* xin, const Acts
     at.row_start = rg->row_start;
   }
   if (c.k_codes && !rg && S <= kKv4Tokens)
-    NML_TRY(kv4_attend(m, c, a.q, a.att, B, S, pos_base, st));
+    NML_TRY(kv4_attend(m, c, a.q, a.att, B, S, pos_base, false, st));
   else
     NML_TRY(launch_attention_prefill(m->dt, at, st));
   LinearArgs wo{};
@@ -458,8 +467,7 @@ int decode_step(nml_model* m, nml_cache* c, const Acts& a, int b0, int Bn, const
     at.dk = m->dk;
     at.scale = sqrtf((float)m->dk);
     if (view.k_codes) {
-      NML_TRY(kv4_append(m, view, B, 1, pos, nullptr, st));
-      NML_TRY(kv4_attend(m, view, a.q, a.att, B, 1, pos, st));
+      NML_TRY(kv4_attend(m, view, a.q, a.att, B, 1, pos, true, st));
     } else {
       NML_TRY(launch_attention_decode(m->dt, at, pos, max_len, a.part, st));
     }

@@ -116,6 +116,31 @@ __device__ __forceinline__ void load8(const T* __restrict__ p, int d0, int dk, f
   }
 }
 
+// Codes and scale byte of a block that four lanes hold, eight values each (the lane's codes).
+template <typename T>
+__device__ __forceinline__ unsigned encode8(const float* x, unsigned& scale) {
+  // max|x| on the bits: infinity and NaN are the largest
+  unsigned top = 0, codes = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const unsigned w = __builtin_bit_cast(unsigned, x[i]) & 0x7fffffffu;
+    top = top > w ? top : w;
+  }
+  top = quad_umax(top);
+  scale = kScaleNaN;
+  if (top < 0x7f800000u) {
+    const int e = block_exponent(top, top_exponent<T>());
+    scale = static_cast<unsigned>(e + 127);
+    const float s = scale_value(scale);
+    // to the nearest code, ties to the even one, saturated at 6
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], s, 0);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], s, 1);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], s, 2);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], s, 3);
+  }
+  return codes;
+}
+
 template <typename T, bool VEC>
 __global__ __launch_bounds__(kWriters) void kv4_write_kernel(Kv4WriteArgs a, Items n) {
   const int b = blockIdx.y;
@@ -144,25 +169,8 @@ __global__ __launch_bounds__(kWriters) void kv4_write_kernel(Kv4WriteArgs a, Ite
 #pragma unroll
   for (int u = 0; u < kEach; ++u) {
     if (!here[u]) continue;
-    // max|x| on the bits: infinity and NaN are the largest
-    unsigned top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const unsigned w = __builtin_bit_cast(unsigned, x[u][i]) & 0x7fffffffu;
-      top = top > w ? top : w;
-    }
-    top = quad_umax(top);
-    unsigned codes = 0, scale = kScaleNaN;
-    if (top < 0x7f800000u) {
-      const int e = block_exponent(top, top_exponent<T>());
-      scale = static_cast<unsigned>(e + 127);
-      const float s = scale_value(scale);
-      // to the nearest code, ties to the even one, saturated at 6
-      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[u][0], x[u][1], s, 0);
-      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[u][2], x[u][3], s, 1);
-      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[u][4], x[u][5], s, 2);
-      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[u][6], x[u][7], s, 3);
-    }
+    unsigned scale;
+    const unsigned codes = encode8<T>(x[u], scale);
     *reinterpret_cast<unsigned*>((is_v ? a.v_codes : a.k_codes) + at[u] * kBlockBytes + part * 4) = codes;
     if (part == 0) (is_v ? a.v_scales : a.k_scales)[at[u]] = static_cast<uint8_t>(scale);
   }
@@ -494,7 +502,9 @@ __device__ __forceinline__ f2 get2(const float* p) {
                                                   __HIP_MEMORY_SCOPE_AGENT));
 }
 
-template <typename T, int NB, int NW>
+// ADD: the row's last key and value come from a.new_k and a.new_v and are not in the cache yet. (Of
+// its own: the calls without it take 2 % longer beside that code, 4 % on long rows.)
+template <typename T, int NB, int NW, bool ADD>
 __global__ __launch_bounds__(64 * NW, NB == 1 ? 6 : NB <= 4 ? 4 : 2) void kv4_attention_kernel(Kv4AttnArgs a) {
   constexpr int NP = sizeof(T) == 2 ? 2 : 3;
   constexpr int W = Kv4Tile<NB>::W, DT = 2 * NB;  // DT: 16-wide tiles of the head dim
@@ -505,6 +515,8 @@ __global__ __launch_bounds__(64 * NW, NB == 1 ? 6 : NB <= 4 ? 4 : 2) void kv4_at
   __shared__ __align__(16) char lds[NW * kWaveLds];
   __shared__ __align__(16) bf8 qs[NP][NB][64];
   __shared__ float sm[NW][16], sl[NW][16];
+  __shared__ __align__(16) unsigned new_codes[2][ADD ? 8 : 1][4];  // of the row's last key and value
+  __shared__ uint8_t new_scales[2][ADD ? 8 : 1];
   __shared__ unsigned arrived;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
@@ -539,6 +551,19 @@ __global__ __launch_bounds__(64 * NW, NB == 1 ? 6 : NB <= 4 ? 4 : 2) void kv4_at
     }
   }
 
+  // A step's own key and value, not in the cache yet: the last wave of the workgroup that has that
+  // key codes them, writes them there and leaves them in LDS for the tile that holds them.
+  const bool adds = ADD && k0 < k1 && k1 == work.len;
+  const int at_v = lane >> 5, at_blk = (lane & 31) >> 2, at_part = lane & 3;
+  float fresh[8];
+  if (adds && w == NW - 1) {
+    const T* p = static_cast<const T*>(at_v ? a.new_v : a.new_k) + work.b * a.new_b + hk * a.new_h +
+                 static_cast<long long>(work.len - 1) * a.dk;
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(a.new_k) | reinterpret_cast<uintptr_t>(a.new_v);
+    if ((bits & 15) == 0 && ((a.dk | a.new_b | a.new_h) & 7) == 0) load8<T, true>(p, 32 * at_blk + 8 * at_part, a.dk, fresh);
+    else load8<T, false>(p, 32 * at_blk + 8 * at_part, a.dk, fresh);
+  }
+
   const size_t base = (static_cast<size_t>(work.b) * a.Hkv + hk) * a.P * nb;
   const uint8_t* kc = a.k_codes + base * kBlockBytes;
   const uint8_t* ks = a.k_scales + base;
@@ -568,6 +593,32 @@ __global__ __launch_bounds__(64 * NW, NB == 1 ? 6 : NB <= 4 ? 4 : 2) void kv4_at
 #pragma unroll
     for (int p = 0; p < NP; ++p) qs[p][w][lane] = q[p];
   }
+  if (adds && w == NW - 1) {
+    unsigned scale_byte;
+    const unsigned codes = encode8<T>(fresh, scale_byte);
+    new_codes[at_v][at_blk][at_part] = codes;
+    if (at_part == 0) new_scales[at_v][at_blk] = static_cast<uint8_t>(scale_byte);
+    if (at_blk < nb) {
+      const size_t to = static_cast<size_t>(work.len - 1) * nb + at_blk;
+      *reinterpret_cast<unsigned*>(const_cast<uint8_t*>((at_v ? vc : kc) + to * kBlockBytes + at_part * 4)) = codes;
+      if (at_part == 0) const_cast<uint8_t*>(at_v ? vs : ks)[to] = static_cast<uint8_t>(scale_byte);
+    }
+  }
+  // that key (and those past it, which repeat it) in a tile from `at` on
+  auto take_new = [&](Kv4Tile<NB>& t, int which, int at) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (at + 16 * h + col >= work.len - 1) {
+#pragma unroll
+        for (int y = 0; y < W; ++y) {
+          const int blk = min(g * NB / 4 + y, nb - 1);
+          t.e[h][y] = new_scales[which][blk];
+#pragma unroll
+          for (int i = 0; i < NB / W; ++i)
+            t.c[h][y * (NB / W) + i] = new_codes[which][blk][NB >= 4 ? i : NB == 2 ? (g & 1) * 2 + i : g];
+        }
+      }
+  };
   int least = lim;
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) least = min(least, __shfl_xor(least, o, 64));
@@ -582,6 +633,10 @@ __global__ __launch_bounds__(64 * NW, NB == 1 ? 6 : NB <= 4 ? 4 : 2) void kv4_at
   __syncthreads();
 
   for (; j < k1; j += kSpan) {
+    if (adds && j + kKeys >= work.len) {
+      take_new(k, 0, j);
+      take_new(v, 1, j);
+    }
     unsigned worst = 0;
 #pragma unroll
     for (int i = 0; i < W; ++i) worst = max(worst, max<unsigned>(k.e[0][i], k.e[1][i]));
@@ -868,7 +923,9 @@ Pieces attention_pieces(int B, int H, int Hkv, int S, int P, int dk) {
 template <typename T, int NB, int NW>
 int attention_launch_nw(const Kv4AttnArgs& a, const Pieces& p, hipStream_t st) {
   // every tile's workgroup, and those that pieces add
-  kv4_attention_kernel<T, NB, NW><<<static_cast<unsigned>(std::min(p.tiles + p.slots, p.tiles * p.most)), 64 * NW, 0, st>>>(a);
+  const unsigned grid = static_cast<unsigned>(std::min(p.tiles + p.slots, p.tiles * p.most));
+  if (a.new_k) kv4_attention_kernel<T, NB, NW, true><<<grid, 64 * NW, 0, st>>>(a);
+  else kv4_attention_kernel<T, NB, NW, false><<<grid, 64 * NW, 0, st>>>(a);
   NML_LAUNCHED();
   return 0;
 }

@@ -239,3 +239,32 @@ def test_no_gradient_under_no_grad(gpu):
     with nm.no_grad():
         out = nm.token_log_probs(m.forward(ids), ids)
     assert not out.requires_grad and out._backward is None
+
+
+def test_a_piece_reads_back_what_steps_wrote(gpu):
+    """Fourteen single tokens and the other nineteen at once, as the whole at once."""
+    m = model(make_weights(CFG, seed=11, dtype=np.float32, rich=True), CFG, np.float32)
+    ids = random_ids((2, 33), CFG.vocab_size, seed=22)
+    want = m.forward_with_cache(ids, kv_bits=4)[0].numpy()
+    cache = None
+    for t in range(14):
+        _, cache = m.forward_with_cache(ids[:, t:t + 1], cache, kv_bits=4)
+    assert np.abs(m.forward_with_cache(ids[:, 14:], cache)[0].numpy() - want[:, 14:]).max() <= 1e-3
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("d, heads", [(64, 2), (64, 1), (160, 2), (128, 1), (256, 1)])
+def test_steps_over_long_rows(gpu, dtype, d, heads):
+    """Two single tokens after prompts that end at a tile's, a wave's and a piece's edge, as both in
+    one call: the step's own key is the last of a tile, the first of one, of a piece."""
+    cfg = GPTConfig(96, d, 1, heads, 4700)
+    m = model(make_weights(cfg, seed=16, dtype=dtype, rich=True), cfg, dtype)
+    tol = 1e-3 if dtype == np.float32 else 3e-2
+    for n in (1, 31, 32, 255, 256, 2047, 2048, 4096, 4510, 4607):
+        ids = random_ids((3, n + 2), cfg.vocab_size, seed=n)
+        _, a = m.forward_with_cache(ids[:, :n], kv_bits=4)
+        want = m.forward_with_cache(ids[:, n:], a)[0].numpy().astype(np.float64)
+        _, b = m.forward_with_cache(ids[:, :n], kv_bits=4)
+        for t in range(2):
+            got = m.forward_with_cache(ids[:, n + t:n + t + 1], b)[0].numpy().astype(np.float64)
+            assert np.abs(got[:, 0] - want[:, t]).max() <= tol, (n, t)
