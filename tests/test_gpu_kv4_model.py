@@ -268,3 +268,24 @@ def test_steps_over_long_rows(gpu, dtype, d, heads):
         for t in range(2):
             got = m.forward_with_cache(ids[:, n + t:n + t + 1], b)[0].numpy().astype(np.float64)
             assert np.abs(got[:, 0] - want[:, t]).max() <= tol, (n, t)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_scoring_and_decoding_between_a_loss_and_its_backward(gpu, dtype):
+    """Neither touches what the loss keeps for its backward: the gradients are bit for bit those
+    without them (the training path sums in a fixed order)."""
+    cfg = GPTConfig(96, 48, 3, 2, 40)
+    w = make_weights(cfg, seed=17, dtype=dtype, rich=True)
+    ids, lab = (random_ids((2, 12), cfg.vocab_size, seed=s) for s in (3, 4))
+    grads = []
+    for between in (False, True):
+        m = model(w, cfg, dtype)
+        loss = m.compute_loss(ids, lab)
+        if between:
+            other = random_ids((3, 30), cfg.vocab_size, seed=5)
+            m.log_probs(other, other, top_k=3)
+            nm.generate(m, other, max_new_tokens=4, temperature=0.0, kv_bits=4)
+        loss.backward()
+        grads.append({n: np.asarray(p.grad) for n, p in nm.named_parameters(m)})
+    for name in grads[0]:
+        assert np.array_equal(grads[0][name], grads[1][name]), name
