@@ -107,18 +107,20 @@ class Tensor:
     def backward(self, grad=None, retain_graph=False):
         """tensor.py:286-332: add ``grad`` (default 1 for a scalar) to this tensor's ``grad``,
         then run every ``_backward`` closure of the graph below it, each after all the
-        closures of the tensors computed from it. Unless ``retain_graph``, the closures and
-        edges are released afterwards."""
+        closures of the tensors computed from it. ``grad`` is taken in the dtype that this
+        tensor keeps its gradient in (the compute dtype or its ``_grad_dtype``). Unless
+        ``retain_graph``, the closures and edges are released afterwards."""
+        gdt = getattr(self, "_grad_dtype", None) or np_backend.dtype
         if grad is None:
             if self.size != 1:
                 raise ValueError("grad must be specified for non-scalar tensors.")
-            grad = np.array([1.0], dtype=np_backend.dtype)
+            grad = np.array([1.0], dtype=gdt)
         elif isinstance(grad, (int, float)):
-            grad = np.array([float(grad)], dtype=np_backend.dtype)
+            grad = np.array([float(grad)], dtype=gdt)
         elif isinstance(grad, Tensor):
             grad = np.asarray(grad.data)
         else:
-            grad = np.asarray(grad, dtype=np_backend.dtype)
+            grad = np.asarray(grad, dtype=gdt)
         self._accumulate_grad(grad)
         topo = _backward_order(self)
         for node in reversed(topo):
