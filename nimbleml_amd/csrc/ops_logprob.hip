@@ -31,9 +31,10 @@ constexpr int kCandidates = 1024;
 
 __device__ __forceinline__ float exp_of(float t) { return __builtin_amdgcn_exp2f(t * 1.44269504088896341f); }
 
-// Order of logits as unsigned words: NaN above everything, −0 equal to +0.
+// Order of logits as unsigned words: NaN above everything (by one word below the largest, which with
+// id 0 would be the bound that the first of the rounds starts under), −0 equal to +0.
 __device__ __forceinline__ unsigned order_of(float x) {
-  if (x != x) return 0xffffffffu;
+  if (x != x) return 0xfffffffeu;
   const unsigned u = __builtin_bit_cast(unsigned, x + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
@@ -327,7 +328,8 @@ __global__ __launch_bounds__(NT) void logprob_kernel(LogprobArgs a) {
     }
     return;
   }
-  // Many equal logits (masked vocabularies) or NaN: the next one in order, top_k times.
+  // Many equal logits (masked vocabularies) or NaN: the next one in order, top_k times (every key is
+  // below the first bound).
   unsigned long long last = ~0ull;
   for (int t = 0; t < a.top_k; ++t) {
     unsigned long long best = 0;
