@@ -623,7 +623,8 @@ __global__ __launch_bounds__(64 * NW, NB == 1 ? 6 : NB <= 4 ? 4 : 2) void kv4_at
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) least = min(least, __shfl_xor(least, o, 64));
   const float scale = 1.44269504088896341f / a.scale;  // scores in powers of two
-  const float slack = kSlack * 0.69314718055994531f * a.scale;
+  // (finite, or −inf + slack would be NaN and the maximum never move: past 6·10^37 of a.scale)
+  const float slack = fminf(kSlack * 0.69314718055994531f * a.scale, 3.402823466e38f);
   floatx4 o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = floatx4{0.f, 0.f, 0.f, 0.f};
