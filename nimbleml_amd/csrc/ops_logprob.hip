@@ -403,9 +403,9 @@ int logprobs_launch(const LogprobArgs& a, hipStream_t st) {
   constexpr int E = RowPieces<T>::E;
   const int pieces = (a.V + 2 * (E - 1)) / E;  // at most, wherever a row starts
 #define NML_LOGPROB(NT, NCH) logprob_kernel<T, NT, NCH><<<b.rows, NT, 0, st>>>(b)
-  for (int r0 = 0; r0 < a.rows; r0 += kLaunchRows) {
+  for (long long r0 = 0; r0 < a.rows; r0 += kLaunchRows) {  // (r0 passes the largest int)
     LogprobArgs b = a;
-    b.rows = a.rows - r0 < kLaunchRows ? a.rows - r0 : kLaunchRows;
+    b.rows = static_cast<int>(a.rows - r0 < kLaunchRows ? a.rows - r0 : kLaunchRows);
     b.logits = static_cast<const T*>(a.logits) + static_cast<size_t>(r0) * a.ld;
     if (a.targets) b.targets = a.targets + r0;
     if (a.logp) b.logp = a.logp + r0;
@@ -433,9 +433,9 @@ template <typename T>
 int logprobs_bwd_launch(const LogprobBwdArgs& a, hipStream_t st) {
   constexpr int E = RowPieces<T>::E;
   const int pieces = (a.V + 2 * (E - 1)) / E;
-  for (int r0 = 0; r0 < a.rows; r0 += 65535) {  // rows of one launch
+  for (long long r0 = 0; r0 < a.rows; r0 += 65535) {  // rows of one launch (r0 passes the largest int)
     LogprobBwdArgs b = a;
-    b.rows = a.rows - r0 < 65535 ? a.rows - r0 : 65535;
+    b.rows = static_cast<int>(a.rows - r0 < 65535 ? a.rows - r0 : 65535);
     b.logits = static_cast<const T*>(a.logits) + static_cast<size_t>(r0) * a.ld;
     b.dlogits = static_cast<T*>(a.dlogits) + static_cast<size_t>(r0) * a.ld_d;
     b.targets = a.targets + r0;
