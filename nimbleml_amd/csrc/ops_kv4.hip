@@ -271,6 +271,9 @@ typedef unsigned u2 __attribute__((ext_vector_type(2)));
 
 constexpr int kKeys = 32;                  // keys of a wave's tile
 constexpr float kSlack = 8.f;              // in powers of two
+// Scale bytes (2^65 and up) of values whose Σ p·v could pass float32's range (2^30 keys, p up to
+// 2^kSlack). Looked for in float32 calls only: a float16 output holds no such values.
+constexpr unsigned kLargeScale = 192;
 
 // Waves of a workgroup: eight, which share a tile's keys where tiles are few; four where there are
 // at least four times the workgroups of eight that the card holds, so that a short tile pays for
@@ -511,6 +514,7 @@ __global__ __launch_bounds__(64 * NW, NB == 1 ? 6 : NB <= 4 ? 4 : 2) void kv4_at
   constexpr int kRow = 64 * NB;                   // bytes of a key's values in LDS
   constexpr int kWaveLds = kKeys * kRow;          // and as many of 16 rows of 32·NB floats
   constexpr int D = 32 * NB, kThreads = 64 * NW, kSpan = NW * kKeys;
+  constexpr unsigned kLarge = NP == 3 ? kLargeScale : kScaleNaN;
   static_assert(NW >= NB, "a wave lays out a step of Q");
   __shared__ __align__(16) char lds[NW * kWaveLds];
   __shared__ __align__(16) bf8 qs[NP][NB][64];
@@ -628,7 +632,8 @@ __global__ __launch_bounds__(64 * NW, NB == 1 ? 6 : NB <= 4 ? 4 : 2) void kv4_at
   floatx4 o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = floatx4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, ref = 0.f, l = 0.f;  // m: of q·k; ref: m·scale, finite; l: of this lane's keys
+  float m = -INFINITY, ref = 0.f, l = 0.f;  // m: of q·k; ref: m·scale + lift, finite; l: of this lane's keys
+  int lift = 0;                             // above 0 once a large value of V has come by
   unsigned nan_blocks = 0;                  // blocks of the output that a NaN block of V reached
   char* mine = lds + w * kWaveLds;
   __syncthreads();
@@ -678,7 +683,7 @@ __global__ __launch_bounds__(64 * NW, NB == 1 ? 6 : NB <= 4 ? 4 : 2) void kv4_at
     worst = 0;
 #pragma unroll
     for (int i = 0; i < W; ++i) worst = max(worst, max<unsigned>(v.e[0][i], v.e[1][i]));
-    if (__ballot(worst == kScaleNaN)) {
+    if (__ballot(worst >= kLarge)) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         unsigned of[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -688,6 +693,20 @@ __global__ __launch_bounds__(64 * NW, NB == 1 ? 6 : NB <= 4 ? 4 : 2) void kv4_at
 #pragma unroll
         for (int i = 0; i < NB; ++i)
           if (of[i] & vis) nan_blocks |= 1u << i;
+      }
+      if constexpr (kLarge < kScaleNaN) {
+        worst = 0;
+#pragma unroll
+        for (int i = 0; i < W; ++i) worst = max(worst, max<unsigned>(v.e[0][i], v.e[1][i]));
+        if (lift == 0 && __ballot(worst >= kLarge)) {
+          // p from here on 2^-lift of what it was: Σ p·v of all the row's keys stays in range
+          lift = static_cast<int>(kSlack) + 32 - __builtin_clz(work.len);
+          ref += static_cast<float>(lift);
+          const float f = __builtin_amdgcn_exp2f(-static_cast<float>(lift));
+          l *= f;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[d] *= f;
+        }
       }
     }
     // V to LDS, a key a row
@@ -716,7 +735,7 @@ __global__ __launch_bounds__(64 * NW, NB == 1 ? 6 : NB <= 4 ? 4 : 2) void kv4_at
     if (__ballot(top > m + slack)) {
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float mn = fmaxf(m, top), rn = mn == -INFINITY ? 0.f : mn * scale;
+      const float mn = fmaxf(m, top), rn = mn == -INFINITY ? 0.f : mn * scale + static_cast<float>(lift);
       const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - rn);
       m = mn;
       ref = rn;
