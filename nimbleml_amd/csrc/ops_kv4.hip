@@ -457,7 +457,8 @@ __device__ __forceinline__ bf8 convert8(unsigned c, float s) {
   return bf8{a.x, a.y, b.x, b.y, d.x, d.y, e.x, e.y};
 }
 
-// As scale_value, of a byte that the write made (never 0; zeroed memory holds codes of 0 only).
+// As scale_value (the conversions to bf16 take the exponent's bits alone: a byte of 0 is 2^-127 here
+// too).
 __device__ __forceinline__ float tile_scale(unsigned e) { return __builtin_bit_cast(float, e << 23); }
 
 // Keys of a 16-key subtile (bit i: key i) that hold a NaN block, from the lanes' scales; the
