@@ -164,7 +164,7 @@ int nml_decode_attention_device(const void* q, const void* kcache, const void* v
 
 /* ---- a KV cache in 4 bits ----
  * No reference counterpart (its generate() keeps no cache, models/generate.py:101-103): the
- * cache of nml_decode_attention_device at 4.25 bits a value. A head's vector of dk values is cut
+ * cache of nml_decode_attention_device at 17 bytes for 32 values. A head's vector of dk values is cut
  * into nb = ⌈dk/32⌉ blocks of 32 (the last padded with zeros); a block is 32 E2M1 codes (0, ½,
  * 1, 1½, 2, 3, 4, 6 and sign; code i in half i % 2 of byte i / 2, the low half first) and a
  * scale byte e for 2^(e − 127), 255 for NaN. With 2^k ≤ max|x| < 2^(k+1) a block's scale is
@@ -199,6 +199,8 @@ int nml_kv4_read_device(const uint8_t* k_codes, const uint8_t* k_scales, const u
  *   s_j = (q·k_j) / scale_div, softmax, Σ_j p_j·v_j     (scores and sums in float32)
  * with the cache's values exactly; a token that sees no key (a length below the count) gives
  * zeros. A NaN block reaches only the tokens that see its key. seq = 1 is a decode step.
+ * scale_div: positive and normal. float32 queries above 3.38e38 in magnitude count as infinite,
+ * and of those below 2^-110 only multiples of 2^-133 are seen.
  *   q: (batch, heads, seq, dk); out: (batch, seq, heads·dk), rows from counts[b] on left as
  *   they were; query head h reads KV head h / (heads / kv_heads)
  *   ws: nml_kv4_attention_workspace bytes, 16-byte aligned, zeroed once before its first use;
@@ -458,9 +460,11 @@ int nml_model_adamw_update(nml_model* m, int kind, int layer, size_t offset, siz
  * The seam generate() probes for (models/generate.py:93-100). */
 int nml_cache_create(nml_model* m, size_t batch, nml_cache** out);
 /* The same cache in 4 bits (blocks of 32 E2M1 codes and a scale, as nml_kv4_write_device makes
- * them): 3.76 times fewer bytes than float16's. Every call that takes a cache takes it; attention
- * sees the values that the cache holds, the new tokens' own among them, whether they come one by
- * one or as a prompt. Beside the codes it holds one layer's K and V in the compute dtype. */
+ * them): 17·⌈dk/32⌉ bytes a vector where float16 takes 2·dk, 3.76 times fewer at head dims that are
+ * multiples of 32, 2.35 at 40, 1.88 at 16, more bytes below 9; beside them one layer's K and V in
+ * the compute dtype, so a model of one layer has nothing to gain. Every call that takes a cache
+ * takes it; attention sees the values that the cache holds, the new tokens' own among them, whether
+ * they come one by one or as a prompt. */
 int nml_cache_create_kv4(nml_model* m, size_t batch, nml_cache** out);
 int nml_cache_destroy(nml_cache* c);
 /* The length of row 0 (rows prefilled with nml_model_prefill_ragged may differ). */

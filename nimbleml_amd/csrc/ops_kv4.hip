@@ -2,9 +2,9 @@
 //
 // Format (one head's vector of dk values, ⌈dk/32⌉ blocks of 32, the last padded with zeros):
 // 32 E2M1 codes (0 ½ 1 1½ 2 3 4 6 with a sign; the first of two in a byte's low half) and one
-// scale byte e that stands for 2^(e − 127), 255 for NaN: 17 bytes a block, 4.25 bits a value,
-// 3.76 times fewer bytes than fp16. gfx950 converts two codes to two values, scale included, in
-// one instruction, and rounds two values to two codes in another.
+// scale byte e that stands for 2^(e − 127), 255 for NaN: 17 bytes a block, 4.25 bits a value and
+// 3.76 times fewer bytes than fp16 where dk is a multiple of 32. gfx950 converts two codes to two
+// values, scale included, in one instruction, and rounds two values to two codes in another.
 //
 // With 2^k ≤ max|x| < 2^(k+1) the scale is 2^(k−2), or 2^(k−1) where max|x| ≥ 1.75·2^k: there
 // saturating the largest value at 6 would cost more than the coarser step (signal to error on
@@ -243,9 +243,9 @@ __global__ __launch_bounds__(kWriters) void kv4_read_kernel(Kv4ReadArgs a, Items
 // loaded and has its operand, no LDS), O = Vᵀ·Pᵀ takes the probabilities from the lanes where S
 // left them, with the keys of the contraction in that order. V passes through LDS for the
 // transpose of its read; Q is split and laid out in LDS once a workgroup. The codes' values are
-// exact in bf16, a query is split in two (float16) or three (float32) bf16 parts without loss and
-// a probability into as many, so every product is exact and scores, statistics and outputs are
-// float32 sums.
+// exact in bf16 and a query is split in two (float16) or three (float32) bf16 parts without loss, so
+// scores are float32 sums of exact products. A float32 probability enters the product with V as as
+// many parts: 24 bits in float32, 17 in float16, whose output has 11; Σ p is of the whole ones.
 //
 // A wave goes through tiles of 32 keys on its own: its loads of the next tile are in flight
 // during this one; the running maximum that the exponentials refer to moves only when a score
@@ -256,9 +256,9 @@ __global__ __launch_bounds__(kWriters) void kv4_read_kernel(Kv4ReadArgs a, Items
 // go to several, as many in all as the card holds at once, and the last to finish merges them in
 // their order.
 //
-// What bounds it: 8 rows of 8 Ki … 32 Ki keys, 8 KV heads of 128 with four query heads each, 39 µs,
-// 4.6 TB/s of memory. 32 rows of 128 … 1280 keys, 16 heads of 64, 12 µs: 2 TB/s, the latency of a
-// workgroup's few rounds. One row of 1023 keys 8 µs: 2.7 until the first tile is there and Q laid
+// What bounds it: 8 rows of 8 Ki … 32 Ki keys, 8 KV heads of 128 with four query heads each, 38–45 µs
+// from card to card, 4.0–4.7 TB/s of memory. 32 rows of 128 … 1280 keys, 16 heads of 64, 12 µs: 2 TB/s,
+// the latency of a workgroup's few rounds. One row of 1023 keys 8 µs: 2.7 until the first tile is there and Q laid
 // out, 0.8 a round, 1.8 for the merge and the store.
 
 typedef float f2 __attribute__((ext_vector_type(2)));

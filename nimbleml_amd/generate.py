@@ -14,8 +14,12 @@ order on the device, so a seeded run gives the reference's tokens. With ``eos_id
 the reference stops drawing at the eos step; the global generator is then rewound
 to the state those fewer draws leave, so later draws of the caller agree too.
 
-``kv_bits=4`` holds the KV cache in 4 bits (blocks of 32 values, a power-of-two scale): a long
-context's attention reads 3.76 times fewer bytes than float16's, and sees the rounded values.
+``kv_bits=4`` holds the KV cache in 4 bits (blocks of 32 values, a power-of-two scale): attention
+sees the rounded values and reads 17·⌈dk/32⌉ bytes a vector of dk where float16 has 2·dk (3.76 times
+fewer where dk is a multiple of 32). It pays where the cache's bytes bound a step: batches, long
+contexts. A batch of one leaves the one-kernel decode step that models of d 1024, head dim 64 and up
+to 2048 positions have, and takes the batched step (24 layers, float16: 0.86 ms a step in place of
+0.37 at 1000 keys, 1.03 and 1.00 at 8000 where neither cache has that kernel, 1.06 and 1.87 at 32000).
 
 Ragged batches: ``input_ids`` may be a list of rows of different lengths; each
 row then generates as if run alone (the result is a list of arrays).

@@ -21,7 +21,10 @@ def token_log_probs(logits, targets, *, ignore_index=None):
 
     With gradients wanted, ``backward(grad)`` with ``grad`` of that shape adds the gradient of
     Σ grad·output to ``logits.grad`` (in the logits' dtype: float16 ones want the loss scaled, as
-    ``compute_loss`` does) and goes on through the graph that made the logits."""
+    ``compute_loss`` does; ``grad`` itself is taken in float32) and goes on through the graph that
+    made the logits. Logits of any vocabulary are scored and differentiated; the backward of a model
+    (``GPT.forward``'s, as ``compute_loss``'s) takes vocabularies that are a multiple of 4 and raises
+    for others."""
     rows = logits.shape[:-1]
     x = logits.data if isinstance(logits.data, N.DeviceArray) else \
         N.DeviceArray.from_host(np.asarray(logits.data))
