@@ -5,7 +5,8 @@
 //   d logits = dlogp·([v = target] − p) − dentropy·p·(log p + entropy)
 // m and Z go from the forward to the gradient apart (m + log Z in one float32 would lose log Z
 // beside a large m, as of a row at the type's lowest value). Sums and statistics are float32 for
-// either dtype. A logit of −inf has probability 0 and adds nothing; a row of nothing else has no distribution: logp and entropy are NaN, as log_softmax's.
+// either dtype. A logit of −inf has probability 0 and adds nothing; a row of nothing else has no
+// distribution: logp and entropy are NaN, as log_softmax's.
 //
 // A workgroup takes a row and goes over it once: each thread keeps Σ exp(t) and Σ exp(t)·t of its
 // logits relative to a reference of its own, which moves only when a logit passes it by 8 (so the
