@@ -272,6 +272,101 @@ int nml_token_logprobs_backward_device(const void* logits, size_t ld, const int6
                                        size_t vocab, int64_t ignore_index, int has_ignore, void* dlogits,
                                        size_t ld_d, int* err, int dtype);
 
+/* Distillation from a teacher's top logits, with no reference kernel: the counterpart, row by row, of
+ * losses/cross_entropy.py:109-192 for a target that is a distribution.
+ * logits: (rows, vocab) at a row stride of ld elements (dtype); top_ids int64, top_logits float32:
+ * (rows, top_k), the teacher's logits (or log probabilities: any offset a row) of the tokens it is
+ * known of, in any order; 1 ≤ top_k ≤ 256.
+ *   q_k = exp(y_k/T) / Σ_j exp(y_j/T) over a row's entries, p = softmax(x/T) over the vocabulary
+ *   loss = Σ_k q_k·(log q_k − log p[id_k])     (KL(q || p): p's tokens outside the entries have q = 0)
+ *   m = max_v x_v, l = Σ_v exp((x_v − m)/T)
+ * T = temperature, in [1e-6, 1e6]; the loss is not multiplied by T². Outputs are float32 (rows); m, l
+ * may each be NULL. An entry of id −1 or logit −inf is absent; a row without any other has no teacher:
+ * its logits are not read and it gives zeros. The same id twice counts twice. A probability of 0 where
+ * q is not: +inf. An id outside [−1, vocab) makes its row NaN and sets bit 0 of *err (device int, may be
+ * NULL; the caller clears it); a NaN or +inf among a row's entries or logits makes it NaN, as does a
+ * row of logits that are all −inf. Asynchronous, no workspace. */
+int nml_distill_device(const void* logits, size_t ld, const int64_t* top_ids, const float* top_logits,
+                       size_t rows, size_t vocab, size_t top_k, double temperature, float* loss,
+                       float* m, float* l, int* err, int dtype);
+/* Its gradient: dlogits (rows, vocab) at stride ld_d, of the logits' dtype, is overwritten with
+ *   dloss/T·(p_v − Σ_{k: id_k = v} q_k)
+ * from the forward's m and l; dloss: float32 (rows). Rows without a teacher: zeros. dlogits may be
+ * logits itself. An id outside [−1, vocab) makes its row NaN and sets bit 0 of *err. Asynchronous, no
+ * workspace. */
+int nml_distill_backward_device(const void* logits, size_t ld, const int64_t* top_ids,
+                                const float* top_logits, const float* m, const float* l,
+                                const float* dloss, size_t rows, size_t vocab, size_t top_k,
+                                double temperature, void* dlogits, size_t ld_d, int* err, int dtype);
+
+/* Drafted tokens verified against the target's distribution, from given uniform numbers: what a
+ * sequence takes of a cheaper model's guesses so that its tokens are distributed as the target's own
+ * (models/generate.py:23-59 with temperature alone, or greedy). No reference counterpart.
+ *   logits: (batch, drafted + 1, vocab), rows at a stride of ld elements (dtype): the target's after the
+ *           row's last token and after each draft
+ *   draft_logits: (batch, drafted, vocab) at ld_draft, the logits that the drafts were drawn from at the
+ *           same temperature; NULL: the drafts were chosen outright (q_i = 1 at the draft)
+ *   drafts: int64 (batch, drafted); counts: int32 (batch), drafts of each row (NULL: all)
+ *   u: float64 (batch, drafted + 1) in [0, 1): a number for each draft, the last for the final token
+ * With p_i, q_i the softmax of logits/T: draft i is accepted iff u_i·q_i(d_i) < p_i(d_i), up to the first
+ * that is not, r (none: r = counts[b]). The token at r is the first v with Σ_{j≤v} w_j > u_last·Σ w,
+ * w = max(p_r − q_r, 0) for a refused draft (p_r if that is 0 throughout), else p_r. Sums in 64 bits.
+ * T ≤ 0: a draft is accepted iff it is the row's largest logit (the lowest id of equal ones), which is
+ * also the final token; draft_logits and u are not read.
+ *   accepted: int32 (batch), r; tokens: int64 (batch, drafted + 1): r drafts, the token, then −1
+ * Logits of −inf have probability 0 (a caller that filters sets them). Rows past counts[b] are not
+ * read. *err (device int, may be NULL): bit 0 for a count outside [0, drafted] (clamped) or a draft
+ * outside [0, vocab) (refused); bit 1 where a row that decides has no distribution (NaN or +inf in it,
+ * for T ≤ 0 NaN alone, or nothing above −inf): the token at r is −1.
+ * 0 ≤ drafted ≤ 63, vocab ≤ 2^24, batch·(2·drafted + 1) ≤ 65535. ws: nml_verify_drafts_workspace bytes,
+ * 16-byte aligned, in any state; calls that can run at the same time need one each. Asynchronous. */
+int nml_verify_drafts_workspace(size_t batch, size_t drafted, size_t vocab, size_t* bytes);
+int nml_verify_drafts_device(const void* logits, size_t ld, const void* draft_logits, size_t ld_draft,
+                             const int64_t* drafts, const int32_t* counts, const double* u,
+                             size_t batch, size_t drafted, size_t vocab, double temperature,
+                             int32_t* accepted, int64_t* tokens, void* ws, size_t ws_bytes, int* err,
+                             int dtype);
+
+/* ---- a KV cache in pages ----
+ * No reference counterpart: the cache of nml_decode_attention_device without a whole max_seq of room for
+ * each row. K and V are two pools (num_pages, kv_heads, page_size, dk) in dtype; position p of row b is
+ * position p % page_size of page table[b·max_pages + p / page_size].
+ *   table: device int32 (batch, max_pages); entries past a row's last position are not read
+ *   page_size: a power of two in [8, 1024]; rows may share pages that none of them writes
+ * pos, counts, lens: device int32 (batch). *err: device int, may be NULL, cleared by the caller; bit 0 is
+ * set for a position outside the table, a page outside [0, num_pages), a count outside [0, seq] or a
+ * length outside [0, max_pages·page_size] (counts and lengths are clamped). Any head dim 1 ≤ dk ≤ 256;
+ * all asynchronous. */
+
+/* Writes seq new tokens of each row: token s of row b, s < counts[b] (NULL: seq), goes to position
+ * pos[b] + s (NULL: s). Element d of head h of that token is at k[b·stride_b + h·stride_h + s·stride_s +
+ * d], v alike (strides in elements). Everything else, and tokens whose position or page is out of
+ * range, is left as it was. No two tokens of a call may go to one place. */
+int nml_paged_write_device(const void* k, const void* v, size_t stride_b, size_t stride_h,
+                           size_t stride_s, void* k_pages, void* v_pages, const int32_t* table,
+                           const int32_t* pos, const int32_t* counts, size_t batch, size_t kv_heads,
+                           size_t seq, size_t max_pages, size_t page_size, size_t num_pages, size_t dk,
+                           int* err, int dtype);
+/* Causal attention of each row's counts[b] (NULL: seq) last cached tokens over its pages, as
+ * nml_kv4_attention_device: token s stands at position lens[b] − counts[b] + s and sees the keys up to
+ * itself, s_j = (q·k_j) / scale_div, softmax, Σ_j p_j·v_j; a token that sees no key gives zeros. What
+ * the pages hold at positions that a token does not see does not matter to it, infinities and NaN
+ * neither. The output of a row with a page out of range is not to be used. scale_div: positive and
+ * normal.
+ *   q: (batch, heads, seq, dk); out: (batch, seq, heads·dk), rows from counts[b] on left as they were;
+ *   query head h reads KV head h / (heads / kv_heads)
+ *   ws: nml_paged_attention_workspace bytes, 16-byte aligned, zeroed once before its first use; every
+ *   call leaves its counters zero, so one serves any number of calls one after another, whatever their
+ *   sizes, and calls that can run at the same time need one each. */
+int nml_paged_attention_workspace(size_t batch, size_t heads, size_t kv_heads, size_t seq,
+                                  size_t max_pages, size_t page_size, size_t dk, int dtype,
+                                  size_t* bytes);
+int nml_paged_attention_device(const void* q, const void* k_pages, const void* v_pages,
+                               const int32_t* table, const int32_t* lens, const int32_t* counts,
+                               void* out, size_t batch, size_t heads, size_t kv_heads, size_t seq,
+                               size_t max_pages, size_t page_size, size_t num_pages, size_t dk,
+                               float scale_div, void* ws, size_t ws_bytes, int* err, int dtype);
+
 /* Optimizer step, float32 state, in place on device buffers.
  * adamw_step (native/src/module.cpp:175-188 → adamw_step_cpu, native/src/adamw.cpp:6-20):
  * the same operation order, so results equal the reference's bit for bit. n elements;

@@ -29,6 +29,7 @@ vp = C.c_void_p
 sz = C.c_size_t
 i32 = C.c_int
 f32 = C.c_float
+f64 = C.c_double
 i64 = C.c_int64
 PI32 = C.POINTER(C.c_int32)
 
@@ -72,6 +73,15 @@ _SIGS = {
     "nml_token_logprobs_device": [vp, sz, vp, sz, sz, i64, i32, sz, vp, vp, vp, vp, vp, vp, vp, i32],
     "nml_token_logprobs_backward_device": [vp, sz, vp, vp, vp, vp, vp, vp, sz, sz, i64, i32, vp,
                                            sz, vp, i32],
+    "nml_distill_device": [vp, sz, vp, vp, sz, sz, sz, f64, vp, vp, vp, vp, i32],
+    "nml_distill_backward_device": [vp, sz, vp, vp, vp, vp, vp, sz, sz, sz, f64, vp, sz, vp, i32],
+    "nml_verify_drafts_workspace": [sz, sz, sz, C.POINTER(sz)],
+    "nml_verify_drafts_device": [vp, sz, vp, sz, vp, vp, vp, sz, sz, sz, f64, vp, vp, vp, sz, vp, i32],
+    "nml_paged_write_device": [vp, vp, sz, sz, sz, vp, vp, vp, vp, vp, sz, sz, sz, sz, sz, sz, sz, vp,
+                               i32],
+    "nml_paged_attention_workspace": [sz, sz, sz, sz, sz, sz, sz, i32, C.POINTER(sz)],
+    "nml_paged_attention_device": [vp, vp, vp, vp, vp, vp, vp, sz, sz, sz, sz, sz, sz, sz, sz, f32, vp,
+                                   sz, vp, i32],
     "nml_sdpa_forward_device": [vp, vp, vp, vp, vp, sz, sz, sz, f32, i32, i32],
     "nml_tied_ce_forward_device": [vp, vp, vp, sz, sz, sz, i64, i32, C.POINTER(C.c_double), i32],
     "nml_tied_ce_forward_device_noalloc": [vp, vp, vp, sz, sz, sz, i64, i32,

@@ -291,6 +291,99 @@ struct LogprobBwdArgs {
 };
 int launch_logprobs_backward(int dt, const LogprobBwdArgs& a, hipStream_t st);
 
+// Distillation from a teacher's top logits (ops_distill.hip): with q the softmax of a row's K teacher
+// logits at temperature T and p that of its logits (rows, V) at stride ld, loss = Σ q_k·(log q_k − log
+// p[id_k]), m = max x, l = Σ exp((x − m)/T); m, l may be null. An entry of id −1 or logit −inf is
+// absent, a row of nothing else gives zeros; an id outside [−1, V) gives NaN and sets bit 0 of *err
+// (may be null).
+constexpr int kMaxDistillTop = 256;
+struct DistillArgs {
+  const void* logits;
+  long long ld;
+  const int64_t* top_ids;
+  const float* top_logits;
+  int rows, V, K;
+  float c, inv_t;  // log₂ e / T, 1 / T
+  float *loss, *m, *l;
+  int* err;
+};
+int launch_distill(int dt, const DistillArgs& a, hipStream_t st);
+
+// Its gradient: dlogits = dloss/T·(p_v − Σ_{k: id_k = v} q_k), from the forward's m and l. May
+// overwrite logits in place.
+struct DistillBwdArgs {
+  const void* logits;
+  long long ld;
+  const int64_t* top_ids;
+  const float* top_logits;
+  const float *m, *l, *dloss;
+  int rows, V, K;
+  float c, inv_t;
+  void* dlogits;
+  long long ld_d;
+  int* err;
+};
+int launch_distill_backward(int dt, const DistillBwdArgs& a, hipStream_t st);
+
+// Drafted tokens verified against the target's distribution (ops_verify.hip): of B sequences' counts[b]
+// (null: n) drafts each, logits (B, n + 1, V) at a row stride of ld, draft logits (B, n, V) or null (drafts
+// chosen outright), uniforms u (B, n + 1), c = log₂ e / T; greedy: draft and u are not read. accepted (B),
+// tokens (B, n + 1): the accepted drafts, one token more, −1 from there on. Bit 0 of *err: a count or
+// a draft out of range; bit 1: a row without a distribution (its token is −1).
+constexpr int kMaxDrafts = 63;
+struct VerifyArgs {
+  const void* logits;
+  long long ld;
+  const void* draft;
+  long long ld_draft;
+  const int64_t* drafts;
+  const int32_t* counts;
+  const double* u;
+  int B, n, V, greedy;
+  double c;
+  int32_t* accepted;
+  int64_t* tokens;
+  int* err;
+  // set by the launch: parts of a row, and the workspace's parts
+  int parts;
+  void *stats, *sums;
+  unsigned* counter;
+};
+size_t verify_workspace(int B, int n, int V);
+int launch_verify(int dt, VerifyArgs a, void* ws, hipStream_t st);
+
+// The KV cache in pages (ops_paged.hip): pools (num_pages, H, 1 << shift, dk) of K and of V; position p of
+// row b is in page table[b·max_pages + (p >> shift)].
+//
+// Write: as Kv4WriteArgs' tokens and strides. A position past the table or of a page outside
+// [0, num_pages) is not written and sets bit 0 of *err (may be null).
+struct PagedWriteArgs {
+  const void* k;
+  const void* v;
+  long long stride_b, stride_h, stride_s;
+  void *k_pages, *v_pages;
+  const int32_t *table, *pos, *counts;
+  int B, H, S, max_pages, shift, num_pages, dk;
+  int* err;
+};
+int launch_paged_write(int dt, const PagedWriteArgs& a, hipStream_t st);
+
+// Attention as Kv4AttnArgs' over the pages. A page outside [0, num_pages) sets bit 0 of *err and is
+// read as page 0.
+struct PagedAttnArgs {
+  const void* q;
+  const void *k_pages, *v_pages;
+  const int32_t *table, *lens, *counts;
+  void* out;
+  int B, H, Hkv, S, max_pages, shift, num_pages, dk;
+  int group;    // H / Hkv
+  float scale;  // divisor of the scores
+  void* ws;
+  int* err;
+};
+size_t paged_attention_workspace(int dt, int B, int H, int Hkv, int S, int P, int dk);
+int launch_paged_attention(int dt, const PagedAttnArgs& a, hipStream_t st);
+
 // ------------------------------------------------------------ training
 // Every launch takes the model's storage type dt (F32 or F16) for the activation-side
 // tensors; parameter gradients, partial sums and the softmax statistics are float32.

@@ -721,4 +721,229 @@ int nml_token_logprobs_backward_device(const void* logits, size_t ld, const int6
   return launch_logprobs_backward(dtype, a, nml::stream());
 }
 
+// Rows of logits and the teacher's entries, common to the distillation's two calls.
+static int distill_ok(const char* what, size_t rows, size_t vocab, size_t ld, size_t top_k, double temperature) {
+  NML_REQUIRE(rows <= 0x7fffffff && vocab >= 1 && vocab <= (size_t)1 << 30 && ld >= vocab && ld < (size_t)1 << 40,
+              "%s: %zu rows of %zu logits at stride %zu out of range", what, rows, vocab, ld);
+  NML_REQUIRE(top_k >= 1 && top_k <= (size_t)kMaxDistillTop, "%s: top_k %zu outside [1, %d]", what, top_k,
+              kMaxDistillTop);
+  NML_REQUIRE(temperature >= 1e-6 && temperature <= 1e6, "%s: temperature %g outside [1e-6, 1e6]", what, temperature);
+  return 0;
+}
+
+constexpr double kLog2e64 = 1.4426950408889634074;
+
+int nml_distill_device(const void* logits, size_t ld, const int64_t* top_ids, const float* top_logits, size_t rows,
+                       size_t vocab, size_t top_k, double temperature, float* loss, float* m, float* l, int* err,
+                       int dtype) {
+  NML_TRY(check_dtype(dtype));
+  NML_TRY(distill_ok("distill", rows, vocab, ld, top_k, temperature));
+  if (rows == 0) return 0;
+  NML_REQUIRE(logits && top_ids && top_logits && loss, "distill: a buffer is null");
+  DistillArgs a{};
+  a.logits = logits;
+  a.ld = (long long)ld;
+  a.top_ids = top_ids;
+  a.top_logits = top_logits;
+  a.rows = (int)rows;
+  a.V = (int)vocab;
+  a.K = (int)top_k;
+  a.c = (float)(kLog2e64 / temperature);
+  a.inv_t = (float)(1.0 / temperature);
+  a.loss = loss;
+  a.m = m;
+  a.l = l;
+  a.err = err;
+  return launch_distill(dtype, a, nml::stream());
+}
+
+int nml_distill_backward_device(const void* logits, size_t ld, const int64_t* top_ids, const float* top_logits,
+                                const float* m, const float* l, const float* dloss, size_t rows, size_t vocab,
+                                size_t top_k, double temperature, void* dlogits, size_t ld_d, int* err, int dtype) {
+  NML_TRY(check_dtype(dtype));
+  NML_TRY(distill_ok("distill backward", rows, vocab, ld, top_k, temperature));
+  NML_REQUIRE(ld_d >= vocab && ld_d < (size_t)1 << 40, "distill backward: stride %zu out of range", ld_d);
+  if (rows == 0) return 0;
+  NML_REQUIRE(logits && top_ids && top_logits && m && l && dloss && dlogits, "distill backward: a buffer is null");
+  DistillBwdArgs a{};
+  a.logits = logits;
+  a.ld = (long long)ld;
+  a.top_ids = top_ids;
+  a.top_logits = top_logits;
+  a.m = m;
+  a.l = l;
+  a.dloss = dloss;
+  a.rows = (int)rows;
+  a.V = (int)vocab;
+  a.K = (int)top_k;
+  a.c = (float)(kLog2e64 / temperature);
+  a.inv_t = (float)(1.0 / temperature);
+  a.dlogits = dlogits;
+  a.ld_d = (long long)ld_d;
+  a.err = err;
+  return launch_distill_backward(dtype, a, nml::stream());
+}
+
+static int verify_ok(size_t batch, size_t drafted, size_t vocab) {
+  NML_REQUIRE(drafted <= (size_t)kMaxDrafts, "verify drafts: %zu drafts a row above %d", drafted, kMaxDrafts);
+  NML_REQUIRE(vocab >= 1 && vocab <= (size_t)1 << 24, "verify drafts: vocabulary %zu outside [1, 2^24]", vocab);
+  NML_REQUIRE(batch * (2 * drafted + 1) <= 65535, "verify drafts: %zu rows of %zu drafts too many", batch, drafted);
+  return 0;
+}
+
+int nml_verify_drafts_workspace(size_t batch, size_t drafted, size_t vocab, size_t* bytes) {
+  NML_REQUIRE(bytes != nullptr, "verify drafts: bytes is null");
+  *bytes = 0;
+  NML_REQUIRE(batch <= 65535, "verify drafts: batch %zu too large", batch);
+  NML_TRY(verify_ok(batch, drafted, vocab));
+  if (batch) *bytes = verify_workspace((int)batch, (int)drafted, (int)vocab);
+  return 0;
+}
+
+int nml_verify_drafts_device(const void* logits, size_t ld, const void* draft_logits, size_t ld_draft,
+                             const int64_t* drafts, const int32_t* counts, const double* u, size_t batch,
+                             size_t drafted, size_t vocab, double temperature, int32_t* accepted, int64_t* tokens,
+                             void* ws, size_t ws_bytes, int* err, int dtype) {
+  NML_TRY(check_dtype(dtype));
+  NML_REQUIRE(batch <= 65535, "verify drafts: batch %zu too large", batch);
+  NML_TRY(verify_ok(batch, drafted, vocab));
+  NML_REQUIRE(ld >= vocab && ld < (size_t)1 << 40 && (!draft_logits || (ld_draft >= vocab && ld_draft < (size_t)1 << 40)),
+              "verify drafts: strides %zu, %zu out of range", ld, ld_draft);
+  const bool greedy = temperature <= 0.0;
+  NML_REQUIRE(greedy || (temperature >= 1e-6 && temperature <= 1e6),
+              "verify drafts: temperature %g above 0 and outside [1e-6, 1e6]", temperature);
+  if (batch == 0) return 0;
+  NML_REQUIRE(logits && (drafts || drafted == 0) && accepted && tokens && (greedy || u), "verify drafts: a buffer is null");
+  const size_t need = verify_workspace((int)batch, (int)drafted, (int)vocab);
+  NML_REQUIRE(ws && ws_bytes >= need, "verify drafts: a workspace of %zu bytes is needed, %zu given", need,
+              ws ? ws_bytes : (size_t)0);
+  NML_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 15) == 0, "verify drafts: the workspace must be 16-byte aligned");
+  VerifyArgs a{};
+  a.logits = logits;
+  a.ld = (long long)ld;
+  a.draft = greedy || drafted == 0 ? nullptr : draft_logits;
+  a.ld_draft = (long long)ld_draft;
+  a.drafts = drafts;
+  a.counts = counts;
+  a.u = u;
+  a.B = (int)batch;
+  a.n = (int)drafted;
+  a.V = (int)vocab;
+  a.greedy = greedy;
+  a.c = greedy ? 0.0 : kLog2e64 / temperature;
+  a.accepted = accepted;
+  a.tokens = tokens;
+  a.err = err;
+  return launch_verify(dtype, a, ws, nml::stream());
+}
+
+// Sizes of a paged cache: positions of a row and elements of a launch in 32 bits.
+static int paged_ok(const char* what, size_t batch, size_t heads, size_t seq, size_t max_pages, size_t page_size,
+                    size_t num_pages, size_t dk) {
+  NML_REQUIRE(dk >= 1 && dk <= (size_t)kMaxHeadDim, "%s: head_dim %zu outside [1, %d]", what, dk, kMaxHeadDim);
+  NML_REQUIRE(batch <= 65535 && heads <= 65535, "%s: %zu rows × %zu heads too many", what, batch, heads);
+  NML_REQUIRE(page_size >= 8 && page_size <= 1024 && (page_size & (page_size - 1)) == 0,
+              "%s: page size %zu is not a power of two in [8, 1024]", what, page_size);
+  NML_REQUIRE(max_pages >= 1 && max_pages <= ((size_t)1 << 30) / page_size, "%s: %zu pages of %zu a row out of range",
+              what, max_pages, page_size);
+  NML_REQUIRE(num_pages >= 1 && num_pages <= 0x7fffffff, "%s: %zu pages out of range", what, num_pages);
+  NML_REQUIRE(seq <= ((size_t)1 << 22) / (heads ? heads : 1), "%s: %zu tokens × %zu heads too many", what, seq, heads);
+  return 0;
+}
+
+static int log2_of(size_t n) {
+  int s = 0;
+  while (((size_t)1 << s) < n) ++s;
+  return s;
+}
+
+int nml_paged_write_device(const void* k, const void* v, size_t stride_b, size_t stride_h, size_t stride_s,
+                           void* k_pages, void* v_pages, const int32_t* table, const int32_t* pos,
+                           const int32_t* counts, size_t batch, size_t kv_heads, size_t seq, size_t max_pages,
+                           size_t page_size, size_t num_pages, size_t dk, int* err, int dtype) {
+  NML_TRY(check_dtype(dtype));
+  NML_TRY(paged_ok("paged write", batch, kv_heads, seq, max_pages, page_size, num_pages, dk));
+  if (batch == 0 || kv_heads == 0 || seq == 0) return 0;
+  NML_REQUIRE(k && v && k_pages && v_pages && table, "paged write: a buffer is null");
+  const size_t limit = (size_t)1 << 40;
+  NML_REQUIRE(stride_b < limit && stride_h < limit && stride_s < limit, "paged write: a stride is out of range");
+  PagedWriteArgs a{};
+  a.k = k;
+  a.v = v;
+  a.stride_b = (long long)stride_b;
+  a.stride_h = (long long)stride_h;
+  a.stride_s = (long long)stride_s;
+  a.k_pages = k_pages;
+  a.v_pages = v_pages;
+  a.table = table;
+  a.pos = pos;
+  a.counts = counts;
+  a.B = (int)batch;
+  a.H = (int)kv_heads;
+  a.S = (int)seq;
+  a.max_pages = (int)max_pages;
+  a.shift = log2_of(page_size);
+  a.num_pages = (int)num_pages;
+  a.dk = (int)dk;
+  a.err = err;
+  return launch_paged_write(dtype, a, nml::stream());
+}
+
+static int paged_attention_ok(size_t batch, size_t heads, size_t kv_heads, size_t seq, size_t max_pages,
+                              size_t page_size, size_t num_pages, size_t dk) {
+  NML_TRY(paged_ok("paged attention", batch, heads, seq, max_pages, page_size, num_pages, dk));
+  NML_REQUIRE(kv_heads >= 1 ? heads % kv_heads == 0 : heads == 0,
+              "paged attention: heads (%zu) must be divisible by kv_heads (%zu)", heads, kv_heads);
+  return 0;
+}
+
+int nml_paged_attention_workspace(size_t batch, size_t heads, size_t kv_heads, size_t seq, size_t max_pages,
+                                  size_t page_size, size_t dk, int dtype, size_t* bytes) {
+  NML_REQUIRE(bytes != nullptr, "paged attention: bytes is null");
+  *bytes = 0;
+  NML_TRY(check_dtype(dtype));
+  NML_TRY(paged_attention_ok(batch, heads, kv_heads, seq, max_pages, page_size, 1, dk));
+  if (batch && heads && seq)
+    *bytes = paged_attention_workspace(dtype, (int)batch, (int)heads, (int)kv_heads, (int)seq,
+                                       (int)(max_pages * page_size), (int)dk);
+  return 0;
+}
+
+int nml_paged_attention_device(const void* q, const void* k_pages, const void* v_pages, const int32_t* table,
+                               const int32_t* lens, const int32_t* counts, void* out, size_t batch, size_t heads,
+                               size_t kv_heads, size_t seq, size_t max_pages, size_t page_size, size_t num_pages,
+                               size_t dk, float scale_div, void* ws, size_t ws_bytes, int* err, int dtype) {
+  NML_TRY(check_dtype(dtype));
+  NML_TRY(paged_attention_ok(batch, heads, kv_heads, seq, max_pages, page_size, num_pages, dk));
+  NML_REQUIRE(scale_div > 0.f && std::isnormal(scale_div), "paged attention: scale_div must be positive and normal");
+  if (batch == 0 || heads == 0 || seq == 0) return 0;
+  NML_REQUIRE(q && k_pages && v_pages && table && lens && out, "paged attention: a buffer is null");
+  const size_t need = paged_attention_workspace(dtype, (int)batch, (int)heads, (int)kv_heads, (int)seq,
+                                                (int)(max_pages * page_size), (int)dk);
+  NML_REQUIRE(ws_bytes >= need && (need == 0 || ws != nullptr),
+              "paged attention: a workspace of %zu bytes is needed, %zu given", need, ws ? ws_bytes : (size_t)0);
+  NML_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 15) == 0, "paged attention: the workspace must be 16-byte aligned");
+  PagedAttnArgs a{};
+  a.q = q;
+  a.k_pages = k_pages;
+  a.v_pages = v_pages;
+  a.table = table;
+  a.lens = lens;
+  a.counts = counts;
+  a.out = out;
+  a.B = (int)batch;
+  a.H = (int)heads;
+  a.Hkv = (int)kv_heads;
+  a.S = (int)seq;
+  a.max_pages = (int)max_pages;
+  a.shift = log2_of(page_size);
+  a.num_pages = (int)num_pages;
+  a.dk = (int)dk;
+  a.group = (int)(heads / kv_heads);
+  a.scale = scale_div;
+  a.ws = ws;
+  a.err = err;
+  return launch_paged_attention(dtype, a, nml::stream());
+}
+
 }  // extern "C"

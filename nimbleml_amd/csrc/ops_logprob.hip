@@ -20,6 +20,7 @@
 // elementary float32 operations). A few rows are bound by the latency of the passes (32 rows of
 // 32000 float32 logits: 5.5 µs, 11.8 with 20 alternatives).
 #include "kernels.hpp"
+#include "row_pieces.hpp"
 
 namespace nml {
 
@@ -31,8 +32,6 @@ constexpr int kFewRows = 512;
 constexpr int kLaunchRows = 1 << 21;
 // Gathered candidates of the alternatives; more than this takes the rounds below.
 constexpr int kCandidates = 1024;
-
-__device__ __forceinline__ float exp_of(float t) { return __builtin_amdgcn_exp2f(t * 1.44269504088896341f); }
 
 // Order of logits as unsigned words: NaN above everything (by one word below the largest, which with
 // id 0 would be the bound that the first of the rounds starts under), −0 equal to +0.
@@ -56,48 +55,7 @@ __device__ __forceinline__ unsigned long long wave_umax64(unsigned long long v) 
   return v;
 }
 
-// The 16-byte pieces of a row: piece c holds elements c·E − off … c·E − off + E − 1.
-template <typename T>
-struct RowPieces {
-  static constexpr int E = 16 / static_cast<int>(sizeof(T));
-  typedef T vec __attribute__((ext_vector_type(E)));
-  const T* row;
-  int V, off, n;
-  __device__ RowPieces(const T* r, int v) : row(r), V(v) {
-    off = static_cast<int>((reinterpret_cast<uintptr_t>(r) & 15) / sizeof(T));
-    n = (V + off + E - 1) / E;
-  }
-  __device__ int first(int c) const { return c * E - off; }
-  __device__ vec load(int c) const {
-    const int i = first(c);
-    if (i >= 0 && i + E <= V) return *reinterpret_cast<const vec*>(row + i);
-    return edge(i);
-  }
-  // (word by word: as a vector its values would take a register each beside the whole pieces)
-  __device__ vec edge(int i) const {
-    typedef unsigned u4 __attribute__((ext_vector_type(4)));
-    u4 r;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      if constexpr (E == 4) {
-        r[w] = i + w >= 0 && i + w < V ? __builtin_bit_cast(unsigned, row[i + w]) : 0xff800000u;
-      } else {
-        unsigned half[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int at = i + 2 * w + e;
-          half[e] = at >= 0 && at < V ? __builtin_bit_cast(unsigned short, row[at]) : 0xfc00u;
-        }
-        r[w] = half[0] | half[1] << 16;
-      }
-    }
-    return __builtin_bit_cast(vec, r);
-  }
-};
-
 constexpr float kLowest = -1e4f;          // exp of it is 0, its product with that too
-constexpr float kNone = -3.402823466e38f;  // a reference below every finite logit
-
 // A thread's part of Σ exp(x − ref) and Σ exp(x − ref)·(x − ref), and the largest x it has seen.
 struct Part {
   float top, ref, z, zt;
@@ -109,21 +67,6 @@ struct Part {
     ref = r;
   }
 };
-
-template <typename T>
-__device__ __forceinline__ float piece_max(const typename RowPieces<T>::vec& v);
-template <>
-__device__ __forceinline__ float piece_max<float>(const typename RowPieces<float>::vec& v) {
-  return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
-}
-template <>
-__device__ __forceinline__ float piece_max<half_t>(const typename RowPieces<half_t>::vec& v) {
-  typedef half_t h2 __attribute__((ext_vector_type(2)));
-  const h2 a = __builtin_elementwise_max(h2{v[0], v[1]}, h2{v[2], v[3]});
-  const h2 b = __builtin_elementwise_max(h2{v[4], v[5]}, h2{v[6], v[7]});
-  const h2 c = __builtin_elementwise_max(a, b);
-  return fmaxf(static_cast<float>(c.x), static_cast<float>(c.y));
-}
 
 template <typename T>
 __device__ __forceinline__ void add_piece(Part& s, const typename RowPieces<T>::vec& v) {
