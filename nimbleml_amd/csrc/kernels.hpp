@@ -377,6 +377,7 @@ struct PagedAttnArgs {
   void* out;
   int B, H, Hkv, S, max_pages, shift, num_pages, dk;
   int group;    // H / Hkv
+  int slots;    // set by the launch
   float scale;  // divisor of the scores
   void* ws;
   int* err;
