@@ -564,6 +564,9 @@ int nml_cache_create_kv4(nml_model* m, size_t batch, nml_cache** out);
 int nml_cache_destroy(nml_cache* c);
 /* The length of row 0 (rows prefilled with nml_model_prefill_ragged may differ). */
 int nml_cache_length(nml_cache* c, size_t* len);
+/* Keep each row's first lens[b] tokens (host int32, one a row, at most the row's length): what drafted
+ * tokens that were not accepted left in the cache is given up, and the rows go on from there. */
+int nml_cache_truncate(nml_cache* c, const int32_t* lens);
 /* Append seq tokens (same count per row, each row at its own position) and return their
  * logits (batch, seq, vocab), or (batch, vocab) for the last position when last_only.
  * seq == 1 is one step of generate()'s decode loop (the same kernels as

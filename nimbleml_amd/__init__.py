@@ -8,6 +8,7 @@ include/nimbleml_hip.h. Importing requires the built library
 """
 from nimbleml_amd import np_backend
 from nimbleml_amd._native import DeviceArray
+from nimbleml_amd.distill import distill_loss
 from nimbleml_amd.generate import generate
 from nimbleml_amd.grad_mode import enable_grad, is_grad_enabled, no_grad
 from nimbleml_amd.gpt import GPT, KVCache
@@ -30,4 +31,5 @@ __all__ = [
     "load_checkpoint", "Adam", "AdamW", "device", "using_gpu",
     "set_device", "set_dtype", "np_backend", "no_grad", "enable_grad", "is_grad_enabled",
     "causal_mask_tensor", "make_causal_mask", "token_log_probs",
+    "distill_loss",
 ]

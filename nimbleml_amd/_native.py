@@ -116,6 +116,7 @@ _SIGS = {
     "nml_cache_create": [vp, sz, C.POINTER(vp)],
     "nml_cache_create_kv4": [vp, sz, C.POINTER(vp)],
     "nml_cache_destroy": [vp],
+    "nml_cache_truncate": [vp, PI32],
     "nml_cache_length": [vp, C.POINTER(sz)],
     "nml_model_forward_cached": [vp, vp, vp, sz, sz, vp, i32],
     "nml_model_prefill_ragged": [vp, vp, vp, sz, PI32, sz, vp],

@@ -1182,6 +1182,18 @@ int nml_cache_length(nml_cache* c, size_t* len) {
   return 0;
 }
 
+int nml_cache_truncate(nml_cache* c, const int32_t* lens) {
+  NML_REQUIRE(c != nullptr && lens != nullptr, "cache truncate: cache or lens is null");
+  for (int b = 0; b < c->B; ++b)
+    NML_REQUIRE(lens[b] >= 0 && lens[b] <= c->len[b], "cache truncate: length %d of row %d is out of range [0, %d]",
+                lens[b], b, c->len[b]);
+  hipStream_t st = nml::stream();
+  NML_HIP(hipMemcpyAsync(c->len_dev, lens, c->B * sizeof(int32_t), hipMemcpyHostToDevice, st));
+  NML_HIP(hipStreamSynchronize(st));  // (lens is the caller's)
+  c->len.assign(lens, lens + c->B);
+  return 0;
+}
+
 int nml_model_forward_cached(nml_model* m, nml_cache* c, const int64_t* ids, size_t batch,
                              size_t seq, void* logits, int last_only) {
   NML_TRY(check_ready(m));

@@ -894,6 +894,12 @@ static int paged_attention_ok(size_t batch, size_t heads, size_t kv_heads, size_
   NML_TRY(paged_ok("paged attention", batch, heads, seq, max_pages, page_size, num_pages, dk));
   NML_REQUIRE(kv_heads >= 1 ? heads % kv_heads == 0 : heads == 0,
               "paged attention: heads (%zu) must be divisible by kv_heads (%zu)", heads, kv_heads);
+  if (batch && heads && seq) {
+    // the kernel numbers spans of 64 keys in 32 bits, and a launch its threads
+    const size_t tiles = (heads / kv_heads * seq + 15) / 16 * kv_heads, keys = max_pages * page_size;
+    NML_REQUIRE(tiles * batch <= 0x7fffffff / ((keys + 63) / 64) && tiles * batch <= (size_t)1 << 22,
+                "paged attention: %zu rows × %zu heads × %zu tokens over %zu positions too many", batch, heads, seq, keys);
+  }
   return 0;
 }
 

@@ -33,16 +33,19 @@ struct Entry {
   float y;
 };
 
-// Entry `k` of row r, and whether its id is out of range.
-__device__ __forceinline__ Entry entry_of(const int64_t* ids, const float* ys, int r, int K, int k, int V, bool& bad) {
+// Entry `k` of row r. An id out of range is told, and is an entry of NaN, as which it makes the row NaN.
+__device__ __forceinline__ Entry entry_of(const int64_t* ids, const float* ys, int r, int K, int k, int V, int* err) {
   Entry e{-1, -INFINITY};
-  bad = false;
   if (k < K) {
     const size_t at = static_cast<size_t>(r) * K + k;
     const int64_t id = ids[at];
     const float y = ys[at];
-    bad = id < -1 || id >= V;
-    if (id >= 0 && !bad && y != -INFINITY) e = Entry{static_cast<int>(id), y};
+    if (id < -1 || id >= V) {
+      if (err) __hip_atomic_fetch_or(err, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      e = Entry{0, __builtin_nanf("")};
+    } else if (id >= 0 && y != -INFINITY) {
+      e = Entry{static_cast<int>(id), y};
+    }
   }
   return e;
 }
@@ -66,10 +69,8 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
   __shared__ float top_w[KW], z_w[KW], s_w[KW];
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const T* x = static_cast<const T*>(a.logits) + static_cast<size_t>(r) * a.ld;
-  bool bad;
-  const Entry e = entry_of(a.top_ids, a.top_logits, r, a.K, tid, a.V, bad);
-  const int any = __syncthreads_or((e.id >= 0 ? 1 : 0) | (bad ? 2 : 0));
-  if (any == 0) {
+  const Entry e = entry_of(a.top_ids, a.top_logits, r, a.K, tid, a.V, a.err);
+  if (!__syncthreads_or(e.id >= 0)) {
     if (tid == 0) {
       a.loss[r] = 0.f;
       if (a.m) a.m[r] = 0.f;
@@ -140,10 +141,9 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
     float q = 0.f, t = 0.f;
 #pragma unroll
     for (int i = 0; i < KW; ++i) q += z_w[i], t += s_w[i];
-    a.loss[r] = any & 2 ? __builtin_nanf("") : t / q * a.inv_t + (logf(z) - logf(q));
+    a.loss[r] = t / q * a.inv_t + (logf(z) - logf(q));
     if (a.m) a.m[r] = m;
     if (a.l) a.l[r] = z;
-    if ((any & 2) && a.err) __hip_atomic_fetch_or(a.err, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
 }
 
@@ -163,19 +163,14 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillBwdArgs a, int 
   const Row row(x, a.V);
   const int c0 = blockIdx.x * steps * F * NT, c1 = min(row.n, c0 + steps * F * NT);
   if (c0 >= c1) return;
-  bool bad;
-  const Entry e = entry_of(a.top_ids, a.top_logits, r, a.K, tid, a.V, bad);
-  const int any = __syncthreads_or((e.id >= 0 ? 1 : 0) | (bad ? 2 : 0));
+  const Entry e = entry_of(a.top_ids, a.top_logits, r, a.K, tid, a.V, blockIdx.x == 0 ? a.err : nullptr);
+  const bool taught = __syncthreads_or(e.id >= 0);
   const float m = a.m[r], c = a.c;
   float s = a.dloss[r] * a.inv_t;  // of q; s / l: of exp((x − m)/T)
-  if (any & 2) {
-    s = __builtin_nanf("");
-    if (tid == 0 && blockIdx.x == 0 && a.err) __hip_atomic_fetch_or(a.err, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
   float z = 0.f;  // of the teacher's exponentials
   const bool here = e.id >= row.first(c0) && e.id < row.first(c1) && e.id >= 0;
   float mine = 0.f;
-  if (any != 0) {
+  if (taught) {
     // (read before the row may be overwritten: the barriers stand between)
     if (here) mine = static_cast<float>(x[e.id]);
     const float t = wave_max_dpp(e.y);
@@ -205,7 +200,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillBwdArgs a, int 
   };
   for (int i = c0 + tid; i < c1; i += F * NT) {
     vec v[F];
-    if (any != 0) {
+    if (taught) {
 #pragma unroll
       for (int k = 0; k < F; ++k)
         if (i + NT * k < c1) v[k] = row.load(i + NT * k);
@@ -216,11 +211,11 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillBwdArgs a, int 
       vec d;
 #pragma unroll
       for (int j = 0; j < E; ++j)
-        d[j] = static_cast<T>(any != 0 ? sp * __builtin_amdgcn_exp2f((static_cast<float>(v[k][j]) - m) * c) : 0.f);
+        d[j] = static_cast<T>(taught ? sp * __builtin_amdgcn_exp2f((static_cast<float>(v[k][j]) - m) * c) : 0.f);
       put(row.first(i + NT * k), d);
     }
   }
-  if (any == 0) return;
+  if (!taught) return;
   __syncthreads();  // (the row's stores are done)
   if (here) {
     float q = 0.f;

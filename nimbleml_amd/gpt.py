@@ -62,6 +62,16 @@ class KVCache:
         N.check(N.lib.nml_cache_length(self._h, C.byref(n)))
         return int(n.value)
 
+    def truncate(self, lengths):
+        """Keep each row's first ``lengths`` (an int, or one a row) tokens: rows go on from there.
+        Raises ValueError for a length outside [0, the row's length]."""
+        want = np.broadcast_to(np.asarray(lengths, dtype=np.int64), (self.batch,))
+        if want.size and (int(want.min()) < 0 or int(want.max()) > self.model.max_seq_len):
+            raise ValueError(f"a length is out of range [0, {self.model.max_seq_len}]")
+        lens = np.ascontiguousarray(want, dtype=np.int32)
+        N.check(N.lib.nml_cache_truncate(self._h, lens.ctypes.data_as(N.PI32)))
+        self.lengths = want.copy()
+
     def __del__(self):
         try:
             if self._h:

@@ -10,9 +10,16 @@ Each takes host arrays or ``DeviceArray``s in the compute dtype and returns
   KV4Cache, kv4_write, kv4_read, kv4_attention
                               a KV cache in 4 bits: quantised as it is written, read back,
                               attended to by one or several new tokens (no reference kernel)
+  PagedKVCache, paged_write, paged_attention
+                              a KV cache in pages: written, attended to by one or several new
+                              tokens (no reference kernel)
   token_logprobs, token_logprobs_backward
                               log probabilities of given tokens, entropies and the best
                               alternatives, and their gradient (no reference kernel)
+  distill, distill_backward   divergence from a teacher's top logits and its gradient (no
+                              reference kernel)
+  verify_drafts               drafted tokens accepted or replaced by the target's distribution
+                              (no reference kernel)
   embedding_lookup            kernels/embedding_scatter.py:25-36
   fused_tied_crossentropy_forward  kernels/fused_tied_crossentropy.py:8-24 (loss only)
   linear                      the `x @ W + b` of neural_network/_fused_arrays.py:25-30
@@ -456,3 +463,212 @@ def token_logprobs_backward(logits, targets, m, lsum, entropy, dlogp=None, dentr
         int(ignore_index) if has else 0, int(has), out.ptr, vocab, err.ptr, code))
     _check_flag(err, f"label out of range [0, {vocab})")
     return out
+
+
+def _page_count(lengths, page_size):
+    return -(-np.maximum(np.asarray(lengths, dtype=np.int64), 0) // page_size)
+
+
+def _check_pages(what, table, lengths, page_size, num_pages):
+    """Raises ValueError where a row of ``lengths`` positions needs a page outside [0, num_pages) or
+    more pages than ``table`` (host arrays) has."""
+    need = _page_count(lengths, page_size)
+    if need.size and int(need.max()) > table.shape[1]:
+        raise ValueError(f"{what}: a row of {int(np.max(lengths))} positions needs {int(need.max())} "
+                         f"pages of {page_size}, the table has {table.shape[1]}")
+    used = np.arange(table.shape[1]) < need[:, None]
+    bad = used & ((table < 0) | (table >= num_pages))
+    if bad.any():
+        raise ValueError(f"{what}: page {int(table[bad][0])} is outside [0, {num_pages})")
+
+
+class PagedKVCache:
+    """K and V in ``num_pages`` pages of ``page_size`` (a power of two in [8, 1024]) positions:
+    ``k_pages``/``v_pages`` (num_pages, kv_heads, page_size, dk) in ``dtype`` (None: the compute
+    dtype). Which pages a row has is the caller's table; rows may share pages that none of them
+    writes. Starts zeroed."""
+
+    def __init__(self, num_pages, page_size, kv_heads, dk, dtype=None):
+        self.num_pages, self.page_size = int(num_pages), int(page_size)
+        self.kv_heads, self.dk = int(kv_heads), int(dk)
+        if self.page_size < 8 or self.page_size > 1024 or self.page_size & (self.page_size - 1):
+            raise ValueError(f"page_size must be a power of two in [8, 1024], got {page_size}")
+        if self.num_pages < 1:
+            raise ValueError(f"num_pages must be at least 1, got {num_pages}")
+        self.dtype = np.dtype(np_backend.dtype if dtype is None else dtype)
+        N.np_dtype_code(self.dtype)
+        shape = (self.num_pages, self.kv_heads, self.page_size, self.dk)
+        self.k_pages, self.v_pages = (N.DeviceArray(shape, self.dtype) for _ in range(2))
+        for a in (self.k_pages, self.v_pages):
+            N.check(N.lib.nml_memset(a.ptr, 0, a.nbytes))
+
+
+def _page_table(cache, table, what):
+    """(the table as a host array or None, its shape (batch, pages of a row))."""
+    host = None if isinstance(table, N.DeviceArray) else np.ascontiguousarray(table, dtype=np.int32)
+    shape = table.shape if host is None else host.shape
+    if len(shape) != 2 or shape[1] < 1:
+        raise ValueError(f"{what}: the table must be (batch, pages of a row), got {shape}")
+    return host, shape
+
+
+def paged_write(cache, k, v, table, pos=None, counts=None):
+    """Write K and V (batch, kv_heads, seq, dk) of new tokens into ``cache``: token s of row b, s <
+    ``counts[b]`` (None: all), goes to position ``pos[b] + s`` (None: s), position p of row b being
+    position p % page_size of page ``table[b, p // page_size]``. No two tokens may go to one place.
+    Raises ValueError for a position past the table, a page outside the cache (the other tokens are
+    written) or a count outside [0, seq]."""
+    host, (batch, max_pages) = _page_table(cache, table, "paged_write")
+    shape = (batch, cache.kv_heads, k.shape[2] if np.ndim(k) == 4 else -1, cache.dk)
+    if tuple(k.shape) != shape or tuple(v.shape) != shape:
+        raise ValueError(f"paged_write: k {k.shape}, v {v.shape} for {batch} rows of a cache of "
+                         f"{cache.kv_heads} heads, head dim {cache.dk}")
+    seq = shape[2]
+    kd, vd = _dev(k, cache.dtype), _dev(v, cache.dtype)
+    td = _dev(host if host is not None else table, np.int32)
+    pd = _rows_i32(pos, batch, "paged_write: pos")
+    cd = _rows_i32(counts, batch, "paged_write: counts")
+    err = N.DeviceArray.from_host(np.zeros(1, np.int32))
+    N.check(N.lib.nml_paged_write_device(
+        kd.ptr, vd.ptr, cache.kv_heads * seq * cache.dk, seq * cache.dk, cache.dk,
+        cache.k_pages.ptr, cache.v_pages.ptr, td.ptr, N.ptr(pd), N.ptr(cd), batch, cache.kv_heads,
+        seq, max_pages, cache.page_size, cache.num_pages, cache.dk, err.ptr,
+        N.np_dtype_code(cache.dtype)))
+    _check_flag(err, f"paged_write: a position is outside [0, {max_pages * cache.page_size}), a page "
+                     f"outside [0, {cache.num_pages}) or a count outside [0, {seq}]")
+
+
+def paged_attention(q, cache, table, lens, scale, counts=None):
+    """Causal attention of each row's ``counts[b]`` (None: all ``seq``) last cached tokens over its
+    pages: ``q`` (batch, heads, seq, dk), ``table`` (batch, pages of a row), ``lens`` (batch,) tokens
+    cached per row, these included, ``scale`` the sqrt(dk) divisor; query head h reads KV head
+    h // (heads // kv_heads). Returns the merged-head output (batch, seq, heads·dk), zeros for
+    tokens from ``counts[b]`` on and for tokens that see no key. Raises ValueError for a length
+    outside the table, a count outside [0, seq] or a page outside the cache."""
+    host, (batch, max_pages) = _page_table(cache, table, "paged_attention")
+    if len(q.shape) != 4 or q.shape[0] != batch or q.shape[3] != cache.dk:
+        raise ValueError(f"paged_attention: q {q.shape} for {batch} rows, head dim {cache.dk}")
+    if lens is None:
+        raise ValueError("paged_attention: lens is required")
+    if host is not None and not isinstance(lens, N.DeviceArray):
+        _check_pages("paged_attention", host, lens, cache.page_size, cache.num_pages)
+    qd = _dev(q, cache.dtype)
+    _, heads, seq, dk = qd.shape
+    td = _dev(host if host is not None else table, np.int32)
+    ld = _rows_i32(lens, batch, "paged_attention: lens")
+    cd = _rows_i32(counts, batch, "paged_attention: counts")
+    code = N.np_dtype_code(cache.dtype)
+    sizes = (batch, heads, cache.kv_heads, seq, max_pages, cache.page_size)
+    need = C.c_size_t()
+    N.check(N.lib.nml_paged_attention_workspace(*sizes, dk, code, C.byref(need)))
+    ws = N.DeviceArray((need.value,), np.uint8) if need.value else None
+    if ws is not None:
+        N.check(N.lib.nml_memset(ws.ptr, 0, ws.nbytes))
+    out = N.DeviceArray((batch, seq, heads * dk), cache.dtype)
+    if cd is not None:
+        N.check(N.lib.nml_memset(out.ptr, 0, out.nbytes))
+    err = N.DeviceArray.from_host(np.zeros(1, np.int32))
+    N.check(N.lib.nml_paged_attention_device(
+        qd.ptr, cache.k_pages.ptr, cache.v_pages.ptr, td.ptr, ld.ptr, N.ptr(cd), out.ptr, *sizes,
+        cache.num_pages, dk, float(scale), N.ptr(ws), need.value, err.ptr, code))
+    _check_flag(err, f"paged_attention: a length is outside [0, {max_pages * cache.page_size}], a page "
+                     f"outside [0, {cache.num_pages}) or a count outside [0, {seq}]")
+    return out
+
+
+def _teacher_rows(logits, top_ids, top_logits, what):
+    """(logits, ids, values, rows, vocab, entries a row) of a distillation's arguments."""
+    dt = _float_dtype(logits)
+    ld = _dev(logits, dt)
+    vocab = ld.shape[-1]
+    rows = ld.size // vocab
+    idd = _dev(top_ids if isinstance(top_ids, N.DeviceArray) else
+               np.ascontiguousarray(top_ids, dtype=np.int64), np.int64)
+    top_k = idd.shape[-1] if idd.shape else 0
+    yd = _dev(top_logits if isinstance(top_logits, N.DeviceArray) else
+              np.ascontiguousarray(top_logits, dtype=np.float32), np.float32)
+    if idd.size != rows * top_k or yd.shape != idd.shape:
+        raise ValueError(f"{what}: top_ids {idd.shape} and top_logits {yd.shape} for {rows} rows")
+    return ld, idd, yd, rows, vocab, top_k
+
+
+def distill(logits, top_ids, top_logits, temperature=1.0):
+    """KL(q || p) of each row of ``logits`` (..., vocab): p its softmax at ``temperature``, q that of
+    the teacher's ``top_logits`` (..., k) of the tokens ``top_ids`` (..., k; log probabilities will
+    do: ``token_logprobs``' alternatives are such entries); ids of −1 are absent, rows of nothing
+    else give zeros. Returns ``(loss, m, l)``, float32 (rows,) ``DeviceArray``s; m, l: the largest
+    logit and Σ exp((x − m) / temperature). Raises ValueError for an id outside [−1, vocab)."""
+    ld, idd, yd, rows, vocab, top_k = _teacher_rows(logits, top_ids, top_logits, "distill")
+    loss, m, lsum = (N.DeviceArray((rows,), np.float32) for _ in range(3))
+    err = N.DeviceArray.from_host(np.zeros(1, np.int32))
+    N.check(N.lib.nml_distill_device(
+        ld.ptr, vocab, idd.ptr, yd.ptr, rows, vocab, top_k, float(temperature), loss.ptr, m.ptr,
+        lsum.ptr, err.ptr, N.np_dtype_code(ld.dtype)))
+    _check_flag(err, f"distill: an id is outside [-1, {vocab})")
+    return loss, m, lsum
+
+
+def distill_backward(logits, top_ids, top_logits, m, lsum, dloss, temperature=1.0):
+    """The gradient with respect to ``logits`` (its shape and dtype) of Σ dloss·loss, from
+    ``distill``'s ``m`` and ``l``; ``dloss`` (rows,) float32."""
+    ld, idd, yd, rows, vocab, top_k = _teacher_rows(logits, top_ids, top_logits, "distill_backward")
+    stats = [_dev(x, np.float32) for x in (m, lsum, dloss)]
+    for name, x in zip(("m", "l", "dloss"), stats):
+        if x.size != rows:
+            raise ValueError(f"distill_backward: {name} must have {rows} values, got {x.size}")
+    out = N.DeviceArray(ld.shape, ld.dtype)
+    err = N.DeviceArray.from_host(np.zeros(1, np.int32))
+    N.check(N.lib.nml_distill_backward_device(
+        ld.ptr, vocab, idd.ptr, yd.ptr, *(x.ptr for x in stats), rows, vocab, top_k,
+        float(temperature), out.ptr, vocab, err.ptr, N.np_dtype_code(ld.dtype)))
+    _check_flag(err, f"distill_backward: an id is outside [-1, {vocab})")
+    return out
+
+
+def verify_drafts(logits, drafts, uniforms=None, *, draft_logits=None, counts=None, temperature=1.0):
+    """Which drafted tokens stand, and the token after them, so that what a row gains is distributed
+    as sampling from the target alone at ``temperature`` (≤ 0: as its largest logits).
+
+    ``logits`` (batch, n + 1, vocab): the target's after the row's last token and after each draft,
+    as ``GPT.forward_with_cache`` gives them for [last token, *drafts]; ``drafts`` (batch, n);
+    ``draft_logits`` (batch, n, vocab): what the drafts were sampled from at the same temperature (None:
+    they were chosen outright); ``uniforms`` (batch, n + 1) float64 in [0, 1), one a draft and the last
+    for the final token; ``counts`` (batch,) drafts of each row (None: n).
+
+    Returns ``(accepted, tokens)`` as ``DeviceArray``s: int32 (batch,) accepted drafts and int64
+    (batch, n + 1), those drafts, one token more, then −1; ``KVCache.truncate`` takes a cache back to
+    them. Raises ValueError for a draft outside [0, vocab), a count outside [0, n] or a row of
+    logits that decides and has no distribution."""
+    dt = _float_dtype(logits)
+    if len(logits.shape) != 3 or logits.shape[1] < 1:
+        raise ValueError(f"verify_drafts: logits must be (batch, n + 1, vocab), got {logits.shape}")
+    batch, n, vocab = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
+    greedy = temperature <= 0
+    if uniforms is None and not greedy:
+        raise ValueError("verify_drafts: uniforms are required at a temperature above 0")
+    for name, x, shape in (("drafts", drafts, (batch, n)), ("uniforms", uniforms, (batch, n + 1)),
+                           ("draft_logits", draft_logits, (batch, n, vocab))):
+        if x is not None and tuple(np.shape(x)) != shape:
+            raise ValueError(f"verify_drafts: {name} must be {shape}, got {tuple(np.shape(x))}")
+    ld = _dev(logits, dt)
+    dd = _dev(drafts if isinstance(drafts, N.DeviceArray) else
+              np.ascontiguousarray(drafts, dtype=np.int64), np.int64)
+    qd = None if draft_logits is None or greedy else _dev(draft_logits, dt)
+    ud = None if greedy else _dev(uniforms if isinstance(uniforms, N.DeviceArray) else
+                                  np.ascontiguousarray(uniforms, dtype=np.float64), np.float64)
+    cd = _rows_i32(counts, batch, "verify_drafts: counts")
+    need = C.c_size_t()
+    N.check(N.lib.nml_verify_drafts_workspace(batch, n, vocab, C.byref(need)))
+    ws = N.DeviceArray((need.value,), np.uint8)
+    accepted, tokens = N.DeviceArray((batch,), np.int32), N.DeviceArray((batch, n + 1), np.int64)
+    err = N.DeviceArray.from_host(np.zeros(1, np.int32))
+    N.check(N.lib.nml_verify_drafts_device(
+        ld.ptr, vocab, N.ptr(qd), vocab, dd.ptr, N.ptr(cd), N.ptr(ud), batch, n, vocab,
+        float(temperature), accepted.ptr, tokens.ptr, ws.ptr, need.value, err.ptr,
+        N.np_dtype_code(dt)))
+    flag = int(err.numpy()[0])
+    if flag & 1:
+        raise ValueError(f"verify_drafts: a draft is outside [0, {vocab}) or a count outside [0, {n}]")
+    if flag:
+        raise ValueError("verify_drafts: a row of logits holds NaN or infinity, or nothing above -inf")
+    return accepted, tokens
