@@ -6,24 +6,13 @@
 #include <algorithm>
 
 #include "kernels.hpp"
+#include "paged.hpp"
 
 namespace nml {
 
 namespace {
 
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ void tell(int* err) {
-  if (err) __hip_atomic_fetch_or(err, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-// New tokens of row b.
-__device__ __forceinline__ int row_count(const int32_t* counts, int b, int S, int* err) {
-  if (!counts) return S;
-  const int n = counts[b], c = n < 0 ? 0 : (n > S ? S : n);
-  if (c != n) tell(err);
-  return c;
-}
 
 // ------------------------------------------------------------------------- write
 
@@ -121,8 +110,6 @@ int write_launch(PagedWriteArgs a, size_t es, hipStream_t st) {
 // several, as many in all as the card holds at once, and the last to finish merges them in their
 // order.
 
-typedef float f2 __attribute__((ext_vector_type(2)));
-typedef half_t h2 __attribute__((ext_vector_type(2)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 
 constexpr float kSlack = 8.f;  // in powers of two
@@ -150,11 +137,9 @@ __host__ __device__ constexpr int capacity(int nb, int waves) { return 256 * 4 *
 // Spans (a tile for each wave) that a piece has at least: what it costs to begin one and to merge it.
 __host__ __device__ constexpr int least_spans(int waves) { return 4 * 8 / waves; }
 
-// ws: a counter for each tile in pieces (zero before and after every launch, in the same place for
-// calls of any size), then for each piece its rows' references and Σ p, then their Σ p·v. Tiles in
-// pieces are fewer than the card's workgroups (a piece is at least their even share), and so their
-// pieces fewer than twice as many.
-constexpr int kCounters = 4096, kCounterStep = 16;  // a line for each
+// ws: a counter for each tile in pieces, then for each piece its rows' references and Σ p, then their
+// Σ p·v. Tiles in pieces are fewer than the card's workgroups (a piece is at least their even share),
+// and so their pieces fewer than twice as many.
 
 // Places for pieces: those that the tiles' own workgroups leave on the card (a quarter of it where
 // they leave none: for a row much longer than the others).
@@ -257,20 +242,6 @@ __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, int each, int 
   w.b = -1;
   return w;
 }
-
-// The pages of one row and KV head.
-struct RowPages {
-  const int32_t* table;
-  int shift, num_pages, Hkv, hk;
-  // Number of the page of a key, as it stands in the table.
-  __device__ __forceinline__ int number(int key) const { return table[key >> shift]; }
-  // Where that key's vector starts, in vectors. `bad`: the page is out of range (page 0 is read).
-  __device__ __forceinline__ size_t place(int key, int page, bool& bad) const {
-    const bool out = static_cast<unsigned>(page) >= static_cast<unsigned>(num_pages);
-    bad |= out;
-    return ((static_cast<size_t>(out ? 0 : page) * Hkv + hk) << shift) + (key & ((1 << shift) - 1));
-  }
-};
 
 // N values from d0 on of a vector of dk, zeros past its end. VEC: one load (dk and the vectors' places
 // are multiples of N values, so that all are in or out).
@@ -415,17 +386,6 @@ struct Tile<float, NB, VEC> {
           o[W * j + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][j][e], p[r], o[W * j + e], 0, 0, 0);
   }
 };
-
-// Partial results pass between workgroups of any XCD: stores and loads at agent scope (past the
-// L2s) and a count that each workgroup adds to once its stores have arrived.
-__device__ __forceinline__ void put2(float* p, f2 v) {
-  __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), __builtin_bit_cast(unsigned long long, v), __ATOMIC_RELAXED,
-                     __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ f2 get2(const float* p) {
-  return __builtin_bit_cast(f2, __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED,
-                                                  __HIP_MEMORY_SCOPE_AGENT));
-}
 
 template <typename T, int NB, int NW, bool VEC>
 __global__ __launch_bounds__(64 * NW, waves_of(NB)) void paged_attention_kernel(PagedAttnArgs a) {
@@ -644,7 +604,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(NB)) void paged_attention_kernel(
   };
   const int slot_rows = min(16, R);
   const size_t parts = a.slots;  // pieces that ws has room for
-  float* ml = reinterpret_cast<float*>(static_cast<char*>(a.ws) + sizeof(unsigned) * kCounters * kCounterStep);
+  float* ml = reinterpret_cast<float*>(static_cast<char*>(a.ws) + kCounterBytes);
   float* po = ml + parts * slot_rows * 2;
   // (float32: parts times 2^-4 and 2^-12, whose sums of near the largest values stay finite)
   constexpr float kRoom1 = sizeof(T) == 2 ? 0.f : 4.f, kRoom2 = sizeof(T) == 2 ? 0.f : 12.f;
@@ -803,13 +763,18 @@ int launch_paged_write(int dt, const PagedWriteArgs& a, hipStream_t st) {
 }
 
 size_t paged_attention_workspace(int dt, int B, int H, int Hkv, int S, int P, int dk) {
+  // (which kernel takes a call depends on its buffers' alignment too)
+  const size_t many = paged_prefill_applies(dt, H, Hkv, S, dk) ? paged_prefill_workspace(B, H, Hkv, S, P, dk) : 0;
   const Pieces p = dt == F16 ? attention_pieces<half_t>(B, H, Hkv, S, P, dk) : attention_pieces<float>(B, H, Hkv, S, P, dk);
-  if (p.slots == 0) return 0;
+  if (p.slots == 0) return many;
   const long long R = static_cast<long long>(H / Hkv) * S, d = 32 * steps_of(dk);
-  return sizeof(unsigned) * kCounters * kCounterStep + sizeof(float) * p.slots * std::min<long long>(16, R) * (2 + d);
+  return std::max<size_t>(many, kCounterBytes + sizeof(float) * p.slots * std::min<long long>(16, R) * (2 + d));
 }
 
 int launch_paged_attention(int dt, const PagedAttnArgs& a, hipStream_t st) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k_pages) |
+                         reinterpret_cast<uintptr_t>(a.v_pages) | reinterpret_cast<uintptr_t>(a.out);
+  if ((bits & 15) == 0 && paged_prefill_applies(dt, a.H, a.Hkv, a.S, a.dk)) return launch_paged_prefill(dt, a, st);
   return dt == F16 ? attention_launch<half_t>(a, st) : attention_launch<float>(a, st);
 }
 

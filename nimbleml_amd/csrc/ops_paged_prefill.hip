@@ -1,0 +1,462 @@
+// Attention over a paged KV cache for many new tokens: a piece of a prompt behind what the cache
+// holds already.
+//
+// A KV head's queries (its group's heads times the new tokens, the heads of a token side by side) are
+// taken 128 at a time by a workgroup of four waves, 32 a wave, over tiles of 64 keys in LDS:
+//   Sᵀ = K·Qᵀ    v_mfma_f32_32x32x16_f16, Qᵀ in registers; lane l then holds query l % 32 and keys
+//                8(r/4) + 4(l/32) + r % 4 of each 32 in register r;
+//   Oᵀ += Vᵀ·Pᵀ  Pᵀ straight from those registers, Vᵀ by transposing reads of V as it lies in memory,
+//                in the same order of the keys;
+// so that each lane has its own query's maximum, sum and output column. The reference of the
+// exponentials moves only when a maximum passes it by 2^8 in p. Probabilities enter the product with V
+// as float16 and Σ p is of the rounded ones: a rounding of at most 2^-12 of each, of either sign, which
+// leaves an output as far off again as its own rounding to float16 does (2.9·10^-4 of its norm in place
+// of 2.1·10^-4); a second product for the rest would cost half as many matrix instructions again.
+//
+// One barrier a tile: K is written to LDS two tiles ahead and V one, from registers that were loaded a
+// tile before, and the scores of the next tile are formed beside the probabilities of this one. A
+// wave's loads of 16 bytes a lane are of whole rows of one page, whose number is known a tile earlier,
+// so that a load's address is a scalar and a fixed offset of the lane.
+//
+// Where the tiles of queries leave CUs idle the keys are cut into pieces, and the last workgroup of a
+// tile merges them in their order.
+#include <algorithm>
+#include <type_traits>
+
+#include "paged.hpp"
+
+namespace nml {
+
+namespace {
+
+constexpr int kQ = 128, kK = 64, kWaves = 4, kThreads = 64 * kWaves;
+constexpr float kLog2e = 1.44269504088896341f;
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+
+// What a workgroup does: 128 queries from q0 on of KV head hk of row b, key tiles t0 … t0 + nt − 1, piece
+// `piece` of `pieces`.
+struct Tile {
+  int b, hk, q0, len, n, kend, t0, nt, piece, pieces, at;
+};
+
+// Keys a piece has at least, in tiles.
+constexpr int kLeastTiles = 8;
+
+// False: nothing to do.
+__device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int nq, int splits, Tile& w) {
+  const int heads = a.B * a.Hkv, each = nq * splits, n = blockIdx.x;
+  int bh, inner;
+  if (heads % 8 == 0) {  // all of a (row, KV head) on one XCD, whose L2 then holds its keys
+    const int slot = n >> 3;
+    bh = (n & 7) + 8 * (slot / each);
+    inner = slot % each;
+  } else {
+    bh = n / each;
+    inner = n % each;
+  }
+  w.b = bh / a.Hkv;
+  w.hk = bh - w.b * a.Hkv;
+  const int qt = nq - 1 - inner / splits;  // (the last queries have the most keys)
+  w.piece = inner % splits;
+  w.at = bh * nq + qt;
+  w.q0 = qt * kQ;
+  const int len0 = a.lens[w.b], n0 = a.counts ? a.counts[w.b] : a.S;
+  w.len = min(max(len0, 0), a.max_pages << a.shift);
+  w.n = min(max(n0, 0), a.S);
+  if (n == 0 || inner == 0)
+    if ((w.len != len0 || w.n != n0) && threadIdx.x == 0) tell(a.err);
+  if (w.q0 >= w.n * a.group) return false;
+  const int last = min((w.q0 + kQ - 1) / a.group, w.n - 1);  // the last token
+  w.kend = max(w.len - w.n + last + 1, 0);
+  const int tiles = (w.kend + kK - 1) / kK;
+  const int per = max(kLeastTiles, (tiles + splits - 1) / splits);
+  w.pieces = max(1, (tiles + per - 1) / per);
+  if (w.piece >= w.pieces) return false;
+  w.t0 = w.piece * per;
+  w.nt = min(per, tiles - w.t0);
+  return true;
+}
+
+// DK: head dims up to it, in steps of 8.
+template <int DK>
+__global__ __launch_bounds__(kThreads, 2) void paged_prefill_f16_kernel(PagedAttnArgs a, int nq, int splits) {
+#pragma clang fp contract(off)
+  constexpr int KS = DK / 16, OT = DK / 32, VG = DK / 8;
+  constexpr int L = DK <= 64 ? 8 : 16;    // lanes of a row, 16 bytes each
+  constexpr int RW = 64 / L;              // rows of a wave's load
+  constexpr int CH = kK / (RW * kWaves);  // loads of a wave for a tile
+  constexpr int KP = DK + 8, VP = DK == 96 ? DK : DK + 32;  // halves of a row in LDS: V's 16 banks apart for its reads
+  __shared__ __align__(16) half_t Ks[2][kK][KP];
+  __shared__ __align__(16) half_t Vs[2][kK][VP];
+  __shared__ unsigned arrived;
+  Tile w;
+  if (!find_tile(a, nq, splits, w)) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int dk = a.dk, R = w.n * a.group, hi = lane >> 5;
+  const int qw = w.q0 + wave * 32, myq = qw + (lane & 31);  // the wave's first query, this lane's
+  const bool live = myq < R;
+  const int tok = min(myq, R - 1) / a.group, head = w.hk * a.group + min(myq, R - 1) % a.group;
+  const int lim = w.len - w.n + tok;  // the last key that this lane's query sees
+  const float cscale = kLog2e / a.scale;
+  constexpr float kUp = 7.f;  // p times 2^7: at most 2^15, with all of float16's bits down to 2^-21
+  const float lazy = fminf(8.0f / cscale, 3.402823466e38f);
+  const half8 z8 = {0, 0, 0, 0, 0, 0, 0, 0};
+  half8 qb[KS];
+  {
+    const half_t* qp = static_cast<const half_t*>(a.q) + ((static_cast<size_t>(w.b) * a.H + head) * a.S + tok) * dk;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      qb[ks] = live && ks * 16 + hi * 8 < dk ? *reinterpret_cast<const half8*>(qp + ks * 16 + hi * 8) : z8;
+  }
+  // tiles that this wave reads, and the first of them that needs its mask ends past `unmasked`
+  const int wlast = w.len - w.n + min((qw + 31) / a.group, w.n - 1);
+  int ntw = qw >= R || wlast < 0 ? 0 : min(w.nt, max(0, wlast / kK + 1 - w.t0));
+  int unmasked = w.len - w.n + qw / a.group;
+  // (as vector values: scalar tests fold into the loop's, the bodies merge, and head dim 128 spills a
+  // hundred registers)
+  asm volatile("" : "+v"(ntw), "+v"(unmasked));
+
+  // Page numbers of a tile's rows, lane i those of load i; a wave's load i takes rows from
+  // (i·kWaves + wave)·RW on. Past the last key: its page (rows in bounds, that the mask takes out).
+  const RowPages pages{a.table + static_cast<size_t>(w.b) * a.max_pages, a.shift, a.num_pages, a.Hkv, w.hk};
+  const int lastkey = max(w.kend - 1, 0);
+  bool bad = false;
+  auto first_row = [&](int i) { return (i * kWaves + wave) * RW; };
+  auto fetch_ids = [&](int t) { return pages.number(min(t * kK + first_row(lane < CH ? lane : 0), lastkey)); };
+  const int col = lane % L, row = lane / L;
+  const int dpos = col * 8;
+  const bool mine = DK == 64 || DK == 128 ? dpos < dk : col < VG && dpos < dk;
+  const unsigned loff = static_cast<unsigned>((row * dk + (mine ? dpos : 0)) * 2);
+  auto fetch = [&](const void* pool, int t, int ids, half8 (&dst)[CH]) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int key = t * kK + first_row(i);
+      const size_t at = pages.place(key, __builtin_amdgcn_readlane(ids, i), bad);
+      const char* p = static_cast<const char*>(pool) + at * dk * 2;
+      dst[i] = mine ? *reinterpret_cast<const half8*>(p + loff) : z8;
+    }
+  };
+  half8 kn[CH], vn[CH];
+  auto put_k = [&](auto buf_c) {
+    constexpr int buf = decltype(buf_c)::value;
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+      if (VG == L || col < VG) *reinterpret_cast<half8*>(&Ks[buf][first_row(i) + row][dpos]) = kn[i];
+  };
+  auto put_v = [&](auto buf_c, int t) {
+    constexpr int buf = decltype(buf_c)::value;
+    if ((t + 1) * kK > w.kend) {  // (what lies past the last key may be anything)
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
+        if (t * kK + first_row(i) + row >= w.kend) vn[i] = z8;
+    }
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+      if (VG == L || col < VG) *reinterpret_cast<half8*>(&Vs[buf][first_row(i) + row][dpos]) = vn[i];
+  };
+  auto scores = [&](auto buf_c, floatx16 (&s)[2]) {
+    constexpr int buf = decltype(buf_c)::value;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const half8 ka = *reinterpret_cast<const half8*>(&Ks[buf][t * 32 + (lane & 31)][ks * 16 + hi * 8]);
+        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qb[ks], s[t], 0, 0, 0);
+      }
+    }
+  };
+
+  float m = -INFINITY, l = 0.f;  // reference (in units of q·k) and Σ p·2^7 of this lane's query
+  float mnew = -INFINITY;
+  bool grow = false;
+  floatx16 o[OT];
+#pragma unroll
+  for (int t = 0; t < OT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
+
+  // Masking of tile t's scores, their maximum, and the reference that its probabilities will use.
+  auto prep = [&](auto mask_c, int t, floatx16 (&s)[2]) {
+    if constexpr (decltype(mask_c)::value) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = t * kK + u * 32 + 8 * (r >> 2) + 4 * hi + (r & 3);
+          if (key > lim) s[u][r] = -INFINITY;
+        }
+    }
+    float mloc = s[0][0];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (u + r > 0) mloc = fmaxf(mloc, s[u][r]);
+    float mx = fmaxf(m, mloc);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    grow = __any(mx > m + lazy);
+    mnew = grow ? mx : m;
+  };
+  auto masked = [&](int t) { return (t + 1) * kK - 1 > unmasked; };
+
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, 1>;
+  using T_ = std::true_type;
+  using F_ = std::false_type;
+  auto body = [&](auto par_c, auto next_c, auto mask_next_c, int t, floatx16 (&cur)[2], floatx16 (&nxt)[2]) {
+    constexpr int PAR = decltype(par_c)::value;
+    constexpr bool NEXT = decltype(next_c)::value;
+    if (grow) {
+      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m * cscale - mnew * cscale);
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < OT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+    }
+    m = mnew;
+    if constexpr (NEXT) scores(std::integral_constant<int, PAR ^ 1>{}, nxt);
+    const float nmx = kUp - (m == -INFINITY ? 0.f : m) * cscale;
+    const half2v ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
+    half8 pb[4];
+#pragma unroll
+    for (int blk = 0; blk < 4; ++blk)
+#pragma unroll
+      for (int jj = 0; jj < 8; jj += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[blk >> 1][8 * (blk & 1) + jj], cscale, nmx));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[blk >> 1][8 * (blk & 1) + jj + 1], cscale, nmx));
+        const half2v pp = {static_cast<_Float16>(p0), static_cast<_Float16>(p1)};
+        l = __builtin_amdgcn_fdot2(pp, ones, l, false);
+        pb[blk][jj] = pp[0];
+        pb[blk][jj + 1] = pp[1];
+      }
+#pragma unroll
+    for (int blk = 0; blk < 4; ++blk) {
+      // k-slot j of lane half hi: key 8(j / 4) + 4·hi + j % 4 of the 16. A transposing read gives a lane
+      // four keys of its dim from the rows that its 16 lanes point at, 8 bytes each.
+      typedef __attribute__((address_space(3))) s4 lds_s4;
+      const half_t* at = &Vs[PAR][blk * 16 + 4 * hi + ((lane & 15) >> 2)][16 * ((lane >> 4) & 1) + 4 * (lane & 3)];
+#pragma unroll
+      for (int d = 0; d < OT; ++d) {
+        const s4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + d * 32));
+        const s4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + d * 32 + 8 * VP));
+        const half8 va = __builtin_bit_cast(half8, s8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pb[blk], o[d], 0, 0, 0);
+      }
+    }
+    if constexpr (NEXT) prep(mask_next_c, t + 1, nxt);
+  };
+  int ids_v = 0, ids_k = 0;  // of the next tiles to load
+  auto iter = [&](auto par_c, int j, floatx16 (&cur)[2], floatx16 (&nxt)[2]) {
+    constexpr int PAR = decltype(par_c)::value;
+    const int t = w.t0 + j;
+    __syncthreads();
+    if (j + 2 < w.nt) put_k(par_c);
+    if (j + 1 < w.nt) put_v(std::integral_constant<int, PAR ^ 1>{}, t + 1);
+    if (j + 2 < w.nt) fetch(a.v_pages, t + 2, ids_v, vn);
+    if (j + 3 < w.nt) fetch(a.k_pages, t + 3, ids_k, kn);
+    ids_v = ids_k;
+    if (j + 4 < w.nt) ids_k = fetch_ids(t + 4);
+    if (j >= ntw) return;
+    if (j + 1 >= ntw)
+      body(par_c, F_{}, F_{}, t, cur, nxt);
+    else if (masked(t + 1))
+      body(par_c, T_{}, T_{}, t, cur, nxt);
+    else
+      body(par_c, T_{}, F_{}, t, cur, nxt);
+  };
+
+  floatx16 sA[2], sB[2];
+  if (w.nt > 0) {  // K(0), V(0), K(1) into LDS; K(2), V(1) into registers; tile 0's scores
+    const int t = w.t0, i0 = fetch_ids(t), i1 = fetch_ids(t + 1);
+    ids_v = fetch_ids(t + 2);
+    ids_k = fetch_ids(t + 3);
+    fetch(a.k_pages, t, i0, kn);
+    fetch(a.v_pages, t, i0, vn);
+    put_k(I0{});
+    put_v(I0{}, t);
+    if (w.nt > 1) {
+      fetch(a.k_pages, t + 1, i1, kn);
+      fetch(a.v_pages, t + 1, i1, vn);
+      put_k(I1{});
+    }
+    if (w.nt > 2) fetch(a.k_pages, t + 2, ids_v, kn);
+    __syncthreads();
+    if (ntw > 0) {
+      scores(I0{}, sA);
+      if (masked(t))
+        prep(T_{}, t, sA);
+      else
+        prep(F_{}, t, sA);
+    }
+  }
+  for (int j = 0; j < w.nt; j += 2) {
+    iter(I0{}, j, sA, sB);
+    if (j + 1 < w.nt) iter(I1{}, j + 1, sB, sA);
+  }
+  if (__any(bad) && lane == 0) tell(a.err);
+  l += __shfl_xor(l, 32, 64);
+
+  // An infinite or NaN value makes 0·∞ of keys that a query does not see: outputs that are not
+  // finite are formed again, key by key, keys without weight left out.
+  {
+    bool wrong = false;
+#pragma unroll
+    for (int d = 0; d < OT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) wrong |= !__builtin_isfinite(o[d][r]);
+    if (__any(wrong && live)) {
+      const float nmx = kUp - (m == -INFINITY ? 0.f : m) * cscale;
+      floatx16 fresh[OT];
+#pragma unroll
+      for (int d = 0; d < OT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) fresh[d][r] = 0.f;
+      const int end = min(min(w.kend, (w.t0 + w.nt) * kK), wlast + 1);
+      for (int key = w.t0 * kK; key < end; ++key) {
+        const size_t at = pages.place(key, pages.number(key), bad) * dk;
+        const half_t *kr = static_cast<const half_t*>(a.k_pages) + at, *vr = static_cast<const half_t*>(a.v_pages) + at;
+        int h = hi;
+        asm volatile("" : "+v"(h));  // (the bounds tests formed here, not kept for the loop)
+        float s = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          if (ks * 16 + h * 8 < dk) {
+            const half8 kk = *reinterpret_cast<const half8*>(kr + ks * 16 + h * 8);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              s = __builtin_fmaf(static_cast<float>(qb[ks][e]), static_cast<float>(kk[e]), s);
+          }
+        s += __shfl_xor(s, 32, 64);
+        const float p = key > lim ? 0.f : static_cast<float>(static_cast<half_t>(__builtin_amdgcn_exp2f(__builtin_fmaf(s, cscale, nmx))));
+        if (p != 0.f) {
+#pragma unroll
+          for (int d = 0; d < OT; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int dim = d * 32 + 8 * (r >> 2) + 4 * h + (r & 3);
+              if (dim < dk) fresh[d][r] = __builtin_fmaf(p, static_cast<float>(vr[dim]), fresh[d][r]);
+            }
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < OT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!__builtin_isfinite(o[d][r])) o[d][r] = fresh[d][r];
+    }
+  }
+
+  half_t* out = static_cast<half_t*>(a.out) + ((static_cast<size_t>(w.b) * a.S + tok) * a.H + head) * dk;
+  if (w.pieces == 1) {
+    if (!live) return;
+    const float inv = lim < 0 ? 0.f : 1.f / l;
+#pragma unroll
+    for (int d = 0; d < OT; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int dim = d * 32 + 8 * g + 4 * hi;
+        half4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = static_cast<half_t>(lim < 0 ? 0.f : o[d][4 * g + e] * inv);
+        if (dim < dk) *reinterpret_cast<half4*>(out + dim) = v;
+      }
+    return;
+  }
+  // A piece's part: per query its reference and Σ p, then its Σ p·v, four dims at a time.
+  float* ml = reinterpret_cast<float*>(static_cast<char*>(a.ws) + kCounterBytes);
+  float* po = ml + static_cast<size_t>(a.slots) * kQ * 2;
+  const size_t slot = static_cast<size_t>(w.at) * splits + w.piece;
+  {
+    const size_t q = slot * kQ + wave * 32 + (lane & 31);
+    if (hi == 0) put2(ml + 2 * q, f2{m == -INFINITY ? m : m * cscale, l});
+#pragma unroll
+    for (int d = 0; d < OT; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float* to = po + q * DK + d * 32 + 8 * g + 4 * hi;
+        put2(to, f2{o[d][4 * g], o[d][4 * g + 1]});
+        put2(to + 2, f2{o[d][4 * g + 2], o[d][4 * g + 3]});
+      }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  unsigned* counter = static_cast<unsigned*>(a.ws) + static_cast<size_t>(w.at) * kCounterStep;
+  if (tid == 0) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (arrived + 1 != static_cast<unsigned>(w.pieces)) return;
+  if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const int rows = min(kQ, R - w.q0);
+  for (int i = tid; i < rows * (DK / 4); i += kThreads) {
+    const int c = i / (DK / 4), d = (i % (DK / 4)) * 4;
+    const size_t first = static_cast<size_t>(w.at) * splits;
+    float top = -INFINITY;
+    for (int y = 0; y < w.pieces; ++y) top = fmaxf(top, get2(ml + 2 * ((first + y) * kQ + c)).x);
+    const float rf = top == -INFINITY ? 0.f : top;
+    float lt = 0.f;
+    floatx4 ot = {0.f, 0.f, 0.f, 0.f};
+    for (int y = 0; y < w.pieces; ++y) {
+      const size_t q = (first + y) * kQ + c;
+      const f2 st = get2(ml + 2 * q), x0 = get2(po + q * DK + d), x1 = get2(po + q * DK + d + 2);
+      const float f = __builtin_amdgcn_exp2f(st.x - rf);
+      lt += st.y * f;
+      ot += floatx4{x0.x, x0.y, x1.x, x1.y} * f;
+    }
+    const int rr = w.q0 + c, tk = rr / a.group;
+    if (d >= dk) continue;
+    half_t* to = static_cast<half_t*>(a.out) + ((static_cast<size_t>(w.b) * a.S + tk) * a.H + w.hk * a.group + rr % a.group) * dk + d;
+    const bool sees = w.len - w.n + tk >= 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) to[e] = static_cast<half_t>(sees ? ot[e] / lt : 0.f);
+  }
+}
+
+// Tiles of 128 queries, and into how many pieces the keys of one are cut: as many workgroups as
+// the card holds at once (two a CU), where the tiles alone are fewer.
+constexpr int kHeld = 512;
+struct Grid {
+  long long tiles;
+  int nq, splits;
+};
+Grid grid_of(int B, int H, int Hkv, int S, int P) {
+  Grid g;
+  g.nq = (H / Hkv * S + kQ - 1) / kQ;
+  g.tiles = static_cast<long long>(g.nq) * Hkv * B;
+  const int most = std::max(1, (P + kK - 1) / kK / kLeastTiles);
+  g.splits = static_cast<int>(std::min<long long>(most, std::max<long long>(1, kHeld / g.tiles)));
+  return g;
+}
+
+template <int DK>
+int launch_f16(PagedAttnArgs a, hipStream_t st) {
+  const Grid g = grid_of(a.B, a.H, a.Hkv, a.S, a.max_pages << a.shift);
+  a.slots = g.splits > 1 ? static_cast<int>(g.tiles * g.splits) : 0;
+  paged_prefill_f16_kernel<DK><<<static_cast<unsigned>(g.tiles * g.splits), kThreads, 0, st>>>(a, g.nq, g.splits);
+  NML_LAUNCHED();
+  return 0;
+}
+
+}  // namespace
+
+bool paged_prefill_applies(int dt, int H, int Hkv, int S, int dk) {
+  return dt == F16 && dk <= 128 && dk % 8 == 0 && S > 1 && H / Hkv * S >= 64;
+}
+
+size_t paged_prefill_workspace(int B, int H, int Hkv, int S, int P, int dk) {
+  const Grid g = grid_of(B, H, Hkv, S, P);
+  if (g.splits == 1) return 0;
+  const size_t d = dk <= 64 ? 64 : dk <= 96 ? 96 : 128;
+  return kCounterBytes + sizeof(float) * g.tiles * g.splits * kQ * (2 + d);
+}
+
+int launch_paged_prefill(int dt, const PagedAttnArgs& a, hipStream_t st) {
+  if (a.dk <= 64) return launch_f16<64>(a, st);
+  if (a.dk <= 96) return launch_f16<96>(a, st);
+  return launch_f16<128>(a, st);
+}
+
+}  // namespace nml
