@@ -764,7 +764,7 @@ int launch_paged_write(int dt, const PagedWriteArgs& a, hipStream_t st) {
 
 size_t paged_attention_workspace(int dt, int B, int H, int Hkv, int S, int P, int dk) {
   // (which kernel takes a call depends on its buffers' alignment too)
-  const size_t many = paged_prefill_applies(dt, H, Hkv, S, dk) ? paged_prefill_workspace(B, H, Hkv, S, P, dk) : 0;
+  const size_t many = paged_prefill_applies(dt, H, Hkv, S, dk) ? paged_prefill_workspace(dt, B, H, Hkv, S, P, dk) : 0;
   const Pieces p = dt == F16 ? attention_pieces<half_t>(B, H, Hkv, S, P, dk) : attention_pieces<float>(B, H, Hkv, S, P, dk);
   if (p.slots == 0) return many;
   const long long R = static_cast<long long>(H / Hkv) * S, d = 32 * steps_of(dk);

@@ -18,8 +18,8 @@
 // wave's loads of 16 bytes a lane are of whole rows of one page, whose number is known a tile earlier,
 // so that a load's address is a scalar and a fixed offset of the lane.
 //
-// Where the tiles of queries leave CUs idle the keys are cut into pieces, and the last workgroup of a
-// tile merges them in their order.
+// Where the tiles of queries leave CUs idle the keys are cut into pieces, whose parts a second launch
+// merges.
 #include <algorithm>
 #include <type_traits>
 
@@ -35,17 +35,37 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 typedef short s8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
-// What a workgroup does: 128 queries from q0 on of KV head hk of row b, key tiles t0 … t0 + nt − 1, piece
-// `piece` of `pieces`.
+// Keys a piece has at least, in tiles.
+constexpr int kLeastTiles = 8;
+
+// The keys of 128 queries, from q0 on of (row, KV head) bh: length and new tokens of the row, keys that a
+// query of them sees, key tiles a piece and pieces. n·group ≤ q0: no queries.
+struct Span {
+  int len, n, kend, per, pieces;
+  bool good;  // length and count were in range
+};
+__device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int bh, int q0, int splits) {
+  Span w;
+  const int b = bh / a.Hkv, len = a.lens[b], n = a.counts ? a.counts[b] : a.S;
+  w.len = min(max(len, 0), a.max_pages << a.shift);
+  w.n = min(max(n, 0), a.S);
+  w.good = w.len == len && w.n == n;
+  const int last = min((q0 + kQ - 1) / a.group, w.n - 1);  // the last token
+  w.kend = max(w.len - w.n + last + 1, 0);
+  const int tiles = (w.kend + kK - 1) / kK;
+  w.per = max(kLeastTiles, (tiles + splits - 1) / splits);
+  w.pieces = q0 >= w.n * a.group ? 0 : max(1, (tiles + w.per - 1) / w.per);
+  return w;
+}
+
+// What a workgroup does: queries from q0 on of KV head hk of row b, key tiles t0 … t0 + nt − 1, piece
+// `piece` of w.pieces of tile `at`.
 struct Tile {
   int b, hk, q0, len, n, kend, t0, nt, piece, pieces, at;
 };
 
-// Keys a piece has at least, in tiles.
-constexpr int kLeastTiles = 8;
-
 // False: nothing to do.
-__device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int nq, int splits, Tile& w) {
+__device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int nq, int splits, Tile& t) {
   const int heads = a.B * a.Hkv, each = nq * splits, n = blockIdx.x;
   int bh, inner;
   if (heads % 8 == 0) {  // all of a (row, KV head) on one XCD, whose L2 then holds its keys
@@ -56,27 +76,66 @@ __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int nq, int sp
     bh = n / each;
     inner = n % each;
   }
-  w.b = bh / a.Hkv;
-  w.hk = bh - w.b * a.Hkv;
+  t.b = bh / a.Hkv;
+  t.hk = bh - t.b * a.Hkv;
   const int qt = nq - 1 - inner / splits;  // (the last queries have the most keys)
-  w.piece = inner % splits;
-  w.at = bh * nq + qt;
-  w.q0 = qt * kQ;
-  const int len0 = a.lens[w.b], n0 = a.counts ? a.counts[w.b] : a.S;
-  w.len = min(max(len0, 0), a.max_pages << a.shift);
-  w.n = min(max(n0, 0), a.S);
-  if (n == 0 || inner == 0)
-    if ((w.len != len0 || w.n != n0) && threadIdx.x == 0) tell(a.err);
-  if (w.q0 >= w.n * a.group) return false;
-  const int last = min((w.q0 + kQ - 1) / a.group, w.n - 1);  // the last token
-  w.kend = max(w.len - w.n + last + 1, 0);
-  const int tiles = (w.kend + kK - 1) / kK;
-  const int per = max(kLeastTiles, (tiles + splits - 1) / splits);
-  w.pieces = max(1, (tiles + per - 1) / per);
-  if (w.piece >= w.pieces) return false;
-  w.t0 = w.piece * per;
-  w.nt = min(per, tiles - w.t0);
+  t.piece = inner % splits;
+  t.at = bh * nq + qt;
+  t.q0 = qt * kQ;
+  const Span w = span_of(a, bh, t.q0, splits);
+  if (inner == 0 && !w.good && threadIdx.x == 0) tell(a.err);
+  if (t.piece >= w.pieces) return false;
+  t.len = w.len;
+  t.n = w.n;
+  t.kend = w.kend;
+  t.pieces = w.pieces;
+  t.t0 = t.piece * w.per;
+  t.nt = min(w.per, (w.kend + kK - 1) / kK - t.t0);
   return true;
+}
+
+// Where a piece's part goes: per query its reference (in powers of two) and Σ p, then its Σ p·v.
+struct Parts {
+  float *ml, *po;
+  __device__ Parts(const PagedAttnArgs& a) {
+    ml = reinterpret_cast<float*>(static_cast<char*>(a.ws) + kCounterBytes);  // (behind what other calls keep there)
+    po = ml + static_cast<size_t>(a.slots) * kQ * 2;
+  }
+};
+
+// The pieces' parts merged in their order, four dims of a query a thread. (A launch of its own: by the
+// last workgroup of a tile, as in ops_paged.hip, 32 pieces of 128 queries took 100 µs.)
+template <typename T, int DK>
+__global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttnArgs a, int nq, int splits) {
+  constexpr int Q = DK / 4, kRows = kThreads / Q, kBlocks = (kQ + kRows - 1) / kRows;
+  const int at = blockIdx.x / kBlocks, bh = at / nq, q0 = (at - bh * nq) * kQ;
+  const Span w = span_of(a, bh, q0, splits);
+  if (w.pieces <= 1) return;
+  const int c = blockIdx.x % kBlocks * kRows + threadIdx.x / Q, d = threadIdx.x % Q * 4;
+  if (threadIdx.x / Q >= kRows || c >= kQ || q0 + c >= w.n * a.group || d >= a.dk) return;
+  const Parts parts(a);
+  const size_t first = static_cast<size_t>(at) * splits;
+  // (float32: parts times 2^-12, whose sums of near the largest values stay finite)
+  constexpr float kRoom = sizeof(T) == 2 ? 0.f : 12.f;
+  float top = -INFINITY;
+  for (int y = 0; y < w.pieces; ++y) top = fmaxf(top, parts.ml[2 * ((first + y) * kQ + c)]);
+  const float rf = (top == -INFINITY ? 0.f : top) + kRoom;
+  float lt = 0.f;
+  floatx4 ot = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int y = 0; y < w.pieces; ++y) {
+    const size_t q = (first + y) * kQ + c;
+    const f2 st = *reinterpret_cast<const f2*>(parts.ml + 2 * q);
+    const floatx4 x = *reinterpret_cast<const floatx4*>(parts.po + q * DK + d);
+    const float f = __builtin_amdgcn_exp2f(st.x - rf);
+    lt += st.y * f;
+    ot += x * f;
+  }
+  const int rr = q0 + c, tk = rr / a.group, b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  T* to = static_cast<T*>(a.out) + ((static_cast<size_t>(b) * a.S + tk) * a.H + hk * a.group + rr % a.group) * a.dk + d;
+  const bool sees = w.len - w.n + tk >= 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) to[e] = static_cast<T>(sees ? ot[e] / lt : 0.f);
 }
 
 // DK: head dims up to it, in steps of 8.
@@ -90,7 +149,6 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prefill_f16_kernel(PagedAtt
   constexpr int KP = DK + 8, VP = DK == 96 ? DK : DK + 32;  // halves of a row in LDS: V's 16 banks apart for its reads
   __shared__ __align__(16) half_t Ks[2][kK][KP];
   __shared__ __align__(16) half_t Vs[2][kK][VP];
-  __shared__ unsigned arrived;
   Tile w;
   if (!find_tile(a, nq, splits, w)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -351,9 +409,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prefill_f16_kernel(PagedAtt
     }
   }
 
-  half_t* out = static_cast<half_t*>(a.out) + ((static_cast<size_t>(w.b) * a.S + tok) * a.H + head) * dk;
   if (w.pieces == 1) {
     if (!live) return;
+    half_t* out = static_cast<half_t*>(a.out) + ((static_cast<size_t>(w.b) * a.S + tok) * a.H + head) * dk;
     const float inv = lim < 0 ? 0.f : 1.f / l;
 #pragma unroll
     for (int d = 0; d < OT; ++d)
@@ -367,52 +425,244 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prefill_f16_kernel(PagedAtt
       }
     return;
   }
-  // A piece's part: per query its reference and Σ p, then its Σ p·v, four dims at a time.
-  float* ml = reinterpret_cast<float*>(static_cast<char*>(a.ws) + kCounterBytes);
-  float* po = ml + static_cast<size_t>(a.slots) * kQ * 2;
-  const size_t slot = static_cast<size_t>(w.at) * splits + w.piece;
+  const Parts parts(a);
+  const size_t q = (static_cast<size_t>(w.at) * splits + w.piece) * kQ + wave * 32 + (lane & 31);
+  if (hi == 0) *reinterpret_cast<f2*>(parts.ml + 2 * q) = f2{m == -INFINITY ? m : m * cscale, l};
+#pragma unroll
+  for (int d = 0; d < OT; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      floatx4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = o[d][4 * g + e];
+      *reinterpret_cast<floatx4*>(parts.po + q * DK + d * 32 + 8 * g + 4 * hi) = v;
+    }
+}
+
+// float32: the same tiles on v_mfma_f32_32x32x2f32, whose two steps of a contraction are dims 8i + e and
+// 8i + 4 + e of K, so that a lane's 16 bytes of a row feed four of them, and whose 32 rows are every W-th
+// dim of V, so that one read feeds W tiles of the output. A tile of keys costs 16 times the cycles on
+// the matrix pipe that its softmax takes beside it: one buffer and two barriers a tile, with the other
+// workgroup of the CU in between.
+template <int DK>
+__global__ __launch_bounds__(kThreads, 2) void paged_prefill_f32_kernel(PagedAttnArgs a, int nq, int splits) {
+  constexpr int KS = DK / 8, OT = DK / 32, VG = DK / 4;
+  constexpr int W = OT == 3 ? 1 : OT;
+  constexpr int L = DK == 32 ? 8 : DK == 64 ? 16 : 32;  // lanes of a row, 16 bytes each
+  constexpr int RW = 64 / L, CH = kK / (RW * kWaves);
+  constexpr int P = DK + 4;  // floats of a row in LDS
+  typedef float vecw __attribute__((ext_vector_type(W)));
+  __shared__ __align__(16) float Ks[kK][P];
+  __shared__ __align__(16) float Vs[kK][P];
+  Tile w;
+  if (!find_tile(a, nq, splits, w)) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int dk = a.dk, R = w.n * a.group, hi = lane >> 5, l32 = lane & 31;
+  const int qw = w.q0 + wave * 32, myq = qw + l32;
+  const bool live = myq < R;
+  const int tok = min(myq, R - 1) / a.group, head = w.hk * a.group + min(myq, R - 1) % a.group;
+  const int lim = w.len - w.n + tok;
+  const float cscale = kLog2e / a.scale;
+  const float lazy = fminf(8.0f / cscale, 3.402823466e38f);
+  const floatx4 z4 = {0.f, 0.f, 0.f, 0.f};
+  floatx4 qb[KS];
   {
-    const size_t q = slot * kQ + wave * 32 + (lane & 31);
-    if (hi == 0) put2(ml + 2 * q, f2{m == -INFINITY ? m : m * cscale, l});
+    const float* qp = static_cast<const float*>(a.q) + ((static_cast<size_t>(w.b) * a.H + head) * a.S + tok) * dk;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      qb[ks] = live && ks * 8 + hi * 4 < dk ? *reinterpret_cast<const floatx4*>(qp + ks * 8 + hi * 4) : z4;
+  }
+  const int wlast = w.len - w.n + min((qw + 31) / a.group, w.n - 1);
+  const int ntw = qw >= R || wlast < 0 ? 0 : min(w.nt, max(0, wlast / kK + 1 - w.t0));
+  const int unmasked = w.len - w.n + qw / a.group;
+
+  const RowPages pages{a.table + static_cast<size_t>(w.b) * a.max_pages, a.shift, a.num_pages, a.Hkv, w.hk};
+  const int lastkey = max(w.kend - 1, 0);
+  bool bad = false;
+  auto first_row = [&](int i) { return (i * kWaves + wave) * RW; };
+  auto fetch_ids = [&](int t) { return pages.number(min(t * kK + first_row(lane < CH ? lane : 0), lastkey)); };
+  const int col = lane % L, row = lane / L, dpos = col * 4;
+  const bool mine = dpos < dk, stores = VG == L || col < VG;
+  const unsigned loff = static_cast<unsigned>((row * dk + (mine ? dpos : 0)) * 4);
+  floatx4 kn[CH], vn[CH];
+  auto fetch = [&](int t, int ids) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const size_t at = pages.place(t * kK + first_row(i), __builtin_amdgcn_readlane(ids, i), bad) * dk * 4 + loff;
+      kn[i] = mine ? *reinterpret_cast<const floatx4*>(static_cast<const char*>(a.k_pages) + at) : z4;
+      vn[i] = mine ? *reinterpret_cast<const floatx4*>(static_cast<const char*>(a.v_pages) + at) : z4;
+    }
+  };
+  auto put = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+      if (stores) {
+        const int r = first_row(i) + row;
+        *reinterpret_cast<floatx4*>(&Ks[r][dpos]) = kn[i];
+        // (what lies past the last key may be anything)
+        *reinterpret_cast<floatx4*>(&Vs[r][dpos]) = t * kK + r < w.kend ? vn[i] : z4;
+      }
+  };
+  float m = -INFINITY, l = 0.f;
+  floatx16 o[OT];
+#pragma unroll
+  for (int d = 0; d < OT; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+  int ids = 0;
+  if (w.nt > 0) {
+    fetch(w.t0, fetch_ids(w.t0));
+    ids = fetch_ids(w.t0 + 1);
+  }
+  for (int j = 0; j < w.nt; ++j) {
+    const int t = w.t0 + j;
+    __syncthreads();  // (the tile before is read)
+    put(t);
+    __syncthreads();
+    if (j + 1 < w.nt) fetch(t + 1, ids);
+    if (j + 2 < w.nt) ids = fetch_ids(t + 2);
+    if (j >= ntw) continue;
+    floatx16 s[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const floatx4 ka = *reinterpret_cast<const floatx4*>(&Ks[u * 32 + l32][ks * 8 + hi * 4]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(ka[e], qb[ks][e], s[u], 0, 0, 0);
+      }
+    }
+    if ((t + 1) * kK - 1 > unmasked) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (t * kK + u * 32 + 8 * (r >> 2) + 4 * hi + (r & 3) > lim) s[u][r] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[u][r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    if (__any(mx > m + lazy)) {
+      mx = fmaxf(mx, m);
+      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mx) * cscale);
+      m = mx;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < OT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float p = __builtin_amdgcn_exp2f((s[u][r] - ref) * cscale);
+        l += p;
+        s[u][r] = p;
+      }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float* vrow = &Vs[u * 32 + 8 * (r >> 2) + 4 * hi + (r & 3)][W * l32];
+#pragma unroll
+        for (int d = 0; d < OT; d += W) {
+          const vecw v = *reinterpret_cast<const vecw*>(vrow + 32 * d);
+#pragma unroll
+          for (int e = 0; e < W; ++e) o[d + e] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[e], s[u][r], o[d + e], 0, 0, 0);
+        }
+      }
+  }
+  if (__any(bad) && lane == 0) tell(a.err);
+  l += __shfl_xor(l, 32, 64);
+  // dim of register r of output tile d
+  auto dim_of = [&](int d, int r, int h) { return 32 * W * (d / W) + W * (8 * (r >> 2) + 4 * h + (r & 3)) + d % W; };
+  float ref = m == -INFINITY ? m : m * cscale;  // in powers of two
+
+  // Outputs that are not finite are formed again, as in the float16 kernel, of probabilities 2^-lift as
+  // large: sums of values near float32's largest pass its range too.
+  {
+    bool wrong = false;
 #pragma unroll
     for (int d = 0; d < OT; ++d)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float* to = po + q * DK + d * 32 + 8 * g + 4 * hi;
-        put2(to, f2{o[d][4 * g], o[d][4 * g + 1]});
-        put2(to + 2, f2{o[d][4 * g + 2], o[d][4 * g + 3]});
-      }
-  }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  unsigned* counter = static_cast<unsigned*>(a.ws) + static_cast<size_t>(w.at) * kCounterStep;
-  if (tid == 0) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  if (arrived + 1 != static_cast<unsigned>(w.pieces)) return;
-  if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  const int rows = min(kQ, R - w.q0);
-  for (int i = tid; i < rows * (DK / 4); i += kThreads) {
-    const int c = i / (DK / 4), d = (i % (DK / 4)) * 4;
-    const size_t first = static_cast<size_t>(w.at) * splits;
-    float top = -INFINITY;
-    for (int y = 0; y < w.pieces; ++y) top = fmaxf(top, get2(ml + 2 * ((first + y) * kQ + c)).x);
-    const float rf = top == -INFINITY ? 0.f : top;
-    float lt = 0.f;
-    floatx4 ot = {0.f, 0.f, 0.f, 0.f};
-    for (int y = 0; y < w.pieces; ++y) {
-      const size_t q = (first + y) * kQ + c;
-      const f2 st = get2(ml + 2 * q), x0 = get2(po + q * DK + d), x1 = get2(po + q * DK + d + 2);
-      const float f = __builtin_amdgcn_exp2f(st.x - rf);
-      lt += st.y * f;
-      ot += floatx4{x0.x, x0.y, x1.x, x1.y} * f;
-    }
-    const int rr = w.q0 + c, tk = rr / a.group;
-    if (d >= dk) continue;
-    half_t* to = static_cast<half_t*>(a.out) + ((static_cast<size_t>(w.b) * a.S + tk) * a.H + w.hk * a.group + rr % a.group) * dk + d;
-    const bool sees = w.len - w.n + tk >= 0;
+      for (int r = 0; r < 16; ++r) wrong |= !__builtin_isfinite(o[d][r]);
+    if (__any(wrong && live)) {
+      const float lift = 40.f - static_cast<float>(__builtin_clz(w.len)), f = __builtin_amdgcn_exp2f(-lift);
+      const float base = m == -INFINITY ? 0.f : m;
+      if (m != -INFINITY) ref += lift;
+      l *= f;
+      floatx16 fresh[OT];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) to[e] = static_cast<half_t>(sees ? ot[e] / lt : 0.f);
+      for (int d = 0; d < OT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) fresh[d][r] = 0.f;
+      const int end = min(min(w.kend, (w.t0 + w.nt) * kK), wlast + 1);
+      for (int key = w.t0 * kK; key < end; ++key) {
+        const size_t at = pages.place(key, pages.number(key), bad) * dk;
+        const float *kr = static_cast<const float*>(a.k_pages) + at, *vr = static_cast<const float*>(a.v_pages) + at;
+        int h = hi, c = l32;
+        asm volatile("" : "+v"(h), "+v"(c));  // (the bounds tests formed here, not kept for the loop)
+        float x = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          if (ks * 8 + h * 4 < dk) {
+            const floatx4 kk = *reinterpret_cast<const floatx4*>(kr + ks * 8 + h * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x = __builtin_fmaf(qb[ks][e], kk[e], x);
+          }
+        x += __shfl_xor(x, 32, 64);
+        const float p = key > lim ? 0.f : __builtin_amdgcn_exp2f((x - base) * cscale - lift);
+        if (p != 0.f) {
+#pragma unroll
+          for (int d = 0; d < OT; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int dim = dim_of(d, r, h);
+              if (dim < dk) fresh[d][r] = __builtin_fmaf(p, vr[dim], fresh[d][r]);
+            }
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < OT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = __builtin_isfinite(o[d][r]) ? o[d][r] * f : fresh[d][r];
+    }
   }
+
+  // two neighbouring dims at a time
+  auto each_pair = [&](auto f) {
+    if constexpr (W == 1) {
+#pragma unroll
+      for (int d = 0; d < OT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) f(dim_of(d, r, hi), f2{o[d][r], o[d][r + 1]});
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int d = 0; d < OT; d += 2) f(dim_of(d, r, hi), f2{o[d][r], o[d + 1][r]});
+    }
+  };
+  if (w.pieces == 1) {
+    if (!live) return;
+    float* out = static_cast<float*>(a.out) + ((static_cast<size_t>(w.b) * a.S + tok) * a.H + head) * dk;
+    const float inv = lim < 0 ? 0.f : 1.f / l;
+    each_pair([&](int dim, f2 v) {
+      if (dim < dk) *reinterpret_cast<f2*>(out + dim) = lim < 0 ? f2{0.f, 0.f} : f2{v.x * inv, v.y * inv};
+    });
+    return;
+  }
+  const Parts parts(a);
+  const size_t q = (static_cast<size_t>(w.at) * splits + w.piece) * kQ + wave * 32 + l32;
+  if (hi == 0) *reinterpret_cast<f2*>(parts.ml + 2 * q) = f2{ref, l};
+  each_pair([&](int dim, f2 v) { *reinterpret_cast<f2*>(parts.po + q * DK + dim) = v; });
 }
 
 // Tiles of 128 queries, and into how many pieces the keys of one are cut: as many workgroups as
@@ -431,11 +681,24 @@ Grid grid_of(int B, int H, int Hkv, int S, int P) {
   return g;
 }
 
+// Columns of the kernel that takes a head dim.
+int columns_of(int dt, int dk) { return dk <= 32 && dt == F32 ? 32 : dk <= 64 ? 64 : dk <= 96 ? 96 : 128; }
+
 template <int DK>
-int launch_f16(PagedAttnArgs a, hipStream_t st) {
-  const Grid g = grid_of(a.B, a.H, a.Hkv, a.S, a.max_pages << a.shift);
-  a.slots = g.splits > 1 ? static_cast<int>(g.tiles * g.splits) : 0;
-  paged_prefill_f16_kernel<DK><<<static_cast<unsigned>(g.tiles * g.splits), kThreads, 0, st>>>(a, g.nq, g.splits);
+int launch_columns(int dt, const PagedAttnArgs& a, const Grid& g, hipStream_t st) {
+  const unsigned n = static_cast<unsigned>(g.tiles * g.splits);
+  if constexpr (DK > 32) {
+    if (dt == F16) paged_prefill_f16_kernel<DK><<<n, kThreads, 0, st>>>(a, g.nq, g.splits);
+  }
+  if (dt == F32) paged_prefill_f32_kernel<DK><<<n, kThreads, 0, st>>>(a, g.nq, g.splits);
+  NML_LAUNCHED();
+  if (g.splits == 1) return 0;
+  constexpr int kRows = kThreads / (DK / 4);
+  const unsigned blocks = static_cast<unsigned>(g.tiles * ((kQ + kRows - 1) / kRows));
+  if constexpr (DK > 32) {
+    if (dt == F16) paged_merge_kernel<half_t, DK><<<blocks, kThreads, 0, st>>>(a, g.nq, g.splits);
+  }
+  if (dt == F32) paged_merge_kernel<float, DK><<<blocks, kThreads, 0, st>>>(a, g.nq, g.splits);
   NML_LAUNCHED();
   return 0;
 }
@@ -443,20 +706,24 @@ int launch_f16(PagedAttnArgs a, hipStream_t st) {
 }  // namespace
 
 bool paged_prefill_applies(int dt, int H, int Hkv, int S, int dk) {
-  return dt == F16 && dk <= 128 && dk % 8 == 0 && S > 1 && H / Hkv * S >= 64;
+  return dk <= 128 && dk % (dt == F16 ? 8 : 4) == 0 && S > 1 && H / Hkv * S >= 64;
 }
 
-size_t paged_prefill_workspace(int B, int H, int Hkv, int S, int P, int dk) {
+size_t paged_prefill_workspace(int dt, int B, int H, int Hkv, int S, int P, int dk) {
   const Grid g = grid_of(B, H, Hkv, S, P);
   if (g.splits == 1) return 0;
-  const size_t d = dk <= 64 ? 64 : dk <= 96 ? 96 : 128;
-  return kCounterBytes + sizeof(float) * g.tiles * g.splits * kQ * (2 + d);
+  return kCounterBytes + sizeof(float) * g.tiles * g.splits * kQ * (2 + columns_of(dt, dk));
 }
 
-int launch_paged_prefill(int dt, const PagedAttnArgs& a, hipStream_t st) {
-  if (a.dk <= 64) return launch_f16<64>(a, st);
-  if (a.dk <= 96) return launch_f16<96>(a, st);
-  return launch_f16<128>(a, st);
+int launch_paged_prefill(int dt, PagedAttnArgs a, hipStream_t st) {
+  const Grid g = grid_of(a.B, a.H, a.Hkv, a.S, a.max_pages << a.shift);
+  a.slots = g.splits > 1 ? static_cast<int>(g.tiles * g.splits) : 0;
+  switch (columns_of(dt, a.dk)) {
+    case 32: return launch_columns<32>(dt, a, g, st);
+    case 64: return launch_columns<64>(dt, a, g, st);
+    case 96: return launch_columns<96>(dt, a, g, st);
+  }
+  return launch_columns<128>(dt, a, g, st);
 }
 
 }  // namespace nml

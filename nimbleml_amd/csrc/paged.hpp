@@ -52,7 +52,7 @@ constexpr size_t kCounterBytes = sizeof(unsigned) * kCounters * kCounterStep;
 // Attention of many new tokens (ops_paged_prefill.hip), for the calls that it takes; the buffers are
 // 16-byte aligned.
 bool paged_prefill_applies(int dt, int H, int Hkv, int S, int dk);
-size_t paged_prefill_workspace(int B, int H, int Hkv, int S, int P, int dk);
-int launch_paged_prefill(int dt, const PagedAttnArgs& a, hipStream_t st);
+size_t paged_prefill_workspace(int dt, int B, int H, int Hkv, int S, int P, int dk);
+int launch_paged_prefill(int dt, PagedAttnArgs a, hipStream_t st);
 
 }  // namespace nml
