@@ -344,8 +344,8 @@ struct VerifyArgs {
   int32_t* accepted;
   int64_t* tokens;
   int* err;
-  // set by the launch: parts of a row, and the workspace's parts
-  int parts;
+  // set by the launch: parts of a row, of the row that decides, and the workspace's parts
+  int row_parts, parts;
   void *stats, *sums;
   unsigned* counter;
 };

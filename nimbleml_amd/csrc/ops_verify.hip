@@ -15,34 +15,81 @@
 //
 // Exponentials and sums are in 64 bits: a token is where a running sum of V weights passes a number,
 // and with 32 bits about one in 10^3 … 10^4 tokens would be the neighbour of the one that the formula
-// gives. A 64-bit multiply-add runs at the rate of a 32-bit one on this card, and the exponential
-// below takes 14 of them.
+// gives. A 64-bit multiply-add runs at the rate of a 32-bit one on this card, and an exponential takes
+// 14 such operations.
 #include "kernels.hpp"
 
 namespace nml {
 
 namespace {
 
-constexpr int kThreads = 256, kEach = 32, kPart = kThreads * kEach;  // elements of a part of a row
-constexpr int kMaxRows = kMaxDrafts + 1;
+constexpr int kThreads = 256, kMaxRows = kMaxDrafts + 1;
+// Elements of a part of a row, a thread's times kThreads: few where the rows are few, so that a lone
+// call's chain is short.
+constexpr int kSmall = 8, kLarge = 32;
 
-// 2^t for t ≤ 0: 2^⌊t⌉ times the exponential series of (t − ⌊t⌉)·ln 2 up to the tenth power (what
-// is left out is below 3·10^-13 of it).
-__device__ __forceinline__ double exp2_64(double t) {
-  t = fmax(t, -1200.0);  // (−inf: 0; a NaN is found by other means)
-  const double n = rint(t), f = (t - n) * 0.693147180559945309417;
-  double p = 1.0 / 3628800.0;
-  p = p * f + 1.0 / 362880.0;
-  p = p * f + 1.0 / 40320.0;
-  p = p * f + 1.0 / 5040.0;
-  p = p * f + 1.0 / 720.0;
-  p = p * f + 1.0 / 120.0;
-  p = p * f + 1.0 / 24.0;
-  p = p * f + 1.0 / 6.0;
-  p = p * f + 0.5;
-  p = p * f + 1.0;
-  p = p * f + 1.0;
-  return ldexp(p, static_cast<int>(n));
+// exp((x − m)/T) of x ≤ m, c = log₂ e / T (the difference first: the logits may be large): 2^n times a
+// polynomial in f, n + f the exponent, |f| ≤ ½, whose coefficients are fitted to 2^f for the least
+// relative error (8·10^-13, by exchange); 0 below 2^-1000, NaN of NaN. The addend 1.5·2^52 rounds to an
+// integer, which the sum's low word then is.
+__device__ __forceinline__ double exp64(float x, double c, double m) {
+  const double t = (static_cast<double>(x) - m) * c;
+  const double k = t + 6755399441055744.0, f = t - (k - 6755399441055744.0);
+  double p = 1.3175858091404474e-06;
+  p = __builtin_fma(p, f, 1.5309737421601964e-05);
+  p = __builtin_fma(p, f, 0.0001540385174883757);
+  p = __builtin_fma(p, f, 0.0013333452062250341);
+  p = __builtin_fma(p, f, 0.0096181285428622344);
+  p = __builtin_fma(p, f, 0.055504109393417086);
+  p = __builtin_fma(p, f, 0.24022650698880371);
+  p = __builtin_fma(p, f, 0.69314718054651414);
+  p = __builtin_fma(p, f, 0.9999999999997623);
+  const unsigned long long bits = __builtin_bit_cast(unsigned long long, p) +
+                                  (static_cast<unsigned long long>(static_cast<unsigned>(__builtin_bit_cast(unsigned long long, k))) << 52);
+  return t < -1000.0 ? 0.0 : __builtin_bit_cast(double, bits);
+}
+// m, but finite where nothing is above −inf (every exponential is 0 then).
+__device__ __forceinline__ double reference(float m) { return m == -INFINITY ? 0.0 : static_cast<double>(m); }
+
+// Lane moves of 64-bit values on the data-parallel-primitive path (lanes without a source: 0).
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double dpp_d(double v) {
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), CTRL, ROWS, 0xf, false);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(double, static_cast<unsigned long long>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double lane_d(double v, int l) {
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+  const unsigned lo = __builtin_amdgcn_readlane(static_cast<int>(b), l), hi = __builtin_amdgcn_readlane(static_cast<int>(b >> 32), l);
+  return __builtin_bit_cast(double, static_cast<unsigned long long>(hi) << 32 | lo);
+}
+// Over the 16 lanes of a row, in each of them.
+__device__ __forceinline__ double row16_sum_d(double v) {
+  v += dpp_d<kDppXor1>(v);
+  v += dpp_d<kDppXor2>(v);
+  v += dpp_d<kDppHalfMirror>(v);
+  return v + dpp_d<kDppMirror>(v);
+}
+__device__ __forceinline__ float row16_max(float v) {
+  v = fmaxf(v, dpp_move<kDppXor1>(v));
+  v = fmaxf(v, dpp_move<kDppXor2>(v));
+  v = fmaxf(v, dpp_move<kDppHalfMirror>(v));
+  return fmaxf(v, dpp_move<kDppMirror>(v));
+}
+__device__ __forceinline__ double wave_sum64(double v) {
+  v = row16_sum_d(v);
+  return (lane_d(v, 0) + lane_d(v, 16)) + (lane_d(v, 32) + lane_d(v, 48));
+}
+// Inclusive sum over the wave's lanes.
+__device__ __forceinline__ double wave_scan64(double v) {
+  v += dpp_d<0x111>(v);       // row_shr:1
+  v += dpp_d<0x112>(v);       // row_shr:2
+  v += dpp_d<0x114>(v);       // row_shr:4
+  v += dpp_d<0x118>(v);       // row_shr:8
+  v += dpp_d<0x142, 0xa>(v);  // row_bcast:15
+  v += dpp_d<0x143, 0xc>(v);  // row_bcast:31
+  return v;
 }
 
 // Of a part of a row (or a row): the largest logit and Σ exp((x − m)/T), NaN where the row has no
@@ -92,10 +139,10 @@ __device__ __forceinline__ int drafted_of(const VerifyArgs& a, int b, bool tell)
   return k;
 }
 
-template <typename T, bool GREEDY>
+template <typename T, int EACH, bool GREEDY>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
   typedef Group<T> G;
-  constexpr int E = G::E, N = kEach / E, NW = kThreads / 64;
+  constexpr int E = G::E, N = EACH / E, NW = kThreads / 64;
   __shared__ float ms[NW];
   __shared__ double zs[NW];
   __shared__ unsigned long long ks[NW];
@@ -109,7 +156,7 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
   if (draft ? i - a.n - 1 >= c : i > c) return;
   const T* x = draft ? static_cast<const T*>(a.draft) + (static_cast<size_t>(b) * a.n + (i - a.n - 1)) * a.ld_draft
                      : static_cast<const T*>(a.logits) + (static_cast<size_t>(b) * (a.n + 1) + i) * a.ld;
-  const int first = part * kPart;
+  const int first = part * kThreads * EACH;
   typename G::vec v[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) {
@@ -119,7 +166,7 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
 #pragma unroll
       for (int e = 0; e < E; ++e) v[k][e] = static_cast<T>(-INFINITY);
   }
-  Stat* out = static_cast<Stat*>(a.stats) + static_cast<size_t>(blockIdx.y) * a.parts + part;
+  Stat* out = static_cast<Stat*>(a.stats) + static_cast<size_t>(blockIdx.y) * a.row_parts + part;
   if (GREEDY) {
     unsigned long long best = 0;
 #pragma unroll
@@ -140,46 +187,39 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
     }
     return;
   }
-  float m = -INFINITY;
-  bool none = false;  // a NaN or +inf
+  float m = -INFINITY;  // (NaN is not seen here; it reaches the sum, and so does +inf, as ∞ − ∞)
 #pragma unroll
   for (int k = 0; k < N; ++k)
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float f = static_cast<float>(v[k][e]);
-      m = fmaxf(m, f);
-      none |= !(f < INFINITY);
-    }
+    for (int e = 0; e < E; ++e) m = fmaxf(m, static_cast<float>(v[k][e]));
   m = wave_max_dpp(m);
   if (lane == 0) ms[w] = m;
-  const bool bad = __syncthreads_or(none);
+  __syncthreads();
   m = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
-  const double ref = m == -INFINITY ? 0.0 : static_cast<double>(m);
+  const double ref = reference(m);
   double z = 0.0;
-  if (!bad) {
 #pragma unroll
-    for (int k = 0; k < N; ++k)
+  for (int k = 0; k < N; ++k)
 #pragma unroll
-      for (int e = 0; e < E; ++e) z += exp2_64((static_cast<double>(static_cast<float>(v[k][e])) - ref) * a.c);
-  }
-  z = wave_sum_d(z);
+    for (int e = 0; e < E; ++e) z += exp64(static_cast<float>(v[k][e]), a.c, ref);
+  z = wave_sum64(z);
   if (lane == 0) zs[w] = z;
   __syncthreads();
-  if (tid == 0) *out = Stat{bad ? __builtin_nan("") : (zs[0] + zs[1]) + (zs[2] + zs[3]), m, 0};
+  if (tid == 0) *out = Stat{(zs[0] + zs[1]) + (zs[2] + zs[3]), m, 0};
 }
 
-// Row `i` of sequence b from its parts, by one wave: m and Σ exp((x − m)/T), NaN without a
+// A row from its parts, by 16 lanes (each has the result): m and Σ exp((x − m)/T), NaN without a
 // distribution.
-__device__ __forceinline__ Stat row_stat(const VerifyArgs& a, int b, int i, int lane) {
-  const int rows = a.n + 1 + (a.draft ? a.n : 0);
-  const Stat* s = static_cast<const Stat*>(a.stats) + (static_cast<size_t>(b) * rows + i) * a.parts;
-  float m = -INFINITY;
-  for (int k = lane; k < a.parts; k += 64) m = fmaxf(m, s[k].m);
-  m = wave_max_dpp(m);
-  double z = 0.0;
-  for (int k = lane; k < a.parts; k += 64)
-    z += s[k].z * exp2_64(s[k].m == m ? 0.0 : (static_cast<double>(s[k].m) - static_cast<double>(m)) * a.c);
-  z = wave_sum_d(z);
+// own: its part l16, loaded ahead.
+__device__ __forceinline__ Stat part_of(const Stat* s, int parts, int l16) { return l16 < parts ? s[l16] : Stat{0.0, -INFINITY, 0}; }
+__device__ __forceinline__ Stat row_stat(const Stat* s, Stat own, int parts, double c, int l16) {
+  float m = own.m;
+  for (int k = l16 + 16; k < parts; k += 16) m = fmaxf(m, s[k].m);
+  m = row16_max(m);
+  const double ref = reference(m);
+  double z = own.z * exp64(own.m, c, ref);
+  for (int k = l16 + 16; k < parts; k += 16) z += s[k].z * exp64(s[k].m, c, ref);
+  z = row16_sum_d(z);
   return Stat{m == -INFINITY ? __builtin_nan("") : z, m, 0};
 }
 
@@ -193,19 +233,10 @@ __device__ __forceinline__ double get64(const double* p) {
                                                       __HIP_MEMORY_SCOPE_AGENT));
 }
 
-__device__ __forceinline__ double wave_scan_d(double v, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double t = __shfl_up(v, o, 64);
-    if (lane >= o) v += t;
-  }
-  return v;
-}
-
 // The answer of sequence b: r accepted drafts and the token after them (−1: no distribution).
-__device__ __forceinline__ void answer(const VerifyArgs& a, int b, int r, int64_t token, int tid) {
+__device__ __forceinline__ void answer(const VerifyArgs& a, const int64_t* drafts, int b, int r, int64_t token, int tid) {
   for (int i = tid; i <= a.n; i += kThreads)
-    a.tokens[static_cast<size_t>(b) * (a.n + 1) + i] = i < r ? a.drafts[static_cast<size_t>(b) * a.n + i] : i == r ? token : -1;
+    a.tokens[static_cast<size_t>(b) * (a.n + 1) + i] = i < r ? drafts[i] : i == r ? token : -1;
   if (tid == 0) {
     a.accepted[b] = r;
     if (token < 0 && a.err) __hip_atomic_fetch_or(a.err, 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -217,11 +248,11 @@ __global__ __launch_bounds__(kThreads) void verify_greedy_kernel(VerifyArgs a) {
   __shared__ unsigned long long best[kMaxRows];
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int c = drafted_of(a, b, false);
-  const Stat* s = static_cast<const Stat*>(a.stats) + static_cast<size_t>(b) * (a.n + 1) * a.parts;
+  const Stat* s = static_cast<const Stat*>(a.stats) + static_cast<size_t>(b) * (a.n + 1) * a.row_parts;
   for (int i = w; i <= c; i += kThreads / 64) {
     unsigned long long k = 0;
-    for (int y = lane; y < a.parts; y += 64) {
-      const unsigned long long o = __builtin_bit_cast(unsigned long long, s[i * a.parts + y].z);
+    for (int y = lane; y < a.row_parts; y += 64) {
+      const unsigned long long o = __builtin_bit_cast(unsigned long long, s[i * a.row_parts + y].z);
       k = k > o ? k : o;
     }
     k = wave_umax64(k);
@@ -238,41 +269,65 @@ __global__ __launch_bounds__(kThreads) void verify_greedy_kernel(VerifyArgs a) {
     if ((d < 0 || d >= a.V) && tid == 0 && a.err) __hip_atomic_fetch_or(a.err, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (d != token) break;
   }
-  answer(a, b, r, token, tid);
+  answer(a, a.drafts + static_cast<size_t>(b) * a.n, b, r, token, tid);
 }
 
-template <typename T>
+template <typename T, int EACH>
 __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
+#pragma clang fp contract(off)  // (equal probabilities leave nothing: no product of one side kept unrounded)
   typedef Group<T> G;
-  constexpr int E = G::E, N = kEach / E, NW = kThreads / 64;
+  constexpr int E = G::E, N = EACH / E, NW = kThreads / 64;
   __shared__ Stat ps[kMaxRows], qs[kMaxRows];
-  __shared__ double sums[2][NW];
-  __shared__ int r_, at_, part_;
-  __shared__ double before_, goal_;
-  __shared__ bool left_, last_;
+  __shared__ int64_t ids[kMaxRows];
+  __shared__ double sums[NW], before_, goal_;
+  __shared__ int r_, part_, hits[NW], ends[NW];
+  __shared__ bool last_;
   const int part = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int c = drafted_of(a, b, false);
-  for (int i = w; i <= c; i += NW) {
-    const Stat p = row_stat(a, b, i, lane);
-    const Stat q = a.draft && i < c ? row_stat(a, b, a.n + 1 + i, lane) : Stat{1.0, 0.f, 0};
-    if (lane == 0) ps[i] = p, qs[i] = q;
-  }
-  __syncthreads();
   const int64_t* drafts = a.drafts + static_cast<size_t>(b) * a.n;
   const double* u = a.u + static_cast<size_t>(b) * (a.n + 1);
   auto target = [&](int i) { return static_cast<const T*>(a.logits) + (static_cast<size_t>(b) * (a.n + 1) + i) * a.ld; };
   auto drafted = [&](int i) { return static_cast<const T*>(a.draft) + (static_cast<size_t>(b) * a.n + i) * a.ld_draft; };
-  if (w == 0) {  // a draft a lane
-    bool ok = true;
-    if (lane < c) {
-      const int64_t d = drafts[lane];
-      ok = d >= 0 && d < a.V;
-      if (!ok && part == 0 && a.err) __hip_atomic_fetch_or(a.err, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (ok) {
-        const double pd = exp2_64((static_cast<double>(static_cast<float>(target(lane)[d])) - ps[lane].m) * a.c) / ps[lane].z;
-        const double qd = !a.draft ? 1.0 : exp2_64((static_cast<double>(static_cast<float>(drafted(lane)[d])) - qs[lane].m) * a.c) / qs[lane].z;
-        ok = u[lane] * qd < pd;  // (false where either has no distribution)
-      }
+  // All that the acceptance takes is loaded before anything is waited for, of drafts past the row's
+  // count too (their rows' parts may hold anything and are not looked at).
+  const int rows = a.n + 1 + (a.draft ? a.n : 0), l16 = tid & 15;
+  const Stat* stats = static_cast<const Stat*>(a.stats) + static_cast<size_t>(b) * rows * a.row_parts;
+  auto row_at = [&](int i) { return stats + static_cast<size_t>(i) * a.row_parts; };
+  int i = tid >> 4;
+  Stat ahead{};
+  if (i < rows) ahead = part_of(row_at(i), a.row_parts, l16);
+  bool ok = true;
+  float dp = 0.f, dq = 0.f;
+  double du = 0.0;
+  if (tid < a.n) {  // (the first wave)
+    const int64_t d = drafts[tid];
+    du = u[tid];
+    ok = d >= 0 && d < a.V;
+    if (ok) {
+      dp = static_cast<float>(target(tid)[d]);
+      if (a.draft) dq = static_cast<float>(drafted(tid)[d]);
+    }
+    ids[tid] = d;
+  }
+  const double last_u = u[a.n];
+  while (i < rows) {
+    const Stat s = row_stat(row_at(i), ahead, a.row_parts, a.c, l16);
+    if (l16 == 0) {
+      if (i <= a.n) ps[i] = s;
+      else qs[i - a.n - 1] = s;
+    }
+    i += kThreads / 16;
+    if (i < rows) ahead = part_of(row_at(i), a.row_parts, l16);
+  }
+  if (!a.draft && tid < a.n) qs[tid] = Stat{1.0, 0.f, 0};
+  const int c = drafted_of(a, b, false);
+  __syncthreads();
+  if (w == 0) {
+    if (lane >= c) ok = true;
+    else if (!ok && part == 0 && a.err) __hip_atomic_fetch_or(a.err, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (lane < c && ok) {
+      const double pd = exp64(dp, a.c, reference(ps[lane].m)) / ps[lane].z;
+      const double qd = a.draft ? exp64(dq, a.c, reference(qs[lane].m)) / qs[lane].z : 1.0;
+      ok = du * qd < pd;  // (false where either has no distribution)
     }
     const unsigned long long no = __ballot(!ok);
     if (lane == 0) r_ = no ? __ffsll(no) - 1 : c;
@@ -282,158 +337,177 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
   const Stat p = ps[r], q = qs[r];
   const bool refused = r < c;
   if (!(p.z > 0.0) || (refused && !(q.z > 0.0))) {
-    if (part == 0) answer(a, b, r, -1, tid);
+    if (part == 0) answer(a, ids, b, r, -1, tid);
     return;
   }
   const T *xp = target(r), *xq = refused && a.draft ? drafted(r) : nullptr;
-  const int64_t d = refused && !a.draft ? drafts[r] : -1;
-  const double ip = 1.0 / p.z, iq = 1.0 / q.z;
-  // the weights of element i: what p has above q, and p
-  auto weigh = [&](float fp, float fq, int i, double& left, double& all) {
-    all = exp2_64((static_cast<double>(fp) - p.m) * a.c) * ip;
-    left = all;
-    if (xq) left = fmax(all - exp2_64((static_cast<double>(fq) - q.m) * a.c) * iq, 0.0);
-    if (i == d) left = 0.0;
+  const int64_t d = refused && !a.draft ? ids[r] : -1;
+  const double ip = 1.0 / p.z, iq = 1.0 / q.z, mp = reference(p.m), mq = xq ? reference(q.m) : 0.0;
+  // The weights of EACH elements, in groups of E that lie `step` apart from `first` on: what p has above q
+  // (`over`), or p; past the row's end 0.
+  double wt[EACH];
+  auto weigh = [&](int first, int step, bool over) {
+    typename G::vec vp[N], vq[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int at = first + k * step;
+#pragma unroll
+      for (int e = 0; e < E; ++e) vp[k][e] = vq[k][e] = static_cast<T>(-INFINITY);
+      if (at < a.V) {
+        vp[k] = G::load(xp, at, a.V);
+        if (xq) vq[k] = G::load(xq, at, a.V);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const double all = exp64(static_cast<float>(vp[k][e]), a.c, mp) * ip;
+        double left = fmax(all - exp64(static_cast<float>(vq[k][e]), a.c, mq) * iq, 0.0);
+        if (first + k * step + e == d) left = 0.0;
+        wt[k * E + e] = over ? left : all;
+      }
   };
-  double left = 0.0, all = 0.0;
-  for (int k = 0; k < N; ++k) {
-    const int at = part * kPart + (k * kThreads + tid) * E;
-    if (at >= a.V) break;
-    const typename G::vec vp = G::load(xp, at, a.V);
-    typename G::vec vq = vp;
-    if (xq) vq = G::load(xq, at, a.V);
+  // Twice through the same code (which the second time is there): for this part's sum of weights; and,
+  // by the last workgroup of the sequence to arrive, for the part where the running sum passes the
+  // goal, EACH elements in a row to a thread. A refused draft whose p is nowhere above q (by
+  // rounding alone): the token is p's, whose sum is 1, part by part.
+  enum { kSum, kFind, kWalk } mode = kSum;
+  double* mine = static_cast<double*>(a.sums) + static_cast<size_t>(b) * a.parts;
+  int at = part, end_before = -1;
+  double before = 0.0, goal = 0.0;
+#pragma unroll 1
+  for (;;) {
+    const int first = mode == kSum ? at * kThreads * EACH + tid * E : (at * kThreads + tid) * EACH;
+    weigh(first, mode == kSum ? kThreads * E : E, mode != kWalk && refused);
+    double own = 0.0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      double l1, a1;
-      weigh(static_cast<float>(vp[e]), static_cast<float>(vq[e]), at + e, l1, a1);
-      left += l1;
-      all += a1;
-    }
-  }
-  left = wave_sum_d(left);
-  all = wave_sum_d(all);
-  if (lane == 0) sums[0][w] = left, sums[1][w] = all;
-  __syncthreads();
-  double* mine = static_cast<double*>(a.sums) + 2 * static_cast<size_t>(b) * a.parts;
-  if (tid == 0) {
-    put64(mine + 2 * part, (sums[0][0] + sums[0][1]) + (sums[0][2] + sums[0][3]));
-    put64(mine + 2 * part + 1, (sums[1][0] + sums[1][1]) + (sums[1][2] + sums[1][3]));
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    last_ = __hip_atomic_fetch_add(a.counter + b, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == static_cast<unsigned>(a.parts);
-  }
-  __syncthreads();
-  if (!last_) return;
-
-  // The last of the sequence: the part where the running sum passes the goal, by one wave.
-  if (w == 0) {
-    double total[2] = {0.0, 0.0};
-    for (int k = lane; k < a.parts; k += 64) total[0] += get64(mine + 2 * k), total[1] += get64(mine + 2 * k + 1);
-    total[0] = wave_sum_d(total[0]);
-    total[1] = wave_sum_d(total[1]);
-    const int which = total[0] > 0.0 ? 0 : 1;
-    const double goal = u[a.n] * total[which];
-    double carry = 0.0, before = 0.0;
-    int found = -1, some = 0;
-    double some_before = 0.0;
-    for (int k0 = 0; k0 < a.parts && found < 0; k0 += 64) {
-      const double s = k0 + lane < a.parts ? get64(mine + 2 * (k0 + lane) + which) : 0.0;
-      const double run = carry + wave_scan_d(s, lane);
-      const unsigned long long past = __ballot(run > goal && s > 0.0), any = __ballot(s > 0.0);
-      const int l = past ? __ffsll(past) - 1 : any ? 63 - __clzll(any) : 0;
-      const double b4 = __shfl(run - s, l, 64);
-      if (past) found = k0 + l, before = b4;
-      else if (any) some = k0 + l, some_before = b4;
-      carry = __shfl(run, 63, 64);
-    }
-    if (lane == 0) {
-      part_ = found < 0 ? some : found;
-      before_ = found < 0 ? some_before : before;
-      goal_ = goal;
-      left_ = which == 0;
-      at_ = 0x7fffffff;
-    }
-  }
-  __syncthreads();
-  // its weights again, kEach in a row to a thread
-  const int first = part_ * kPart + tid * kEach;
-  double own = 0.0, wt[kEach];
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const int at = first + k * E;
-    typename G::vec vp, vq;
-    if (at < a.V) {
-      vp = G::load(xp, at, a.V);
-      vq = vp;
-      if (xq) vq = G::load(xq, at, a.V);
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      double l1 = 0.0, a1 = 0.0;
-      if (at < a.V) weigh(static_cast<float>(vp[e]), static_cast<float>(vq[e]), at + e, l1, a1);
-      own += wt[k * E + e] = left_ ? l1 : a1;
-    }
-  }
-  const double scan = wave_scan_d(own, lane);
-  if (lane == 63) sums[0][w] = scan;
-  __syncthreads();
-  double run = before_ + (scan - own);
-  for (int y = 0; y < w; ++y) run += sums[0][y];
-  int hit = 0x7fffffff, end = -1;
-#pragma unroll
-  for (int k = 0; k < kEach; ++k) {
-    run += wt[k];
-    if (wt[k] > 0.0) {
-      end = first + k;
-      if (hit == 0x7fffffff && run > goal_) hit = first + k;
-    }
-  }
-  atomicMin(&at_, hit);
-  __syncthreads();
-  int at = at_;
-  if (at == 0x7fffffff) {  // the running sum ends below what its parts add up to: the last with a weight
+    for (int k = 0; k < EACH; ++k) own += wt[k];
+    const double scan = wave_scan64(own);
+    __syncthreads();  // (what the time before left in LDS is read)
+    if (lane == 63) sums[w] = scan;
     __syncthreads();
-    if (tid == 0) at_ = -1;
+    if (mode == kSum) {
+      if (tid == 0) {
+        put64(mine + part, (sums[0] + sums[1]) + (sums[2] + sums[3]));
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        last_ = __hip_atomic_fetch_add(a.counter + b, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == static_cast<unsigned>(a.parts);
+      }
+      __syncthreads();
+      if (!last_) return;
+      if (w == 0) {  // the part where the running sum passes the goal (none: the last with a weight)
+        const double kept = lane < a.parts ? get64(mine + lane) : 0.0;  // (the first 64)
+        double total = kept;
+        for (int k = lane + 64; k < a.parts; k += 64) total += get64(mine + k);
+        total = wave_sum64(total);
+        const double to = last_u * total;
+        double carry = 0.0, start = 0.0;
+        int found = -1;
+        for (int k0 = 0; k0 < a.parts; k0 += 64) {
+          const double s = k0 == 0 ? kept : k0 + lane < a.parts ? get64(mine + k0 + lane) : 0.0;
+          const double run = carry + wave_scan64(s);
+          const unsigned long long past = __ballot(run > to && s > 0.0), any = __ballot(s > 0.0);
+          if (any) {
+            const int l = past ? __ffsll(past) - 1 : 63 - __clzll(any);
+            found = k0 + l;
+            start = lane_d(run - s, l);
+          }
+          if (past) break;
+          carry = lane_d(run, 63);
+        }
+        if (lane == 0) part_ = found, before_ = start, goal_ = to;
+      }
+      __syncthreads();
+      mode = part_ < 0 ? kWalk : kFind;
+      at = max(part_, 0);
+      before = part_ < 0 ? 0.0 : before_;
+      goal = part_ < 0 ? last_u : goal_;
+      continue;
+    }
+    double run = before + (scan - own);
+    for (int y = 0; y < w; ++y) run += sums[y];
+    // this thread's first element past the goal, and its last with a weight; then the part's
+    int hit = -1, end = -1;
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      run += wt[k];
+      if (wt[k] > 0.0) {
+        end = first + k;
+        if (hit < 0 && run > goal) hit = end;
+      }
+    }
+    const unsigned long long past = __ballot(hit >= 0), any = __ballot(end >= 0);
+    if (lane == (past ? __ffsll(past) - 1 : 0)) hits[w] = hit;
+    if (lane == (any ? 63 - __clzll(any) : 0)) ends[w] = end;
     __syncthreads();
-    atomicMax(&at_, end);
-    __syncthreads();
-    at = at_;
+    int token = -1;
+#pragma unroll
+    for (int y = NW - 1; y >= 0; --y) {
+      if (hits[y] >= 0) token = hits[y];
+      end_before = max(end_before, ends[y]);
+    }
+    if (mode == kWalk && token < 0 && at + 1 < a.parts) {
+      before += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+      ++at;
+      continue;
+    }
+    // (none: the running sum ends below what its parts add up to, by rounding: the last with a weight)
+    answer(a, ids, b, r, token < 0 ? end_before : token, tid);
+    return;
   }
-  answer(a, b, r, at, tid);
 }
 
-template <typename T>
-int verify_launch(const VerifyArgs& a, hipStream_t st) {
-  const int rows = a.n + 1 + (a.draft ? a.n : 0);
-  const dim3 grid(a.parts, static_cast<unsigned>(a.B) * rows);
-  if (a.greedy) {
-    verify_stats_kernel<T, true><<<grid, kThreads, 0, st>>>(a);
-    NML_LAUNCHED();
-    verify_greedy_kernel<T><<<a.B, kThreads, 0, st>>>(a);
-  } else {
-    verify_stats_kernel<T, false><<<grid, kThreads, 0, st>>>(a);
-    NML_LAUNCHED();
-    verify_draw_kernel<T><<<dim3(a.parts, a.B), kThreads, 0, st>>>(a);
-  }
+// Elements of a part to a thread, of `rows` rows of V: as many as leave two workgroups for every CU.
+int each_of(long long rows, int V) { return rows * V >= 512LL * kThreads * kLarge ? kLarge : kSmall; }
+int parts_of(long long rows, int V) {
+  const int part = kThreads * each_of(rows, V);
+  return (V + part - 1) / part;
+}
+// Rows of logits that a call may have to go over.
+long long rows_of(int B, int n) { return static_cast<long long>(B) * (2 * n + 1); }
+
+template <typename T, int EACH>
+int stats_launch(const VerifyArgs& a, hipStream_t st) {
+  const dim3 grid(a.row_parts, static_cast<unsigned>(a.B) * (a.n + 1 + (a.draft ? a.n : 0)));
+  if (a.greedy) verify_stats_kernel<T, EACH, true><<<grid, kThreads, 0, st>>>(a);
+  else verify_stats_kernel<T, EACH, false><<<grid, kThreads, 0, st>>>(a);
   NML_LAUNCHED();
   return 0;
 }
 
-size_t stats_bytes(int B, int n, int parts) { return sizeof(Stat) * (2 * static_cast<size_t>(n) + 1) * parts * B; }
-int parts_of(int V) { return (V + kPart - 1) / kPart; }
+template <typename T>
+int verify_launch(const VerifyArgs& a, hipStream_t st) {
+  NML_TRY((each_of(rows_of(a.B, a.n), a.V) == kLarge ? stats_launch<T, kLarge>(a, st) : stats_launch<T, kSmall>(a, st)));
+  const dim3 grid(a.parts, a.B);
+  if (a.greedy) verify_greedy_kernel<T><<<a.B, kThreads, 0, st>>>(a);
+  else if (each_of(a.B, a.V) == kLarge) verify_draw_kernel<T, kLarge><<<grid, kThreads, 0, st>>>(a);
+  else verify_draw_kernel<T, kSmall><<<grid, kThreads, 0, st>>>(a);
+  NML_LAUNCHED();
+  return 0;
+}
+
+// The workspace: a Stat for each part of a row, a sum for each part of a sequence's deciding row, a counter.
+struct Layout {
+  size_t stats, sums, all;
+  Layout(int B, int n, int V) {
+    stats = sizeof(Stat) * rows_of(B, n) * parts_of(rows_of(B, n), V);
+    sums = stats + sizeof(double) * parts_of(B, V) * B;
+    all = sums + sizeof(unsigned) * B;
+  }
+};
 
 }  // namespace
 
-size_t verify_workspace(int B, int n, int V) {
-  const size_t parts = parts_of(V);
-  return stats_bytes(B, n, static_cast<int>(parts)) + 2 * sizeof(double) * parts * B + sizeof(unsigned) * B;
-}
+size_t verify_workspace(int B, int n, int V) { return Layout(B, n, V).all; }
 
 int launch_verify(int dt, VerifyArgs a, void* ws, hipStream_t st) {
-  a.parts = parts_of(a.V);
+  const Layout at(a.B, a.n, a.V);
+  a.row_parts = parts_of(rows_of(a.B, a.n), a.V);
+  a.parts = parts_of(a.B, a.V);
   char* p = static_cast<char*>(ws);
   a.stats = p;
-  a.sums = p + stats_bytes(a.B, a.n, a.parts);
-  a.counter = reinterpret_cast<unsigned*>(static_cast<double*>(a.sums) + 2 * static_cast<size_t>(a.parts) * a.B);
+  a.sums = p + at.stats;
+  a.counter = reinterpret_cast<unsigned*>(p + at.sums);
   return dt == F16 ? verify_launch<half_t>(a, st) : verify_launch<float>(a, st);
 }
 

@@ -60,6 +60,25 @@ def test_the_same_distribution_accepts_everything(gpu):
     assert (a.numpy() == 5).all() and np.array_equal(tok.numpy()[:, :5], drafts)
 
 
+def test_a_refusal_that_leaves_nothing(gpu):
+    """The draft's distribution is the target's, and a number of 1, out of range, refuses it: the token is
+    then one of p's."""
+    r = np.random.RandomState(11)
+    for vocab in (3, 5000, 20001):
+        logits = r.randn(64, 2, vocab).astype(np.float32)
+        logits[:, :, 1::2] = -np.inf
+        drafts = 2 * r.randint(0, vocab // 2, (64, 1))
+        for last in (0.0, 0.3, np.nextafter(1.0, 0.0)):
+            u = np.tile([1.0, last], (64, 1))
+            a, tok = (x.numpy() for x in K.verify_drafts(logits, drafts, u, draft_logits=logits[:, :1].copy()))
+            assert (a == 0).all()
+            end = tok[np.arange(64), a]
+            assert (end >= 0).all() and (end < vocab).all() and (end % 2 == 0).all()
+            p = np.exp(R.log_softmax(logits[np.arange(64), a], 1.0))
+            run = np.cumsum(p, -1)[np.arange(64), end]
+            assert (run >= last - 1e-9).all() and (run - p[np.arange(64), end] <= last + 1e-9).all()
+
+
 def test_uniforms_at_the_ends(gpu):
     logits, draft, drafts, u, _ = case(6, 3, 700, np.float32, seed=4)
     for x in (0.0, np.nextafter(1.0, 0.0)):
