@@ -27,6 +27,7 @@ constexpr int kThreads = 256, kMaxRows = kMaxDrafts + 1;
 // Elements of a part of a row, a thread's times kThreads: few where the rows are few, so that a lone
 // call's chain is short.
 constexpr int kSmall = 8, kLarge = 32;
+constexpr int kLine = 32;  // words from one sequence's counter to the next: a line of its own
 
 // exp((x − m)/T) of x ≤ m, c = log₂ e / T (the difference first: the logits may be large): 2^n times a
 // polynomial in f, n + f the exponent, |f| ≤ ½, whose coefficients are fitted to 2^f for the least
@@ -150,7 +151,7 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
   const int b = blockIdx.y / rows, i = blockIdx.y - b * rows;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   // (the second launch's counter of this sequence)
-  if (part == 0 && i == 0 && tid == 0) a.counter[b] = 0;
+  if (part == 0 && i == 0 && tid == 0) a.counter[b * kLine] = 0;
   const int c = drafted_of(a, b, part == 0 && i == 0 && tid == 0);
   const bool draft = i > a.n;
   if (draft ? i - a.n - 1 >= c : i > c) return;
@@ -391,7 +392,7 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
       if (tid == 0) {
         put64(mine + part, (sums[0] + sums[1]) + (sums[2] + sums[3]));
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        last_ = __hip_atomic_fetch_add(a.counter + b, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == static_cast<unsigned>(a.parts);
+        last_ = __hip_atomic_fetch_add(a.counter + b * kLine, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == static_cast<unsigned>(a.parts);
       }
       __syncthreads();
       if (!last_) return;
@@ -492,7 +493,7 @@ struct Layout {
   Layout(int B, int n, int V) {
     stats = sizeof(Stat) * rows_of(B, n) * parts_of(rows_of(B, n), V);
     sums = stats + sizeof(double) * parts_of(B, V) * B;
-    all = sums + sizeof(unsigned) * B;
+    all = sums + sizeof(unsigned) * kLine * B;
   }
 };
 
