@@ -127,15 +127,19 @@ constexpr float up_log2() {
 
 // Head dims in steps of 32: 1, 2, 4 or 8 of them.
 constexpr int steps_of(int dk) { return dk <= 32 ? 1 : dk <= 64 ? 2 : dk <= 128 ? 4 : 8; }
-// Workgroups of eight waves where tiles are few, of four where there are at least four times as many as
-// the card holds.
-constexpr int kManyTiles = 4;
+// Waves of a workgroup. Few begin and merge sooner, and more workgroups even out rows of different length
+// (µs with four and eight: 16 rows of 1 to 8 Ki keys, 32 heads over 8 of 128, 54 and 70; one row of 1023, 16
+// heads of 64, 10.7 and 12.2, 9.2 with two; 128 rows of 100 to 1000 60.9 with four and 57.1 with two). At
+// head dim 256 a wave's tile fills its registers and eight keep the CU's four pipes busy (16 rows of 1
+// to 4 Ki keys, 16 heads over 2, 42.9 and 37.9).
+__host__ __device__ constexpr int group_waves(int nb) { return nb == 2 ? 2 : nb == 8 ? 8 : 4; }
 // Waves a SIMD that the registers are held to, and the workgroups that the card's 256 CUs then
 // hold at once.
 __host__ __device__ constexpr int waves_of(int nb) { return nb <= 2 ? 4 : 2; }
-__host__ __device__ constexpr int capacity(int nb, int waves) { return 256 * 4 * waves_of(nb) / waves; }
-// Spans (a tile for each wave) that a piece has at least: what it costs to begin one and to merge it.
-__host__ __device__ constexpr int least_spans(int waves) { return 4 * 8 / waves; }
+__host__ __device__ constexpr int capacity(int nb) { return 256 * 4 * waves_of(nb) / group_waves(nb); }
+// Spans (a tile for each wave) that a piece has at least: what it costs to begin one and to merge it. (One row
+// of 1023 keys, 16 heads of 64: 9.2 µs at two spans of 64 keys, 10.6 at four, 8.9 at one; of 100 keys 6.9, 6.9, 8.7.)
+__host__ __device__ constexpr int least_spans(int nb) { return nb == 2 ? 2 : 1; }
 
 // ws: a counter for each tile in pieces, then for each piece its rows' references and Σ p, then their
 // Σ p·v. Tiles in pieces are fewer than the card's workgroups (a piece is at least their even share),
@@ -170,7 +174,7 @@ struct Work {
 };
 // More than 64 rows are shared out to the waves, a run of rows each; sums: of the waves.
 template <int SPAN, int NW>
-__device__ __forceinline__ Work find_work(const PagedAttnArgs& a, int each, int cap, int lane, int wave, int (*sums)[3]) {
+__device__ __forceinline__ Work find_work(const PagedAttnArgs& a, int each, int cap, int fewest, int lane, int wave, int (*sums)[3]) {
   Work w{};
   Rows<SPAN> rows;
   const int run = a.B <= 64 ? 64 : (a.B + 64 * NW - 1) / (64 * NW) * 64;
@@ -192,7 +196,7 @@ __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, int each, int 
     for (int i = 0; i < NW; ++i) total += sums[i][0];
   }
   const int room = room_for(static_cast<long long>(each) * a.B, cap);
-  const int least = max(least_spans(NW), static_cast<int>((static_cast<long long>(total) * each + room - 1) / room));
+  const int least = max(fewest, static_cast<int>((static_cast<long long>(total) * each + room - 1) / room));
   auto pieces_of = [&](int spans) { return spans <= least ? min(spans, 1) : (spans + least - 1) / least; };
   const int at = static_cast<int>(blockIdx.x / each);
   int before = 0, slots = 0, from = 0;
@@ -387,9 +391,10 @@ struct Tile<float, NB, VEC> {
   }
 };
 
-template <typename T, int NB, int NW, bool VEC>
-__global__ __launch_bounds__(64 * NW, waves_of(NB)) void paged_attention_kernel(PagedAttnArgs a) {
+template <typename T, int NB, bool VEC>
+__global__ __launch_bounds__(64 * group_waves(NB), waves_of(NB)) void paged_attention_kernel(PagedAttnArgs a) {
   typedef Tile<T, NB, VEC> Keys;
+  constexpr int NW = group_waves(NB);
   constexpr int KT = tile_keys<T>(), KX = KT / 4, DT = Keys::kTiles;
   constexpr int D = 32 * NB, kWaveLds = 64 * D;  // 16 rows of D floats; a tile of V takes as much
   constexpr int kThreads = 64 * NW, kSpan = NW * KT, kIds = 2;
@@ -404,7 +409,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(NB)) void paged_attention_kernel(
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
   const int R = a.group * a.S, tiles = (R + 15) / 16;
-  const Work work = find_work<kSpan, NW>(a, a.Hkv * tiles, capacity(NB, NW), lane, w, reinterpret_cast<int(*)[3]>(lds));
+  const Work work = find_work<kSpan, NW>(a, a.Hkv * tiles, capacity(NB), least_spans(NB), lane, w, reinterpret_cast<int(*)[3]>(lds));
   if (work.b < 0 || work.n == 0) return;
   const int hk = tiles == 1 ? work.e : work.e / tiles, tile = work.e - hk * tiles;
   const int per = work.pieces == 1 ? work.spans : (work.spans + work.pieces - 1) / work.pieces;
@@ -701,21 +706,17 @@ __global__ __launch_bounds__(64 * NW, waves_of(NB)) void paged_attention_kernel(
   }
 }
 
-// Waves of a workgroup; most pieces of one tile, and in all those of tiles in pieces that there
-// can be.
+// Most pieces of one tile, and in all those of tiles in pieces that there can be.
 struct Pieces {
-  int waves;
   long long tiles, most, slots;
 };
 template <typename T>
 Pieces attention_pieces(int B, int H, int Hkv, int S, int P, int dk) {
   Pieces p;
-  const int nb = steps_of(dk);
+  const int nb = steps_of(dk), span = group_waves(nb) * tile_keys<T>(), spans = (P - 1) / span + 1;
   p.tiles = (static_cast<long long>(H / Hkv) * S + 15) / 16 * Hkv * B;
-  p.waves = p.tiles >= kManyTiles * capacity(nb, 8) ? 4 : 8;
-  const int span = p.waves * tile_keys<T>(), spans = (P - 1) / span + 1;
-  p.most = (spans - 1) / least_spans(p.waves) + 1;
-  p.slots = p.most == 1 ? 0 : std::min(p.tiles * p.most, 2LL * room_for(p.tiles, capacity(nb, p.waves)));
+  p.most = (spans - 1) / least_spans(nb) + 1;
+  p.slots = p.most == 1 ? 0 : std::min(p.tiles * p.most, 2LL * room_for(p.tiles, capacity(nb)));
   return p;
 }
 
@@ -725,8 +726,7 @@ int attention_launch_nb(PagedAttnArgs a, hipStream_t st) {
   a.slots = static_cast<int>(p.slots);
   // every tile's workgroup, and those that pieces add
   const unsigned grid = static_cast<unsigned>(std::min(p.tiles + p.slots, p.tiles * p.most));
-  if (p.waves == 8) paged_attention_kernel<T, NB, 8, VEC><<<grid, 512, 0, st>>>(a);
-  else paged_attention_kernel<T, NB, 4, VEC><<<grid, 256, 0, st>>>(a);
+  paged_attention_kernel<T, NB, VEC><<<grid, 64 * group_waves(NB), 0, st>>>(a);
   NML_LAUNCHED();
   return 0;
 }
