@@ -46,11 +46,11 @@ def check(cache, q, lens, counts, scale=None):
     want, size, spread = R.paged_attention(q, cache.k, cache.v, cache.table, lens, full, scale)
     # a score is a float32 sum of dk products and is rounded three times more, the exponential of that
     # error is a relative one of p, twice (the sum of them); the sums over the keys round once a
-    # key at most; a float16 probability is held in two parts of 11 bits, or, for 64 queries of a KV
-    # head and more, in one: half a step of 2^-10 of it, and of the sum of them
+    # key at most; a float16 probability is held in two parts of 11 bits, or, for more than 32 queries
+    # of a KV head, in one: half a step of 2^-10 of it, and of the sum of them
     n = max(int(np.max(lens)), 1)
     ds = 2.0 ** -24 * (dk + 4) * spread
-    one = dtype == np.float16 and seq > 1 and heads // cache.k.shape[1] * seq >= 64 and dk <= 128 and dk % 8 == 0
+    one = dtype == np.float16 and seq > 1 and heads // cache.k.shape[1] * seq > 32 and dk <= 128 and dk % 8 == 0
     part = 2.0 ** -10 if one else 2.0 ** -21
     tol = size * (2 * ds + 2.0 ** -24 * (n + 32) + part) + HALF[dtype] * np.abs(want) + 2.0 ** -25 * (dtype == np.float16)
     assert np.isfinite(got).all()
