@@ -39,6 +39,11 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 // four, 18.8 at eight, 19.9 at one).
 constexpr int kLeastTiles = 4;
 
+// Workgroups that the card holds at once, two a CU: where the tiles are fewer their keys are cut into
+// pieces. (Pieces for twice as many: 6 ragged rows of up to 512 tokens, 12 heads of 80, 53 in place of 47
+// µs, 128 tokens over 16 Ki keys 83 in place of 64.)
+constexpr int kHeld = 512;
+
 // The keys of 128 queries, from q0 on of (row, KV head) bh: length and new tokens of the row, keys that a
 // query of them sees, key tiles a piece and pieces. n·group ≤ q0: no queries.
 struct Span {
@@ -54,7 +59,12 @@ __device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int bh, int q0, 
   const int last = min((q0 + kQ - 1) / a.group, w.n - 1);  // the last token
   w.kend = max(w.len - w.n + last + 1, 0);
   const int tiles = (w.kend + kK - 1) / kK;
-  w.per = max(kLeastTiles, (tiles + splits - 1) / splits);
+  // a piece: an even share, for as many workgroups as the card holds, of what all rows would have to do
+  // were they as this one (the first queries have fewer keys than the last)
+  const long long queries = (w.n * static_cast<long long>(a.group) + kQ - 1) / kQ;
+  const int mean = (max(w.len - w.n + kQ / a.group, 0) + w.len) / (2 * kK) + 1;
+  const int share = static_cast<int>((queries * mean * a.B * a.Hkv + kHeld - 1) / kHeld);
+  w.per = max(max(kLeastTiles, share), (tiles + splits - 1) / splits);
   w.pieces = q0 >= w.n * a.group ? 0 : max(1, (tiles + w.per - 1) / w.per);
   return w;
 }
@@ -67,24 +77,18 @@ struct Tile {
 
 // False: nothing to do.
 __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int nq, int splits, Tile& t) {
-  const int heads = a.B * a.Hkv, each = nq * splits, n = blockIdx.x;
-  int bh, inner;
-  if (heads % 8 == 0) {  // all of a (row, KV head) on one XCD, whose L2 then holds its keys
-    const int slot = n >> 3;
-    bh = (n & 7) + 8 * (slot / each);
-    inner = slot % each;
-  } else {
-    bh = n / each;
-    inner = n % each;
-  }
+  // (row, KV head) fastest: with a multiple of 8 of them each has its XCD, whose L2 then holds its keys. The
+  // last queries, which have the most keys, first; and pieces that a tile does not have behind all others
+  // (among them they leave half of the CUs idle).
+  const int heads = a.B * a.Hkv, n = blockIdx.x, rest = n / heads, bh = n - rest * heads;
   t.b = bh / a.Hkv;
   t.hk = bh - t.b * a.Hkv;
-  const int qt = nq - 1 - inner / splits;  // (the last queries have the most keys)
-  t.piece = inner % splits;
+  const int qt = nq - 1 - rest % nq;
+  t.piece = rest / nq;
   t.at = bh * nq + qt;
   t.q0 = qt * kQ;
   const Span w = span_of(a, bh, t.q0, splits);
-  if (inner == 0 && !w.good && threadIdx.x == 0) tell(a.err);
+  if (rest == 0 && !w.good && threadIdx.x == 0) tell(a.err);
   if (t.piece >= w.pieces) return false;
   t.len = w.len;
   t.n = w.n;
@@ -666,10 +670,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prefill_f32_kernel(PagedAtt
   each_pair([&](int dim, f2 v) { *reinterpret_cast<f2*>(parts.po + q * DK + dim) = v; });
 }
 
-// Tiles of 128 queries, and into how many pieces the keys of one are cut: as many workgroups at least as
-// the card holds at once (two a CU), where the tiles alone are fewer. (Twice as many: 6 ragged rows of up
-// to 512 tokens, 12 heads of 80, 48 µs in place of 53, but 128 tokens over 16 Ki keys 83 in place of 64.)
-constexpr int kHeld = 512;
+// Tiles of 128 queries, and the most pieces that the keys of one are cut into.
 struct Grid {
   long long tiles;
   int nq, splits;
@@ -679,7 +680,7 @@ Grid grid_of(int B, int H, int Hkv, int S, int P) {
   g.nq = (H / Hkv * S + kQ - 1) / kQ;
   g.tiles = static_cast<long long>(g.nq) * Hkv * B;
   const int most = std::max(1, (P + kK - 1) / kK / kLeastTiles);
-  g.splits = static_cast<int>(std::min<long long>(most, (kHeld + g.tiles - 1) / g.tiles));
+  g.splits = g.tiles >= kHeld ? 1 : static_cast<int>(std::min<long long>(most, (2 * kHeld + g.tiles - 1) / g.tiles));
   return g;
 }
 
