@@ -2,7 +2,7 @@
 // holds already.
 //
 // A KV head's queries (its group's heads times the new tokens, the heads of a token side by side) are
-// taken 128 at a time by a workgroup of four waves, 32 a wave, over tiles of 64 keys in LDS:
+// taken 128 or 256 at a time by a workgroup of four or eight waves, 32 a wave, over tiles of 64 keys in LDS:
 //   Sᵀ = K·Qᵀ    v_mfma_f32_32x32x16_f16, Qᵀ in registers; lane l then holds query l % 32 and keys
 //                8(r/4) + 4(l/32) + r % 4 of each 32 in register r;
 //   Oᵀ += Vᵀ·Pᵀ  Pᵀ straight from those registers, Vᵀ by transposing reads of V as it lies in memory,
@@ -29,7 +29,7 @@ namespace nml {
 
 namespace {
 
-constexpr int kQ = 128, kK = 64, kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kK = 64;  // keys of a tile
 constexpr float kLog2e = 1.44269504088896341f;
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef short s8 __attribute__((ext_vector_type(8)));
@@ -39,31 +39,32 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 // four, 18.8 at eight, 19.9 at one).
 constexpr int kLeastTiles = 4;
 
-// Workgroups that the card holds at once, two a CU: where the tiles are fewer their keys are cut into
-// pieces. (Pieces for twice as many: 6 ragged rows of up to 512 tokens, 12 heads of 80, 53 in place of 47
+// Workgroups that the card holds at once, eight waves a CU: where the tiles are fewer their keys are cut
+// into pieces. (Pieces for twice as many: 6 ragged rows of up to 512 tokens, 12 heads of 80, 53 in place of 47
 // µs, 128 tokens over 16 Ki keys 83 in place of 64.)
-constexpr int kHeld = 512;
+__host__ __device__ constexpr int held(int Q) { return 256 * 256 / Q; }
 
-// The keys of 128 queries, from q0 on of (row, KV head) bh: length and new tokens of the row, keys that a
+// The keys of Q queries, from q0 on of (row, KV head) bh: length and new tokens of the row, keys that a
 // query of them sees, key tiles a piece and pieces. n·group ≤ q0: no queries.
 struct Span {
   int len, n, kend, per, pieces;
   bool good;  // length and count were in range
 };
+template <int Q>
 __device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int bh, int q0, int splits) {
   Span w;
   const int b = bh / a.Hkv, len = a.lens[b], n = a.counts ? a.counts[b] : a.S;
   w.len = min(max(len, 0), a.max_pages << a.shift);
   w.n = min(max(n, 0), a.S);
   w.good = w.len == len && w.n == n;
-  const int last = min((q0 + kQ - 1) / a.group, w.n - 1);  // the last token
+  const int last = min((q0 + Q - 1) / a.group, w.n - 1);  // the last token
   w.kend = max(w.len - w.n + last + 1, 0);
   const int tiles = (w.kend + kK - 1) / kK;
   // a piece: an even share, for as many workgroups as the card holds, of what all rows would have to do
   // were they as this one (the first queries have fewer keys than the last)
-  const long long queries = (w.n * static_cast<long long>(a.group) + kQ - 1) / kQ;
-  const int mean = (max(w.len - w.n + kQ / a.group, 0) + w.len) / (2 * kK) + 1;
-  const int share = static_cast<int>((queries * mean * a.B * a.Hkv + kHeld - 1) / kHeld);
+  const long long queries = (w.n * static_cast<long long>(a.group) + Q - 1) / Q;
+  const int mean = (max(w.len - w.n + Q / a.group, 0) + w.len) / (2 * kK) + 1;
+  const int share = static_cast<int>((queries * mean * a.B * a.Hkv + held(Q) - 1) / held(Q));
   w.per = max(max(kLeastTiles, share), (tiles + splits - 1) / splits);
   w.pieces = q0 >= w.n * a.group ? 0 : max(1, (tiles + w.per - 1) / w.per);
   return w;
@@ -76,6 +77,7 @@ struct Tile {
 };
 
 // False: nothing to do.
+template <int Q>
 __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int nq, int splits, Tile& t) {
   // (row, KV head) fastest: with a multiple of 8 of them each has its XCD, whose L2 then holds its keys. The
   // last queries, which have the most keys, first; and pieces that a tile does not have behind all others
@@ -86,8 +88,8 @@ __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int nq, int sp
   const int qt = nq - 1 - rest % nq;
   t.piece = rest / nq;
   t.at = bh * nq + qt;
-  t.q0 = qt * kQ;
-  const Span w = span_of(a, bh, t.q0, splits);
+  t.q0 = qt * Q;
+  const Span w = span_of<Q>(a, bh, t.q0, splits);
   if (rest == 0 && !w.good && threadIdx.x == 0) tell(a.err);
   if (t.piece >= w.pieces) return false;
   t.len = w.len;
@@ -102,34 +104,35 @@ __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int nq, int sp
 // Where a piece's part goes: per query its reference (in powers of two) and Σ p, then its Σ p·v.
 struct Parts {
   float *ml, *po;
-  __device__ Parts(const PagedAttnArgs& a) {
+  __device__ Parts(const PagedAttnArgs& a, int Q) {
     ml = reinterpret_cast<float*>(static_cast<char*>(a.ws) + kCounterBytes);  // (behind what other calls keep there)
-    po = ml + static_cast<size_t>(a.slots) * kQ * 2;
+    po = ml + static_cast<size_t>(a.slots) * Q * 2;
   }
 };
 
 // The pieces' parts merged in their order, four dims of a query a thread. (A launch of its own: by the
 // last workgroup of a tile, as in ops_paged.hip, 32 pieces of 128 queries took 100 µs.)
-template <typename T, int DK>
-__global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttnArgs a, int nq, int splits) {
-  constexpr int Q = DK / 4, kRows = kThreads / Q, kBlocks = (kQ + kRows - 1) / kRows;
-  const int at = blockIdx.x / kBlocks, bh = at / nq, q0 = (at - bh * nq) * kQ;
-  const Span w = span_of(a, bh, q0, splits);
+constexpr int kMergers = 256;
+template <typename T, int DK, int Q>
+__global__ __launch_bounds__(kMergers) void paged_merge_kernel(PagedAttnArgs a, int nq, int splits) {
+  constexpr int L = DK / 4, kRows = kMergers / L, kBlocks = (Q + kRows - 1) / kRows;
+  const int at = blockIdx.x / kBlocks, bh = at / nq, q0 = (at - bh * nq) * Q;
+  const Span w = span_of<Q>(a, bh, q0, splits);
   if (w.pieces <= 1) return;
-  const int c = blockIdx.x % kBlocks * kRows + threadIdx.x / Q, d = threadIdx.x % Q * 4;
-  if (threadIdx.x / Q >= kRows || c >= kQ || q0 + c >= w.n * a.group || d >= a.dk) return;
-  const Parts parts(a);
+  const int c = blockIdx.x % kBlocks * kRows + threadIdx.x / L, d = threadIdx.x % L * 4;
+  if (threadIdx.x / L >= kRows || c >= Q || q0 + c >= w.n * a.group || d >= a.dk) return;
+  const Parts parts(a, Q);
   const size_t first = static_cast<size_t>(at) * splits;
   // (float32: parts times 2^-12, whose sums of near the largest values stay finite)
   constexpr float kRoom = sizeof(T) == 2 ? 0.f : 12.f;
   float top = -INFINITY;
-  for (int y = 0; y < w.pieces; ++y) top = fmaxf(top, parts.ml[2 * ((first + y) * kQ + c)]);
+  for (int y = 0; y < w.pieces; ++y) top = fmaxf(top, parts.ml[2 * ((first + y) * Q + c)]);
   const float rf = (top == -INFINITY ? 0.f : top) + kRoom;
   float lt = 0.f;
   floatx4 ot = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int y = 0; y < w.pieces; ++y) {
-    const size_t q = (first + y) * kQ + c;
+    const size_t q = (first + y) * Q + c;
     const f2 st = *reinterpret_cast<const f2*>(parts.ml + 2 * q);
     const floatx4 x = *reinterpret_cast<const floatx4*>(parts.po + q * DK + d);
     const float f = __builtin_amdgcn_exp2f(st.x - rf);
@@ -144,9 +147,10 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttnArgs a, 
 }
 
 // DK: head dims up to it, in steps of 8.
-template <int DK>
-__global__ __launch_bounds__(kThreads, 2) void paged_prefill_f16_kernel(PagedAttnArgs a, int nq, int splits) {
+template <int DK, int kWaves>
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_prefill_f16_kernel(PagedAttnArgs a, int nq, int splits) {
 #pragma clang fp contract(off)
+  constexpr int kThreads = 64 * kWaves, kQ = 32 * kWaves;
   constexpr int KS = DK / 16, OT = DK / 32, VG = DK / 8;
   constexpr int L = DK <= 64 ? 8 : 16;    // lanes of a row, 16 bytes each
   constexpr int RW = 64 / L;              // rows of a wave's load
@@ -155,7 +159,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prefill_f16_kernel(PagedAtt
   __shared__ __align__(16) half_t Ks[2][kK][KP];
   __shared__ __align__(16) half_t Vs[2][kK][VP];
   Tile w;
-  if (!find_tile(a, nq, splits, w)) return;
+  if (!find_tile<kQ>(a, nq, splits, w)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int dk = a.dk, R = w.n * a.group, hi = lane >> 5;
   const int qw = w.q0 + wave * 32, myq = qw + (lane & 31);  // the wave's first query, this lane's
@@ -430,7 +434,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prefill_f16_kernel(PagedAtt
       }
     return;
   }
-  const Parts parts(a);
+  const Parts parts(a, kQ);
   const size_t q = (static_cast<size_t>(w.at) * splits + w.piece) * kQ + wave * 32 + (lane & 31);
   if (hi == 0) *reinterpret_cast<f2*>(parts.ml + 2 * q) = f2{m == -INFINITY ? m : m * cscale, l};
 #pragma unroll
@@ -450,7 +454,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prefill_f16_kernel(PagedAtt
 // the matrix pipe that its softmax takes beside it: one buffer and two barriers a tile, with the other
 // workgroup of the CU in between.
 template <int DK>
-__global__ __launch_bounds__(kThreads, 2) void paged_prefill_f32_kernel(PagedAttnArgs a, int nq, int splits) {
+__global__ __launch_bounds__(256, 2) void paged_prefill_f32_kernel(PagedAttnArgs a, int nq, int splits) {
+  constexpr int kWaves = 4, kQ = 32 * kWaves;
   constexpr int KS = DK / 8, OT = DK / 32, VG = DK / 4;
   constexpr int W = OT == 3 ? 1 : OT;
   constexpr int L = DK == 32 ? 8 : DK == 64 ? 16 : 32;  // lanes of a row, 16 bytes each
@@ -460,7 +465,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prefill_f32_kernel(PagedAtt
   __shared__ __align__(16) float Ks[kK][P];
   __shared__ __align__(16) float Vs[kK][P];
   Tile w;
-  if (!find_tile(a, nq, splits, w)) return;
+  if (!find_tile<kQ>(a, nq, splits, w)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int dk = a.dk, R = w.n * a.group, hi = lane >> 5, l32 = lane & 31;
   const int qw = w.q0 + wave * 32, myq = qw + l32;
@@ -664,46 +669,56 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prefill_f32_kernel(PagedAtt
     });
     return;
   }
-  const Parts parts(a);
+  const Parts parts(a, kQ);
   const size_t q = (static_cast<size_t>(w.at) * splits + w.piece) * kQ + wave * 32 + l32;
   if (hi == 0) *reinterpret_cast<f2*>(parts.ml + 2 * q) = f2{ref, l};
   each_pair([&](int dim, f2 v) { *reinterpret_cast<f2*>(parts.po + q * DK + dim) = v; });
 }
 
-// Tiles of 128 queries, and the most pieces that the keys of one are cut into.
-struct Grid {
-  long long tiles;
-  int nq, splits;
-};
-Grid grid_of(int B, int H, int Hkv, int S, int P) {
-  Grid g;
-  g.nq = (H / Hkv * S + kQ - 1) / kQ;
-  g.tiles = static_cast<long long>(g.nq) * Hkv * B;
-  const int most = std::max(1, (P + kK - 1) / kK / kLeastTiles);
-  g.splits = g.tiles >= kHeld ? 1 : static_cast<int>(std::min<long long>(most, (2 * kHeld + g.tiles - 1) / g.tiles));
-  return g;
-}
-
+// Queries of a workgroup: float16 at head dims above 64 eight waves, which share what is written to LDS (a
+// piece of 2048 tokens over 8192 keys of 128: 307 µs, 322 with four; of 64 215 and 189), where a KV head has
+// more than four take.
+int queries_of(int dt, int R, int dk) { return dt == F16 && dk > 64 && R > 128 ? 256 : 128; }
 // Columns of the kernel that takes a head dim.
 int columns_of(int dt, int dk) { return dk <= 32 && dt == F32 ? 32 : dk <= 64 ? 64 : dk <= 96 ? 96 : 128; }
 
-template <int DK>
-int launch_columns(int dt, const PagedAttnArgs& a, const Grid& g, hipStream_t st) {
+// Tiles of queries, and the most pieces that the keys of one are cut into.
+struct Grid {
+  long long tiles;
+  int q, nq, splits;
+};
+Grid grid_of(int dt, int B, int H, int Hkv, int S, int P, int dk) {
+  Grid g;
+  const int R = H / Hkv * S;
+  g.q = queries_of(dt, R, dk);
+  g.nq = (R + g.q - 1) / g.q;
+  g.tiles = static_cast<long long>(g.nq) * Hkv * B;
+  const int most = std::max(1, (P + kK - 1) / kK / kLeastTiles), all = held(g.q);
+  g.splits = g.tiles >= all ? 1 : static_cast<int>(std::min<long long>(most, (2 * all + g.tiles - 1) / g.tiles));
+  return g;
+}
+
+template <typename T, int DK, int Q>
+int launch_kernels(const PagedAttnArgs& a, const Grid& g, hipStream_t st) {
   const unsigned n = static_cast<unsigned>(g.tiles * g.splits);
-  if constexpr (DK > 32) {
-    if (dt == F16) paged_prefill_f16_kernel<DK><<<n, kThreads, 0, st>>>(a, g.nq, g.splits);
-  }
-  if (dt == F32) paged_prefill_f32_kernel<DK><<<n, kThreads, 0, st>>>(a, g.nq, g.splits);
+  if constexpr (sizeof(T) == 2) paged_prefill_f16_kernel<DK, Q / 32><<<n, 2 * Q, 0, st>>>(a, g.nq, g.splits);
+  else paged_prefill_f32_kernel<DK><<<n, 2 * Q, 0, st>>>(a, g.nq, g.splits);
   NML_LAUNCHED();
   if (g.splits == 1) return 0;
-  constexpr int kRows = kThreads / (DK / 4);
-  const unsigned blocks = static_cast<unsigned>(g.tiles * ((kQ + kRows - 1) / kRows));
-  if constexpr (DK > 32) {
-    if (dt == F16) paged_merge_kernel<half_t, DK><<<blocks, kThreads, 0, st>>>(a, g.nq, g.splits);
-  }
-  if (dt == F32) paged_merge_kernel<float, DK><<<blocks, kThreads, 0, st>>>(a, g.nq, g.splits);
+  constexpr int kRows = kMergers / (DK / 4);
+  const unsigned blocks = static_cast<unsigned>(g.tiles * ((Q + kRows - 1) / kRows));
+  paged_merge_kernel<T, DK, Q><<<blocks, kMergers, 0, st>>>(a, g.nq, g.splits);
   NML_LAUNCHED();
   return 0;
+}
+
+template <int DK>
+int launch_columns(int dt, const PagedAttnArgs& a, const Grid& g, hipStream_t st) {
+  if (dt == F32) return launch_kernels<float, DK, 128>(a, g, st);
+  if constexpr (DK > 64) {
+    if (g.q == 256) return launch_kernels<half_t, DK, 256>(a, g, st);
+  }
+  return launch_kernels<half_t, DK, 128>(a, g, st);
 }
 
 }  // namespace
@@ -716,16 +731,16 @@ bool paged_prefill_applies(int dt, int H, int Hkv, int S, int dk) {
 }
 
 size_t paged_prefill_workspace(int dt, int B, int H, int Hkv, int S, int P, int dk) {
-  const Grid g = grid_of(B, H, Hkv, S, P);
+  const Grid g = grid_of(dt, B, H, Hkv, S, P, dk);
   if (g.splits == 1) return 0;
-  return kCounterBytes + sizeof(float) * g.tiles * g.splits * kQ * (2 + columns_of(dt, dk));
+  return kCounterBytes + sizeof(float) * g.tiles * g.splits * g.q * (2 + columns_of(dt, dk));
 }
 
 int launch_paged_prefill(int dt, PagedAttnArgs a, hipStream_t st) {
-  const Grid g = grid_of(a.B, a.H, a.Hkv, a.S, a.max_pages << a.shift);
+  const Grid g = grid_of(dt, a.B, a.H, a.Hkv, a.S, a.max_pages << a.shift, a.dk);
   a.slots = g.splits > 1 ? static_cast<int>(g.tiles * g.splits) : 0;
   switch (columns_of(dt, a.dk)) {
-    case 32: return launch_columns<32>(dt, a, g, st);
+    case 32: return launch_kernels<float, 32, 128>(a, g, st);
     case 64: return launch_columns<64>(dt, a, g, st);
     case 96: return launch_columns<96>(dt, a, g, st);
   }

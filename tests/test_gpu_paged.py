@@ -93,6 +93,16 @@ def test_attention(gpu, batch, kv, group, dk, page, pages, seq, dtype):
 
 
 @pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("group, dk", [(1, 64), (3, 72), (5, 96), (2, 128)])
+def test_many_new_tokens_behind_a_long_cache(gpu, group, dk, dtype):
+    """Several tiles of queries of a row, whose keys are cut into pieces of a size that differs with the row."""
+    cache = Cache(3, 2, dk, 16, 130, dtype, dk)
+    q = queries(3, 2 * group, 257, dk, dtype, dk)
+    check(cache, q, np.array([2080, 700, 257], np.int32), None)
+    check(cache, q, np.array([1999, 100, 0], np.int32), np.array([129, 256, 3], np.int32))
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
 @pytest.mark.parametrize("seq", [1, 5, 150])
 def test_what_is_not_seen_does_not_matter(gpu, dtype, seq):
     """NaN and infinities past a row's length, in other pages, and in the tokens after a token."""
