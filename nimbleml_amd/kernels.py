@@ -579,6 +579,9 @@ def paged_attention(q, cache, table, lens, scale, counts=None):
 def _teacher_rows(logits, top_ids, top_logits, what):
     """(logits, ids, values, rows, vocab, entries a row) of a distillation's arguments."""
     dt = _float_dtype(logits)
+    shape = tuple(np.shape(logits))
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"{what}: logits must be (..., vocab), got {shape}")
     ld = _dev(logits, dt)
     vocab = ld.shape[-1]
     rows = ld.size // vocab

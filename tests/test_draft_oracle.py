@@ -155,5 +155,8 @@ def test_wrappers_check_before_they_touch_the_device():
         K.verify_drafts(x, np.zeros((2, 4)), temperature=0.0)
     with pytest.raises(ValueError, match="draft_logits must be"):
         K.verify_drafts(x, np.zeros((2, 3)), np.zeros((2, 4)), draft_logits=x)
+    for empty in (np.zeros((2, 0), np.float32), np.float32(1)):
+        with pytest.raises(ValueError, match="logits must be"):
+            K.distill(empty, np.zeros((2, 3)), np.zeros((2, 3)))
     with pytest.raises(ValueError, match="power of two"):
         K.PagedKVCache(4, 24, 1, 64)

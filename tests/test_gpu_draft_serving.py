@@ -217,3 +217,67 @@ def test_captured_and_replayed(gpu, hip):  # noqa: F811
                 assert np.array_equal(a, b, equal_nan=True), i
     finally:
         graph.close()
+
+
+def test_two_streams_at_once(gpu, hip):  # noqa: F811
+    """Calls on two streams, each with its own workspaces, over one cache: as one after another."""
+    r = np.random.RandomState(5)
+    cache = Cache(2, 2, 128, 16, 130, np.float16, 23)
+    lens = upload(np.array([2080, 900], np.int32))
+    table = upload(cache.table)
+    V, batch, n = 20001, 5, 4
+    need = N.sz()
+    sides = []
+    for seq in (4, 300):
+        q = upload(queries(2, 4, seq, 128, np.float16, seq))
+        N.check(N.lib.nml_paged_attention_workspace(2, 4, 2, seq, 130, 16, 128, 1, C.byref(need)))
+        ws = upload(np.zeros(need.value, np.uint8))
+        N.check(N.lib.nml_verify_drafts_workspace(batch, n, V, C.byref(need)))
+        vws = upload(r.randint(0, 256, need.value).astype(np.uint8))
+        logits, drafts, u = upload(r.randn(batch, n + 1, V).astype(np.float32)), upload(r.randint(0, V, (batch, n))), \
+            upload(r.rand(batch, n + 1))
+        out, acc, tok = N.DeviceArray((2, seq, 512), np.float16), N.DeviceArray((batch,), np.int32), \
+            N.DeviceArray((batch, n + 1), np.int64)
+
+        def work(seq=seq, q=q, ws=ws, vws=vws, logits=logits, drafts=drafts, u=u, out=out, acc=acc, tok=tok):
+            N.check(N.lib.nml_paged_attention_device(
+                q.ptr, cache.c.k_pages.ptr, cache.c.v_pages.ptr, table.ptr, lens.ptr, None, out.ptr, 2, 4, 2, seq, 130, 16,
+                cache.c.num_pages, 128, 11.0, ws.ptr, ws.nbytes, None, 1))
+            N.check(N.lib.nml_verify_drafts_device(
+                logits.ptr, V, None, 0, drafts.ptr, None, u.ptr, batch, n, V, 1.0, acc.ptr, tok.ptr, vws.ptr, vws.nbytes,
+                None, 0))
+
+        work()
+        N.synchronize()
+        sides.append((work, (out, acc, tok), [o.numpy() for o in (out, acc, tok)]))
+        for o in (out, acc, tok):
+            N.check(N.lib.nml_memset(o.ptr, 0xff, o.nbytes))
+    N.synchronize()
+    graphs = [Graph(hip, side[0]) for side in sides]  # (each on a stream of its own)
+    try:
+        for _ in range(3):
+            for _ in range(5):
+                for g in graphs:
+                    g.run()
+            for g in graphs:
+                g.wait()
+            for _, outs, want in sides:
+                for o, w in zip(outs, want):
+                    assert np.array_equal(o.numpy(), w)
+    finally:
+        for g in graphs:
+            g.close()
+
+
+def test_empty_batches(gpu):
+    loss, m, lsum = K.distill(np.zeros((0, 7), np.float32), np.zeros((0, 2)), np.zeros((0, 2)))
+    assert loss.shape == m.shape == lsum.shape == (0,)
+    accepted, tokens = K.verify_drafts(np.zeros((0, 3, 7), np.float32), np.zeros((0, 2)), np.zeros((0, 3)))
+    assert accepted.shape == (0,) and tokens.shape == (0, 3)
+    cache = K.PagedKVCache(2, 8, 1, 16, np.float16)
+    none = np.zeros((0, 1, 2, 16), np.float16)
+    K.paged_write(cache, none, none, np.zeros((0, 1)))
+    assert K.paged_attention(none, cache, np.zeros((0, 1)), np.zeros(0), 4.0).shape == (0, 2, 16)
+    no_tokens = np.zeros((2, 1, 0, 16), np.float16)
+    K.paged_write(cache, no_tokens, no_tokens, np.zeros((2, 1)))
+    assert K.paged_attention(no_tokens, cache, np.zeros((2, 1)), np.zeros(2), 4.0).shape == (2, 0, 16)
