@@ -278,3 +278,23 @@ def test_pages_past_32_bits(gpu):
         x.reshape(1024, dk)[:1000] = new[0, 0]
     want, _, _ = R.paged_attention(q, *fill, np.arange(4)[None], [1000], [3], np.sqrt(dk))
     assert np.abs(got - want[0]).max() <= 2.0 ** -11 * np.abs(want).max() * 2
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_out_of_range_is_told_with_many_new_tokens(gpu, dtype):
+    cache = Cache(2, 1, 32, 8, 40, dtype, 15)
+    q, lens = queries(2, 1, 150, 32, dtype, 15), np.array([320, 200], np.int32)
+    good = K.paged_attention(q, cache.c, cache.table, lens, 4.0).numpy().reshape(2, 150, 32)
+    for page in (-1, cache.c.num_pages, 1 << 30):
+        bad = cache.table.copy()
+        bad[1, 24] = page  # (its keys 192 … 199, the last that it has)
+        with pytest.raises(ValueError, match="page"):
+            K.paged_attention(q, cache.c, upload(bad), lens, 4.0)
+        short = np.array([320, 192], np.int32)  # (the page is not read then)
+        got = K.paged_attention(q, cache.c, upload(bad), short, 4.0).numpy().reshape(2, 150, 32)
+        assert np.array_equal(got[0], good[0])
+    for lens, counts, match in (([321, 200], [150, 3], "length"), ([320, -1], [150, 3], "length"),
+                                ([320, 200], [151, 3], "count"), ([320, 200], [150, -1], "count")):
+        with pytest.raises(ValueError, match=match):
+            K.paged_attention(q, cache.c, upload(cache.table), upload(np.array(lens, np.int32)), 4.0,
+                              np.array(counts, np.int32))
