@@ -29,8 +29,8 @@ __device__ __forceinline__ unsigned quotient(unsigned n, Div d) { return (__umul
 
 // A writing workgroup, and the units that a lane of it takes (their loads in flight together: 4 × 4096 tokens
 // of 16 heads of 128 float16 values, µs with four 57.9, two 52.7, eight 151). Written past the caches, which
-// a prompt's keys leave again before they are read: 39.9, 6.7 TB/s of reads and writes (the reads partly from
-// the last cache).
+// a prompt's keys leave again before they are read: 39.5, 6.8 TB/s of reads and writes (the reads partly from
+// the last cache; with inputs that were not there 59, 4.6). One token of 32 rows, 16 heads of 64: 3.0.
 constexpr int kWriters = 256, kEach = 4;
 
 // Units of one row: (head, token, unit of its vector), the unit fastest: the order of the pages, so
@@ -112,6 +112,11 @@ int write_launch(PagedWriteArgs a, size_t es, hipStream_t st) {
 // A (row, KV head, 16 queries) is one workgroup's unless its keys are many: pieces of a long one go to
 // several, as many in all as the card holds at once, and the last to finish merges them in their
 // order.
+//
+// Bound by HBM where keys are many: 16 rows of 1 to 8 Ki keys, 32 heads over 8 of 128, float16, 68 µs,
+// 4.4 TB/s of keys and values (a copy 4.8). Where few, by a chain of dependent steps: lengths, page
+// numbers, keys, rounds, merge and the pieces' merge: one row of 1023 keys, 16 heads of 64, 8.8 µs; 16
+// rows of up to 2048 and up to 5 tokens, 8 heads of 32, float32, 14.8.
 
 typedef short s4 __attribute__((ext_vector_type(4)));
 

@@ -16,7 +16,9 @@
 // Exponentials and sums are in 64 bits: a token is where a running sum of V weights passes a number,
 // and with 32 bits about one in 10^3 … 10^4 tokens would be the neighbour of the one that the formula
 // gives. A 64-bit multiply-add runs at the rate of a 32-bit one on this card, and an exponential takes
-// 14 such operations.
+// 14 such operations: the first launch is bound by them (and the loads before), the second by its
+// chain of dependent steps, two passes over a part with a count of arrivals in between. One sequence of four
+// drafts, 32000 float32 logits a row: 3.1 and 8.3 µs; 32 of up to five, 50304 float16 logits: 14.9 and 12.8.
 #include "kernels.hpp"
 
 namespace nml {
@@ -25,7 +27,9 @@ namespace {
 
 constexpr int kThreads = 256, kMaxRows = kMaxDrafts + 1;
 // Elements of a part of a row, a thread's times kThreads: few where the rows are few, so that a lone
-// call's chain is short.
+// call's chain is short. (µs of both launches, few or many by size / always few / always many: one
+// sequence of four drafts, 32000 float32, 11.4 / 11.8 / 19.8; 32 of up to five, 50304 float16, 27.0 / 27.4 /
+// 29.0; 64 of eight, 32000 float16, 40.9 / 47.2 / 42.2.)
 constexpr int kSmall = 8, kLarge = 32;
 constexpr int kLine = 32;  // words from one sequence's counter to the next: a line of its own
 
