@@ -4,6 +4,7 @@
 // of one row, a head's positions in a run. Row b's position p is position p % page of page
 // table[b·max_pages + p / page].
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels.hpp"
 #include "paged.hpp"
@@ -116,7 +117,8 @@ int write_launch(PagedWriteArgs a, size_t es, hipStream_t st) {
 // Bound by HBM where keys are many: 16 rows of 1 to 8 Ki keys, 32 heads over 8 of 128, float16, 68 µs,
 // 4.4 TB/s of keys and values (a copy 4.8). Where few, by a chain of dependent steps: lengths, page
 // numbers, keys, rounds, merge and the pieces' merge: one row of 1023 keys, 16 heads of 64, 8.8 µs; 16
-// rows of up to 2048 and up to 5 tokens, 8 heads of 32, float32, 14.8.
+// rows of up to 2048 and up to 5 tokens, 8 heads of 32, float32, 14.8. (Where work is cut finely enough the
+// merge is what is left: its loads are in batches of 16 pieces, of four where there are no more.)
 
 typedef short s4 __attribute__((ext_vector_type(4)));
 
@@ -137,17 +139,21 @@ constexpr float up_log2() {
 constexpr int steps_of(int dk) { return dk <= 32 ? 1 : dk <= 64 ? 2 : dk <= 128 ? 4 : 8; }
 // Waves of a workgroup. Few begin and merge sooner, and more workgroups even out rows of different length
 // (µs with four and eight: 16 rows of 1 to 8 Ki keys, 32 heads over 8 of 128, 54 and 70; one row of 1023, 16
-// heads of 64, 10.7 and 12.2, 9.2 with two; 128 rows of 100 to 1000 60.9 with four and 57.1 with two). At
-// head dim 256 a wave's tile fills its registers and eight keep the CU's four pipes busy (16 rows of 1
-// to 4 Ki keys, 16 heads over 2, 42.9 and 37.9).
-__host__ __device__ constexpr int group_waves(int nb) { return nb == 2 ? 2 : nb == 8 ? 8 : 4; }
-// Waves a SIMD that the registers are held to, and the workgroups that the card's 256 CUs then
-// hold at once.
-__host__ __device__ constexpr int waves_of(int nb) { return nb <= 2 ? 4 : 2; }
-__host__ __device__ constexpr int capacity(int nb) { return 256 * 4 * waves_of(nb) / group_waves(nb); }
+// heads of 64, 10.7 and 12.2, 9.2 with two; 128 rows of 100 to 1000 60.9 with four and 57.1 with two).
+__host__ __device__ constexpr int group_waves(int nb) { return nb == 2 ? 2 : 4; }
+// Waves a SIMD that the registers are held to (at head dim 256 a wave's tile takes more than half of them: 16
+// rows of 1 to 4 Ki keys, 16 heads over 2, float16 33 µs and float32 47; held to two waves 38 and 68, with
+// spills), and the workgroups that the card's CUs then hold at once.
+__host__ __device__ constexpr int waves_of(int nb) { return nb <= 2 ? 4 : nb == 8 ? 1 : 2; }
+constexpr int kCus = 256;
+__host__ __device__ constexpr int capacity(int nb) { return kCus * 4 * waves_of(nb) / group_waves(nb); }
 // Spans (a tile for each wave) that a piece has at least: what it costs to begin one and to merge it. (One row
 // of 1023 keys, 16 heads of 64: 9.2 µs at two spans of 64 keys, 10.6 at four, 8.9 at one; of 100 keys 6.9, 6.9, 8.7.)
 __host__ __device__ constexpr int least_spans(int nb) { return nb == 2 ? 2 : 1; }
+// Pieces that a thread of a merge takes its four values of in the time of a round (16000 keys, 16 heads over one
+// of 128: 26 µs, 27 at eight, 65 with a piece for each span and batches of four; 8000 keys, 32 heads over 4 of
+// 64: 14.0, 13.4, 17.7).
+constexpr float kMerged = 16.f;
 
 // ws: a counter for each tile in pieces, then for each piece its rows' references and Σ p, then their
 // Σ p·v. Tiles in pieces are fewer than the card's workgroups (a piece is at least their even share),
@@ -175,16 +181,17 @@ struct Rows {
   }
 };
 
-// What this workgroup does: piece `piece` of `pieces` of tile (b, e), whose row has len keys and n
+// What this workgroup does: piece `piece` of `pieces` of tile (b, hk, tile), whose row has len keys and n
 // new tokens; `slot`: where the tile's first piece is in ws. b < 0: nothing.
 struct Work {
-  int b, e, piece, pieces, slot, len, n, spans;
+  int b, hk, tile, piece, pieces, slot, len, n, spans;
 };
 // More than 64 rows are shared out to the waves, a run of rows each; sums: of the waves.
 template <int SPAN, int NW>
-__device__ __forceinline__ Work find_work(const PagedAttnArgs& a, int each, int cap, int fewest, int lane, int wave, int (*sums)[3]) {
+__device__ __forceinline__ Work find_work(const PagedAttnArgs& a, int tiles, int cap, int fewest, float merge, int lane, int wave, int (*sums)[3]) {
   Work w{};
   Rows<SPAN> rows;
+  const int each = a.Hkv * tiles;
   const int run = a.B <= 64 ? 64 : (a.B + 64 * NW - 1) / (64 * NW) * 64;
   const int first = a.B <= 64 ? 0 : wave * run, end = min(first + run, a.B);
   int total = 0;
@@ -204,7 +211,17 @@ __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, int each, int 
     for (int i = 0; i < NW; ++i) total += sums[i][0];
   }
   const int room = room_for(static_cast<long long>(each) * a.B, cap);
-  const int least = max(fewest, static_cast<int>((static_cast<long long>(total) * each + room - 1) / room));
+  int least = max(fewest, static_cast<int>((static_cast<long long>(total) * each + room - 1) / room));
+  // What a piece takes of the merge, `merge` of a round, against its own rounds: s spans to a piece, s² = merge ·
+  // the row's in the mean.
+  const float mean = static_cast<float>(total) * __builtin_amdgcn_rcpf(static_cast<float>(a.B));
+  least = max(least, static_cast<int>(__builtin_ceilf(__builtin_amdgcn_sqrtf(mean * merge))));
+  // Few tiles, which pieces of any size leave even: a wave for each SIMD, beside which a second one adds
+  // pieces to merge but no bandwidth (30000 keys, 32 heads over 8 of 128: 29.5 µs, 33.5 with two). More tiles, of
+  // different length, are evener in more pieces (16 rows of 1 to 8 Ki: 55, 73 with one).
+  constexpr int kEven = kCus * 4 / NW;
+  if (static_cast<long long>(each) * a.B <= kEven / 4)
+    least = max(least, static_cast<int>((static_cast<long long>(total) * each + kEven - 1) / kEven));
   auto pieces_of = [&](int spans) { return spans <= least ? min(spans, 1) : (spans + least - 1) / least; };
   const int at = static_cast<int>(blockIdx.x / each);
   int before = 0, slots = 0, from = 0;
@@ -243,9 +260,19 @@ __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, int each, int 
       const int start = before + __builtin_amdgcn_readlane(sum, l) - w.pieces;
       const int local = static_cast<int>(blockIdx.x) - start * each;
       w.b = i + l;
-      w.e = w.pieces == 1 ? local : local / w.pieces;
-      w.piece = local - w.e * w.pieces;
-      w.slot = (slots + __builtin_amdgcn_readlane(sum_slots, l) - w.pieces) * each + w.e * w.pieces;
+      // A KV head's piece is of all of its tiles: they are 8 workgroups apart, on one XCD, whose L2 has its
+      // keys for them (five tokens over 30000 keys, two tiles: 52 µs, 58 with a tile's pieces side by side).
+      int both = local;
+      w.tile = 0;
+      if (tiles > 1) {
+        const int heads = a.Hkv * w.pieces, turn = local / (8 * tiles), in = local - turn * (8 * tiles);
+        const int width = min(8, heads - 8 * turn);
+        w.tile = width == 8 ? in >> 3 : in / width;
+        both = 8 * turn + in - w.tile * width;
+      }
+      w.hk = w.pieces == 1 ? both : both / w.pieces;
+      w.piece = both - w.hk * w.pieces;
+      w.slot = (slots + __builtin_amdgcn_readlane(sum_slots, l) - w.pieces) * each + (w.hk * tiles + w.tile) * w.pieces;
       return w;
     }
     before += __builtin_amdgcn_readlane(sum, 63);
@@ -417,9 +444,10 @@ __global__ __launch_bounds__(64 * group_waves(NB), waves_of(NB)) void paged_atte
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
   const int R = a.group * a.S, tiles = (R + 15) / 16;
-  const Work work = find_work<kSpan, NW>(a, a.Hkv * tiles, capacity(NB), least_spans(NB), lane, w, reinterpret_cast<int(*)[3]>(lds));
+  const float merge = static_cast<float>(min(16, R)) * (D / (4.f * kThreads * kMerged));
+  const Work work = find_work<kSpan, NW>(a, tiles, capacity(NB), least_spans(NB), merge, lane, w, reinterpret_cast<int(*)[3]>(lds));
   if (work.b < 0 || work.n == 0) return;
-  const int hk = tiles == 1 ? work.e : work.e / tiles, tile = work.e - hk * tiles;
+  const int hk = work.hk, tile = work.tile;
   const int per = work.pieces == 1 ? work.spans : (work.spans + work.pieces - 1) / work.pieces;
 
   // The query of column c of this tile: row r of the KV head's R, token r / group of head hk·group +
@@ -657,7 +685,7 @@ __global__ __launch_bounds__(64 * group_waves(NB), waves_of(NB)) void paged_atte
   if (arrived + 1 != static_cast<unsigned>(work.pieces)) return;
   if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   // four dims of a row a thread, the pieces over as many threads as there are
-  constexpr int Q = D / 4, kBatch = 4;
+  constexpr int Q = D / 4;
   struct Sum {
     floatx4 o;
     float m, l;
@@ -668,33 +696,38 @@ __global__ __launch_bounds__(64 * group_waves(NB), waves_of(NB)) void paged_atte
   for (int i = threadIdx.x - way * cols; i < cols; i += kThreads) {
     const int c = i / Q, dq = i % Q;
     Sum t{floatx4{0.f, 0.f, 0.f, 0.f}, -INFINITY, 0.f};
-    for (int y = way; y < work.pieces && way < ways; y += kBatch * ways) {
-      f2 st[kBatch], p[kBatch][2];
+    auto add = [&](auto batch) {  // pieces whose loads are in flight together
+      constexpr int kBatch = decltype(batch)::value;
+      for (int y = way; y < work.pieces && way < ways; y += kBatch * ways) {
+        f2 st[kBatch], p[kBatch][2];
 #pragma unroll
-      for (int z = 0; z < kBatch; ++z) {  // (every load of a batch before the first use)
-        st[z] = f2{-INFINITY, 0.f};
-        p[z][0] = p[z][1] = f2{0.f, 0.f};
-        if (y + z * ways < work.pieces) {
-          const size_t at = static_cast<size_t>(work.slot + y + z * ways) * slot_rows + c;
-          st[z] = get2(ml + 2 * at);
-          p[z][0] = get2(po + at * D + 4 * dq);
-          p[z][1] = get2(po + at * D + 4 * dq + 2);
+        for (int z = 0; z < kBatch; ++z) {  // (every load of a batch before the first use)
+          st[z] = f2{-INFINITY, 0.f};
+          p[z][0] = p[z][1] = f2{0.f, 0.f};
+          if (y + z * ways < work.pieces) {
+            const size_t at = static_cast<size_t>(work.slot + y + z * ways) * slot_rows + c;
+            st[z] = get2(ml + 2 * at);
+            p[z][0] = get2(po + at * D + 4 * dq);
+            p[z][1] = get2(po + at * D + 4 * dq + 2);
+          }
+        }
+        float mn = t.m;
+#pragma unroll
+        for (int z = 0; z < kBatch; ++z) mn = fmaxf(mn, st[z].x + kRoom2);
+        const float rf = mn == -INFINITY ? 0.f : mn, f0 = __builtin_amdgcn_exp2f(t.m - rf);
+        t.m = mn;
+        t.l *= f0;
+        t.o *= f0;
+#pragma unroll
+        for (int z = 0; z < kBatch; ++z) {
+          const float f = __builtin_amdgcn_exp2f(st[z].x - rf);
+          t.l += st[z].y * f;
+          t.o += floatx4{p[z][0].x, p[z][0].y, p[z][1].x, p[z][1].y} * f;
         }
       }
-      float mn = t.m;
-#pragma unroll
-      for (int z = 0; z < kBatch; ++z) mn = fmaxf(mn, st[z].x + kRoom2);
-      const float rf = mn == -INFINITY ? 0.f : mn, f0 = __builtin_amdgcn_exp2f(t.m - rf);
-      t.m = mn;
-      t.l *= f0;
-      t.o *= f0;
-#pragma unroll
-      for (int z = 0; z < kBatch; ++z) {
-        const float f = __builtin_amdgcn_exp2f(st[z].x - rf);
-        t.l += st[z].y * f;
-        t.o += floatx4{p[z][0].x, p[z][0].y, p[z][1].x, p[z][1].y} * f;
-      }
-    }
+    };
+    if (work.pieces > 8 * ways) add(std::integral_constant<int, 16>{});
+    else add(std::integral_constant<int, 4>{});
     if (ways > 1) {
       sums[threadIdx.x] = t;
       __syncthreads();

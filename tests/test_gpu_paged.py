@@ -103,6 +103,19 @@ def test_many_new_tokens_behind_a_long_cache(gpu, group, dk, dtype):
 
 
 @pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("batch, kv, group, dk, seq", [
+    (1, 1, 16, 128, 1), (1, 3, 4, 64, 6), (2, 1, 1, 256, 3), (1, 2, 5, 200, 9), (5, 3, 9, 32, 2), (1, 11, 1, 16, 1), (3, 5, 1, 96, 30)])
+def test_many_pieces(gpu, batch, kv, group, dk, seq, dtype):
+    """Few rows of many keys: pieces of every tile merged, KV heads in eights and not, one tile and several."""
+    cache = Cache(batch, kv, dk, 64, 130, dtype, dk + seq)
+    q, r = queries(batch, kv * group, seq, dk, dtype, dk), np.random.RandomState(seq)
+    check(cache, q, np.full(batch, 8320, np.int32), None)
+    lens = r.randint(0, 8321, batch).astype(np.int32)
+    lens[0] = 8001
+    check(cache, q, lens, r.randint(0, seq + 1, batch).astype(np.int32))
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
 @pytest.mark.parametrize("seq", [1, 5, 150])
 def test_what_is_not_seen_does_not_matter(gpu, dtype, seq):
     """NaN and infinities past a row's length, in other pages, and in the tokens after a token."""
