@@ -23,7 +23,8 @@
 //
 // Bound by the matrix pipe and the exponentials beside it. 2048 tokens over 8192 keys, 32 heads of 128 over
 // 8, float16: 306 µs, 786 TFLOP/s, where a product of 8192³ reaches 1089; two rows of them with 16 heads of
-// 64: 188, 640 (as many exponentials for half the products).
+// 64: 188, 640 (as many exponentials for half the products); 16 over 4 of 256: 624, 385 (one wave a SIMD, and
+// values moved between its two halves of the registers).
 #include <algorithm>
 #include <type_traits>
 
@@ -43,10 +44,10 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 // four, 18.8 at eight, 19.9 at one).
 constexpr int kLeastTiles = 4;
 
-// Workgroups that the card holds at once, eight waves a CU: where the tiles are fewer their keys are cut
-// into pieces. (Pieces for twice as many: 6 ragged rows of up to 512 tokens, 12 heads of 80, 53 in place of 47
+// Workgroups that the card holds at once, eight waves a CU (columns above 128, which take more than half of
+// the registers: four): where the tiles are fewer their keys are cut into pieces. (Pieces for twice as many: 6 ragged rows of up to 512 tokens, 12 heads of 80, 53 in place of 47
 // µs, 128 tokens over 16 Ki keys 83 in place of 64.)
-__host__ __device__ constexpr int held(int Q) { return 256 * 256 / Q; }
+__host__ __device__ constexpr int held(int Q, int DK) { return DK > 128 ? 256 : 256 * 256 / Q; }
 
 // The keys of Q queries, from q0 on of (row, KV head) bh: length and new tokens of the row, keys that a
 // query of them sees, key tiles a piece and pieces. n·group ≤ q0: no queries.
@@ -54,7 +55,7 @@ struct Span {
   int len, n, kend, per, pieces;
   bool good;  // length and count were in range
 };
-template <int Q>
+template <int Q, int DK>
 __device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int bh, int q0, int splits) {
   Span w;
   const int b = bh / a.Hkv, len = a.lens[b], n = a.counts ? a.counts[b] : a.S;
@@ -68,7 +69,7 @@ __device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int bh, int q0, 
   // were they as this one (the first queries have fewer keys than the last)
   const long long queries = (w.n * static_cast<long long>(a.group) + Q - 1) / Q;
   const int mean = (max(w.len - w.n + Q / a.group, 0) + w.len) / (2 * kK) + 1;
-  const int share = static_cast<int>((queries * mean * a.B * a.Hkv + held(Q) - 1) / held(Q));
+  const int share = static_cast<int>((queries * mean * a.B * a.Hkv + held(Q, DK) - 1) / held(Q, DK));
   w.per = max(max(kLeastTiles, share), (tiles + splits - 1) / splits);
   w.pieces = q0 >= w.n * a.group ? 0 : max(1, (tiles + w.per - 1) / w.per);
   return w;
@@ -81,7 +82,7 @@ struct Tile {
 };
 
 // False: nothing to do.
-template <int Q>
+template <int Q, int DK>
 __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int nq, int splits, Tile& t) {
   // (row, KV head) fastest: with a multiple of 8 of them each has its XCD, whose L2 then holds its keys. The
   // last queries, which have the most keys, first; and pieces that a tile does not have behind all others
@@ -93,7 +94,7 @@ __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int nq, int sp
   t.piece = rest / nq;
   t.at = bh * nq + qt;
   t.q0 = qt * Q;
-  const Span w = span_of<Q>(a, bh, t.q0, splits);
+  const Span w = span_of<Q, DK>(a, bh, t.q0, splits);
   if (rest == 0 && !w.good && threadIdx.x == 0) tell(a.err);
   if (t.piece >= w.pieces) return false;
   t.len = w.len;
@@ -121,7 +122,7 @@ template <typename T, int DK, int Q>
 __global__ __launch_bounds__(kMergers) void paged_merge_kernel(PagedAttnArgs a, int nq, int splits) {
   constexpr int L = DK / 4, kRows = kMergers / L, kBlocks = (Q + kRows - 1) / kRows;
   const int at = blockIdx.x / kBlocks, bh = at / nq, q0 = (at - bh * nq) * Q;
-  const Span w = span_of<Q>(a, bh, q0, splits);
+  const Span w = span_of<Q, DK>(a, bh, q0, splits);
   if (w.pieces <= 1) return;
   const int c = blockIdx.x % kBlocks * kRows + threadIdx.x / L, d = threadIdx.x % L * 4;
   if (threadIdx.x / L >= kRows || c >= Q || q0 + c >= w.n * a.group || d >= a.dk) return;
@@ -152,18 +153,18 @@ __global__ __launch_bounds__(kMergers) void paged_merge_kernel(PagedAttnArgs a, 
 
 // DK: head dims up to it, in steps of 8.
 template <int DK, int kWaves>
-__global__ __launch_bounds__(64 * kWaves, 2) void paged_prefill_f16_kernel(PagedAttnArgs a, int nq, int splits) {
+__global__ __launch_bounds__(64 * kWaves, DK > 128 ? 1 : 2) void paged_prefill_f16_kernel(PagedAttnArgs a, int nq, int splits) {
 #pragma clang fp contract(off)
   constexpr int kThreads = 64 * kWaves, kQ = 32 * kWaves;
   constexpr int KS = DK / 16, OT = DK / 32, VG = DK / 8;
-  constexpr int L = DK <= 64 ? 8 : 16;    // lanes of a row, 16 bytes each
+  constexpr int L = DK <= 64 ? 8 : DK <= 128 ? 16 : 32;  // lanes of a row, 16 bytes each
   constexpr int RW = 64 / L;              // rows of a wave's load
   constexpr int CH = kK / (RW * kWaves);  // loads of a wave for a tile
   constexpr int KP = DK + 8, VP = DK == 96 ? DK : DK + 32;  // halves of a row in LDS: V's 16 banks apart for its reads
   __shared__ __align__(16) half_t Ks[2][kK][KP];
   __shared__ __align__(16) half_t Vs[2][kK][VP];
   Tile w;
-  if (!find_tile<kQ>(a, nq, splits, w)) return;
+  if (!find_tile<kQ, DK>(a, nq, splits, w)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int dk = a.dk, R = w.n * a.group, hi = lane >> 5;
   const int qw = w.q0 + wave * 32, myq = qw + (lane & 31);  // the wave's first query, this lane's
@@ -198,7 +199,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_prefill_f16_kernel(Paged
   auto fetch_ids = [&](int t) { return pages.number(min(t * kK + first_row(lane < CH ? lane : 0), lastkey)); };
   const int col = lane % L, row = lane / L;
   const int dpos = col * 8;
-  const bool mine = DK == 64 || DK == 128 ? dpos < dk : col < VG && dpos < dk;
+  const bool mine = VG == L ? dpos < dk : col < VG && dpos < dk;
   const unsigned loff = static_cast<unsigned>((row * dk + (mine ? dpos : 0)) * 2);
   auto fetch = [&](const void* pool, int t, int ids, half8 (&dst)[CH]) {
 #pragma unroll
@@ -470,7 +471,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_f32_kernel(PagedAttnArgs
   __shared__ __align__(16) float Ks[kK][P];
   __shared__ __align__(16) float Vs[kK][P];
   Tile w;
-  if (!find_tile<kQ>(a, nq, splits, w)) return;
+  if (!find_tile<kQ, DK>(a, nq, splits, w)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int dk = a.dk, R = w.n * a.group, hi = lane >> 5, l32 = lane & 31;
   const int qw = w.q0 + wave * 32, myq = qw + l32;
@@ -682,10 +683,12 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_f32_kernel(PagedAttnArgs
 
 // Queries of a workgroup: float16 at head dims above 64 eight waves, which share what is written to LDS (a
 // piece of 2048 tokens over 8192 keys of 128: 307 µs, 322 with four; of 64 215 and 189), where a KV head has
-// more than four take.
-int queries_of(int dt, int R, int dk) { return dt == F16 && dk > 64 && R > 128 ? 256 : 128; }
+// more than four take; above 128 the registers are four waves'.
+int queries_of(int dt, int R, int dk) { return dt == F16 && dk > 64 && dk <= 128 && R > 128 ? 256 : 128; }
 // Columns of the kernel that takes a head dim.
-int columns_of(int dt, int dk) { return dk <= 32 && dt == F32 ? 32 : dk <= 64 ? 64 : dk <= 96 ? 96 : 128; }
+int columns_of(int dt, int dk) {
+  return dk <= 32 && dt == F32 ? 32 : dk <= 64 ? 64 : dk <= 96 ? 96 : dk <= 128 ? 128 : dk <= 192 ? 192 : 256;
+}
 
 // Tiles of queries, and the most pieces that the keys of one are cut into.
 struct Grid {
@@ -698,7 +701,7 @@ Grid grid_of(int dt, int B, int H, int Hkv, int S, int P, int dk) {
   g.q = queries_of(dt, R, dk);
   g.nq = (R + g.q - 1) / g.q;
   g.tiles = static_cast<long long>(g.nq) * Hkv * B;
-  const int most = std::max(1, (P + kK - 1) / kK / kLeastTiles), all = held(g.q);
+  const int most = std::max(1, (P + kK - 1) / kK / kLeastTiles), all = held(g.q, columns_of(dt, dk));
   g.splits = g.tiles >= all ? 1 : static_cast<int>(std::min<long long>(most, (2 * all + g.tiles - 1) / g.tiles));
   return g;
 }
@@ -719,8 +722,9 @@ int launch_kernels(const PagedAttnArgs& a, const Grid& g, hipStream_t st) {
 
 template <int DK>
 int launch_columns(int dt, const PagedAttnArgs& a, const Grid& g, hipStream_t st) {
-  if (dt == F32) return launch_kernels<float, DK, 128>(a, g, st);
-  if constexpr (DK > 64) {
+  if constexpr (DK > 128) return launch_kernels<half_t, DK, 128>(a, g, st);
+  else if (dt == F32) return launch_kernels<float, DK, 128>(a, g, st);
+  if constexpr (DK > 64 && DK <= 128) {
     if (g.q == 256) return launch_kernels<half_t, DK, 256>(a, g, st);
   }
   return launch_kernels<half_t, DK, 128>(a, g, st);
@@ -729,10 +733,11 @@ int launch_columns(int dt, const PagedAttnArgs& a, const Grid& g, hipStream_t st
 }  // namespace
 
 // Queries of a KV head from which on this pays: float16, 48 over 4000 keys of 128, 32.8 µs (42.9 with 16 at a
-// time), 32 no less; float32, whose matrix instructions cost what they multiply, padding or not, 100 over
+// time), 32 no less; 33 over 2000 keys of 256 42.1 (47.4), 2048 over 8192 624 (1705), 64 over 200 26.8 (20.4);
+// float32, whose matrix instructions cost what they multiply, padding or not, 100 over
 // up to 1000 keys 54 (44).
 bool paged_prefill_applies(int dt, int H, int Hkv, int S, int dk) {
-  return dk <= 128 && dk % (dt == F16 ? 8 : 4) == 0 && S > 1 && H / Hkv * S >= (dt == F16 ? 33 : 128);
+  return dk <= (dt == F16 ? 256 : 128) && dk % (dt == F16 ? 8 : 4) == 0 && S > 1 && H / Hkv * S >= (dt == F16 ? 33 : 128);
 }
 
 size_t paged_prefill_workspace(int dt, int B, int H, int Hkv, int S, int P, int dk) {
@@ -748,8 +753,10 @@ int launch_paged_prefill(int dt, PagedAttnArgs a, hipStream_t st) {
     case 32: return launch_kernels<float, 32, 128>(a, g, st);
     case 64: return launch_columns<64>(dt, a, g, st);
     case 96: return launch_columns<96>(dt, a, g, st);
+    case 128: return launch_columns<128>(dt, a, g, st);
+    case 192: return launch_columns<192>(dt, a, g, st);
   }
-  return launch_columns<128>(dt, a, g, st);
+  return launch_columns<256>(dt, a, g, st);
 }
 
 }  // namespace nml
