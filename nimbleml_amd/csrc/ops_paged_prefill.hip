@@ -458,18 +458,21 @@ __global__ __launch_bounds__(64 * kWaves, DK > 128 ? 1 : 2) void paged_prefill_f
 // dim of V, so that one read feeds W tiles of the output. A tile of keys costs 16 times the cycles on
 // the matrix pipe that its softmax takes beside it: one buffer and two barriers a tile, with the other
 // workgroup of the CU in between. (1024 tokens over 4096 keys: 8 heads of 64, 87 µs, 86 TFLOP/s; 8 over 2 of
-// 128, 159, 94; a product of 8192³ reaches 153.)
+// 128, 157, 96; 16 over 4 of 192, 1000 over 4000, 470, 92; a product of 8192³ reaches 153.)
 template <int DK>
-__global__ __launch_bounds__(256, 2) void paged_prefill_f32_kernel(PagedAttnArgs a, int nq, int splits) {
+__global__ __launch_bounds__(256, DK > 128 ? 1 : 2) void paged_prefill_f32_kernel(PagedAttnArgs a, int nq, int splits) {
   constexpr int kWaves = 4, kQ = 32 * kWaves;
+  // Keys of a tile here: 32 where 64 would take more registers than there are (1000 tokens over 4000 keys, 16
+  // heads over 4 of 192, 470 µs, 475; 512 over 2048, 8 of 256, 105, 135; of 128 156.7, 158.5).
+  constexpr int KT = DK > 96 ? 32 : kK;
   constexpr int KS = DK / 8, OT = DK / 32, VG = DK / 4;
-  constexpr int W = OT == 3 ? 1 : OT;
-  constexpr int L = DK == 32 ? 8 : DK == 64 ? 16 : 32;  // lanes of a row, 16 bytes each
-  constexpr int RW = 64 / L, CH = kK / (RW * kWaves);
+  constexpr int W = OT % 4 == 0 ? 4 : OT % 2 == 0 ? 2 : 1;
+  constexpr int L = DK == 32 ? 8 : DK == 64 ? 16 : DK <= 128 ? 32 : 64;  // lanes of a row, 16 bytes each
+  constexpr int RW = 64 / L, CH = KT / (RW * kWaves);
   constexpr int P = DK + 4;  // floats of a row in LDS
   typedef float vecw __attribute__((ext_vector_type(W)));
-  __shared__ __align__(16) float Ks[kK][P];
-  __shared__ __align__(16) float Vs[kK][P];
+  __shared__ __align__(16) float Ks[KT][P];
+  __shared__ __align__(16) float Vs[KT][P];
   Tile w;
   if (!find_tile<kQ, DK>(a, nq, splits, w)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -488,15 +491,16 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_f32_kernel(PagedAttnArgs
     for (int ks = 0; ks < KS; ++ks)
       qb[ks] = live && ks * 8 + hi * 4 < dk ? *reinterpret_cast<const floatx4*>(qp + ks * 8 + hi * 4) : z4;
   }
+  const int t0 = w.t0 * (kK / KT), nt = min(w.nt * (kK / KT), (w.kend + KT - 1) / KT - t0);
   const int wlast = w.len - w.n + min((qw + 31) / a.group, w.n - 1);
-  const int ntw = qw >= R || wlast < 0 ? 0 : min(w.nt, max(0, wlast / kK + 1 - w.t0));
+  const int ntw = qw >= R || wlast < 0 ? 0 : min(nt, max(0, wlast / KT + 1 - t0));
   const int unmasked = w.len - w.n + qw / a.group;
 
   const RowPages pages{a.table + static_cast<size_t>(w.b) * a.max_pages, a.shift, a.num_pages, a.Hkv, w.hk};
   const int lastkey = max(w.kend - 1, 0);
   bool bad = false;
   auto first_row = [&](int i) { return (i * kWaves + wave) * RW; };
-  auto fetch_ids = [&](int t) { return pages.number(min(t * kK + first_row(lane < CH ? lane : 0), lastkey)); };
+  auto fetch_ids = [&](int t) { return pages.number(min(t * KT + first_row(lane < CH ? lane : 0), lastkey)); };
   const int col = lane % L, row = lane / L, dpos = col * 4;
   const bool mine = dpos < dk, stores = VG == L || col < VG;
   const unsigned loff = static_cast<unsigned>((row * dk + (mine ? dpos : 0)) * 4);
@@ -504,7 +508,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_f32_kernel(PagedAttnArgs
   auto fetch = [&](int t, int ids) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const size_t at = pages.place(t * kK + first_row(i), __builtin_amdgcn_readlane(ids, i), bad) * dk * 4 + loff;
+      const size_t at = pages.place(t * KT + first_row(i), __builtin_amdgcn_readlane(ids, i), bad) * dk * 4 + loff;
       kn[i] = mine ? *reinterpret_cast<const floatx4*>(static_cast<const char*>(a.k_pages) + at) : z4;
       vn[i] = mine ? *reinterpret_cast<const floatx4*>(static_cast<const char*>(a.v_pages) + at) : z4;
     }
@@ -516,7 +520,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_f32_kernel(PagedAttnArgs
         const int r = first_row(i) + row;
         *reinterpret_cast<floatx4*>(&Ks[r][dpos]) = kn[i];
         // (what lies past the last key may be anything)
-        *reinterpret_cast<floatx4*>(&Vs[r][dpos]) = t * kK + r < w.kend ? vn[i] : z4;
+        *reinterpret_cast<floatx4*>(&Vs[r][dpos]) = t * KT + r < w.kend ? vn[i] : z4;
       }
   };
   float m = -INFINITY, l = 0.f;
@@ -526,21 +530,21 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_f32_kernel(PagedAttnArgs
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
   int ids = 0;
-  if (w.nt > 0) {
-    fetch(w.t0, fetch_ids(w.t0));
-    ids = fetch_ids(w.t0 + 1);
+  if (nt > 0) {
+    fetch(t0, fetch_ids(t0));
+    ids = fetch_ids(t0 + 1);
   }
-  for (int j = 0; j < w.nt; ++j) {
-    const int t = w.t0 + j;
+  for (int j = 0; j < nt; ++j) {
+    const int t = t0 + j;
     __syncthreads();  // (the tile before is read)
     put(t);
     __syncthreads();
-    if (j + 1 < w.nt) fetch(t + 1, ids);
-    if (j + 2 < w.nt) ids = fetch_ids(t + 2);
+    if (j + 1 < nt) fetch(t + 1, ids);
+    if (j + 2 < nt) ids = fetch_ids(t + 2);
     if (j >= ntw) continue;
-    floatx16 s[2];
+    floatx16 s[KT / 32];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < KT / 32; ++u) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
 #pragma unroll
@@ -550,16 +554,16 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_f32_kernel(PagedAttnArgs
         for (int e = 0; e < 4; ++e) s[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(ka[e], qb[ks][e], s[u], 0, 0, 0);
       }
     }
-    if ((t + 1) * kK - 1 > unmasked) {
+    if ((t + 1) * KT - 1 > unmasked) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (t * kK + u * 32 + 8 * (r >> 2) + 4 * hi + (r & 3) > lim) s[u][r] = -INFINITY;
+          if (t * KT + u * 32 + 8 * (r >> 2) + 4 * hi + (r & 3) > lim) s[u][r] = -INFINITY;
     }
     float mx = s[0][0];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[u][r]);
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
@@ -575,7 +579,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_f32_kernel(PagedAttnArgs
     }
     const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float p = __builtin_amdgcn_exp2f((s[u][r] - ref) * cscale);
@@ -583,7 +587,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_f32_kernel(PagedAttnArgs
         s[u][r] = p;
       }
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float* vrow = &Vs[u * 32 + 8 * (r >> 2) + 4 * hi + (r & 3)][W * l32];
@@ -619,8 +623,8 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_f32_kernel(PagedAttnArgs
       for (int d = 0; d < OT; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) fresh[d][r] = 0.f;
-      const int end = min(min(w.kend, (w.t0 + w.nt) * kK), wlast + 1);
-      for (int key = w.t0 * kK; key < end; ++key) {
+      const int end = min(min(w.kend, (t0 + nt) * KT), wlast + 1);
+      for (int key = t0 * KT; key < end; ++key) {
         const size_t at = pages.place(key, pages.number(key), bad) * dk;
         const float *kr = static_cast<const float*>(a.k_pages) + at, *vr = static_cast<const float*>(a.v_pages) + at;
         int h = hi, c = l32;
@@ -722,8 +726,7 @@ int launch_kernels(const PagedAttnArgs& a, const Grid& g, hipStream_t st) {
 
 template <int DK>
 int launch_columns(int dt, const PagedAttnArgs& a, const Grid& g, hipStream_t st) {
-  if constexpr (DK > 128) return launch_kernels<half_t, DK, 128>(a, g, st);
-  else if (dt == F32) return launch_kernels<float, DK, 128>(a, g, st);
+  if (dt == F32) return launch_kernels<float, DK, 128>(a, g, st);
   if constexpr (DK > 64 && DK <= 128) {
     if (g.q == 256) return launch_kernels<half_t, DK, 256>(a, g, st);
   }
@@ -735,9 +738,10 @@ int launch_columns(int dt, const PagedAttnArgs& a, const Grid& g, hipStream_t st
 // Queries of a KV head from which on this pays: float16, 48 over 4000 keys of 128, 32.8 µs (42.9 with 16 at a
 // time), 32 no less; 33 over 2000 keys of 256 42.1 (47.4), 2048 over 8192 624 (1705), 64 over 200 26.8 (20.4);
 // float32, whose matrix instructions cost what they multiply, padding or not, 100 over
-// up to 1000 keys 54 (44).
+// up to 1000 keys 54 (44), 128 over 128 keys of 256 50 (22), 512 over 2048 105 (130), 1000 over 4000 of 192
+// 470 (778).
 bool paged_prefill_applies(int dt, int H, int Hkv, int S, int dk) {
-  return dk <= (dt == F16 ? 256 : 128) && dk % (dt == F16 ? 8 : 4) == 0 && S > 1 && H / Hkv * S >= (dt == F16 ? 33 : 128);
+  return dk % (dt == F16 ? 8 : 4) == 0 && S > 1 && H / Hkv * S >= (dt == F16 ? 33 : dk <= 128 ? 128 : 256);
 }
 
 size_t paged_prefill_workspace(int dt, int B, int H, int Hkv, int S, int P, int dk) {

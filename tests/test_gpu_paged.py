@@ -93,7 +93,7 @@ def test_attention(gpu, batch, kv, group, dk, page, pages, seq, dtype):
 
 
 @pytest.mark.parametrize("dtype", [np.float32, np.float16])
-@pytest.mark.parametrize("group, dk", [(1, 64), (3, 72), (5, 96), (2, 128), (1, 136), (2, 192), (3, 200), (2, 256)])
+@pytest.mark.parametrize("group, dk", [(1, 64), (3, 72), (5, 96), (2, 128), (1, 136), (2, 192), (3, 200), (2, 256), (1, 252)])
 def test_many_new_tokens_behind_a_long_cache(gpu, group, dk, dtype):
     """Several tiles of queries of a row, whose keys are cut into pieces of a size that differs with the row."""
     cache = Cache(3, 2, dk, 16, 130, dtype, dk)
