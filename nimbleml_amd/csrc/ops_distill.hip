@@ -16,7 +16,7 @@
 // order of atomics.
 //
 // Both are bound by HBM where rows are many. 4096 rows of 32000 float16 logits, 64 entries each: the loss
-// 52 µs, 5.1 TB/s of reads; the gradient 110 µs, 4.8 TB/s of reads and writes. 2048 rows of 4096 float32
+// 53 µs, 5.0 TB/s of reads; the gradient 110 µs, 4.8 TB/s of reads and writes. 2048 rows of 4096 float32
 // logits: 8.6 and 11.6 µs, in part from the last cache. A single row of 50304: 7.4 and 6.4 µs with its
 // launch.
 #include "kernels.hpp"
