@@ -114,10 +114,10 @@ int write_launch(PagedWriteArgs a, size_t es, hipStream_t st) {
 // several, as many in all as the card holds at once, and the last to finish merges them in their
 // order.
 //
-// Bound by HBM where keys are many: 16 rows of 1 to 8 Ki keys, 32 heads over 8 of 128, float16, 68 µs,
-// 4.4 TB/s of keys and values (a copy 4.8). Where few, by a chain of dependent steps: lengths, page
-// numbers, keys, rounds, merge and the pieces' merge: one row of 1023 keys, 16 heads of 64, 8.8 µs; 16
-// rows of up to 2048 and up to 5 tokens, 8 heads of 32, float32, 14.8. (Where work is cut finely enough the
+// Bound by HBM where keys are many: 16 rows of 1 to 8 Ki keys, 32 heads over 8 of 128, float16, 66 µs,
+// 4.6 TB/s of keys and values (a copy 4.8). Where few, by a chain of dependent steps: lengths, page
+// numbers, keys, rounds, merge and the pieces' merge: one row of 1023 keys, 16 heads of 64, 9.1 µs; 16
+// rows of up to 2048 and up to 5 tokens, 8 heads of 32, float32, 14.2. (Where work is cut finely enough the
 // merge is what is left: its loads are in batches of 16 pieces, of four where there are no more.)
 
 typedef short s4 __attribute__((ext_vector_type(4)));
@@ -147,6 +147,8 @@ __host__ __device__ constexpr int group_waves(int nb) { return nb == 2 ? 2 : 4; 
 __host__ __device__ constexpr int waves_of(int nb) { return nb <= 2 ? 4 : nb == 8 ? 1 : 2; }
 constexpr int kCus = 256;
 __host__ __device__ constexpr int capacity(int nb) { return kCus * 4 * waves_of(nb) / group_waves(nb); }
+// Pieces that few tiles are cut into, and one more for each of them at most: a wave for each SIMD.
+__host__ __device__ constexpr int even_pieces(int waves) { return kCus * 4 / waves; }
 // Spans (a tile for each wave) that a piece has at least: what it costs to begin one and to merge it. (One row
 // of 1023 keys, 16 heads of 64: 9.2 µs at two spans of 64 keys, 10.6 at four, 8.9 at one; of 100 keys 6.9, 6.9, 8.7.)
 __host__ __device__ constexpr int least_spans(int nb) { return nb == 2 ? 2 : 1; }
@@ -219,9 +221,9 @@ __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, int tiles, int
   // Few tiles, which pieces of any size leave even: a wave for each SIMD, beside which a second one adds
   // pieces to merge but no bandwidth (30000 keys, 32 heads over 8 of 128: 29.5 µs, 33.5 with two). More tiles, of
   // different length, are evener in more pieces (16 rows of 1 to 8 Ki: 55, 73 with one).
-  constexpr int kEven = kCus * 4 / NW;
-  if (static_cast<long long>(each) * a.B <= kEven / 4)
-    least = max(least, static_cast<int>((static_cast<long long>(total) * each + kEven - 1) / kEven));
+  constexpr int even = even_pieces(NW);
+  if (static_cast<long long>(each) * a.B <= even / 4)
+    least = max(least, static_cast<int>((static_cast<long long>(total) * each + even - 1) / even));
   auto pieces_of = [&](int spans) { return spans <= least ? min(spans, 1) : (spans + least - 1) / least; };
   const int at = static_cast<int>(blockIdx.x / each);
   int before = 0, slots = 0, from = 0;
@@ -789,6 +791,8 @@ Pieces attention_pieces(int B, int H, int Hkv, int S, int P, int dk) {
   p.tiles = (static_cast<long long>(H / Hkv) * S + 15) / 16 * Hkv * B;
   p.most = (spans - 1) / least_spans(nb) + 1;
   p.slots = p.most == 1 ? 0 : std::min(p.tiles * p.most, 2LL * room_for(p.tiles, capacity(nb)));
+  const int even = even_pieces(group_waves(nb));
+  if (p.tiles <= even / 4) p.slots = std::min(p.slots, even + p.tiles);
   return p;
 }
 
