@@ -13,7 +13,7 @@
 // those below 2^-21 of the largest, 2^-31 of that), and Σ p is of the two, so that an output is off by
 // little more than its own rounding to float16. As one float16 value an output would be off as far
 // again (2.9·10^-4 of its norm, 2.1·10^-4), for a third fewer matrix instructions: 2048 tokens over 8192 keys,
-// 32 heads of 128 over 8, 341 µs and 439; two rows of them with 16 heads of 64, 244 and 277.
+// 32 heads of 128 over 8, 341 µs and 425; two rows of them with 16 heads of 64, 244 and 277.
 //
 // One barrier a tile: K is written to LDS two tiles ahead and V one, from registers that were loaded a
 // tile before, and the scores of the next tile are formed beside the probabilities of this one. A
@@ -315,14 +315,23 @@ __global__ __launch_bounds__(64 * kWaves, DK > 128 ? 1 : 2) void paged_prefill_f
       // k-slot j of lane half hi: key 8(j / 4) + 4·hi + j % 4 of the 16. A transposing read gives a lane
       // four keys of its dim from the rows that its 16 lanes point at, 8 bytes each.
       typedef __attribute__((address_space(3))) s4 lds_s4;
+      // (the two products of an output apart: 2048 tokens over 8192 keys, 32 heads of 128 over 8, 420 µs in pairs
+      // and 428 side by side; 16 over 4 of 256 737 in pairs, 720 in fours, 763)
+      constexpr int F = DK > 128 ? 4 : 2;
       const half_t* at = &Vs[PAR][blk * 16 + 4 * hi + ((lane & 15) >> 2)][16 * ((lane >> 4) & 1) + 4 * (lane & 3)];
 #pragma unroll
-      for (int d = 0; d < OT; ++d) {
-        const s4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + d * 32));
-        const s4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + d * 32 + 8 * VP));
-        const half8 va = __builtin_bit_cast(half8, s8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pb[0], o[d], 0, 0, 0);
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pb[1], o[d], 0, 0, 0);
+      for (int d = 0; d < OT; d += F) {
+        half8 va[F];
+#pragma unroll
+        for (int f = 0; f < F && d + f < OT; ++f) {
+          const s4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + (d + f) * 32));
+          const s4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + (d + f) * 32 + 8 * VP));
+          va[f] = __builtin_bit_cast(half8, s8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int f = 0; f < F && d + f < OT; ++f) o[d + f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[f], pb[c], o[d + f], 0, 0, 0);
       }
     }
     if constexpr (NEXT) prep(mask_next_c, t + 1, nxt);
