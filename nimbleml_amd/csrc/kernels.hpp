@@ -382,6 +382,9 @@ struct PagedAttnArgs {
   void* ws;
   int* err;
 };
+// Keys that a workgroup takes at once, 64 at most: Σ over the rows of their spans, for each tile of 16 queries
+// of a KV head, is to be in 32 bits.
+int paged_attention_span(int dt, int dk);
 size_t paged_attention_workspace(int dt, int B, int H, int Hkv, int S, int P, int dk);
 int launch_paged_attention(int dt, const PagedAttnArgs& a, hipStream_t st);
 

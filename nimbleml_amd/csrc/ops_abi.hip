@@ -890,14 +890,15 @@ int nml_paged_write_device(const void* k, const void* v, size_t stride_b, size_t
 }
 
 static int paged_attention_ok(size_t batch, size_t heads, size_t kv_heads, size_t seq, size_t max_pages,
-                              size_t page_size, size_t num_pages, size_t dk) {
+                              size_t page_size, size_t num_pages, size_t dk, int dtype) {
   NML_TRY(paged_ok("paged attention", batch, heads, seq, max_pages, page_size, num_pages, dk));
   NML_REQUIRE(kv_heads >= 1 ? heads % kv_heads == 0 : heads == 0,
               "paged attention: heads (%zu) must be divisible by kv_heads (%zu)", heads, kv_heads);
   if (batch && heads && seq) {
-    // the kernel numbers spans of 64 keys in 32 bits, and a launch its threads
+    // the kernel numbers the spans of keys that its workgroups take in 32 bits, and a launch its threads
     const size_t tiles = (heads / kv_heads * seq + 15) / 16 * kv_heads, keys = max_pages * page_size;
-    NML_REQUIRE(tiles * batch <= 0x7fffffff / ((keys + 63) / 64) && tiles * batch <= (size_t)1 << 22,
+    const size_t span = (size_t)paged_attention_span(dtype, (int)dk);
+    NML_REQUIRE(tiles * batch <= 0x7fffffff / ((keys + span - 1) / span) && tiles * batch <= (size_t)1 << 22,
                 "paged attention: %zu rows × %zu heads × %zu tokens over %zu positions too many", batch, heads, seq, keys);
   }
   return 0;
@@ -908,7 +909,7 @@ int nml_paged_attention_workspace(size_t batch, size_t heads, size_t kv_heads, s
   NML_REQUIRE(bytes != nullptr, "paged attention: bytes is null");
   *bytes = 0;
   NML_TRY(check_dtype(dtype));
-  NML_TRY(paged_attention_ok(batch, heads, kv_heads, seq, max_pages, page_size, 1, dk));
+  NML_TRY(paged_attention_ok(batch, heads, kv_heads, seq, max_pages, page_size, 1, dk, dtype));
   if (batch && heads && seq)
     *bytes = paged_attention_workspace(dtype, (int)batch, (int)heads, (int)kv_heads, (int)seq,
                                        (int)(max_pages * page_size), (int)dk);
@@ -920,7 +921,7 @@ int nml_paged_attention_device(const void* q, const void* k_pages, const void* v
                                size_t kv_heads, size_t seq, size_t max_pages, size_t page_size, size_t num_pages,
                                size_t dk, float scale_div, void* ws, size_t ws_bytes, int* err, int dtype) {
   NML_TRY(check_dtype(dtype));
-  NML_TRY(paged_attention_ok(batch, heads, kv_heads, seq, max_pages, page_size, num_pages, dk));
+  NML_TRY(paged_attention_ok(batch, heads, kv_heads, seq, max_pages, page_size, num_pages, dk, dtype));
   NML_REQUIRE(scale_div > 0.f && std::isnormal(scale_div), "paged attention: scale_div must be positive and normal");
   if (batch == 0 || heads == 0 || seq == 0) return 0;
   NML_REQUIRE(q && k_pages && v_pages && table && lens && out, "paged attention: a buffer is null");

@@ -839,6 +839,10 @@ int launch_paged_write(int dt, const PagedWriteArgs& a, hipStream_t st) {
   return es == 2 ? write_launch<unsigned short>(a, es, st) : write_launch<unsigned>(a, es, st);
 }
 
+int paged_attention_span(int dt, int dk) {
+  return std::min(64, group_waves(steps_of(dk)) * (dt == F16 ? tile_keys<half_t>() : tile_keys<float>()));
+}
+
 size_t paged_attention_workspace(int dt, int B, int H, int Hkv, int S, int P, int dk) {
   // (which kernel takes a call depends on its buffers' alignment too)
   const size_t many = paged_prefill_applies(dt, H, Hkv, S, dk) ? paged_prefill_workspace(dt, B, H, Hkv, S, P, dk) : 0;
