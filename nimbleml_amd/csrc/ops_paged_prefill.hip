@@ -70,7 +70,7 @@ __device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int bh, int q0, 
   // a piece: an even share, for as many workgroups as the card holds, of what all rows would have to do
   // were they as this one (the first queries have fewer keys than the last)
   const long long queries = (w.n * static_cast<long long>(a.group) + Q - 1) / Q;
-  const int mean = (max(w.len - w.n + Q / a.group, 0) + w.len) / (2 * kK) + 1;
+  const int mean = static_cast<int>((max(w.len - w.n + Q / a.group, 0) + static_cast<long long>(w.len)) / (2 * kK)) + 1;
   const int share = static_cast<int>((queries * mean * a.B * a.Hkv + held(Q, DK) - 1) / held(Q, DK));
   w.per = max(max(kLeastTiles, share), (tiles + splits - 1) / splits);
   w.pieces = q0 >= w.n * a.group ? 0 : max(1, (tiles + w.per - 1) / w.per);
