@@ -292,8 +292,10 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
   const double* u = a.u + static_cast<size_t>(b) * (a.n + 1);
   auto target = [&](int i) { return static_cast<const T*>(a.logits) + (static_cast<size_t>(b) * (a.n + 1) + i) * a.ld; };
   auto drafted = [&](int i) { return static_cast<const T*>(a.draft) + (static_cast<size_t>(b) * a.n + i) * a.ld_draft; };
-  // All that the acceptance takes is loaded before anything is waited for, of drafts past the row's
-  // count too (their rows' parts may hold anything and are not looked at).
+  // All that the acceptance takes is loaded before anything is waited for but the drafts and their count, which
+  // say what logits are read: those of drafts past the count are not there. (Of their rows' parts, which may
+  // hold anything, nothing is used.)
+  const int c = drafted_of(a, b, false);
   const int rows = a.n + 1 + (a.draft ? a.n : 0), l16 = tid & 15;
   const Stat* stats = static_cast<const Stat*>(a.stats) + static_cast<size_t>(b) * rows * a.row_parts;
   auto row_at = [&](int i) { return stats + static_cast<size_t>(i) * a.row_parts; };
@@ -307,7 +309,7 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
     const int64_t d = drafts[tid];
     du = u[tid];
     ok = d >= 0 && d < a.V;
-    if (ok) {
+    if (ok && tid < c) {
       dp = static_cast<float>(target(tid)[d]);
       if (a.draft) dq = static_cast<float>(drafted(tid)[d]);
     }
@@ -324,7 +326,6 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
     if (i < rows) ahead = part_of(row_at(i), a.row_parts, l16);
   }
   if (!a.draft && tid < a.n) qs[tid] = Stat{1.0, 0.f, 0};
-  const int c = drafted_of(a, b, false);
   __syncthreads();
   if (w == 0) {
     if (lane >= c) ok = true;
