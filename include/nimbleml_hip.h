@@ -316,9 +316,9 @@ int nml_distill_backward_device(const void* logits, size_t ld, const int64_t* to
  *   accepted: int32 (batch), r; tokens: int64 (batch, drafted + 1): r drafts, the token, then −1
  * Logits of −inf have probability 0 (a caller that filters sets them). Rows of logits past
  * counts[b], and of draft logits from counts[b] on, are not read; drafts and u are, and what they hold from
- * counts[b] on does not matter (but for u's last). *err (device int, may be NULL): bit 0 for a count outside [0, drafted] (clamped) or a draft
- * outside [0, vocab) (refused); bit 1 where a row that decides has no distribution (NaN or +inf in it,
- * for T ≤ 0 NaN alone, or nothing above −inf): the token at r is −1.
+ * counts[b] on does not matter (but for u's last). *err (device int, may be NULL): bit 0 for a count outside
+ * [0, drafted] (clamped) or a draft before it outside [0, vocab) (refused); bit 1 where a row that decides has
+ * no distribution (NaN or +inf in it, for T ≤ 0 NaN alone, or nothing above −inf): the token at r is −1.
  * 0 ≤ drafted ≤ 63, vocab ≤ 2^24, batch·(2·drafted + 1) ≤ 65535. ws: nml_verify_drafts_workspace bytes,
  * 16-byte aligned, in any state; calls that can run at the same time need one each. Asynchronous. */
 int nml_verify_drafts_workspace(size_t batch, size_t drafted, size_t vocab, size_t* bytes);

@@ -253,6 +253,10 @@ __global__ __launch_bounds__(kThreads) void verify_greedy_kernel(VerifyArgs a) {
   __shared__ unsigned long long best[kMaxRows];
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int c = drafted_of(a, b, false);
+  if (tid < c) {  // (drafts behind the first that is refused are told too)
+    const int64_t d = a.drafts[static_cast<size_t>(b) * a.n + tid];
+    if ((d < 0 || d >= a.V) && a.err) __hip_atomic_fetch_or(a.err, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
   const Stat* s = static_cast<const Stat*>(a.stats) + static_cast<size_t>(b) * (a.n + 1) * a.row_parts;
   for (int i = w; i <= c; i += kThreads / 64) {
     unsigned long long k = 0;
@@ -271,7 +275,6 @@ __global__ __launch_bounds__(kThreads) void verify_greedy_kernel(VerifyArgs a) {
     token = o == 0xffffffffu || o <= 0x007fffffu ? -1 : static_cast<int64_t>(~static_cast<unsigned>(best[r]));
     if (r == c || token < 0) break;
     const int64_t d = a.drafts[static_cast<size_t>(b) * a.n + r];
-    if ((d < 0 || d >= a.V) && tid == 0 && a.err) __hip_atomic_fetch_or(a.err, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (d != token) break;
   }
   answer(a, a.drafts + static_cast<size_t>(b) * a.n, b, r, token, tid);

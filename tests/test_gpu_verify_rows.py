@@ -56,3 +56,20 @@ def test_rows_past_the_last_count_need_not_be_there(gpu, t):
     full = np.concatenate([rows, np.zeros((n, vocab), np.float32)]).reshape(2, n + 1, vocab)
     wa, wt = R.verify(full, drafts, u, np.concatenate([draft, draft]).reshape(2, n, vocab), counts, t)
     assert err == 0 and np.array_equal(a, wa) and np.array_equal(tok, wt)
+
+
+@pytest.mark.parametrize("t", [1.0, 0.0])
+@pytest.mark.parametrize("wrong", [-1, 400, -(1 << 40), 1 << 40])
+def test_a_draft_out_of_range_behind_a_refusal_is_told(gpu, t, wrong):
+    """The first draft is refused, a later one is no token; past a count it does not matter."""
+    logits, _, drafts, u, _ = case(3, 4, 400, np.float32, t, seed=23)
+    drafts[:, 0] = logits[:, 0].argmin(-1)
+    u[:, 0] = 1.0  # (chosen outright: refused unless p = 1)
+    counts = np.array([4, 3, 4], np.int32)
+    wa, wt = R.verify(logits, drafts, u, None, counts, t)
+    assert (wa == 0).all()
+    drafts[1, 3] = wrong
+    assert call(logits, None, drafts, u, counts, t, 400, 0)[2] == 0
+    drafts[2, 3] = wrong
+    a, tok, err = call(logits, None, drafts, u, counts, t, 400, 0)
+    assert err == 1 and np.array_equal(a, wa) and np.array_equal(tok, wt)
