@@ -292,7 +292,7 @@ int nml_distill_device(const void* logits, size_t ld, const int64_t* top_ids, co
 /* Its gradient: dlogits (rows, vocab) at stride ld_d, of the logits' dtype, is overwritten with
  *   dloss/T·(p_v − Σ_{k: id_k = v} q_k)
  * from the forward's m and l; dloss: float32 (rows). Rows without a teacher: zeros. dlogits may be
- * logits itself. An id outside [−1, vocab) makes its row NaN and sets bit 0 of *err. Asynchronous, no
+ * logits itself, at the same stride. An id outside [−1, vocab) makes its row NaN and sets bit 0 of *err. Asynchronous, no
  * workspace. */
 int nml_distill_backward_device(const void* logits, size_t ld, const int64_t* top_ids,
                                 const float* top_logits, const float* m, const float* l,

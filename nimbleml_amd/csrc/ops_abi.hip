@@ -765,6 +765,8 @@ int nml_distill_backward_device(const void* logits, size_t ld, const int64_t* to
   NML_REQUIRE(ld_d >= vocab && ld_d < (size_t)1 << 40, "distill backward: stride %zu out of range", ld_d);
   if (rows == 0) return 0;
   NML_REQUIRE(logits && top_ids && top_logits && m && l && dloss && dlogits, "distill backward: a buffer is null");
+  NML_REQUIRE(dlogits != logits || ld_d == ld || rows == 1, "distill backward: in place, but strides %zu and %zu differ", ld,
+              ld_d);
   DistillBwdArgs a{};
   a.logits = logits;
   a.ld = (long long)ld;
