@@ -31,6 +31,9 @@ constexpr int kFewRows = 512;
 constexpr int kLaunchRows = 1 << 21;  // of one launch: its threads are counted in 32 bits
 constexpr int kTeachers = kMaxDistillTop;
 constexpr float kLog2e = 1.44269504088896341f;
+// Differences of logits times a power of two, exactly: those of float32's largest, and their sums, stay finite
+// where the temperature brings the loss back into its range.
+constexpr float kFar = 0x1p-10f;
 
 // A thread's entry of the teacher's.
 struct Entry {
@@ -135,7 +138,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
     if (e.id >= 0) {
       q = __builtin_amdgcn_exp2f((e.y - y) * c);
       // (the teacher's and the model's logits each from their own largest: an offset costs nothing)
-      if (q != 0.f) t = q * ((e.y - y) - (mine - m));
+      if (q != 0.f) t = q * ((e.y - y) * kFar - (mine * kFar - m * kFar));
     }
     q = wave_sum_dpp(q);
     t = wave_sum_dpp(t);
@@ -146,7 +149,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
     float q = 0.f, t = 0.f;
 #pragma unroll
     for (int i = 0; i < KW; ++i) q += z_w[i], t += s_w[i];
-    a.loss[r] = t / q * a.inv_t + (logf(z) - logf(q));
+    a.loss[r] = t / q * (a.inv_t / kFar) + (logf(z) - logf(q));
     if (a.m) a.m[r] = m;
     if (a.l) a.l[r] = z;
   }
