@@ -175,6 +175,8 @@ __global__ __launch_bounds__(64 * kWaves, DK > 128 ? 1 : 2) void paged_prefill_f
   const int lim = w.len - w.n + tok;  // the last key that this lane's query sees
   const float cscale = kLog2e / a.scale;
   constexpr float kUp = 7.f;  // p times 2^7: at most 2^15, with all of float16's bits down to 2^-21
+  // What a score in powers of two is raised by under reference x (rounded once: all that refers to x takes this)
+  auto raise_of = [&](float x) { return kUp - (x == -INFINITY ? 0.f : x) * cscale; };
   const float lazy = fminf(8.0f / cscale, 3.402823466e38f);
   const half8 z8 = {0, 0, 0, 0, 0, 0, 0, 0};
   half8 qb[KS];
@@ -285,7 +287,7 @@ __global__ __launch_bounds__(64 * kWaves, DK > 128 ? 1 : 2) void paged_prefill_f
     constexpr int PAR = decltype(par_c)::value;
     constexpr bool NEXT = decltype(next_c)::value;
     if (grow) {
-      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m * cscale - mnew * cscale);
+      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(raise_of(mnew) - raise_of(m));
       l *= alpha;
 #pragma unroll
       for (int d = 0; d < OT; ++d)
@@ -294,7 +296,7 @@ __global__ __launch_bounds__(64 * kWaves, DK > 128 ? 1 : 2) void paged_prefill_f
     }
     m = mnew;
     if constexpr (NEXT) scores(std::integral_constant<int, PAR ^ 1>{}, nxt);
-    const float nmx = kUp - (m == -INFINITY ? 0.f : m) * cscale;
+    const float nmx = raise_of(m);
     const half2v ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
 #pragma unroll
     for (int blk = 0; blk < 4; ++blk) {
@@ -396,7 +398,7 @@ __global__ __launch_bounds__(64 * kWaves, DK > 128 ? 1 : 2) void paged_prefill_f
 #pragma unroll
       for (int r = 0; r < 16; ++r) wrong |= !__builtin_isfinite(o[d][r]);
     if (__any(wrong && live)) {
-      const float nmx = kUp - (m == -INFINITY ? 0.f : m) * cscale;
+      const float nmx = raise_of(m);
       floatx16 fresh[OT];
 #pragma unroll
       for (int d = 0; d < OT; ++d)
@@ -455,7 +457,7 @@ __global__ __launch_bounds__(64 * kWaves, DK > 128 ? 1 : 2) void paged_prefill_f
   }
   const Parts parts(a, kQ);
   const size_t q = (static_cast<size_t>(w.at) * splits + w.piece) * kQ + wave * 32 + (lane & 31);
-  if (hi == 0) *reinterpret_cast<f2*>(parts.ml + 2 * q) = f2{m == -INFINITY ? m : m * cscale, l};
+  if (hi == 0) *reinterpret_cast<f2*>(parts.ml + 2 * q) = f2{m == -INFINITY ? m : -raise_of(m), l};
 #pragma unroll
   for (int d = 0; d < OT; ++d)
 #pragma unroll
@@ -617,7 +619,7 @@ __global__ __launch_bounds__(256, DK > 128 ? 1 : 2) void paged_prefill_f32_kerne
   l += __shfl_xor(l, 32, 64);
   // dim of register r of output tile d
   auto dim_of = [&](int d, int r, int h) { return 32 * W * (d / W) + W * (8 * (r >> 2) + 4 * h + (r & 3)) + d % W; };
-  float ref = m == -INFINITY ? m : m * cscale;  // in powers of two
+  float lifted = 0.f;  // the part is 2^-lifted of what its reference m makes it
 
   // Outputs that are not finite are formed again, as in the float16 kernel, of probabilities 2^-lift as
   // large: sums of values near float32's largest pass its range too.
@@ -630,7 +632,7 @@ __global__ __launch_bounds__(256, DK > 128 ? 1 : 2) void paged_prefill_f32_kerne
     if (__any(wrong && live)) {
       const float lift = 40.f - static_cast<float>(__builtin_clz(w.len)), f = __builtin_amdgcn_exp2f(-lift);
       const float base = m == -INFINITY ? 0.f : m;
-      if (m != -INFINITY) ref += lift;
+      lifted = lift;
       l *= f;
       floatx16 fresh[OT];
 #pragma unroll
@@ -695,8 +697,17 @@ __global__ __launch_bounds__(256, DK > 128 ? 1 : 2) void paged_prefill_f32_kerne
   }
   const Parts parts(a, kQ);
   const size_t q = (static_cast<size_t>(w.at) * splits + w.piece) * kQ + wave * 32 + l32;
-  if (hi == 0) *reinterpret_cast<f2*>(parts.ml + 2 * q) = f2{ref, l};
-  each_pair([&](int dim, f2 v) { *reinterpret_cast<f2*>(parts.po + q * DK + dim) = v; });
+  // A part's reference is in powers of two: what m·cscale, which may be large, and its sum with the lift are off
+  // by their roundings goes into the part (halved first, so that the largest values stay finite).
+  lifted += 1.f;
+  float ref = -INFINITY, f = 0.5f;
+  if (m != -INFINITY) {
+    const float up = m * cscale;
+    ref = up + lifted;
+    if (__builtin_isfinite(ref)) f *= __builtin_amdgcn_exp2f(__builtin_fmaf(m, cscale, -up) + (up - (ref - lifted)));
+  }
+  if (hi == 0) *reinterpret_cast<f2*>(parts.ml + 2 * q) = f2{ref, l * f};
+  each_pair([&](int dim, f2 v) { *reinterpret_cast<f2*>(parts.po + q * DK + dim) = f2{v.x * f, v.y * f}; });
 }
 
 // Queries of a workgroup: float16 at head dims above 64 eight waves, which share what is written to LDS (a
