@@ -51,61 +51,185 @@ constexpr int kLeastTiles = 4;
 // µs, 128 tokens over 16 Ki keys 83 in place of 64.)
 __host__ __device__ constexpr int held(int Q, int DK) { return DK > 128 ? 256 : 256 * 256 / Q; }
 
-// The keys of Q queries, from q0 on of (row, KV head) bh: length and new tokens of the row, keys that a
-// query of them sees, key tiles a piece and pieces. n·group ≤ q0: no queries.
-struct Span {
-  int len, n, kend, per, pieces;
+// A row of the batch: its length and new tokens, in range, tiles of Q queries of a KV head (0: nothing to
+// do), tiles of keys. Every lane has one where the rows are gone through 64 at a time.
+struct Row {
+  int len, n, nq, kt;
   bool good;  // length and count were in range
+  template <int Q>
+  static __device__ __forceinline__ Row load(const PagedAttnArgs& a, int b) {
+    const int at = min(b, a.B - 1);
+    return make<Q>(a, a.lens[at], a.counts ? a.counts[at] : a.S, b < a.B);
+  }
+  // One row for all lanes, in scalars.
+  template <int Q>
+  static __device__ __forceinline__ Row one(const PagedAttnArgs& a, int b) {
+    const int y = a.counts ? a.counts[b] : a.S;
+    return make<Q>(a, __builtin_amdgcn_readfirstlane(a.lens[b]), __builtin_amdgcn_readfirstlane(y), true);
+  }
+  template <int Q>
+  static __device__ __forceinline__ Row make(const PagedAttnArgs& a, int x, int y, bool there) {
+    Row r;
+    r.len = min(max(x, 0), a.max_pages << a.shift);
+    r.n = min(max(y, 0), a.S);
+    r.good = r.len == x && r.n == y;
+    r.nq = there ? (r.n * a.group + Q - 1) / Q : 0;
+    r.kt = (r.len + kK - 1) / kK;
+    return r;
+  }
+  // What its queries have to go over, in pairs of tiles: the first of them have fewer keys than the last. (At least
+  // half of nq·kt.)
+  template <int Q>
+  __device__ __forceinline__ long long work(int group) const {
+    const long long keys = max(len - n + Q / group, 0) + static_cast<long long>(len);
+    return nq * (keys / (2 * kK) + 1);
+  }
 };
+
+// Where the keys are in pieces, a piece has `per` tiles of them: an even share, for as many workgroups as the
+// card holds (H), of what all rows have to do, W. Row b's tiles of queries have up to p_b = ⌈kt_b / per⌉
+// pieces, and those that are in pieces places for p_b parts each. As p_b − 1 < kt_b / per and Σ nq_b·kt_b·Hkv ≤ 2W
+// ≤ 2H·per, the pieces past the tiles' first are at most 2H, and so are the tiles in pieces. What the host makes
+// room for is bounded the same way (grid_of). A row of little more than a piece stays whole: two rows of 2048 tokens
+// over 8192 keys, 16 heads of 64, 277 µs, 297 with a second piece of an eighth and its merge.
+struct Plan {
+  int per, live;  // key tiles of a piece; tiles of queries of all rows and KV heads
+  int same;       // tiles of queries of each row, where all have as many, else 0
+  // Pieces of a row's tiles at most.
+  __host__ __device__ int pieces(int kt) const { return 4 * kt <= 5 * per ? 1 : (kt + per - 1) / per; }
+};
+// mine: this lane's row, where there are no more than 64.
 template <int Q, int DK>
-__device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int bh, int q0, int splits) {
-  Span w;
-  const int b = bh / a.Hkv, len = a.lens[b], n = a.counts ? a.counts[b] : a.S;
-  w.len = min(max(len, 0), a.max_pages << a.shift);
-  w.n = min(max(n, 0), a.S);
-  w.good = w.len == len && w.n == n;
-  const int last = min((q0 + Q - 1) / a.group, w.n - 1);  // the last token
-  w.kend = max(w.len - w.n + last + 1, 0);
-  const int tiles = (w.kend + kK - 1) / kK;
-  // a piece: an even share, for as many workgroups as the card holds, of what all rows would have to do
-  // were they as this one (the first queries have fewer keys than the last)
-  const long long queries = (w.n * static_cast<long long>(a.group) + Q - 1) / Q;
-  const int mean = static_cast<int>((max(w.len - w.n + Q / a.group, 0) + static_cast<long long>(w.len)) / (2 * kK)) + 1;
-  const int share = static_cast<int>((queries * mean * a.B * a.Hkv + held(Q, DK) - 1) / held(Q, DK));
-  w.per = max(max(kLeastTiles, share), (tiles + splits - 1) / splits);
-  w.pieces = q0 >= w.n * a.group ? 0 : max(1, (tiles + w.per - 1) / w.per);
-  return w;
+__device__ __forceinline__ Plan plan_of(const PagedAttnArgs& a, int lane, bool first, Row& mine) {
+  long long work;
+  int live, nq0;
+  bool good, same = true;
+  if (a.B == 1) {  // (the scans and their vector values take two launches 1.5 µs)
+    mine = Row::one<Q>(a, 0);
+    work = mine.work<Q>(a.group);
+    live = nq0 = mine.nq;
+    good = mine.good;
+  } else {
+    work = live = nq0 = 0;
+    good = true;
+    for (int i = 0; i < a.B; i += 64) {
+      mine = Row::load<Q>(a, i + lane);
+      work += mine.work<Q>(a.group);
+      live += mine.nq;
+      good &= mine.good;
+      if (i == 0) nq0 = __builtin_amdgcn_readfirstlane(mine.nq);
+      same &= i + lane >= a.B || mine.nq == nq0;
+    }
+    auto sum = [](int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); };
+    // (W is below 2^46: 2^22 queries by 2^24 pairs of tiles)
+    work = (static_cast<long long>(sum(static_cast<int>(work >> 20))) << 20) + sum(static_cast<int>(work & 0xfffff));
+    live = sum(live);
+    same = __all(same);
+  }
+  if (!good && first) tell(a.err);
+  constexpr int H = held(Q, DK);
+  const long long share = (work * a.Hkv + H - 1) / H;
+  return Plan{static_cast<int>(max(static_cast<long long>(kLeastTiles), min(share, 1LL << 28))), live * a.Hkv, same ? nq0 : 0};
 }
 
 // What a workgroup does: queries from q0 on of KV head hk of row b, key tiles t0 … t0 + nt − 1, piece
-// `piece` of w.pieces of tile `at`.
+// `piece` of `pieces`, whose first has its part at `slot`.
 struct Tile {
-  int b, hk, q0, len, n, kend, t0, nt, piece, pieces, at;
+  int b, hk, q0, len, n, kend, t0, nt, piece, pieces, slot;
+  // The keys of the Q queries, in pieces of per tiles. False: this piece is not there.
+  template <int Q>
+  __device__ __forceinline__ bool cut(const PagedAttnArgs& a, int per) {
+    const int last = min((q0 + Q - 1) / a.group, n - 1);  // the last token
+    kend = max(len - n + last + 1, 0);
+    const int tiles = (kend + kK - 1) / kK;
+    pieces = max(1, (tiles + per - 1) / per);
+    t0 = piece * per;
+    nt = min(per, tiles - t0);
+    return piece < pieces;
+  }
+  // All of it in scalar registers: the compiler does not see that lanes agree on it, and spills 56 vector registers at
+  // float32 head dims of 256 in place of 10.
+  __device__ __forceinline__ void scalars() {
+    for (int* x : {&b, &hk, &q0, &len, &n, &kend, &t0, &nt, &piece, &pieces, &slot}) *x = __builtin_amdgcn_readfirstlane(*x);
+  }
 };
 
-// False: nothing to do.
+// The row that has item `at` of items that the rows have one after another: `items` of a row with p pieces
+// (of a tile) of them. False: none has it. t.piece: the item's number in its row.
+template <int Q, typename F>
+__device__ __forceinline__ bool find_row(const PagedAttnArgs& a, const Plan& plan, const Row& mine, int at, int lane, F items, Tile& t, int& nq, int& p) {
+  if (a.B == 1) {
+    const Row r = Row::one<Q>(a, 0);
+    t.b = t.slot = 0;
+    t.len = r.len;
+    t.n = r.n;
+    t.piece = at;
+    nq = r.nq;
+    p = plan.pieces(r.kt);
+    return at < items(nq * a.Hkv, p);
+  }
+  int before = 0, slots = 0;
+  for (int i = 0; i < a.B; i += 64) {
+    const Row r = a.B <= 64 ? mine : Row::load<Q>(a, i + lane);
+    const int pieces = plan.pieces(r.kt), tiles = r.nq * a.Hkv;
+    const int own = items(tiles, pieces), own_slots = pieces > 1 ? tiles * pieces : 0;
+    const int sum = wave_scan(own), sum_slots = wave_scan(own_slots);
+    const unsigned long long past = __ballot(before + sum > at);
+    if (past) {
+      const int l = __ffsll(past) - 1;
+      t.b = i + l;
+      t.len = __builtin_amdgcn_readlane(r.len, l);
+      t.n = __builtin_amdgcn_readlane(r.n, l);
+      t.piece = at - before - __builtin_amdgcn_readlane(sum - own, l);
+      t.slot = slots + __builtin_amdgcn_readlane(sum_slots - own_slots, l);
+      nq = __builtin_amdgcn_readlane(r.nq, l);
+      p = __builtin_amdgcn_readlane(pieces, l);
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(sum, 63);
+    slots += __builtin_amdgcn_readlane(sum_slots, 63);
+  }
+  return false;
+}
+
+// False: nothing to do. a.slots: 0 where no keys are in pieces.
 template <int Q, int DK>
-__device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int nq, int splits, Tile& t) {
-  // (row, KV head) fastest: with a multiple of 8 of them each has its XCD, whose L2 then holds its keys. The
-  // last queries, which have the most keys, first; and pieces that a tile does not have behind all others
-  // (among them they leave half of the CUs idle).
-  const int heads = a.B * a.Hkv, n = blockIdx.x, rest = n / heads, bh = n - rest * heads;
-  t.b = bh / a.Hkv;
-  t.hk = bh - t.b * a.Hkv;
-  const int qt = nq - 1 - rest % nq;
-  t.piece = rest / nq;
-  t.at = bh * nq + qt;
+__device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int nq, Tile& t) {
+  const int lane = threadIdx.x & 63;
+  if (a.slots == 0) {
+    // (row, KV head) fastest: with a multiple of 8 of them each has its XCD, whose L2 then holds its keys. The
+    // last queries, which have the most keys, first.
+    const int heads = a.B * a.Hkv, rest = static_cast<int>(blockIdx.x) / heads, bh = static_cast<int>(blockIdx.x) - rest * heads;
+    t.b = bh / a.Hkv;
+    t.hk = bh - t.b * a.Hkv;
+    t.q0 = (nq - 1 - rest) * Q;
+    const Row r = Row::one<Q>(a, t.b);
+    if (rest == 0 && !r.good && threadIdx.x == 0) tell(a.err);
+    t.len = r.len;
+    t.n = r.n;
+    t.piece = t.slot = 0;
+    return t.q0 < t.n * a.group && t.cut<Q>(a, 1 << 30);
+  }
+  // Every tile's first piece, then the others, which a tile of few keys may not have (among the first they leave
+  // half of the CUs idle). Where all rows have as many tiles of queries, in the order above; else row after row.
+  Row mine;
+  const Plan plan = plan_of<Q, DK>(a, lane, blockIdx.x == 0, mine);
+  const int first = static_cast<int>(blockIdx.x);
+  const bool more = first >= plan.live;
+  int at = more ? first - plan.live : first, p = 1;
+  if (!more && plan.same > 0) {
+    const int heads = a.B * a.Hkv, rest = at / heads, bh = at - rest * heads, b = bh / a.Hkv;
+    at = (b * plan.same + rest) * a.Hkv + (bh - b * a.Hkv);
+  }
+  if (!find_row<Q>(a, plan, mine, at, lane, [&](int tiles, int pieces) { return more ? tiles * (pieces - 1) : tiles; }, t, nq, p))
+    return false;
+  const int rest = t.piece / a.Hkv;
+  t.hk = t.piece - rest * a.Hkv;
+  const int turn = rest / nq, qt = nq - 1 - (rest - turn * nq);
+  t.piece = turn + (more ? 1 : 0);
   t.q0 = qt * Q;
-  const Span w = span_of<Q, DK>(a, bh, t.q0, splits);
-  if (rest == 0 && !w.good && threadIdx.x == 0) tell(a.err);
-  if (t.piece >= w.pieces) return false;
-  t.len = w.len;
-  t.n = w.n;
-  t.kend = w.kend;
-  t.pieces = w.pieces;
-  t.t0 = t.piece * w.per;
-  t.nt = min(w.per, (w.kend + kK - 1) / kK - t.t0);
-  return true;
+  t.slot += (t.hk * nq + qt) * p;
+  return t.cut<Q>(a, p == 1 ? 1 << 30 : plan.per);
 }
 
 // Where a piece's part goes: per query its reference (in powers of two) and Σ p, then its Σ p·v.
@@ -121,15 +245,27 @@ struct Parts {
 // last workgroup of a tile, as in ops_paged.hip, 32 pieces of 128 queries took 100 µs.)
 constexpr int kMergers = 256;
 template <typename T, int DK, int Q>
-__global__ __launch_bounds__(kMergers) void paged_merge_kernel(PagedAttnArgs a, int nq, int splits) {
+__global__ __launch_bounds__(kMergers) void paged_merge_kernel(PagedAttnArgs a) {
   constexpr int L = DK / 4, kRows = kMergers / L, kBlocks = (Q + kRows - 1) / kRows;
-  const int at = blockIdx.x / kBlocks, bh = at / nq, q0 = (at - bh * nq) * Q;
-  const Span w = span_of<Q, DK>(a, bh, q0, splits);
-  if (w.pieces <= 1) return;
+  // (a block of rows of a tile in pieces)
+  const int lane = threadIdx.x & 63;
+  Row mine;
+  const Plan plan = plan_of<Q, DK>(a, lane, false, mine);
+  Tile w;
+  int nq = 1, p = 1;
+  if (!find_row<Q>(a, plan, mine, static_cast<int>(blockIdx.x) / kBlocks, lane, [](int tiles, int pieces) { return pieces > 1 ? tiles : 0; }, w, nq, p))
+    return;
+  w.hk = w.piece / nq;
+  const int qt = w.piece - w.hk * nq;
+  w.q0 = qt * Q;
+  w.slot += w.piece * p;
+  w.piece = 0;
+  w.cut<Q>(a, plan.per);
+  if (w.pieces == 1) return;
   const int c = blockIdx.x % kBlocks * kRows + threadIdx.x / L, d = threadIdx.x % L * 4;
-  if (threadIdx.x / L >= kRows || c >= Q || q0 + c >= w.n * a.group || d >= a.dk) return;
+  if (threadIdx.x / L >= kRows || c >= Q || w.q0 + c >= w.n * a.group || d >= a.dk) return;
   const Parts parts(a, Q);
-  const size_t first = static_cast<size_t>(at) * splits;
+  const size_t first = w.slot;
   // (float32: parts times 2^-12, whose sums of near the largest values stay finite)
   constexpr float kRoom = sizeof(T) == 2 ? 0.f : 12.f;
   float top = -INFINITY;
@@ -146,8 +282,8 @@ __global__ __launch_bounds__(kMergers) void paged_merge_kernel(PagedAttnArgs a, 
     lt += st.y * f;
     ot += x * f;
   }
-  const int rr = q0 + c, tk = rr / a.group, b = bh / a.Hkv, hk = bh - b * a.Hkv;
-  T* to = static_cast<T*>(a.out) + ((static_cast<size_t>(b) * a.S + tk) * a.H + hk * a.group + rr % a.group) * a.dk + d;
+  const int rr = w.q0 + c, tk = rr / a.group;
+  T* to = static_cast<T*>(a.out) + ((static_cast<size_t>(w.b) * a.S + tk) * a.H + w.hk * a.group + rr % a.group) * a.dk + d;
   const bool sees = w.len - w.n + tk >= 0;
 #pragma unroll
   for (int e = 0; e < 4; ++e) to[e] = static_cast<T>(sees ? ot[e] / lt : 0.f);
@@ -155,7 +291,7 @@ __global__ __launch_bounds__(kMergers) void paged_merge_kernel(PagedAttnArgs a, 
 
 // DK: head dims up to it, in steps of 8.
 template <int DK, int kWaves>
-__global__ __launch_bounds__(64 * kWaves, DK > 128 ? 1 : 2) void paged_prefill_f16_kernel(PagedAttnArgs a, int nq, int splits) {
+__global__ __launch_bounds__(64 * kWaves, DK > 128 ? 1 : 2) void paged_prefill_f16_kernel(PagedAttnArgs a, int nq) {
 #pragma clang fp contract(off)
   constexpr int kThreads = 64 * kWaves, kQ = 32 * kWaves;
   constexpr int KS = DK / 16, OT = DK / 32, VG = DK / 8;
@@ -166,7 +302,8 @@ __global__ __launch_bounds__(64 * kWaves, DK > 128 ? 1 : 2) void paged_prefill_f
   __shared__ __align__(16) half_t Ks[2][kK][KP];
   __shared__ __align__(16) half_t Vs[2][kK][VP];
   Tile w;
-  if (!find_tile<kQ, DK>(a, nq, splits, w)) return;
+  if (!find_tile<kQ, DK>(a, nq, w)) return;
+  w.scalars();
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int dk = a.dk, R = w.n * a.group, hi = lane >> 5;
   const int qw = w.q0 + wave * 32, myq = qw + (lane & 31);  // the wave's first query, this lane's
@@ -456,7 +593,7 @@ __global__ __launch_bounds__(64 * kWaves, DK > 128 ? 1 : 2) void paged_prefill_f
     return;
   }
   const Parts parts(a, kQ);
-  const size_t q = (static_cast<size_t>(w.at) * splits + w.piece) * kQ + wave * 32 + (lane & 31);
+  const size_t q = (static_cast<size_t>(w.slot) + w.piece) * kQ + wave * 32 + (lane & 31);
   if (hi == 0) *reinterpret_cast<f2*>(parts.ml + 2 * q) = f2{m == -INFINITY ? m : -raise_of(m), l};
 #pragma unroll
   for (int d = 0; d < OT; ++d)
@@ -476,7 +613,7 @@ __global__ __launch_bounds__(64 * kWaves, DK > 128 ? 1 : 2) void paged_prefill_f
 // workgroup of the CU in between. (1024 tokens over 4096 keys: 8 heads of 64, 87 µs, 86 TFLOP/s; 8 over 2 of
 // 128, 157, 96; 16 over 4 of 192, 1000 over 4000, 470, 92; a product of 8192³ reaches 153.)
 template <int DK>
-__global__ __launch_bounds__(256, DK > 128 ? 1 : 2) void paged_prefill_f32_kernel(PagedAttnArgs a, int nq, int splits) {
+__global__ __launch_bounds__(256, DK > 128 ? 1 : 2) void paged_prefill_f32_kernel(PagedAttnArgs a, int nq) {
   constexpr int kWaves = 4, kQ = 32 * kWaves;
   // Keys of a tile here: 32 where 64 would take more registers than there are (1000 tokens over 4000 keys, 16
   // heads over 4 of 192, 470 µs, 475; 512 over 2048, 8 of 256, 105, 135; of 128 156.7, 158.5).
@@ -490,7 +627,8 @@ __global__ __launch_bounds__(256, DK > 128 ? 1 : 2) void paged_prefill_f32_kerne
   __shared__ __align__(16) float Ks[KT][P];
   __shared__ __align__(16) float Vs[KT][P];
   Tile w;
-  if (!find_tile<kQ, DK>(a, nq, splits, w)) return;
+  if (!find_tile<kQ, DK>(a, nq, w)) return;
+  w.scalars();
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int dk = a.dk, R = w.n * a.group, hi = lane >> 5, l32 = lane & 31;
   const int qw = w.q0 + wave * 32, myq = qw + l32;
@@ -696,7 +834,7 @@ __global__ __launch_bounds__(256, DK > 128 ? 1 : 2) void paged_prefill_f32_kerne
     return;
   }
   const Parts parts(a, kQ);
-  const size_t q = (static_cast<size_t>(w.at) * splits + w.piece) * kQ + wave * 32 + l32;
+  const size_t q = (static_cast<size_t>(w.slot) + w.piece) * kQ + wave * 32 + l32;
   // A part's reference is in powers of two: what m·cscale, which may be large, and its sum with the lift are off
   // by their roundings goes into the part (halved first, so that the largest values stay finite).
   lifted += 1.f;
@@ -719,32 +857,40 @@ int columns_of(int dt, int dk) {
   return dk <= 32 && dt == F32 ? 32 : dk <= 64 ? 64 : dk <= 96 ? 96 : dk <= 128 ? 128 : dk <= 192 ? 192 : 256;
 }
 
-// Tiles of queries, and the most pieces that the keys of one are cut into.
+// Tiles of queries, the workgroups that take them and their pieces, places for parts (0: no keys are in pieces) and
+// tiles that may be in pieces.
 struct Grid {
-  long long tiles;
-  int q, nq, splits;
+  int q, nq;
+  long long groups, slots, split;
 };
 Grid grid_of(int dt, int B, int H, int Hkv, int S, int P, int dk) {
   Grid g;
   const int R = H / Hkv * S;
   g.q = queries_of(dt, R, dk);
   g.nq = (R + g.q - 1) / g.q;
-  g.tiles = static_cast<long long>(g.nq) * Hkv * B;
-  const int most = std::max(1, (P + kK - 1) / kK / kLeastTiles), all = held(g.q, columns_of(dt, dk));
-  g.splits = g.tiles >= all ? 1 : static_cast<int>(std::min<long long>(most, (2 * all + g.tiles - 1) / g.tiles));
+  const long long tiles = static_cast<long long>(g.nq) * Hkv * B, all = held(g.q, columns_of(dt, dk));
+  const int most = Plan{kLeastTiles, 0, 0}.pieces((P - 1) / kK + 1);  // pieces of a tile
+  g.groups = tiles;
+  g.slots = g.split = 0;
+  // One row's tiles that fill the card stay whole. Those of several may be of one row alone that has many new
+  // tokens, or many more keys than the others. (Of more than 512 the workgroups would spend their time on
+  // lengths.)
+  if (most == 1 || (B == 1 && tiles >= all) || B > 512) return g;
+  g.groups = tiles + std::min(2 * all, tiles * (most - 1));
+  g.split = std::min(tiles, 2 * all);
+  g.slots = std::min(2 * all + g.split, tiles * most);
   return g;
 }
 
 template <typename T, int DK, int Q>
 int launch_kernels(const PagedAttnArgs& a, const Grid& g, hipStream_t st) {
-  const unsigned n = static_cast<unsigned>(g.tiles * g.splits);
-  if constexpr (sizeof(T) == 2) paged_prefill_f16_kernel<DK, Q / 32><<<n, 2 * Q, 0, st>>>(a, g.nq, g.splits);
-  else paged_prefill_f32_kernel<DK><<<n, 2 * Q, 0, st>>>(a, g.nq, g.splits);
+  const unsigned n = static_cast<unsigned>(g.groups);
+  if constexpr (sizeof(T) == 2) paged_prefill_f16_kernel<DK, Q / 32><<<n, 2 * Q, 0, st>>>(a, g.nq);
+  else paged_prefill_f32_kernel<DK><<<n, 2 * Q, 0, st>>>(a, g.nq);
   NML_LAUNCHED();
-  if (g.splits == 1) return 0;
+  if (g.slots == 0) return 0;
   constexpr int kRows = kMergers / (DK / 4);
-  const unsigned blocks = static_cast<unsigned>(g.tiles * ((Q + kRows - 1) / kRows));
-  paged_merge_kernel<T, DK, Q><<<blocks, kMergers, 0, st>>>(a, g.nq, g.splits);
+  paged_merge_kernel<T, DK, Q><<<static_cast<unsigned>(g.split * ((Q + kRows - 1) / kRows)), kMergers, 0, st>>>(a);
   NML_LAUNCHED();
   return 0;
 }
@@ -771,13 +917,12 @@ bool paged_prefill_applies(int dt, int H, int Hkv, int S, int dk) {
 
 size_t paged_prefill_workspace(int dt, int B, int H, int Hkv, int S, int P, int dk) {
   const Grid g = grid_of(dt, B, H, Hkv, S, P, dk);
-  if (g.splits == 1) return 0;
-  return kCounterBytes + sizeof(float) * g.tiles * g.splits * g.q * (2 + columns_of(dt, dk));
+  return g.slots == 0 ? 0 : kCounterBytes + sizeof(float) * g.slots * g.q * (2 + columns_of(dt, dk));
 }
 
 int launch_paged_prefill(int dt, PagedAttnArgs a, hipStream_t st) {
   const Grid g = grid_of(dt, a.B, a.H, a.Hkv, a.S, a.max_pages << a.shift, a.dk);
-  a.slots = g.splits > 1 ? static_cast<int>(g.tiles * g.splits) : 0;
+  a.slots = static_cast<int>(g.slots);
   switch (columns_of(dt, a.dk)) {
     case 32: return launch_kernels<float, 32, 128>(a, g, st);
     case 64: return launch_columns<64>(dt, a, g, st);
