@@ -469,14 +469,16 @@ def _page_count(lengths, page_size):
     return -(-np.maximum(np.asarray(lengths, dtype=np.int64), 0) // page_size)
 
 
-def _check_pages(what, table, lengths, page_size, num_pages):
-    """Raises ValueError where a row of ``lengths`` positions needs a page outside [0, num_pages) or
-    more pages than ``table`` (host arrays) has."""
+def _check_pages(what, table, lengths, page_size, num_pages, counts=None):
+    """Raises ValueError where a row of ``lengths`` positions needs more pages than ``table`` (host
+    arrays) has or, unless its count is 0, one outside [0, num_pages)."""
     need = _page_count(lengths, page_size)
     if need.size and int(need.max()) > table.shape[1]:
         raise ValueError(f"{what}: a row of {int(np.max(lengths))} positions needs {int(need.max())} "
                          f"pages of {page_size}, the table has {table.shape[1]}")
     used = np.arange(table.shape[1]) < need[:, None]
+    if counts is not None:
+        used &= np.asarray(counts)[:, None] != 0
     bad = used & ((table < 0) | (table >= num_pages))
     if bad.any():
         raise ValueError(f"{what}: page {int(table[bad][0])} is outside [0, {num_pages})")
@@ -550,10 +552,14 @@ def paged_attention(q, cache, table, lens, scale, counts=None):
         raise ValueError(f"paged_attention: q {q.shape} for {batch} rows, head dim {cache.dk}")
     if lens is None:
         raise ValueError("paged_attention: lens is required")
-    if host is not None and not isinstance(lens, N.DeviceArray):
-        _check_pages("paged_attention", host, lens, cache.page_size, cache.num_pages)
+    for name, x in (("lens", lens), ("counts", counts)):
+        if x is not None and np.shape(x) != (batch,):
+            raise ValueError(f"paged_attention: {name} must be ({batch},), got {np.shape(x)}")
+    heads, seq, dk = q.shape[1:]
+    # what is on the host is checked here, anything else by the kernel: pages of rows that attend
+    if host is not None and seq and not any(isinstance(x, N.DeviceArray) for x in (lens, counts)):
+        _check_pages("paged_attention", host, lens, cache.page_size, cache.num_pages, counts)
     qd = _dev(q, cache.dtype)
-    _, heads, seq, dk = qd.shape
     td = _dev(host if host is not None else table, np.int32)
     ld = _rows_i32(lens, batch, "paged_attention: lens")
     cd = _rows_i32(counts, batch, "paged_attention: counts")
