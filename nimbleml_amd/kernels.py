@@ -35,6 +35,7 @@ import numpy as np
 
 from nimbleml_amd import _native as N
 from nimbleml_amd import np_backend
+from nimbleml_amd.tensor import Tensor
 
 EPI_NONE, EPI_BIAS, EPI_BIAS_GELU, EPI_BIAS_RESID = 0, 1, 2, 3
 
@@ -647,7 +648,9 @@ def verify_drafts(logits, drafts, uniforms=None, *, draft_logits=None, counts=No
     Returns ``(accepted, tokens)`` as ``DeviceArray``s: int32 (batch,) accepted drafts and int64
     (batch, n + 1), those drafts, one token more, then −1; ``KVCache.truncate`` takes a cache back to
     them. Raises ValueError for a draft outside [0, vocab), a count outside [0, n] or a row of
-    logits that decides and has no distribution."""
+    logits that decides and has no distribution. Both logits may be Tensors."""
+    logits, draft_logits = (x.data.reshape(x.shape) if isinstance(x, Tensor) else x
+                            for x in (logits, draft_logits))
     dt = _float_dtype(logits)
     if len(logits.shape) != 3 or logits.shape[1] < 1:
         raise ValueError(f"verify_drafts: logits must be (batch, n + 1, vocab), got {logits.shape}")
