@@ -27,8 +27,8 @@ def distill_loss(logits, top_ids, top_logits, *, temperature=1.0):
     x = logits.data if isinstance(logits.data, N.DeviceArray) else \
         N.DeviceArray.from_host(np.asarray(logits.data))
     x = x.reshape(logits.shape)
-    ids, top = (a if isinstance(a, N.DeviceArray) else N.DeviceArray.from_host(np.asarray(
-        a.data if isinstance(a, Tensor) else a, dtype=dt).reshape(a.shape))
+    ids, top = (a if isinstance(a, N.DeviceArray) else N.DeviceArray.from_host(
+        np.asarray(a.data, dtype=dt).reshape(a.shape) if isinstance(a, Tensor) else np.asarray(a, dtype=dt))
         for a, dt in ((top_ids, np.int64), (top_logits, np.float32)))
     loss, m, lsum = K.distill(x, ids, top, temperature)
     needs = is_grad_enabled() and logits.requires_grad
