@@ -906,13 +906,14 @@ int launch_columns(int dt, const PagedAttnArgs& a, const Grid& g, hipStream_t st
 
 }  // namespace
 
-// Queries of a KV head from which on this pays: float16, 48 over 4000 keys of 128, 32.8 µs (42.9 with 16 at a
-// time), 32 no less; 33 over 2000 keys of 256 42.1 (47.4), 2048 over 8192 624 (1705), 64 over 200 26.8 (20.4);
-// float32, whose matrix instructions cost what they multiply, padding or not, 100 over
-// up to 1000 keys 54 (44), 128 over 128 keys of 256 50 (22), 512 over 2048 105 (130), 1000 over 4000 of 192
-// 470 (778).
+// Queries of a KV head from which on this pays (µs here and with 16 queries at a time). float16: 64, one row of
+// 3000 keys, 16 heads of 64 22.4 and 20.7, 8 of 128 27.2 and 22.5, 4 of 256 41 and 36, 8 rows of 1500 32 and 37, 36 and
+// 37, 47 and 62; 96 22.8 and 24.9, 27.8 and 26.1, 42 and 36, 8 rows 33 and 48, 38 and 54, 49 and 62; the fewer
+// the tiles and the keys the later, one row of 400 past 256 (17.0 and 15.9). float32, whose matrix
+// instructions cost what they multiply, padding or not: 100 over 4000 keys of 128 58 and 33, 200 over 2000 of 64 36 and 42;
+// of 256 200 over 2048 103 and 87, 512 110 and 145.
 bool paged_prefill_applies(int dt, int H, int Hkv, int S, int dk) {
-  return dk % (dt == F16 ? 8 : 4) == 0 && S > 1 && H / Hkv * S >= (dt == F16 ? 33 : dk <= 128 ? 128 : 256);
+  return dk % (dt == F16 ? 8 : 4) == 0 && S > 1 && H / Hkv * S >= (dt == F16 ? 65 : dk <= 128 ? 128 : 256);
 }
 
 size_t paged_prefill_workspace(int dt, int B, int H, int Hkv, int S, int P, int dk) {
