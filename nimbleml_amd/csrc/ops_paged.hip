@@ -28,11 +28,11 @@ inline Div div_by(unsigned d) {
 }
 __device__ __forceinline__ unsigned quotient(unsigned n, Div d) { return (__umulhi(d.mul, n) + n) >> d.shift; }
 
-// A writing workgroup, and the units that a lane of it takes (their loads in flight together: 4 × 4096 tokens
-// of 16 heads of 128 float16 values, µs with four 57.9, two 52.7, eight 151). Written past the caches, which
-// a prompt's keys leave again before they are read: 39.5, 6.8 TB/s of reads and writes (the reads partly from
-// the last cache; with inputs that were not there 59, 4.6). One token of 32 rows, 16 heads of 64: 3.0.
-constexpr int kWriters = 256, kEach = 4;
+// A writing workgroup, and the units that a lane of it takes, their loads in flight together. With inputs that change
+// from call to call: 4 × 4096 tokens of 16 heads of 128 float16 values, 55.7 µs with two, 4.8 TB/s of reads and
+// writes; 59.7 with one, 60.1 with four, 172 with eight; stored past the caches, which a prompt's keys leave again before
+// they are read: 59 with stores that stay there. One token of 32 rows, 16 heads of 64: 3.0 with its launch.
+constexpr int kWriters = 256, kEach = 2;
 
 // Units of one row: (head, token, unit of its vector), the unit fastest: the order of the pages, so
 // that a workgroup writes runs of them.
@@ -137,9 +137,11 @@ constexpr float up_log2() {
 
 // Head dims in steps of 32: 1, 2, 4 or 8 of them.
 constexpr int steps_of(int dk) { return dk <= 32 ? 1 : dk <= 64 ? 2 : dk <= 128 ? 4 : 8; }
-// Waves of a workgroup. Few begin and merge sooner, and more workgroups even out rows of different length
-// (µs with four and eight: 16 rows of 1 to 8 Ki keys, 32 heads over 8 of 128, 54 and 70; one row of 1023, 16
-// heads of 64, 10.7 and 12.2, 9.2 with two; 128 rows of 100 to 1000 60.9 with four and 57.1 with two).
+// Waves of a workgroup. Few begin and merge sooner, and more workgroups even out rows of different length; at a head dim
+// of 64 two, else four. (µs, with inputs that change from call to call: 16 rows of 1 to 8 Ki keys, 32 heads over 8 of 128, 66
+// with four and 76 with eight; of 64, 43 with two and 41 with four, one row of 1023, 16 heads of 64, 9.9 and 11.5,
+// 128 rows of 100 to 1000 64.6 and 66.0; the same three of 32 24.2 and 21.2, 8.9 and 10.1, 33 and 35, and 16 rows of up
+// to 2048 and five tokens, 8 heads of 32, float32, 18.6 and 15.5.)
 __host__ __device__ constexpr int group_waves(int nb) { return nb == 2 ? 2 : 4; }
 // Waves a SIMD that the registers are held to (at head dim 256 a wave's tile takes more than half of them: 16
 // rows of 1 to 4 Ki keys, 16 heads over 2, float16 33 µs and float32 47; held to two waves 38 and 68, with
