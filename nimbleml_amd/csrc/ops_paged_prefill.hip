@@ -2,7 +2,7 @@
 // holds already.
 //
 // A KV head's queries (its group's heads times the new tokens, the heads of a token side by side) are
-// taken 128 or 256 at a time by a workgroup of four or eight waves, 32 a wave, over tiles of 64 keys in LDS:
+// taken 128 at a time by a workgroup of four waves, 32 a wave, over tiles of 64 keys in LDS:
 //   Sᵀ = K·Qᵀ    v_mfma_f32_32x32x16_f16, Qᵀ in registers; lane l then holds query l % 32 and keys
 //                8(r/4) + 4(l/32) + r % 4 of each 32 in register r;
 //   Oᵀ += Vᵀ·Pᵀ  Pᵀ straight from those registers, Vᵀ by transposing reads of V as it lies in memory,
@@ -37,51 +37,52 @@ namespace nml {
 namespace {
 
 constexpr int kK = 64;  // keys of a tile
+// Waves of a workgroup, and the queries of its tile. (Eight waves, which share what is written to LDS: 1024 tokens over
+// 4096 keys, 16 heads over 4 of 96, 76 µs, 71 with four; 6 ragged rows of up to 512 tokens, 12 heads of 80, 64 and 57;
+// 2048 over 8192, 32 over 8 of 128, 440 and 439; two rows of them, 16 heads of 64, 324 and 286.)
+constexpr int kWaves = 4, kQ = 32 * kWaves;
 constexpr float kLog2e = 1.44269504088896341f;
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef short s8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
-// Keys a piece has at least, in tiles (2 rows of 100 tokens over up to 1000 keys, 16 heads of 64: 15.1 µs at
-// four, 18.8 at eight, 19.9 at one).
+// Keys a piece has at least, in tiles (2 rows of 100 tokens over up to 1000 keys, 16 heads of 64: 17.7 µs at
+// four, 22.4 at eight, 18.2 at one).
 constexpr int kLeastTiles = 4;
 
 // Workgroups that the card holds at once, eight waves a CU (columns above 128, which take more than half of
-// the registers: four): where the tiles are fewer their keys are cut into pieces. (Pieces for twice as many: 6 ragged rows of up to 512 tokens, 12 heads of 80, 53 in place of 47
-// µs, 128 tokens over 16 Ki keys 83 in place of 64.)
-__host__ __device__ constexpr int held(int Q, int DK) { return DK > 128 ? 256 : 256 * 256 / Q; }
+// the registers: four): where the tiles are fewer their keys are cut into pieces. (Pieces for twice as many: 128 tokens
+// over 16 Ki keys, 16 heads over 4 of 128, 88 in place of 62 µs, 1024 over 4096, 16 over 4 of 192, 170 in place of 161;
+// 2048 over 8192, 16 over 4 of 256, which are 256 tiles whole, 700 in place of 723.)
+__host__ __device__ constexpr int held(int DK) { return DK > 128 ? 256 : 512; }
 
-// A row of the batch: its length and new tokens, in range, tiles of Q queries of a KV head (0: nothing to
+// A row of the batch: its length and new tokens, in range, tiles of queries of a KV head (0: nothing to
 // do), tiles of keys. Every lane has one where the rows are gone through 64 at a time.
 struct Row {
   int len, n, nq, kt;
   bool good;  // length and count were in range
-  template <int Q>
   static __device__ __forceinline__ Row load(const PagedAttnArgs& a, int b) {
     const int at = min(b, a.B - 1);
-    return make<Q>(a, a.lens[at], a.counts ? a.counts[at] : a.S, b < a.B);
+    return make(a, a.lens[at], a.counts ? a.counts[at] : a.S, b < a.B);
   }
   // One row for all lanes, in scalars.
-  template <int Q>
   static __device__ __forceinline__ Row one(const PagedAttnArgs& a, int b) {
     const int y = a.counts ? a.counts[b] : a.S;
-    return make<Q>(a, __builtin_amdgcn_readfirstlane(a.lens[b]), __builtin_amdgcn_readfirstlane(y), true);
+    return make(a, __builtin_amdgcn_readfirstlane(a.lens[b]), __builtin_amdgcn_readfirstlane(y), true);
   }
-  template <int Q>
   static __device__ __forceinline__ Row make(const PagedAttnArgs& a, int x, int y, bool there) {
     Row r;
     r.len = min(max(x, 0), a.max_pages << a.shift);
     r.n = min(max(y, 0), a.S);
     r.good = r.len == x && r.n == y;
-    r.nq = there ? (r.n * a.group + Q - 1) / Q : 0;
+    r.nq = there ? (r.n * a.group + kQ - 1) / kQ : 0;
     r.kt = (r.len + kK - 1) / kK;
     return r;
   }
   // What its queries have to go over, in pairs of tiles: the first of them have fewer keys than the last. (At least
   // half of nq·kt.)
-  template <int Q>
   __device__ __forceinline__ long long work(int group) const {
-    const long long keys = max(len - n + Q / group, 0) + static_cast<long long>(len);
+    const long long keys = max(len - n + kQ / group, 0) + static_cast<long long>(len);
     return nq * (keys / (2 * kK) + 1);
   }
 };
@@ -99,22 +100,22 @@ struct Plan {
   __host__ __device__ int pieces(int kt) const { return 4 * kt <= 5 * per ? 1 : (kt + per - 1) / per; }
 };
 // mine: this lane's row, where there are no more than 64.
-template <int Q, int DK>
+template <int DK>
 __device__ __forceinline__ Plan plan_of(const PagedAttnArgs& a, int lane, bool first, Row& mine) {
   long long work;
   int live, nq0;
   bool good, same = true;
   if (a.B == 1) {  // (the scans and their vector values take two launches 1.5 µs)
-    mine = Row::one<Q>(a, 0);
-    work = mine.work<Q>(a.group);
+    mine = Row::one(a, 0);
+    work = mine.work(a.group);
     live = nq0 = mine.nq;
     good = mine.good;
   } else {
     work = live = nq0 = 0;
     good = true;
     for (int i = 0; i < a.B; i += 64) {
-      mine = Row::load<Q>(a, i + lane);
-      work += mine.work<Q>(a.group);
+      mine = Row::load(a, i + lane);
+      work += mine.work(a.group);
       live += mine.nq;
       good &= mine.good;
       if (i == 0) nq0 = __builtin_amdgcn_readfirstlane(mine.nq);
@@ -127,7 +128,7 @@ __device__ __forceinline__ Plan plan_of(const PagedAttnArgs& a, int lane, bool f
     same = __all(same);
   }
   if (!good && first) tell(a.err);
-  constexpr int H = held(Q, DK);
+  constexpr int H = held(DK);
   const long long share = (work * a.Hkv + H - 1) / H;
   return Plan{static_cast<int>(max(static_cast<long long>(kLeastTiles), min(share, 1LL << 28))), live * a.Hkv, same ? nq0 : 0};
 }
@@ -136,10 +137,9 @@ __device__ __forceinline__ Plan plan_of(const PagedAttnArgs& a, int lane, bool f
 // `piece` of `pieces`, whose first has its part at `slot`.
 struct Tile {
   int b, hk, q0, len, n, kend, t0, nt, piece, pieces, slot;
-  // The keys of the Q queries, in pieces of per tiles. False: this piece is not there.
-  template <int Q>
+  // The keys of the queries, in pieces of per tiles. False: this piece is not there.
   __device__ __forceinline__ bool cut(const PagedAttnArgs& a, int per) {
-    const int last = min((q0 + Q - 1) / a.group, n - 1);  // the last token
+    const int last = min((q0 + kQ - 1) / a.group, n - 1);  // the last token
     kend = max(len - n + last + 1, 0);
     const int tiles = (kend + kK - 1) / kK;
     pieces = max(1, (tiles + per - 1) / per);
@@ -156,10 +156,10 @@ struct Tile {
 
 // The row that has item `at` of items that the rows have one after another: `items` of a row with p pieces
 // (of a tile) of them. False: none has it. t.piece: the item's number in its row.
-template <int Q, typename F>
+template <typename F>
 __device__ __forceinline__ bool find_row(const PagedAttnArgs& a, const Plan& plan, const Row& mine, int at, int lane, F items, Tile& t, int& nq, int& p) {
   if (a.B == 1) {
-    const Row r = Row::one<Q>(a, 0);
+    const Row r = Row::one(a, 0);
     t.b = t.slot = 0;
     t.len = r.len;
     t.n = r.n;
@@ -170,7 +170,7 @@ __device__ __forceinline__ bool find_row(const PagedAttnArgs& a, const Plan& pla
   }
   int before = 0, slots = 0;
   for (int i = 0; i < a.B; i += 64) {
-    const Row r = a.B <= 64 ? mine : Row::load<Q>(a, i + lane);
+    const Row r = a.B <= 64 ? mine : Row::load(a, i + lane);
     const int pieces = plan.pieces(r.kt), tiles = r.nq * a.Hkv;
     const int own = items(tiles, pieces), own_slots = pieces > 1 ? tiles * pieces : 0;
     const int sum = wave_scan(own), sum_slots = wave_scan(own_slots);
@@ -193,7 +193,7 @@ __device__ __forceinline__ bool find_row(const PagedAttnArgs& a, const Plan& pla
 }
 
 // False: nothing to do. a.slots: 0 where no keys are in pieces.
-template <int Q, int DK>
+template <int DK>
 __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int nq, Tile& t) {
   const int lane = threadIdx.x & 63;
   if (a.slots == 0) {
@@ -202,18 +202,18 @@ __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int nq, Tile& 
     const int heads = a.B * a.Hkv, rest = static_cast<int>(blockIdx.x) / heads, bh = static_cast<int>(blockIdx.x) - rest * heads;
     t.b = bh / a.Hkv;
     t.hk = bh - t.b * a.Hkv;
-    t.q0 = (nq - 1 - rest) * Q;
-    const Row r = Row::one<Q>(a, t.b);
+    t.q0 = (nq - 1 - rest) * kQ;
+    const Row r = Row::one(a, t.b);
     if (rest == 0 && !r.good && threadIdx.x == 0) tell(a.err);
     t.len = r.len;
     t.n = r.n;
     t.piece = t.slot = 0;
-    return t.q0 < t.n * a.group && t.cut<Q>(a, 1 << 30);
+    return t.q0 < t.n * a.group && t.cut(a, 1 << 30);
   }
   // Every tile's first piece, then the others, which a tile of few keys may not have (among the first they leave
   // half of the CUs idle). Where all rows have as many tiles of queries, in the order above; else row after row.
   Row mine;
-  const Plan plan = plan_of<Q, DK>(a, lane, blockIdx.x == 0, mine);
+  const Plan plan = plan_of<DK>(a, lane, blockIdx.x == 0, mine);
   const int first = static_cast<int>(blockIdx.x);
   const bool more = first >= plan.live;
   int at = more ? first - plan.live : first, p = 1;
@@ -221,61 +221,61 @@ __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int nq, Tile& 
     const int heads = a.B * a.Hkv, rest = at / heads, bh = at - rest * heads, b = bh / a.Hkv;
     at = (b * plan.same + rest) * a.Hkv + (bh - b * a.Hkv);
   }
-  if (!find_row<Q>(a, plan, mine, at, lane, [&](int tiles, int pieces) { return more ? tiles * (pieces - 1) : tiles; }, t, nq, p))
+  if (!find_row(a, plan, mine, at, lane, [&](int tiles, int pieces) { return more ? tiles * (pieces - 1) : tiles; }, t, nq, p))
     return false;
   const int rest = t.piece / a.Hkv;
   t.hk = t.piece - rest * a.Hkv;
   const int turn = rest / nq, qt = nq - 1 - (rest - turn * nq);
   t.piece = turn + (more ? 1 : 0);
-  t.q0 = qt * Q;
+  t.q0 = qt * kQ;
   t.slot += (t.hk * nq + qt) * p;
-  return t.cut<Q>(a, p == 1 ? 1 << 30 : plan.per);
+  return t.cut(a, p == 1 ? 1 << 30 : plan.per);
 }
 
 // Where a piece's part goes: per query its reference (in powers of two) and Σ p, then its Σ p·v.
 struct Parts {
   float *ml, *po;
-  __device__ Parts(const PagedAttnArgs& a, int Q) {
+  __device__ explicit Parts(const PagedAttnArgs& a) {
     ml = reinterpret_cast<float*>(static_cast<char*>(a.ws) + kCounterBytes);  // (behind what other calls keep there)
-    po = ml + static_cast<size_t>(a.slots) * Q * 2;
+    po = ml + static_cast<size_t>(a.slots) * kQ * 2;
   }
 };
 
 // The pieces' parts merged in their order, four dims of a query a thread. (A launch of its own: by the
 // last workgroup of a tile, as in ops_paged.hip, 32 pieces of 128 queries took 100 µs.)
 constexpr int kMergers = 256;
-template <typename T, int DK, int Q>
+template <typename T, int DK>
 __global__ __launch_bounds__(kMergers) void paged_merge_kernel(PagedAttnArgs a) {
-  constexpr int L = DK / 4, kRows = kMergers / L, kBlocks = (Q + kRows - 1) / kRows;
+  constexpr int L = DK / 4, kRows = kMergers / L, kBlocks = (kQ + kRows - 1) / kRows;
   // (a block of rows of a tile in pieces)
   const int lane = threadIdx.x & 63;
   Row mine;
-  const Plan plan = plan_of<Q, DK>(a, lane, false, mine);
+  const Plan plan = plan_of<DK>(a, lane, false, mine);
   Tile w;
   int nq = 1, p = 1;
-  if (!find_row<Q>(a, plan, mine, static_cast<int>(blockIdx.x) / kBlocks, lane, [](int tiles, int pieces) { return pieces > 1 ? tiles : 0; }, w, nq, p))
+  if (!find_row(a, plan, mine, static_cast<int>(blockIdx.x) / kBlocks, lane, [](int tiles, int pieces) { return pieces > 1 ? tiles : 0; }, w, nq, p))
     return;
   w.hk = w.piece / nq;
   const int qt = w.piece - w.hk * nq;
-  w.q0 = qt * Q;
+  w.q0 = qt * kQ;
   w.slot += w.piece * p;
   w.piece = 0;
-  w.cut<Q>(a, plan.per);
+  w.cut(a, plan.per);
   if (w.pieces == 1) return;
   const int c = blockIdx.x % kBlocks * kRows + threadIdx.x / L, d = threadIdx.x % L * 4;
-  if (threadIdx.x / L >= kRows || c >= Q || w.q0 + c >= w.n * a.group || d >= a.dk) return;
-  const Parts parts(a, Q);
+  if (threadIdx.x / L >= kRows || c >= kQ || w.q0 + c >= w.n * a.group || d >= a.dk) return;
+  const Parts parts(a);
   const size_t first = w.slot;
   // (float32: parts times 2^-12, whose sums of near the largest values stay finite)
   constexpr float kRoom = sizeof(T) == 2 ? 0.f : 12.f;
   float top = -INFINITY;
-  for (int y = 0; y < w.pieces; ++y) top = fmaxf(top, parts.ml[2 * ((first + y) * Q + c)]);
+  for (int y = 0; y < w.pieces; ++y) top = fmaxf(top, parts.ml[2 * ((first + y) * kQ + c)]);
   const float rf = (top == -INFINITY ? 0.f : top) + kRoom;
   float lt = 0.f;
   floatx4 ot = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int y = 0; y < w.pieces; ++y) {
-    const size_t q = (first + y) * Q + c;
+    const size_t q = (first + y) * kQ + c;
     const f2 st = *reinterpret_cast<const f2*>(parts.ml + 2 * q);
     const floatx4 x = *reinterpret_cast<const floatx4*>(parts.po + q * DK + d);
     const float f = __builtin_amdgcn_exp2f(st.x - rf);
@@ -290,10 +290,9 @@ __global__ __launch_bounds__(kMergers) void paged_merge_kernel(PagedAttnArgs a) 
 }
 
 // DK: head dims up to it, in steps of 8.
-template <int DK, int kWaves>
+template <int DK>
 __global__ __launch_bounds__(64 * kWaves, DK > 128 ? 1 : 2) void paged_prefill_f16_kernel(PagedAttnArgs a, int nq) {
 #pragma clang fp contract(off)
-  constexpr int kThreads = 64 * kWaves, kQ = 32 * kWaves;
   constexpr int KS = DK / 16, OT = DK / 32, VG = DK / 8;
   constexpr int L = DK <= 64 ? 8 : DK <= 128 ? 16 : 32;  // lanes of a row, 16 bytes each
   constexpr int RW = 64 / L;              // rows of a wave's load
@@ -302,7 +301,7 @@ __global__ __launch_bounds__(64 * kWaves, DK > 128 ? 1 : 2) void paged_prefill_f
   __shared__ __align__(16) half_t Ks[2][kK][KP];
   __shared__ __align__(16) half_t Vs[2][kK][VP];
   Tile w;
-  if (!find_tile<kQ, DK>(a, nq, w)) return;
+  if (!find_tile<DK>(a, nq, w)) return;
   w.scalars();
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int dk = a.dk, R = w.n * a.group, hi = lane >> 5;
@@ -592,7 +591,7 @@ __global__ __launch_bounds__(64 * kWaves, DK > 128 ? 1 : 2) void paged_prefill_f
       }
     return;
   }
-  const Parts parts(a, kQ);
+  const Parts parts(a);
   const size_t q = (static_cast<size_t>(w.slot) + w.piece) * kQ + wave * 32 + (lane & 31);
   if (hi == 0) *reinterpret_cast<f2*>(parts.ml + 2 * q) = f2{m == -INFINITY ? m : -raise_of(m), l};
 #pragma unroll
@@ -614,7 +613,6 @@ __global__ __launch_bounds__(64 * kWaves, DK > 128 ? 1 : 2) void paged_prefill_f
 // 128, 157, 96; 16 over 4 of 192, 1000 over 4000, 470, 92; a product of 8192³ reaches 153.)
 template <int DK>
 __global__ __launch_bounds__(256, DK > 128 ? 1 : 2) void paged_prefill_f32_kernel(PagedAttnArgs a, int nq) {
-  constexpr int kWaves = 4, kQ = 32 * kWaves;
   // Keys of a tile here: 32 where 64 would take more registers than there are (1000 tokens over 4000 keys, 16
   // heads over 4 of 192, 470 µs, 475; 512 over 2048, 8 of 256, 105, 135; of 128 156.7, 158.5).
   constexpr int KT = DK > 96 ? 32 : kK;
@@ -627,7 +625,7 @@ __global__ __launch_bounds__(256, DK > 128 ? 1 : 2) void paged_prefill_f32_kerne
   __shared__ __align__(16) float Ks[KT][P];
   __shared__ __align__(16) float Vs[KT][P];
   Tile w;
-  if (!find_tile<kQ, DK>(a, nq, w)) return;
+  if (!find_tile<DK>(a, nq, w)) return;
   w.scalars();
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int dk = a.dk, R = w.n * a.group, hi = lane >> 5, l32 = lane & 31;
@@ -833,7 +831,7 @@ __global__ __launch_bounds__(256, DK > 128 ? 1 : 2) void paged_prefill_f32_kerne
     });
     return;
   }
-  const Parts parts(a, kQ);
+  const Parts parts(a);
   const size_t q = (static_cast<size_t>(w.slot) + w.piece) * kQ + wave * 32 + l32;
   // A part's reference is in powers of two: what m·cscale, which may be large, and its sum with the lift are off
   // by their roundings goes into the part (halved first, so that the largest values stay finite).
@@ -848,10 +846,6 @@ __global__ __launch_bounds__(256, DK > 128 ? 1 : 2) void paged_prefill_f32_kerne
   each_pair([&](int dim, f2 v) { *reinterpret_cast<f2*>(parts.po + q * DK + dim) = f2{v.x * f, v.y * f}; });
 }
 
-// Queries of a workgroup: float16 at head dims above 64 eight waves, which share what is written to LDS (a
-// piece of 2048 tokens over 8192 keys of 128: 307 µs, 322 with four; of 64 215 and 189), where a KV head has
-// more than four take; above 128 the registers are four waves'.
-int queries_of(int dt, int R, int dk) { return dt == F16 && dk > 64 && dk <= 128 && R > 128 ? 256 : 128; }
 // Columns of the kernel that takes a head dim.
 int columns_of(int dt, int dk) {
   return dk <= 32 && dt == F32 ? 32 : dk <= 64 ? 64 : dk <= 96 ? 96 : dk <= 128 ? 128 : dk <= 192 ? 192 : 256;
@@ -860,15 +854,13 @@ int columns_of(int dt, int dk) {
 // Tiles of queries, the workgroups that take them and their pieces, places for parts (0: no keys are in pieces) and
 // tiles that may be in pieces.
 struct Grid {
-  int q, nq;
+  int nq;
   long long groups, slots, split;
 };
 Grid grid_of(int dt, int B, int H, int Hkv, int S, int P, int dk) {
   Grid g;
-  const int R = H / Hkv * S;
-  g.q = queries_of(dt, R, dk);
-  g.nq = (R + g.q - 1) / g.q;
-  const long long tiles = static_cast<long long>(g.nq) * Hkv * B, all = held(g.q, columns_of(dt, dk));
+  g.nq = (H / Hkv * S + kQ - 1) / kQ;
+  const long long tiles = static_cast<long long>(g.nq) * Hkv * B, all = held(columns_of(dt, dk));
   const int most = Plan{kLeastTiles, 0, 0}.pieces((P - 1) / kK + 1);  // pieces of a tile
   g.groups = tiles;
   g.slots = g.split = 0;
@@ -882,26 +874,22 @@ Grid grid_of(int dt, int B, int H, int Hkv, int S, int P, int dk) {
   return g;
 }
 
-template <typename T, int DK, int Q>
+template <typename T, int DK>
 int launch_kernels(const PagedAttnArgs& a, const Grid& g, hipStream_t st) {
   const unsigned n = static_cast<unsigned>(g.groups);
-  if constexpr (sizeof(T) == 2) paged_prefill_f16_kernel<DK, Q / 32><<<n, 2 * Q, 0, st>>>(a, g.nq);
-  else paged_prefill_f32_kernel<DK><<<n, 2 * Q, 0, st>>>(a, g.nq);
+  if constexpr (sizeof(T) == 2) paged_prefill_f16_kernel<DK><<<n, 64 * kWaves, 0, st>>>(a, g.nq);
+  else paged_prefill_f32_kernel<DK><<<n, 64 * kWaves, 0, st>>>(a, g.nq);
   NML_LAUNCHED();
   if (g.slots == 0) return 0;
   constexpr int kRows = kMergers / (DK / 4);
-  paged_merge_kernel<T, DK, Q><<<static_cast<unsigned>(g.split * ((Q + kRows - 1) / kRows)), kMergers, 0, st>>>(a);
+  paged_merge_kernel<T, DK><<<static_cast<unsigned>(g.split * ((kQ + kRows - 1) / kRows)), kMergers, 0, st>>>(a);
   NML_LAUNCHED();
   return 0;
 }
 
 template <int DK>
 int launch_columns(int dt, const PagedAttnArgs& a, const Grid& g, hipStream_t st) {
-  if (dt == F32) return launch_kernels<float, DK, 128>(a, g, st);
-  if constexpr (DK > 64 && DK <= 128) {
-    if (g.q == 256) return launch_kernels<half_t, DK, 256>(a, g, st);
-  }
-  return launch_kernels<half_t, DK, 128>(a, g, st);
+  return dt == F32 ? launch_kernels<float, DK>(a, g, st) : launch_kernels<half_t, DK>(a, g, st);
 }
 
 }  // namespace
@@ -918,14 +906,14 @@ bool paged_prefill_applies(int dt, int H, int Hkv, int S, int dk) {
 
 size_t paged_prefill_workspace(int dt, int B, int H, int Hkv, int S, int P, int dk) {
   const Grid g = grid_of(dt, B, H, Hkv, S, P, dk);
-  return g.slots == 0 ? 0 : kCounterBytes + sizeof(float) * g.slots * g.q * (2 + columns_of(dt, dk));
+  return g.slots == 0 ? 0 : kCounterBytes + sizeof(float) * g.slots * kQ * (2 + columns_of(dt, dk));
 }
 
 int launch_paged_prefill(int dt, PagedAttnArgs a, hipStream_t st) {
   const Grid g = grid_of(dt, a.B, a.H, a.Hkv, a.S, a.max_pages << a.shift, a.dk);
   a.slots = static_cast<int>(g.slots);
   switch (columns_of(dt, a.dk)) {
-    case 32: return launch_kernels<float, 32, 128>(a, g, st);
+    case 32: return launch_kernels<float, 32>(a, g, st);
     case 64: return launch_columns<64>(dt, a, g, st);
     case 96: return launch_columns<96>(dt, a, g, st);
     case 128: return launch_columns<128>(dt, a, g, st);
