@@ -5,6 +5,7 @@ import pytest
 
 from nimbleml_amd import _native as N
 from nimbleml_amd import kernels as K
+from test_gpu_kv4_graphs import Graph, hip  # noqa: F401  (the fixture)
 from test_gpu_paged import Cache, check, queries, upload
 
 pytestmark = pytest.mark.gpu
@@ -64,3 +65,41 @@ def test_one_workspace_serves_calls_of_any_mixture(gpu, dtype):
             d[0].ptr, cache.c.k_pages.ptr, cache.c.v_pages.ptr, table.ptr, d[1].ptr, d[2].ptr, out.ptr, batch, kv, kv, s,
             pages, page, cache.c.num_pages, dk, 8.0, ws.ptr, most, None, code))
         assert np.array_equal(out.numpy(), K.paged_attention(q, cache.c, cache.table, lens, 8.0, counts).numpy())
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_a_captured_call_follows_lengths_and_counts(gpu, hip, dtype):  # noqa: F811
+    """One graph, replayed over batches that are cut into pieces in other ways each time."""
+    batch, kv, group, dk, page, pages, seq = 8, 4, 1, 64, 16, 160, 130
+    cache, room, code, heads = Cache(batch, kv, dk, page, pages, dtype, 2), page * pages, N.np_dtype_code(dtype), kv * group
+    r, need = np.random.RandomState(6), N.sz()
+    q = queries(batch, heads, seq, dk, dtype, 9)
+    d = [upload(x) for x in (q, cache.table, np.zeros(batch, np.int32), np.zeros(batch, np.int32))]
+    N.check(N.lib.nml_paged_attention_workspace(batch, heads, kv, seq, pages, page, dk, code, N.C.byref(need)))
+    ws, out = upload(np.zeros(need.value, np.uint8)), upload(np.zeros((batch, seq, heads * dk), dtype))
+
+    def work():
+        N.check(N.lib.nml_paged_attention_device(
+            d[0].ptr, cache.c.k_pages.ptr, cache.c.v_pages.ptr, d[1].ptr, d[2].ptr, d[3].ptr, out.ptr, batch, heads, kv,
+            seq, pages, page, cache.c.num_pages, dk, 8.0, ws.ptr, need.value, None, code))
+
+    graph = Graph(hip, work)
+    try:
+        for i in range(6):
+            lens = r.randint(0, room + 1, batch).astype(np.int32)
+            counts = r.randint(0, (seq if i % 2 else 3) + 1, batch).astype(np.int32)
+            lens[i], counts[i] = room, seq
+            if i == 2:
+                lens[:], counts[:] = room, seq
+            if i == 3:
+                counts[:] = 0
+            for x, new in zip((d[2], d[3], out), (lens, counts, np.zeros(out.shape, dtype))):
+                N.check(N.lib.nml_memcpy_h2d(x.ptr, new.ctypes.data, new.nbytes))
+            N.synchronize()
+            graph.run()
+            graph.wait()
+            got = out.numpy()
+            assert np.array_equal(got, K.paged_attention(q, cache.c, cache.table, lens, 8.0, counts).numpy()), i
+            assert counts.any() or not got.any()
+    finally:
+        graph.close()
