@@ -10,7 +10,7 @@ Each takes host arrays or ``DeviceArray``s in the compute dtype and returns
   KV4Cache, kv4_write, kv4_read, kv4_attention
                               a KV cache in 4 bits: quantised as it is written, read back,
                               attended to by one or several new tokens (no reference kernel)
-  PagedKVCache, paged_write, paged_attention
+  PagedKVCache, paged_write, paged_attention, paged_attention_workspace
                               a KV cache in pages: written, attended to by one or several new
                               tokens (no reference kernel)
   token_logprobs, token_logprobs_backward
@@ -541,13 +541,32 @@ def paged_write(cache, k, v, table, pos=None, counts=None):
                      f"outside [0, {cache.num_pages}) or a count outside [0, {seq}]")
 
 
-def paged_attention(q, cache, table, lens, scale, counts=None):
+def _paged_attention_bytes(cache, *sizes):
+    need = C.c_size_t()
+    N.check(N.lib.nml_paged_attention_workspace(*sizes, cache.page_size, cache.dk,
+                                                N.np_dtype_code(cache.dtype), C.byref(need)))
+    return need.value
+
+
+def paged_attention_workspace(cache, batch, heads, seq, max_pages):
+    """A workspace for ``paged_attention`` over ``cache`` by ``heads`` query heads, ``seq`` new tokens
+    and tables of (batch, max_pages): a uint8 ``DeviceArray``, zeroed, which calls that run one after
+    another may share, also with other sizes that need no more. Calls of several threads that can
+    run at the same time need one each."""
+    ws = N.DeviceArray((_paged_attention_bytes(cache, batch, heads, cache.kv_heads, seq, max_pages),), np.uint8)
+    N.check(N.lib.nml_memset(ws.ptr, 0, ws.nbytes))
+    return ws
+
+
+def paged_attention(q, cache, table, lens, scale, counts=None, *, workspace=None):
     """Causal attention of each row's ``counts[b]`` (None: all ``seq``) last cached tokens over its
     pages: ``q`` (batch, heads, seq, dk), ``table`` (batch, pages of a row), ``lens`` (batch,) tokens
     cached per row, these included, ``scale`` the sqrt(dk) divisor; query head h reads KV head
     h // (heads // kv_heads). Returns the merged-head output (batch, seq, heads·dk), zeros for
-    tokens from ``counts[b]`` on and for tokens that see no key. Raises ValueError for a length
-    outside the table, a count outside [0, seq] or a page outside the cache."""
+    tokens from ``counts[b]`` on and for tokens that see no key. ``workspace``: what
+    ``paged_attention_workspace`` gave (None: made and freed here, for which a call takes 8 to 40 µs
+    longer). Raises ValueError for a length outside the table, a count outside [0, seq], a page
+    outside the cache or a workspace that is too small."""
     host, (batch, max_pages) = _page_table(cache, table, "paged_attention")
     if len(q.shape) != 4 or q.shape[0] != batch or q.shape[3] != cache.dk:
         raise ValueError(f"paged_attention: q {q.shape} for {batch} rows, head dim {cache.dk}")
@@ -566,18 +585,17 @@ def paged_attention(q, cache, table, lens, scale, counts=None):
     cd = _rows_i32(counts, batch, "paged_attention: counts")
     code = N.np_dtype_code(cache.dtype)
     sizes = (batch, heads, cache.kv_heads, seq, max_pages, cache.page_size)
-    need = C.c_size_t()
-    N.check(N.lib.nml_paged_attention_workspace(*sizes, dk, code, C.byref(need)))
-    ws = N.DeviceArray((need.value,), np.uint8) if need.value else None
-    if ws is not None:
-        N.check(N.lib.nml_memset(ws.ptr, 0, ws.nbytes))
+    if workspace is None:
+        workspace = paged_attention_workspace(cache, batch, heads, seq, max_pages)
+    elif workspace.nbytes < (need := _paged_attention_bytes(cache, *sizes[:-1])):
+        raise ValueError(f"paged_attention: a workspace of {need} bytes is needed, got {workspace.nbytes}")
     out = N.DeviceArray((batch, seq, heads * dk), cache.dtype)
     if cd is not None:
         N.check(N.lib.nml_memset(out.ptr, 0, out.nbytes))
     err = N.DeviceArray.from_host(np.zeros(1, np.int32))
     N.check(N.lib.nml_paged_attention_device(
         qd.ptr, cache.k_pages.ptr, cache.v_pages.ptr, td.ptr, ld.ptr, N.ptr(cd), out.ptr, *sizes,
-        cache.num_pages, dk, float(scale), N.ptr(ws), need.value, err.ptr, code))
+        cache.num_pages, dk, float(scale), N.ptr(workspace), workspace.nbytes, err.ptr, code))
     _check_flag(err, f"paged_attention: a length is outside [0, {max_pages * cache.page_size}], a page "
                      f"outside [0, {cache.num_pages}) or a count outside [0, {seq}]")
     return out
