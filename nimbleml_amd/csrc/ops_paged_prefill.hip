@@ -87,17 +87,23 @@ struct Row {
   }
 };
 
-// Where the keys are in pieces, a piece has `per` tiles of them: an even share, for as many workgroups as the
-// card holds (H), of what all rows have to do, W. Row b's tiles of queries have up to p_b = ⌈kt_b / per⌉
-// pieces, and those that are in pieces places for p_b parts each. As p_b − 1 < kt_b / per and Σ nq_b·kt_b·Hkv ≤ 2W
-// ≤ 2H·per, the pieces past the tiles' first are at most 2H, and so are the tiles in pieces. What the host makes
-// room for is bounded the same way (grid_of). A row of little more than a piece stays whole: two rows of 2048 tokens
-// over 8192 keys, 16 heads of 64, 277 µs, 297 with a second piece of an eighth and its merge.
+// Where the keys are in pieces, a piece has about `per` tiles of them: an even share, for as many workgroups as the
+// card holds (H), of what all rows have to do, W. Row b's tiles of queries have up to p_b ≤ ⌈kt_b / per⌉ pieces,
+// and those that are in pieces places for p_b parts each. As p_b − 1 < kt_b / per and Σ nq_b·kt_b·Hkv ≤ 2W ≤
+// 2H·per, the pieces past the tiles' first are at most 2H, and so are the tiles in pieces. What the host makes room
+// for is bounded the same way (grid_of).
 struct Plan {
   int per, live;  // key tiles of a piece; tiles of queries of all rows and KV heads
   int same;       // tiles of queries of each row, where all have as many, else 0
-  // Pieces of a row's tiles at most.
-  __host__ __device__ int pieces(int kt) const { return 4 * kt <= 5 * per ? 1 : (kt + per - 1) / per; }
+  // Pieces of a row's tiles at most, as long as each other, of a quarter more than `per` at most: so that they do not
+  // pass what the card holds by little (1024 tokens over 4096 keys, 16 heads over 4 of 96, 73 µs, 96 where pieces are `per`
+  // at most), and that a row of little more than a piece stays whole (two rows of 2048 tokens over 8192 keys, 16
+  // heads of 64, 283 µs, 297 with a second piece of an eighth). Pieces of `per` and a short one behind them took 90 in
+  // place of 63 for 30 rows of 128 tokens over 2000 keys, 8 heads of 64.
+  __host__ __device__ int pieces(int kt) const {
+    const int p = (kt - per / 2 + per - 1) / per;
+    return 4 * kt <= 5 * per ? 1 : p < 2 ? 2 : p;
+  }
 };
 // mine: this lane's row, where there are no more than 64.
 template <int DK>
@@ -137,11 +143,11 @@ __device__ __forceinline__ Plan plan_of(const PagedAttnArgs& a, int lane, bool f
 // `piece` of `pieces`, whose first has its part at `slot`.
 struct Tile {
   int b, hk, q0, len, n, kend, t0, nt, piece, pieces, slot;
-  // The keys of the queries, in pieces of per tiles. False: this piece is not there.
-  __device__ __forceinline__ bool cut(const PagedAttnArgs& a, int per) {
+  // The keys of the queries, in pieces of which the row's keys have p. False: this piece is not there.
+  __device__ __forceinline__ bool cut(const PagedAttnArgs& a, int p) {
     const int last = min((q0 + kQ - 1) / a.group, n - 1);  // the last token
     kend = max(len - n + last + 1, 0);
-    const int tiles = (kend + kK - 1) / kK;
+    const int tiles = (kend + kK - 1) / kK, per = p == 1 ? max(tiles, 1) : ((len + kK - 1) / kK + p - 1) / p;
     pieces = max(1, (tiles + per - 1) / per);
     t0 = piece * per;
     nt = min(per, tiles - t0);
@@ -208,7 +214,7 @@ __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int nq, Tile& 
     t.len = r.len;
     t.n = r.n;
     t.piece = t.slot = 0;
-    return t.q0 < t.n * a.group && t.cut(a, 1 << 30);
+    return t.q0 < t.n * a.group && t.cut(a, 1);
   }
   // Every tile's first piece, then the others, which a tile of few keys may not have (among the first they leave
   // half of the CUs idle). Where all rows have as many tiles of queries, in the order above; else row after row.
@@ -229,7 +235,7 @@ __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int nq, Tile& 
   t.piece = turn + (more ? 1 : 0);
   t.q0 = qt * kQ;
   t.slot += (t.hk * nq + qt) * p;
-  return t.cut(a, p == 1 ? 1 << 30 : plan.per);
+  return t.cut(a, p);
 }
 
 // Where a piece's part goes: per query its reference (in powers of two) and Σ p, then its Σ p·v.
@@ -251,6 +257,7 @@ __global__ __launch_bounds__(kMergers) void paged_merge_kernel(PagedAttnArgs a) 
   const int lane = threadIdx.x & 63;
   Row mine;
   const Plan plan = plan_of<DK>(a, lane, false, mine);
+  if (a.B <= 64 && !__any(plan.pieces(mine.kt) > 1)) return;
   Tile w;
   int nq = 1, p = 1;
   if (!find_row(a, plan, mine, static_cast<int>(blockIdx.x) / kBlocks, lane, [](int tiles, int pieces) { return pieces > 1 ? tiles : 0; }, w, nq, p))
@@ -260,7 +267,7 @@ __global__ __launch_bounds__(kMergers) void paged_merge_kernel(PagedAttnArgs a) 
   w.q0 = qt * kQ;
   w.slot += w.piece * p;
   w.piece = 0;
-  w.cut(a, plan.per);
+  w.cut(a, p);
   if (w.pieces == 1) return;
   const int c = blockIdx.x % kBlocks * kRows + threadIdx.x / L, d = threadIdx.x % L * 4;
   if (threadIdx.x / L >= kRows || c >= kQ || w.q0 + c >= w.n * a.group || d >= a.dk) return;
@@ -865,9 +872,9 @@ Grid grid_of(int dt, int B, int H, int Hkv, int S, int P, int dk) {
   g.groups = tiles;
   g.slots = g.split = 0;
   // One row's tiles that fill the card stay whole. Those of several may be of one row alone that has many new
-  // tokens, or many more keys than the others. (Of more than 512 the workgroups would spend their time on
-  // lengths.)
-  if (most == 1 || (B == 1 && tiles >= all) || B > 512) return g;
+  // tokens, or many more keys than the others; of more than 64, whose lengths a workgroup has to go through in several
+  // turns, only where tiles are few (500 rows of 80 tokens over 400 keys, 4 heads of 64: 162 µs, 99 whole).
+  if (most == 1 || (B == 1 && tiles >= all) || (B > 64 && 2 * tiles > all)) return g;
   g.groups = tiles + std::min(2 * all, tiles * (most - 1));
   g.split = std::min(tiles, 2 * all);
   g.slots = std::min(2 * all + g.split, tiles * most);
