@@ -15,10 +15,9 @@
 // entries of one id meet in the lowest of them, added in their order, so nothing depends on the
 // order of atomics.
 //
-// Both are bound by HBM where rows are many. 4096 rows of 32000 float16 logits, 64 entries each: the loss
-// 53 µs, 5.0 TB/s of reads; the gradient 110 µs, 4.8 TB/s of reads and writes. 2048 rows of 4096 float32
-// logits: 8.6 and 11.6 µs, in part from the last cache. A single row of 50304: 7.4 and 6.4 µs with its
-// launch.
+// Both are bound by HBM where rows are many. With inputs that change from call to call, 4096 rows of 32000 float16
+// logits, 64 entries each: the loss 54 µs, 4.9 TB/s of reads; the gradient 120 µs, 4.4 TB/s of reads and
+// writes. 2048 rows of 4096 float32 logits: 9.9 and 13.0 µs. A single row of 50304: 7.4 and 6.4 µs with its launch.
 #include "kernels.hpp"
 #include "row_pieces.hpp"
 
@@ -207,7 +206,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillBwdArgs a, int 
   const float sp = s / a.l[r];
   auto put = [&](int i0, const vec& d) {
     if (i0 >= 0 && i0 + E <= a.V && (reinterpret_cast<uintptr_t>(out + i0) & 15) == 0) {
-      __builtin_nontemporal_store(d, reinterpret_cast<vec*>(out + i0));  // (a row of 32000: 111 µs, 126 kept in the caches)
+      __builtin_nontemporal_store(d, reinterpret_cast<vec*>(out + i0));  // (4096 rows of 32000: 120 µs, 133 with stores kept in the caches)
     } else {
 #pragma unroll
       for (int j = 0; j < E; ++j)

@@ -116,9 +116,10 @@ int write_launch(PagedWriteArgs a, size_t es, hipStream_t st) {
 //
 // Bound by HBM where keys are many: 16 rows of 1 to 8 Ki keys, 32 heads over 8 of 128, float16, 66 µs,
 // 4.6 TB/s of keys and values (a copy 4.8). Where few, by a chain of dependent steps: lengths, page
-// numbers, keys, rounds, merge and the pieces' merge: one row of 1023 keys, 16 heads of 64, 9.1 µs; 16
-// rows of up to 2048 and up to 5 tokens, 8 heads of 32, float32, 14.2. (Where work is cut finely enough the
-// merge is what is left: its loads are in batches of 16 pieces, of four where there are no more.)
+// numbers, keys, rounds, merge and the pieces' merge: one row of 1023 keys, 16 heads of 64, 9.0 µs; 16
+// rows of up to 2048 and up to 5 tokens, 8 heads of 32, float32, 14.0. (Where work is cut finely enough the
+// merge is what is left: its loads are in batches of 16 pieces, of four where there are no more.) Below, where
+// changing inputs are not mentioned, both sides of a choice were timed over one set.
 
 typedef short s4 __attribute__((ext_vector_type(4)));
 

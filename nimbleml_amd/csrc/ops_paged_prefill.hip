@@ -13,7 +13,7 @@
 // those below 2^-21 of the largest, 2^-31 of that), and Σ p is of the two, so that an output is off by
 // little more than its own rounding to float16. As one float16 value an output would be off as far
 // again (2.9·10^-4 of its norm, 2.1·10^-4), for a third fewer matrix instructions: 2048 tokens over 8192 keys,
-// 32 heads of 128 over 8, 341 µs and 425; two rows of them with 16 heads of 64, 244 and 277.
+// 32 heads of 128 over 8, 341 µs and 425 on one box; two rows of them with 16 heads of 64, 244 and 277.
 //
 // One barrier a tile: K is written to LDS two tiles ahead and V one, from registers that were loaded a
 // tile before, and the scores of the next tile are formed beside the probabilities of this one. A
@@ -23,10 +23,11 @@
 // Where the tiles of queries leave CUs idle the keys are cut into pieces, whose parts a second launch
 // merges.
 //
-// Bound by the matrix pipe and the exponentials beside it. 2048 tokens over 8192 keys, 32 heads of 128 over
-// 8, float16: 306 µs, 786 TFLOP/s, where a product of 8192³ reaches 1089; two rows of them with 16 heads of
-// 64: 188, 640 (as many exponentials for half the products); 16 over 4 of 256: 624, 385 (one wave a SIMD, and
-// values moved between its two halves of the registers).
+// Bound by the matrix pipe, which has three products for the formula's two, and the exponentials beside it. 2048 tokens
+// over 8192 keys, 32 heads of 128 over 8, float16: 405 to 440 µs by the box, 594 TFLOP/s of the formula's and 890 on the
+// pipe, where a product of 8192³ reaches 1464; two rows of them with 16 heads of 64: 284, 420 and 630 (as many
+// exponentials for half the products); 16 over 4 of 256: 722, 330 and 500 (one wave a SIMD, and values moved between
+// its two halves of the registers).
 #include <algorithm>
 #include <type_traits>
 
@@ -616,8 +617,8 @@ __global__ __launch_bounds__(64 * kWaves, DK > 128 ? 1 : 2) void paged_prefill_f
 // 8i + 4 + e of K, so that a lane's 16 bytes of a row feed four of them, and whose 32 rows are every W-th
 // dim of V, so that one read feeds W tiles of the output. A tile of keys costs 16 times the cycles on
 // the matrix pipe that its softmax takes beside it: one buffer and two barriers a tile, with the other
-// workgroup of the CU in between. (1024 tokens over 4096 keys: 8 heads of 64, 87 µs, 86 TFLOP/s; 8 over 2 of
-// 128, 157, 96; 16 over 4 of 192, 1000 over 4000, 470, 92; a product of 8192³ reaches 153.)
+// workgroup of the CU in between. (1024 tokens over 4096 keys: 8 heads of 64, 90 µs, 84 TFLOP/s; 8 over 2 of
+// 128, 161, 93; 16 over 4 of 192, 1000 over 4000, 470, 92; a product of 8192³ reaches 153.)
 template <int DK>
 __global__ __launch_bounds__(256, DK > 128 ? 1 : 2) void paged_prefill_f32_kernel(PagedAttnArgs a, int nq) {
   // Keys of a tile here: 32 where 64 would take more registers than there are (1000 tokens over 4000 keys, 16

@@ -18,7 +18,7 @@
 // gives. A 64-bit multiply-add runs at the rate of a 32-bit one on this card, and an exponential takes
 // 14 such operations: the first launch is bound by them (and the loads before), the second by its
 // chain of dependent steps, two passes over a part with a count of arrivals in between. One sequence of four
-// drafts, 32000 float32 logits a row: 3.1 and 8.3 µs; 32 of up to five, 50304 float16 logits: 14.9 and 12.8.
+// drafts, 32000 float32 logits a row: 3.5 and 8.6 µs; 32 of up to five, 50304 float16 logits: 15.2 and 11.8.
 #include "kernels.hpp"
 
 namespace nml {
@@ -28,8 +28,8 @@ namespace {
 constexpr int kThreads = 256, kMaxRows = kMaxDrafts + 1;
 // Elements of a part of a row, a thread's times kThreads: few where the rows are few, so that a lone
 // call's chain is short. (µs of both launches, few or many by size / always few / always many: one
-// sequence of four drafts, 32000 float32, 11.4 / 11.8 / 19.8; 32 of up to five, 50304 float16, 27.0 / 27.4 /
-// 29.0; 64 of eight, 32000 float16, 40.9 / 47.2 / 42.2.)
+// sequence of four drafts, 32000 float32, 11.5 / 11.7 / 19.7; 32 of up to five, 50304 float16, 27.0 / 27.0 /
+// 29.4; 64 of eight, 32000 float16, 44.8 / 51.8 / 46.3.)
 constexpr int kSmall = 8, kLarge = 32;
 constexpr int kLine = 32;  // words from one sequence's counter to the next: a line of its own
 
