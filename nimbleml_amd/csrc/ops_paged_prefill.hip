@@ -106,6 +106,7 @@ struct Plan {
     return 4 * kt <= 5 * per ? 1 : p < 2 ? 2 : p;
   }
 };
+
 // mine: this lane's row, where there are no more than 64.
 template <int DK>
 __device__ __forceinline__ Plan plan_of(const PagedAttnArgs& a, int lane, bool first, Row& mine) {
